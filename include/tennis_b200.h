@@ -38,6 +38,15 @@ extern "C" {
 #define TSB_ACT_NONE 0
 #define TSB_ACT_RELU 1       /* src/kernels/cpu/relu.cpp:30-52 */
 #define TSB_ACT_LEAKY_RELU 2 /* src/kernels/cpu/leaky_relu.cpp:39-67, attribute "scale" */
+/* ... and, beyond the convolutions' three, after tsb_inner_prod_i8 and tsb_group_norm_nhwc */
+#define TSB_ACT_SILU 3       /* v / (1 + exp(-v)) */
+#define TSB_ACT_GELU 4       /* v / 2 * (1 + erf(v / sqrt(2))) */
+
+/* element types of the operators that take more than one */
+#define TSB_TYPE_F32 0
+#define TSB_TYPE_F16 1
+#define TSB_TYPE_BF16 2
+#define TSB_TYPE_I8 3
 
 /* memory layouts of activations */
 #define TSB_LAYOUT_NCHW 0     /* the operator-visible layout of TenniS tensors */
@@ -340,6 +349,93 @@ TSB_API int tsb_inner_prod_f32(const float *x, const float *w, const float *bias
  */
 TSB_API int tsb_concat_i8_nhwc(const int8_t *a, int channels_a, const int8_t *b, int channels_b, int8_t *y, int64_t pixels,
                                void *stream);
+
+/*
+ * quantize with a scale for each row, taken from the row (this and the next two operators have no counterpart in the
+ * reference, whose quantize scales are attributes; they are what int8 networks of matrix products and group norms need
+ * next to its convolutions).
+ *   a = max_c |x[r][c]|;  y[r][c] = half_even(x[r][c] * fp32(127 / a));  scales[r] = fp32(a / 127)
+ * so that scales[r] * y[r][c] stands for x[r][c].  Rows are tokens of an activation or output channels of a weight tensor.
+ *   - x: fp32, fp16 or bf16 [rows, cols], rows x_pitch elements apart (0: the same row again);  y: rows y_pitch bytes apart; only the
+ *     cols bytes of a row are written.  A y_pitch that is a multiple of 16 (and a 16-byte aligned y) is what tsb_inner_prod_i8
+ *     reads fastest.  x and y do not overlap.
+ *   - Rows whose largest magnitude is below 2^-100 count as zero: zeros and a scale of zero.
+ *   - A NaN in the row makes its scale NaN and all its values -128; an infinity makes the scale infinite, finite values 0 and
+ *     infinite ones -128 (the conversion rule of tsb_quantize_f32_i8): either way what is computed from the row shows it.
+ */
+TSB_API int tsb_quantize_rows_i8(const void *x, int x_type, int64_t x_pitch, int8_t *y, int64_t y_pitch, float *scales,
+                                 int64_t rows, int64_t cols, void *stream);
+
+/*
+ * inner product on int8 operands with a scale per token (row of x) and per output channel (row of w): operator "inner_prod"
+ * (src/kernels/gpu/inner_prod.cu) the way conv2d_quantized is operator conv2d.
+ *   acc = sum_k x[m][k] * w[n][k]                                     int32, exact (k at most 131071)
+ *   v = float(acc) * w_scales[n] * x_scales[m] (+ bias[n]) (+ residual[m][n]);  v = activation(v);  y[m][n] = v
+ * Every step is a separately rounded fp32 operation, with one more rounding to y's type; the bits of a result depend neither on
+ * the kernel that computes it nor on the number of rows that are computed with it.
+ *   - x: int8 rows with x_scales, or floating rows without: those are quantized as tsb_quantize_rows_i8 does it, with the
+ *     same bits as a call of that function in front.
+ *   - Any pitch and alignment is right; operands whose address and pitch are multiples of 16 bytes (tsb_quantize_rows_i8's
+ *     with such a pitch, NHWC_PAD tensors with k = channels) run on the tensor cores.
+ *   - y does not overlap the other tensors, but may be the residual itself (same address and pitch).
+ *   - m = 0 or n = 0: nothing is done.
+ */
+typedef struct tsb_inner_prod_args {
+    int64_t m, n, k;                 /* y [m, n] = x [m, k] . w [n, k] */
+    const void *x;
+    int64_t x_pitch;                 /* elements between rows, here and below */
+    const float *x_scales;           /* device; NULL with a floating x */
+    int64_t x_scales_stride;         /* floats between two rows' scales: 1, or 0 where one scale is all rows' */
+    const int8_t *w;
+    int64_t w_pitch;
+    const float *w_scales;           /* [n] device */
+    const float *bias;               /* [n] device or NULL */
+    const void *residual;            /* device or NULL, of y's type */
+    int64_t residual_pitch;
+    void *y;
+    int64_t y_pitch;
+    int x_type;                      /* TSB_TYPE_I8, or a floating type */
+    int y_type;                      /* TSB_TYPE_F32, F16 or BF16 */
+    int activation;                  /* TSB_ACT_* */
+    float leaky_scale;
+    int residual_after_activation;   /* 0: act(v + residual); 1: act(v) + residual */
+    int kernel;                      /* TSB_KERNEL_AUTO; another one is tests' (same bits, TSB_ERR_UNSUPPORTED where it cannot) */
+} tsb_inner_prod_args;
+
+/* Scratch of a call with floating rows (256-byte aligned device memory, at least this many bytes, used until the call's work
+ * on the stream is done; calls that may overlap have one each); 0 for int8 rows. */
+TSB_API size_t tsb_inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *args);
+TSB_API int tsb_inner_prod_i8(const tsb_inner_prod_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Group norm with an activation on channels-last tensors: x [n, pixels, channels], channels in `groups` equal runs.
+ *   mean, variance (biased) of an image's group over its pixels and channels, summed in 64 bits
+ *   v = (x - mean) * (1 / sqrt(variance + eps)) * gamma[c] + beta[c];  y = activation(v)
+ * mean and reciprocal deviation are rounded to fp32 once; the steps behind are separately rounded fp32 operations.
+ *   - x: fp32, fp16 or bf16, channels next to each other, pixels and images any number of elements apart.
+ *   - y of x's type, pixels and images apart likewise; it may be x itself (same address and strides), else they do not overlap.
+ *   - y of TSB_TYPE_I8: quantize(v) with the rules of tsb_quantize_f32_i8 on the channel-major element index and one
+ *     requantize scale for the batch or one per image, written as NHWC_PAD (dense, padding channels zero; y's strides
+ *     are not looked at): what tsb_conv2d_i8_run takes as TSB_LAYOUT_NHWC_PAD and tsb_inner_prod_i8 as int8 rows of one scale.
+ */
+typedef struct tsb_group_norm_desc {
+    int64_t n, pixels, channels, groups;
+    const void *x;
+    int64_t x_pixel_stride, x_image_stride;   /* elements, here and below */
+    void *y;
+    int64_t y_pixel_stride, y_image_stride;
+    const float *gamma, *beta;                /* [channels] device, or NULL: 1 and 0 */
+    double eps;
+    const float *requant_scales_host;         /* int8 output: host, 1 or n scales, at most TSB_MAX_REQUANT_SCALES */
+    int n_requant_scales;
+    int x_type, y_type;
+    int activation;                           /* TSB_ACT_* */
+    float leaky_scale;
+} tsb_group_norm_desc;
+
+/* Scratch of a call, as for tsb_inner_prod_i8. */
+TSB_API size_t tsb_group_norm_workspace_bytes(const tsb_group_norm_desc *desc);
+TSB_API int tsb_group_norm_nhwc(const tsb_group_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef TSB_ENABLE_TRACE
 /* Profiling builds only (compile the library with -DTSB_ENABLE_TRACE; release builds carry neither this symbol nor the

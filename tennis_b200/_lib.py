@@ -5,6 +5,7 @@ to build it.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtennis_b200.so")
@@ -15,7 +16,8 @@ ERR_UNSUPPORTED = -2
 ERR_WORKSPACE_TOO_SMALL = -3
 ERR_DEVICE_TIMEOUT = -4
 
-ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_LEAKY_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
 LAYOUT_NCHW, LAYOUT_NHWC_PAD, LAYOUT_STAGED = 0, 1, 2
 KERNEL_AUTO, KERNEL_DIRECT, KERNEL_TCGEN05 = 0, 1, 2
 TUNE_AUTO, TUNE_OFF, TUNE_ON = 0, 1, 2
@@ -48,6 +50,11 @@ class ConvEpilogue(ctypes.Structure):
         ("out_acc", ctypes.c_void_p),
         ("residual_after_activation", ctypes.c_int),
     ]
+
+
+# tsb_inner_prod_args and tsb_group_norm_desc, packed field by field (both have their wide fields first)
+INNER_PROD_ARGS = struct.Struct("@3q P q P q P q P P P q P q i i i f i i")
+GROUP_NORM_DESC = struct.Struct("@4q P 2q P 2q P P d P i i i i f 0q")
 
 
 # name -> (restype, argtypes); every symbol include/tennis_b200.h declares
@@ -90,6 +97,11 @@ SYMBOLS = {
     "tsb_global_avgpool_f32_nhwc": (_i, [_vp, _vp, _i, _i, _i, _vp]),
     "tsb_inner_prod_f32": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
     "tsb_concat_i8_nhwc": (_i, [_vp, _i, _vp, _i, _vp, _i64, _vp]),
+    "tsb_quantize_rows_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "tsb_inner_prod_i8_workspace_bytes": (_sz, [ctypes.c_char_p]),
+    "tsb_inner_prod_i8": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
+    "tsb_group_norm_workspace_bytes": (_sz, [ctypes.c_char_p]),
+    "tsb_group_norm_nhwc": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
     "tsb_kernel_launch_count": (_i64, []),
 }
 

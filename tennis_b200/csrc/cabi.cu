@@ -31,6 +31,12 @@ int maxpool_i8_nhwc(const int8_t *, int8_t *, int, int, int, int, int, int, int,
 int global_avgpool_f32_nhwc(const float *, float *, int, int, int, cudaStream_t);
 int inner_prod_f32(const float *, const float *, const float *, float *, int, int, int, cudaStream_t);
 int concat_i8_nhwc(const int8_t *, int, const int8_t *, int, int8_t *, int64_t, cudaStream_t);
+// quantize_rows.cu, inner_prod_i8.cu, group_norm.cu
+int quantize_rows_i8(const void *, int, int64_t, int8_t *, int64_t, float *, int64_t, int64_t, cudaStream_t);
+size_t inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *);
+int inner_prod_i8(const tsb_inner_prod_args *, void *, size_t, cudaStream_t);
+size_t group_norm_workspace_bytes(const tsb_group_norm_desc *);
+int group_norm_nhwc(const tsb_group_norm_desc *, void *, size_t, cudaStream_t);
 
 namespace {
 
@@ -132,6 +138,19 @@ int tsb_relu_f32(const float *x, float *y, int64_t count, void *stream) {
 }
 int tsb_leaky_relu_f32(const float *x, float *y, int64_t count, float scale, void *stream) {
     return activation_f32(x, y, count, TSB_ACT_LEAKY_RELU, scale, (cudaStream_t)stream);
+}
+
+int tsb_quantize_rows_i8(const void *x, int x_type, int64_t x_pitch, int8_t *y, int64_t y_pitch, float *scales, int64_t rows, int64_t cols,
+                         void *stream) {
+    return quantize_rows_i8(x, x_type, x_pitch, y, y_pitch, scales, rows, cols, (cudaStream_t)stream);
+}
+size_t tsb_inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *args) { return inner_prod_i8_workspace_bytes(args); }
+int tsb_inner_prod_i8(const tsb_inner_prod_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+    return inner_prod_i8(args, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+size_t tsb_group_norm_workspace_bytes(const tsb_group_norm_desc *desc) { return group_norm_workspace_bytes(desc); }
+int tsb_group_norm_nhwc(const tsb_group_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream) {
+    return group_norm_nhwc(desc, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 int tsb_pool_out_dim(int x, int pad_lo, int pad_hi, int k, int stride) {

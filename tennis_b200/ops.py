@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (ACT_LEAKY_RELU, ACT_NONE, ACT_RELU, KERNEL_AUTO, KERNEL_DIRECT, KERNEL_TCGEN05, LAYOUT_NCHW,
+from ._lib import (ACT_GELU, ACT_LEAKY_RELU, ACT_NONE, ACT_RELU, ACT_SILU, KERNEL_AUTO, KERNEL_DIRECT, KERNEL_TCGEN05, LAYOUT_NCHW,
                    LAYOUT_NHWC_PAD, LAYOUT_STAGED, ConvDesc, ConvEpilogue, TsbError, check, float_array)
 
 REQUIRED, OPTIONAL = "required", "optional"
@@ -517,3 +517,199 @@ def repack_nhwc_to_nchw(x, channels, stream=None):
     y = torch.empty((n, channels, h, w), dtype=torch.int8, device=x.device)
     check(_lib.load().tsb_repack_i8_nhwc_to_nchw(_ptr(x), _ptr(y), n, channels, h, w, _stream_ptr(stream)))
     return y
+
+
+# ---- int8 layers with scales per token: quantize_rows, inner_prod_quantized, group_norm_nhwc --------------------------------
+# These three work on the device that their tensors are on, on its current stream or on `stream`; what they allocate (outputs,
+# workspace) belongs to that stream.  Memory of an input that another stream allocated is the caller's to keep until the work is done.
+_TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16, torch.int8: _lib.TYPE_I8}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _on(x, stream):
+    """A context on x's device and on `stream`, or None where the program is there already."""
+    if stream is None:
+        return None if x.get_device() == _current_device() else torch.cuda.device(x.device)
+    _auto_check(stream.device == x.device, "stream.device == x.device")
+    return torch.cuda.stream(stream)
+
+
+def _rows_of(t):
+    """t [..., k] as rows: a tensor [m, k] whose values of a row are neighbours (a copy only where no view is)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _check_vector(t, size, x, name):
+    _auto_check(t.dtype == torch.float32 and t.numel() == size and t.is_contiguous() and t.device == x.device,
+                "%s: %d contiguous float32 values on x's device" % (name, size))
+
+
+def quantize_rows(x, out=None, scales=None, stream=None):
+    """int8 values of x [..., k] (fp32, fp16 or bf16) with a scale for each row, taken from the row: (q, scales) with
+    ``scales[..., None] * q`` standing for x (tsb_quantize_rows_i8 says how it rounds, and what rows of zeros, NaN and infinities give).
+
+    q is [..., k]; its rows start a multiple of 16 bytes apart, the way inner_prod_quantized reads them fastest.  The rows of x are
+    tokens of an activation, or output channels of a weight tensor.  ``out`` (int8, x's shape, values of a row next to each other)
+    and ``scales`` take the results where they are given."""
+    _auto_check(x.is_cuda, "x.is_cuda")
+    there = _on(x, stream)
+    if there is not None:
+        with there:
+            return quantize_rows(x, out, scales)
+    _auto_check(x.dtype in _FLOATS, "x.dtype: float32, float16 or bfloat16, not %s" % x.dtype)
+    _auto_check(x.dim() >= 1 and x.shape[-1] > 0, "x_tensor.size(-1) > 0")
+    shape, k = x.shape, x.shape[-1]
+    rows = _rows_of(x)
+    if out is None:
+        out = torch.empty(shape[:-1] + ((k + 15) // 16 * 16,), dtype=torch.int8, device=x.device)[..., :k]
+    else:
+        _auto_check(out.dtype == torch.int8 and out.shape == shape and out.device == x.device and (out.stride(-1) == 1 or k == 1),
+                    "out: int8 of x's shape on x's device, values of a row next to each other")
+    # (a view: an `out` whose rows lie no fixed step apart is refused, as it could only be written through a copy)
+    try:
+        q = out if out.dim() == 2 else out.view(-1, k)
+    except RuntimeError:
+        raise EjectionException("out: its rows lie no fixed step apart")
+    if scales is None:
+        scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    else:
+        _check_vector(scales, rows.shape[0], x, "scales")
+    status = _lib.load().tsb_quantize_rows_i8(rows.data_ptr(), _TYPE[x.dtype], rows.stride(0), q.data_ptr(), q.stride(0), scales.data_ptr(),
+                                              rows.shape[0], k, _stream_ptr())
+    if status:
+        check(status)
+    return out, scales
+
+
+def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, activation=ACT_NONE, leaky=0.0, out_dtype=None, out=None,
+                         residual_after_activation=False, kernel=KERNEL_AUTO, stream=None):
+    """x [..., k] times w [n, k] transposed, in int8 with int32 sums, a scale per token and per output channel:
+    ``activation(sum * w_scales * x_scales + bias + residual)`` (or ``activation(...) + residual``), [..., n].
+
+    x is int8 with ``x_scales`` (one per row, or one value for all), as quantize_rows gives them, or floating with ``x_scales=None``: then its rows are
+    quantized in the call.  w int8 and w_scales [n] are what quantize_rows makes of a float weight tensor.  ``residual``
+    has the output's type and shape.  ``out_dtype`` is x's type (of int8 rows: float32) unless given; ``out`` takes the result where
+    it is given (it may be ``residual``, and no other operand)."""
+    _auto_check(x.is_cuda, "x.is_cuda")
+    there = _on(x, stream)
+    if there is not None:
+        with there:
+            return inner_prod_quantized(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, out, residual_after_activation, kernel)
+    dynamic = x_scales is None
+    dev = x.device
+    _auto_check(x.dtype in _FLOATS if dynamic else x.dtype == torch.int8,
+                "x.dtype: int8 with x_scales; float32, float16 or bfloat16 without; not %s" % x.dtype)
+    _auto_check(w.dtype == torch.int8 and w.dim() == 2 and w.device == dev, "w: an int8 matrix on x's device")
+    _auto_check(x.dim() >= 1 and x.shape[-1] == w.shape[1], "w_tensor.size(1) == x_tensor.size(-1)")
+    lead, n = x.shape[:-1], w.shape[0]
+    rows = _rows_of(x)
+    m, k = rows.shape
+    w = _rows_of(w)
+    _check_vector(w_scales, n, x, "w_scales")
+    if not dynamic:
+        _check_vector(x_scales, 1 if x_scales.numel() == 1 else m, x, "x_scales")
+    if bias is not None:
+        _check_vector(bias, n, x, "bias")
+    if out is None:
+        dtype = out_dtype if out_dtype is not None else (x.dtype if dynamic else torch.float32)
+        _auto_check(dtype in _FLOATS, "out_dtype: float32, float16 or bfloat16, not %s" % dtype)
+        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+    else:
+        dtype = out.dtype
+        _auto_check(dtype in _FLOATS and out_dtype in (None, dtype) and out.shape == lead + (n,) and out.device == dev and (n <= 1 or out.stride(-1) == 1),
+                    "out: a floating [..., n] on x's device, values of a row next to each other")
+    if residual is not None:
+        _auto_check(residual.dtype == dtype and residual.shape == lead + (n,) and residual.device == dev, "residual: of the output's type and shape on x's device")
+    if not out.numel():
+        return out
+    try:
+        y = out if out.dim() == 2 else out.view(-1, n)
+    except RuntimeError:
+        raise EjectionException("out: its rows lie no fixed step apart")
+    if residual is not None:
+        residual = _rows_of(residual)
+    lib = _lib.load()
+    args = _lib.INNER_PROD_ARGS.pack(m, n, k, rows.data_ptr(), rows.stride(0), 0 if dynamic else x_scales.data_ptr(),
+                                     0 if dynamic or x_scales.numel() == 1 else 1, w.data_ptr(), w.stride(0), w_scales.data_ptr(),
+                                     0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
+                                     0 if residual is None else residual.stride(0), y.data_ptr(), y.stride(0), _TYPE[x.dtype], _TYPE[dtype],
+                                     activation, leaky, 1 if residual_after_activation else 0, kernel)
+    workspace, size = None, 0
+    if dynamic:
+        size = lib.tsb_inner_prod_i8_workspace_bytes(args)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
+    status = lib.tsb_inner_prod_i8(args, _ptr(workspace), size, _stream_ptr())
+    if status:
+        check(status)
+    return out
+
+
+def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_NONE, leaky=0.0, out_dtype=None, requant_scales=None,
+                    out=None, stream=None):
+    """Group norm and activation of a channels-last x [n, ..., channels] (fp32, fp16 or bf16): mean and variance of each image's
+    ``groups`` equal runs of channels over all its pixels, ``activation((x - mean) / sqrt(variance + eps) * gamma + beta)``.
+
+    The result has x's type and shape (``out`` takes it where it is given; it may be x).  ``out_dtype=torch.int8`` with ``requant_scales`` (one, or one per image)
+    gives ``quantize`` of it as NHWC_PAD [n, ..., padded_channels(channels)] instead, what a convolution plan reads."""
+    _auto_check(x.is_cuda, "x.is_cuda")
+    there = _on(x, stream)
+    if there is not None:
+        with there:
+            return group_norm_nhwc(x, groups, gamma, beta, eps, activation, leaky, out_dtype, requant_scales, out)
+    _auto_check(x.dtype in _FLOATS, "x.dtype: float32, float16 or bfloat16, not %s" % x.dtype)
+    _auto_check(x.dim() >= 3, "x_tensor.dims() >= 3")
+    dtype = out_dtype if out_dtype is not None else (x.dtype if out is None else out.dtype)
+    _auto_check(dtype == x.dtype or dtype == torch.int8, "out_dtype: x's type or int8, not %s" % dtype)
+    shape, n, c = x.shape, x.shape[0], x.shape[-1]
+    _auto_check(c > 0, "x_tensor.size(-1) > 0")
+    pixels = x.numel() // (n * c) if n else 0
+    for v, name in ((gamma, "gamma"), (beta, "beta")):
+        if v is not None:
+            _check_vector(v, c, x, name)
+    scales, n_scales = None, 0
+    if dtype == torch.int8:
+        _auto_check(requant_scales is not None, "out_dtype int8 comes with requant_scales")
+        scales = _scales_of(requant_scales)
+        n_scales = len(scales)
+    x_step = _pixel_step(x)
+    if x_step is None:
+        x, x_step = x.contiguous(), c
+    want = shape[:-1] + (padded_channels(c),) if scales is not None else shape
+    if out is None:
+        out = torch.empty(want, dtype=dtype, device=x.device)
+    else:
+        _auto_check(out.dtype == dtype and out.shape == want and out.device == x.device, "out: x's shape (int8: NHWC_PAD) and the output's type on x's device")
+    y_step = _pixel_step(out)
+    _auto_check(y_step is not None and (scales is None or out.is_contiguous()), "out: pixels of an image a fixed step apart, channels next to each other")
+    lib = _lib.load()
+    desc = _lib.GROUP_NORM_DESC.pack(n, pixels, c, groups, x.data_ptr(), x_step, x.stride(0), out.data_ptr(), y_step, out.stride(0),
+                                     0 if gamma is None else gamma.data_ptr(), 0 if beta is None else beta.data_ptr(), eps,
+                                     0 if scales is None else ctypes.addressof(scales), n_scales, _TYPE[x.dtype], _TYPE[dtype], activation, leaky)
+    size = lib.tsb_group_norm_workspace_bytes(desc)
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    status = lib.tsb_group_norm_nhwc(desc, _ptr(workspace), size, _stream_ptr())
+    if status:
+        check(status)
+    return out
+
+
+def _pixel_step(x):
+    """Elements between neighbouring pixels of an image of x [n, ..., c]; None where they lie no fixed step apart, or a pixel's
+    channels not next to each other."""
+    c = x.shape[-1]
+    if x.is_contiguous():
+        return c
+    if x.stride(-1) != 1 and c > 1:
+        return None
+    first = step = None
+    for size, stride in zip(x.shape[-2:0:-1], x.stride()[-2:0:-1]):
+        if size != 1:
+            if first is None:
+                first = stride
+            elif stride != step:
+                return None
+            step = stride * size
+    return c if first is None else first

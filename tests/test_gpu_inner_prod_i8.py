@@ -1,0 +1,203 @@
+"""inner_prod_quantized against the product in 64 bits, at sizes, layouts and epilogues where it can go wrong."""
+import numpy as np
+import pytest
+import torch
+
+import int8_layers as plain
+
+pytestmark = pytest.mark.gpu
+
+FLOATS = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def int8(m, k, gen, pitch=None, at=0):
+    """An int8 matrix whose rows lie `pitch` apart, all of [-128, 127] in it."""
+    pitch = pitch or (k + 15) // 16 * 16
+    room = torch.empty(m * pitch + at + 16, dtype=torch.int8, device="cuda").random_(-128, 128, generator=gen)
+    return room[at:].as_strided((m, k), (pitch, 1))
+
+
+def case(m, n, k, out, seed=0, residual=True, bias=True, **layout):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    d = dict(x=int8(m, k, g, layout.get("x_pitch"), layout.get("x_at", 0)), w=int8(n, k, g, layout.get("w_pitch"), layout.get("w_at", 0)),
+             xs=torch.empty(m, device="cuda").uniform_(0.5, 2.0, generator=g), ws=torch.empty(n, device="cuda").uniform_(0.5, 2.0, generator=g) / (5000.0 * k ** 0.5),
+             bias=torch.randn(n, device="cuda", generator=g) if bias else None,
+             residual=torch.randn((m, n), device="cuda", generator=g).to(out) if residual else None)
+    return d
+
+
+def numbers(t):
+    return None if t is None else t.float().cpu().double().numpy()
+
+
+def check(got, d, act=0, leaky=0.0, after=False):
+    want, bound = plain.inner_prod(d["x"].cpu().numpy(), d["xs"].cpu().numpy(), d["w"].cpu().numpy(), d["ws"].cpu().numpy(), numbers(d["bias"]), numbers(d["residual"]),
+                                   act, leaky, after)
+    plain.assert_close(got, want, bound, got.dtype)
+
+
+SIZES = [(1, 1, 1), (1, 8, 16), (1, 1000, 2048), (1, 37, 4099), (2, 129, 64), (3, 64, 100), (4, 1024, 1024), (5, 4096, 512), (7, 333, 8192), (8, 250, 1040),
+         (9, 65, 333), (16, 1000, 2048), (17, 128, 128), (24, 511, 192), (31, 2048, 272), (32, 96, 4096), (33, 100, 48), (63, 777, 130), (64, 1000, 2048),
+         (65, 257, 1000), (100, 130, 4096), (127, 64, 127), (128, 128, 128), (129, 256, 256), (130, 512, 4112), (200, 40, 96), (255, 300, 144), (256, 256, 1024),
+         (257, 255, 2048), (300, 1024, 512), (500, 1000, 500), (700, 512, 640), (1000, 96, 64), (1025, 513, 1009), (2049, 64, 32), (4096, 200, 128), (333, 777, 1021),
+         (2300, 1300, 400), (6000, 16, 16)]
+
+
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_sizes(m, n, k):
+    """Every size with the layout that quantize_rows gives, with contiguous (odd) rows and with each output type."""
+    from tennis_b200 import ops
+    for i, out in enumerate(FLOATS):
+        d = case(m, n, k, out, m + n + k + i, residual=i != 1, bias=i != 2)
+        got = ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], out_dtype=out)
+        assert got.dtype == out and got.shape == (m, n)
+        check(got, d)
+    d["x"], d["w"] = d["x"].contiguous(), d["w"].contiguous()
+    check(ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], out_dtype=out), d)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 200, 512), (12, 200, 512), (40, 200, 500), (150, 200, 512), (400, 520, 1024)])
+@pytest.mark.parametrize("act,leaky", [(0, 0.0), (1, 0.0), (2, 0.1), (2, -0.25), (3, 0.0), (4, 0.0)])
+def test_activations(m, n, k, act, leaky):
+    from tennis_b200 import ops
+    for out in FLOATS:
+        for after in (False, True):
+            d = case(m, n, k, out, act)
+            got = ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], act, leaky, out, residual_after_activation=after)
+            check(got, d, act, leaky, after)
+
+
+@pytest.mark.parametrize("m", [1, 6, 30, 140, 700])
+def test_kernels_agree_bit_for_bit(m):
+    """The result's bits depend neither on the kernel nor on the rows that are computed with a row."""
+    from tennis_b200 import _lib, ops
+    d = case(m, 330, 1056, torch.float32, m)
+    args = (d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], _lib.ACT_SILU)
+    got = ops.inner_prod_quantized(*args)
+    assert torch.equal(got, ops.inner_prod_quantized(*args, kernel=_lib.KERNEL_DIRECT))
+    assert torch.equal(got[m // 2:], ops.inner_prod_quantized(d["x"][m // 2:], d["xs"][m // 2:], *args[2:5], d["residual"][m // 2:], _lib.ACT_SILU))
+
+
+@pytest.mark.parametrize("x_pitch,x_at,w_pitch,w_at", [(512, 0, 512, 0), (512, 0, 500, 0), (501, 0, 512, 0), (512, 1, 512, 0), (512, 0, 512, 4), (520, 8, 504, 8), (1024, 16, 640, 32)])
+@pytest.mark.parametrize("m", [1, 13, 50, 300])
+def test_layouts(m, x_pitch, x_at, w_pitch, w_at):
+    from tennis_b200 import ops
+    d = case(m, 150, 500, torch.float16, x_pitch, x_pitch=x_pitch, x_at=x_at, w_pitch=w_pitch, w_at=w_at)
+    check(ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], out_dtype=torch.float16), d)
+
+
+@pytest.mark.parametrize("out", FLOATS, ids=str)
+@pytest.mark.parametrize("m,n,pitch,at", [(1, 100, 100, 0), (9, 100, 112, 0), (40, 99, 99, 0), (200, 128, 128, 0), (200, 128, 129, 1), (300, 250, 256, 8), (300, 256, 512, 3)])
+def test_outputs_of_the_callers(m, n, pitch, at, out):
+    """Rows anywhere: nothing between or behind them is written; the residual may be the output."""
+    from tennis_b200 import ops
+    d = case(m, n, 272, out, m)
+    room = torch.full((m * pitch + at + 64,), 7.0, dtype=out, device="cuda")
+    y = room[at:].as_strided((m, n), (pitch, 1))
+    y.copy_(d["residual"])
+    got = ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], y, out=y)
+    assert got is y
+    check(got, d)
+    written = torch.zeros_like(room, dtype=torch.bool)
+    written[at:].as_strided((m, n), (pitch, 1)).fill_(True)
+    assert (room[~written] == 7.0).all()
+
+
+def test_shapes_and_scales():
+    """More than two dimensions, transposed weights, one scale for all rows, broadcast rows."""
+    from tennis_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = int8(2 * 5 * 7, 48, g, pitch=64).as_strided((2, 5, 7, 48), (35 * 64, 7 * 64, 64, 1))
+    w = int8(48, 24, g).t()
+    ws = torch.rand(24, device="cuda", generator=g) * 1e-3
+    for xs in (torch.rand((2, 5, 7), device="cuda", generator=g), torch.full((1,), 0.25, device="cuda")):
+        got = ops.inner_prod_quantized(x, xs, w, ws)
+        assert got.shape == (2, 5, 7, 24) and got.dtype == torch.float32
+        want, bound = plain.inner_prod(x.reshape(70, 48).cpu().numpy(), xs.expand(2, 5, 7).cpu().numpy().reshape(-1), w.cpu().numpy(), ws.cpu().numpy())
+        plain.assert_close(got.view(70, 24), want, bound, torch.float32)
+    one = int8(1, 48, g).expand(20, 48)
+    got = ops.inner_prod_quantized(one, torch.rand(1, device="cuda"), w, ws)
+    assert (got == got[0]).all()
+    vec = ops.inner_prod_quantized(one[0], torch.ones(1, device="cuda"), w, ws)
+    assert vec.shape == (24,)
+
+
+@pytest.mark.parametrize("k", [131071, 131056])
+def test_largest_sums(k):
+    """k at its limit and every product the largest there is: -128 x -128 and -128 x 127."""
+    from tennis_b200 import ops
+    for m in (1, 20, 200):
+        x = torch.full((m, (k + 15) // 16 * 16), -128, dtype=torch.int8, device="cuda")[:, :k]
+        w = torch.full((70, (k + 15) // 16 * 16), -128, dtype=torch.int8, device="cuda")[:, :k]
+        w[35:] = 127
+        got = ops.inner_prod_quantized(x, torch.ones(m, device="cuda"), w, torch.ones(70, device="cuda"))
+        want = torch.tensor([float(np.float32(k * 16384))] * 35 + [float(np.float32(-k * 128 * 127))] * 35, device="cuda")
+        assert torch.equal(got, want.expand(m, 70))
+
+
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("m,n,k", [(1, 300, 1000), (1, 64, 16), (2, 300, 4096), (3, 77, 333), (4, 128, 8192), (8, 1000, 2048), (11, 256, 130), (16, 512, 16384), (33, 300, 512), (150, 200, 300)])
+def test_floating_rows(dtype, m, n, k):
+    """Bit for bit what quantize_rows and the product on its result give; rows of zeros and NaN as that says."""
+    from tennis_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x = (torch.randn((m, k), device="cuda", generator=g) * 2).to(dtype)
+    if m > 2:
+        x[1] = 0
+        x[2, k // 3] = float("nan")
+    d = case(m, n, k, dtype, 5)
+    q, s = ops.quantize_rows(x)
+    for rows in (x, torch.cat([x, x], 1)[:, :k], torch.cat([x[:, :1], x], 1)[:, 1:]):
+        got = ops.inner_prod_quantized(rows, None, d["w"], d["ws"], d["bias"], d["residual"])
+        want = ops.inner_prod_quantized(q, s, d["w"], d["ws"], d["bias"], d["residual"], out_dtype=dtype)
+        assert got.dtype == dtype and torch.equal(got.nan_to_num(-5.0), want.nan_to_num(-5.0))
+        assert m <= 2 or (torch.isnan(got[2]).all() and not torch.isnan(got[0]).any())
+
+
+def test_far_offsets():
+    """Outputs and operands whose offsets pass 32 bits, of elements and of bytes."""
+    from tennis_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for m in (3, 150):
+        pitch = ((1 << 32) // (m - 1) + 64) // 64 * 64
+        d = case(m, 40, 64, torch.bfloat16, 1, residual=False)
+        x = torch.empty((m - 1) * pitch + 64, dtype=torch.int8, device="cuda").as_strided((m, 64), (pitch, 1))
+        x.copy_(d["x"])
+        y = torch.empty((m - 1) * pitch + 64, dtype=torch.bfloat16, device="cuda").as_strided((m, 40), (pitch, 1))
+        check(ops.inner_prod_quantized(x, d["xs"], d["w"], d["ws"], d["bias"], out=y), d)
+
+
+def test_streams_and_graphs():
+    """Two graphs of the same layer and an eager call on a third stream, all at once: no call uses another's memory."""
+    from tennis_b200 import ops
+    for m in (1, 16, 200):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        d = case(m, 512, 1024, torch.float32, 3, residual=False)
+        xs = [torch.randn((m, 1024), device="cuda", generator=g) for _ in range(3)]
+        want = [ops.inner_prod_quantized(x, None, d["w"], d["ws"], d["bias"]) for x in xs]
+        graphs, outs = [], []
+        for x in xs[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = x
+                for _ in range(4):
+                    y = ops.inner_prod_quantized(x, None, d["w"], d["ws"], d["bias"])
+            graphs.append(graph)
+            outs.append(y)
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for s, graph in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    graph.replay()
+            eager = ops.inner_prod_quantized(xs[2], None, d["w"], d["ws"], d["bias"], stream=streams[2])
+        torch.cuda.synchronize()
+        for got, ref in zip(outs + [eager], want):
+            assert torch.equal(got, ref)
+
+
+def test_empty():
+    from tennis_b200 import ops
+    w, ws = torch.ones((8, 16), dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")
+    assert ops.inner_prod_quantized(torch.empty((0, 16), device="cuda"), None, w, ws).shape == (0, 8)
+    assert ops.inner_prod_quantized(torch.ones((3, 16), device="cuda"), None, w[:0], ws[:0]).shape == (3, 0)
