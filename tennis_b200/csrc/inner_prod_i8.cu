@@ -124,7 +124,11 @@ int check_args(const tsb_inner_prod_args *a) {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 int64_t rows_pitch(int64_t k) { return (k + 15) / 16 * 16; }
 
-int run(const InnerProdParams &p, int y_type, cudaStream_t stream) {
+int run(const InnerProdParams &p, int y_type, int kernel, cudaStream_t stream) {
+    const char *why = "";
+    const bool tc_can = tc::inner_prod_can(p, &why);
+    if (kernel == TSB_KERNEL_TCGEN05 && !tc_can) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: no tensor-core kernel: %s", why);
+    if (kernel == TSB_KERNEL_TCGEN05 || (kernel == TSB_KERNEL_AUTO && tc_can)) return tc::inner_prod(p, y_type, stream);
     switch (y_type) {
         case TSB_TYPE_F32: return launch_direct<float>(p, stream);
         case TSB_TYPE_F16: return launch_direct<__half>(p, stream);
@@ -177,7 +181,7 @@ int inner_prod_i8(const tsb_inner_prod_args *a, void *workspace, size_t workspac
         p.x_scales = s;
         p.xs_stride = 1;
     }
-    return run(p, a->y_type, stream);
+    return run(p, a->y_type, a->kernel, stream);
 }
 
 }  // namespace tsb

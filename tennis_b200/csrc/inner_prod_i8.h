@@ -35,4 +35,11 @@ __device__ __forceinline__ float inner_prod_value(int acc, float ws, float xs, f
 }
 #endif
 
+// inner_prod_tc.cu: the tensor-core kernel
+namespace tc {
+bool inner_prod_can(const InnerProdParams &p, const char **why);     // whether it takes these operands, and if not, why
+int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream);
+int inner_prod_status(cudaStream_t stream);
+}  // namespace tc
+
 }  // namespace tsb

@@ -1,0 +1,401 @@
+// The int8 inner product on the sm_100a tensor cores: y [m, n] = x [m, k] . w [n, k], both operands K-major as they lie in memory.
+//
+//   tile       128 tokens x BN output channels, 128 bytes of K a stage: two TMA boxes (128-byte swizzle; rows and columns behind the
+//              matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums in tensor memory, two buffers of them
+//   roles      warp 0 loads, warp 1 issues the MMAs, eight warps turn finished sums into outputs while the next tile is computed
+//   epilogue   a thread owns a token: tcgen05.ld gives it 32 channels, the rows of a warp go through 4 KB of shared memory so that
+//              residuals are read and outputs written as whole 128-byte lines
+//   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
+//              the L2 then serves
+//
+// Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and
+// all roles go to the common exit.
+#include "inner_prod_i8.h"
+#include "tc_ptx.cuh"
+
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+
+namespace tsb {
+namespace tc {
+namespace {
+
+constexpr int kKBytes = 128;                 // bytes of K a stage
+constexpr int kEpiWarps = 8;
+constexpr int kWarps = 2 + kEpiWarps;
+constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
+constexpr uint32_t kABytes = kBM * kKBytes;
+constexpr uint32_t kStageRow = 128;          // bytes of a staged output row, at most
+constexpr uint32_t kTableFloats = 128;       // a warp's scales and biases: 64 channels each
+constexpr uint32_t kSmem = 227 * 1024;
+constexpr int kMaxStages = 8;
+
+// code of the wait that ran out: 1 stage free, 2 stage full, 3 sums free, 4 sums complete
+__device__ int g_status;
+
+struct TcParams {
+    InnerProdParams p;
+    int tiles_m, tiles_n, kblocks, stages;
+};
+
+template <int BN>
+struct Layout {
+    static constexpr uint32_t kBBytes = BN * kKBytes;
+    static constexpr uint32_t kStage = kABytes + kBBytes;
+    static constexpr uint32_t kOut = kEpiWarps * 32 * kStageRow;                  // staged output rows
+    static constexpr uint32_t kTables = kEpiWarps * kTableFloats * 4;
+    static constexpr uint32_t kBars = 256;
+    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kTables - kBars) / kStage) < kMaxStages
+                                       ? (int)((kSmem - 1024 - kOut - kTables - kBars) / kStage) : kMaxStages;
+    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kTables + kBars;
+};
+
+__device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, int &n_tile) {
+    const int per_group = kGroupM * t.tiles_n;
+    const int g = i / per_group, r = i - g * per_group;
+    const int rows = min(kGroupM, t.tiles_m - g * kGroupM);
+    n_tile = r / rows;
+    m_tile = g * kGroupM + r - n_tile * rows;
+}
+
+// The 16-byte unit u of row r of a warp's staged rows: the units of eight neighbouring rows lie in different banks.
+template <int UNITS>
+__device__ __forceinline__ uint32_t staged(int r, int u) {
+    return (uint32_t)(r * UNITS * 16 + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4));
+}
+
+template <typename T> struct Vec16;        // 16 bytes of a type as fp32 values, and back
+template <> struct Vec16<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[4]) {
+        v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <> struct Vec16<__half> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Vec16<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// CH channels (32 or 64) of a warp's 32 tokens: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel.
+template <typename T, int CH>
+__device__ __forceinline__ void epilogue_chunk(const InnerProdParams &p, uint32_t taddr, int64_t m0, int c0, float xs, uint8_t *rows, float *table, bool y_vec, bool res_vec) {
+    constexpr int kN = Vec16<T>::kN, kUnits = CH / kN;        // values of a 16-byte unit, units of a row: 8 (or 4 of 2-byte values, CH = 32)
+    static_assert(kUnits == 8 || kUnits == 4, "rows of 64 or 128 bytes");
+    const int lane = threadIdx.x & 31;
+    const int live = (int)min((int64_t)32, p.m - m0), cols = min(CH, p.n - c0);
+#pragma unroll
+    for (int i = 0; i < CH / 32; ++i) {
+        const int c = c0 + i * 32 + lane;
+        table[i * 32 + lane] = c < p.n ? __ldg(p.w_scales + c) : 0.0f;
+        table[64 + i * 32 + lane] = c < p.n && p.bias ? __ldg(p.bias + c) : 0.0f;
+    }
+    if (p.residual) {
+        const T *res = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int r = i * (32 / kUnits) + lane / kUnits, u = lane % kUnits;
+            if (r >= live || u * kN >= cols) continue;
+            const T *at = res + r * p.residual_pitch + u * kN;
+            uint8_t *to = rows + staged<kUnits>(r, u);
+            if (res_vec && u * kN + kN <= cols) {
+                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kN; ++j)
+                    if (u * kN + j < cols) reinterpret_cast<T *>(to)[j] = at[j];
+            }
+        }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < CH / 32; ++h) {
+        int acc[32];
+        tmem_ld32(taddr + h * 32, acc);
+        tmem_ld_wait();
+#pragma unroll
+        for (int u = 0; u < 32 / kN; ++u) {
+            uint4 *unit = reinterpret_cast<uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u));
+            float res[kN] = {}, v[kN];
+            if (p.residual) Vec16<T>::get(*unit, res);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const int c = h * 32 + u * kN + j;
+                v[j] = inner_prod_value(acc[u * kN + j], table[c], xs, table[64 + c], p.bias != nullptr, res[j], p.residual != nullptr, p.residual_after != 0,
+                                        p.activation, p.leaky);
+            }
+            *unit = Vec16<T>::put(v);
+        }
+    }
+    __syncwarp();
+    T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+        const int r = i * (32 / kUnits) + lane / kUnits, u = lane % kUnits;
+        if (r >= live || u * kN >= cols) continue;
+        T *to = y + r * p.y_pitch + u * kN;
+        const uint8_t *at = rows + staged<kUnits>(r, u);
+        if (y_vec && u * kN + kN <= cols) {
+            *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j)
+                if (u * kN + j < cols) to[j] = reinterpret_cast<const T *>(at)[j];
+        }
+    }
+    __syncwarp();
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TcParams t,
+                        int y_vec, int res_vec) {
+    using L = Layout<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t *out_rows = smem_raw + (base - raw) + L::kStages * L::kStage;
+    float *tables = reinterpret_cast<float *>(out_rows + L::kOut);
+    uint8_t *bars_ptr = out_rows + L::kOut + L::kTables;
+    const uint32_t bar_full = smem_u32(bars_ptr), bar_empty = bar_full + 8 * kMaxStages, bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars_ptr + 8 * (2 * kMaxStages + 4));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(bars_ptr + 8 * (2 * kMaxStages + 4) + 4);
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int tiles = t.tiles_m * t.tiles_n;
+
+    if (warp == 0) {
+        if (lane < L::kStages) {
+            mbar_init(bar_full + 8 * lane, 1);
+            mbar_init(bar_empty + 8 * lane, 1);
+        }
+        if (lane < 2) {
+            mbar_init(bar_tfull + 8 * lane, 1);
+            mbar_init(bar_tempty + 8 * lane, kEpiWarps);
+        }
+        if (lane == 0) {
+            *abort_flag = 0;
+            prefetch_tensormap(&map_x);
+            prefetch_tensormap(&map_w);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_sync();
+    auto give_up = [&](int code) {
+        if (!*abort_flag) { *abort_flag = 1; atomicExch(&g_status, code); }
+    };
+
+    if (warp == 0) {
+        uint32_t s = 0;
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+            int mt, nt;
+            tile_of(t, i, mt, nt);
+            for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
+                const uint32_t stage = s % L::kStages, round = s / L::kStages;
+                if (!mbar_wait_warp(bar_empty + 8 * stage, (round & 1) ^ 1, abort_flag)) { give_up(1); goto done; }
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar_full + 8 * stage, L::kStage);
+                    tma_load_2d(base + stage * L::kStage, &map_x, bar_full + 8 * stage, kb * kKBytes, mt * kBM);
+                    tma_load_2d(base + stage * L::kStage + kABytes, &map_w, bar_full + 8 * stage, kb * kKBytes, nt * BN);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1) {
+        uint32_t s = 0, n = 0;
+        constexpr uint64_t kDescHi = smem_desc_hi<kKBytes>(8 * kKBytes);
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
+            const uint32_t acc = n & 1;
+            if (!mbar_wait_warp(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag)) { give_up(3); goto done; }
+            tc_fence_after();
+            for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
+                const uint32_t stage = s % L::kStages, round = s / L::kStages;
+                if (!mbar_wait_warp(bar_full + 8 * stage, round & 1, abort_flag)) { give_up(2); goto done; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t a = kDescHi | ((base + stage * L::kStage) >> 4), b = kDescHi | ((base + stage * L::kStage + kABytes) >> 4);
+#pragma unroll
+                    for (int q = 0; q < kKBytes / 32; ++q) mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, instr_desc<BN>(), kb > 0 || q > 0);
+                    tc_commit(bar_empty + 8 * stage);
+                    if (kb == t.kblocks - 1) tc_commit(bar_tfull + 8 * acc);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        const int e = warp - 2, quarter = warp & 3, half = e >> 2;      // tensor memory lanes of this warp: 32 * (warp % 4); channels: half of the tile
+        constexpr int kCh = BN / 2 >= 64 && sizeof(T) == 2 ? 64 : 32;
+        uint8_t *rows = out_rows + e * 32 * kStageRow;
+        float *table = tables + e * kTableFloats;
+        uint32_t n = 0;
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
+            int mt, nt;
+            tile_of(t, i, mt, nt);
+            const uint32_t acc = n & 1;
+            const int64_t m0 = (int64_t)mt * kBM + quarter * 32;
+            const float xs = m0 + lane < t.p.m ? t.p.x_scales[(m0 + lane) * t.p.xs_stride] : 0.0f;
+            if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
+            tc_fence_after();
+            if (m0 < t.p.m)
+                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && nt * BN + c < t.p.n; c += kCh)
+                    epilogue_chunk<T, kCh>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32) << 16) + c, m0, nt * BN + c, xs, rows, table, y_vec != 0, res_vec != 0);
+            tc_fence_before();
+            if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
+            __syncwarp();
+        }
+    }
+done:
+    if (*abort_flag) {
+        // copies that may still be in flight get time to land before shared memory is released
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// cuTensorMapEncodeTiled, looked up once
+PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void *f = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return fn;
+}
+
+// Tiles of `box_rows` rows x 128 bytes of an int8 matrix
+int encode(CUtensorMap *map, const int8_t *at, int64_t rows, int cols, int64_t pitch, int box_rows) {
+    const auto fn = encode_tiled();
+    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? pitch : (cols + 15) / 16 * 16)};
+    cuuint32_t box[2] = {(cuuint32_t)kKBytes, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(at), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: cuTensorMapEncodeTiled failed with %d", (int)r);
+    return TSB_OK;
+}
+
+template <typename T, int BN>
+int launch(const InnerProdParams &p, cudaStream_t stream) {
+    using L = Layout<BN>;
+    CUtensorMap mx, mw;
+    int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
+    if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, BN);
+    if (st != TSB_OK) return st;
+    static std::atomic<uint64_t> configured{0};      // devices that this kernel's shared-memory limit was raised on
+    auto kernel = inner_prod_i8_tc_kernel<T, BN>;
+    int dev = 0;
+    TSB_CUDA(cudaGetDevice(&dev));
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (!(configured.load(std::memory_order_acquire) & bit)) {
+        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
+        configured.fetch_or(bit, std::memory_order_release);
+    }
+    TcParams t = {p, (int)ceil_div64(p.m, kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
+    const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
+    const int y_vec = aligned16(p.y, p.y_pitch, type), res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
+    const int grid = (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148);
+    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(32 * kWarps), L::kBytes, stream, mx, mw, t, y_vec, res_vec));
+    TSB_LAUNCHED("inner_prod_i8_tc_kernel");
+    return TSB_OK;
+}
+
+template <typename T>
+int pick(const InnerProdParams &p, cudaStream_t stream) {
+    if (p.n <= 64) return launch<T, 64>(p, stream);
+    if (p.n <= 128 || ceil_div64(p.m, kBM) * ceil_div(p.n, 256) < 148) return launch<T, 128>(p, stream);
+    return launch<T, 256>(p, stream);
+}
+
+}  // namespace
+
+bool inner_prod_can(const InnerProdParams &p, const char **why) {
+    auto operand = [](const int8_t *at, int64_t rows, int64_t pitch, int k) {
+        return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows == 1 || (pitch % 16 == 0 && pitch >= k && pitch < (int64_t)1 << 40));
+    };
+    if (!operand(p.x, p.m, p.x_pitch, p.k) || !operand(p.w, p.n, p.w_pitch, p.k)) { *why = "an operand's address or pitch is no multiple of 16 bytes, or its rows overlap"; return false; }
+    if (ceil_div64(p.m, kBM) * ceil_div(p.n, 64) > INT32_MAX / 2) { *why = "too many tiles"; return false; }
+    return true;
+}
+
+int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream) {
+    switch (y_type) {
+        case TSB_TYPE_F32: return pick<float>(p, stream);
+        case TSB_TYPE_F16: return pick<__half>(p, stream);
+        default: return pick<__nv_bfloat16>(p, stream);
+    }
+}
+
+// The device's status word: waits for the stream, reads and clears it.
+int inner_prod_status(cudaStream_t stream) {
+    int word = 0, zero = 0;
+    void *at = nullptr;
+    TSB_CUDA(cudaGetSymbolAddress(&at, g_status));
+    TSB_CUDA(cudaMemcpyAsync(&word, at, sizeof(word), cudaMemcpyDeviceToHost, stream));
+    TSB_CUDA(cudaStreamSynchronize(stream));
+    if (word == 0) return TSB_OK;
+    TSB_CUDA(cudaMemcpyAsync(at, &zero, sizeof(zero), cudaMemcpyHostToDevice, stream));
+    TSB_CUDA(cudaStreamSynchronize(stream));
+    static const char *const kWaits[] = {"a stage to be free", "a stage to be loaded", "sums to be read", "sums to be complete"};
+    return fail(TSB_ERR_DEVICE_TIMEOUT, "inner_prod_i8: the wait for %s ran out; results since the last check are not to be used",
+                word >= 1 && word <= 4 ? kWaits[word - 1] : "an unknown event");
+}
+
+}  // namespace tc
+}  // namespace tsb

@@ -647,6 +647,13 @@ def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, act
     return out
 
 
+def inner_prod_status(device=None, stream=None):
+    """Waits for ``stream`` (the device's current one) and raises TsbError where a wait inside a tensor-core inner product on that
+    device ran out since the last check: its results are not to be used."""
+    with torch.cuda.device(device):
+        check(_lib.load().tsb_inner_prod_i8_status(_stream_ptr(stream)))
+
+
 def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_NONE, leaky=0.0, out_dtype=None, requant_scales=None,
                     out=None, stream=None):
     """Group norm and activation of a channels-last x [n, ..., channels] (fp32, fp16 or bf16): mean and variance of each image's

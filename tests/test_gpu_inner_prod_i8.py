@@ -196,6 +196,14 @@ def test_streams_and_graphs():
             assert torch.equal(got, ref)
 
 
+def test_operands_that_the_tensor_cores_cannot_read():
+    from tennis_b200 import _lib, ops
+    d = case(20, 64, 100, torch.float32, 1, x_pitch=100)
+    with pytest.raises(_lib.TsbError, match="16 bytes"):
+        ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], kernel=_lib.KERNEL_TCGEN05)
+    ops.inner_prod_status()
+
+
 def test_empty():
     from tennis_b200 import ops
     w, ws = torch.ones((8, 16), dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")
