@@ -105,7 +105,9 @@ group_norm_apply_kernel(GroupNormParams p, const float2 *__restrict__ stats) {
         float v = __fmul_rn(__fsub_rn(to_f32(static_cast<const T *>(p.x)[image * p.x_image + q * p.x_pixel + c]), st.x), st.y);
         if (p.gamma) v = __fmul_rn(v, p.gamma[c]);
         if (p.beta) v = __fadd_rn(v, p.beta[c]);
-        v = activate(v, p.activation, p.leaky);
+        float one[1] = {v};
+        activate<Y>(one, p.activation, p.leaky);
+        v = one[0];
         if constexpr (sizeof(Y) == 1) {
             const int64_t at = (image * p.channels + c) * p.pixels + q;
             *y = (Y)q8(v, p.scales[p.nscales == 1 ? 0 : image], at < p.rne_limit);

@@ -70,16 +70,15 @@ inner_prod_i8_direct_kernel(InnerProdParams p, int vec_x, int vec_w) {
         for (int i = 0; i < 4; ++i) {
             const int64_t m = m0 + tm + 16 * i;
             if (m >= p.m) continue;
-            const float xs = p.x_scales[m * p.xs_stride];
+            // (a channel that does not exist reads the last one's vectors and is not written)
+            const int last = p.n - 1;
+            auto at = [&](int j) { return min(n0 + tn + 16 * j, last); };
+            float v[4];
+            inner_prod_values<T>(p, acc[i], p.x_scales[m * p.xs_stride], [&](int j) { return p.w_scales[at(j)]; }, [&](int j) { return p.bias ? p.bias[at(j)] : 0.0f; },
+                                 [&](int j) { return to_f32(static_cast<const T *>(p.residual)[m * p.residual_pitch + at(j)]); }, v);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + tn + 16 * j;
-                if (n >= p.n) continue;
-                const float res = p.residual ? to_f32(static_cast<const T *>(p.residual)[m * p.residual_pitch + n]) : 0.0f;
-                const float v = inner_prod_value(acc[i][j], p.w_scales[n], xs, p.bias ? p.bias[n] : 0.0f, p.bias != nullptr, res, p.residual != nullptr,
-                                                 p.residual_after != 0, p.activation, p.leaky);
-                static_cast<T *>(p.y)[m * p.y_pitch + n] = from_f32<T>(v);
-            }
+            for (int j = 0; j < 4; ++j)
+                if (n0 + tn + 16 * j < p.n) static_cast<T *>(p.y)[m * p.y_pitch + n0 + tn + 16 * j] = from_f32<T>(v[j]);
         }
     }
 }

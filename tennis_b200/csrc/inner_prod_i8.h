@@ -22,16 +22,21 @@ struct InnerProdParams {
 };
 
 #ifdef __CUDACC__
-// One value: sum -> fp32, times the output channel's scale, times the token's, + bias, + residual, activation (+ residual); every step
-// is rounded by itself, so the value does not depend on which kernel computed it.
-__device__ __forceinline__ float inner_prod_value(int acc, float ws, float xs, float bias, bool has_bias, float residual, bool has_residual,
-                                                  bool residual_after, int activation, float leaky) {
-    float v = __fmul_rn(__fmul_rn(__int2float_rn(acc), ws), xs);
-    if (has_bias) v = __fadd_rn(v, bias);
-    if (has_residual && !residual_after) v = __fadd_rn(v, residual);
-    v = activate(v, activation, leaky);
-    if (has_residual && residual_after) v = __fadd_rn(v, residual);
-    return v;
+// N values of a token: sum -> fp32, times the output channel's scale, times the token's, + bias (a missing one is 0), + residual,
+// activation (+ residual); every step is rounded by itself, so the values do not depend on which kernel computed them.
+template <typename T, int N, typename Ws, typename Bias, typename Res>
+__device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, const int (&acc)[N], float xs, Ws ws, Bias bias, Res res, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(acc[i]), ws(i)), xs), bias(i));
+    if (p.residual && !p.residual_after) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
+    }
+    activate<T>(v, p.activation, p.leaky);
+    if (p.residual && p.residual_after) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
+    }
 }
 #endif
 

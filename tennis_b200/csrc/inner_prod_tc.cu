@@ -153,19 +153,17 @@ __device__ __forceinline__ void epilogue_chunk(const InnerProdParams &p, uint32_
         int acc[32];
         tmem_ld32(taddr + h * 32, acc);
         tmem_ld_wait();
+        float v[32], res[32];
+        if (p.residual) {
 #pragma unroll
-        for (int u = 0; u < 32 / kN; ++u) {
-            uint4 *unit = reinterpret_cast<uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u));
-            float res[kN] = {}, v[kN];
-            if (p.residual) Vec16<T>::get(*unit, res);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const int c = h * 32 + u * kN + j;
-                v[j] = inner_prod_value(acc[u * kN + j], table[c], xs, table[64 + c], p.bias != nullptr, res[j], p.residual != nullptr, p.residual_after != 0,
-                                        p.activation, p.leaky);
-            }
-            *unit = Vec16<T>::put(v);
+            for (int u = 0; u < 32 / kN; ++u)
+                Vec16<T>::get(*reinterpret_cast<const uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u)), *reinterpret_cast<float (*)[kN]>(&res[u * kN]));
         }
+        inner_prod_values<T>(p, acc, xs, [&](int j) { return table[h * 32 + j]; }, [&](int j) { return table[64 + h * 32 + j]; },
+                             [&](int j) { return res[j]; }, v);
+#pragma unroll
+        for (int u = 0; u < 32 / kN; ++u)
+            *reinterpret_cast<uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u)) = Vec16<T>::put(*reinterpret_cast<float (*)[kN]>(&v[u * kN]));
     }
     __syncwarp();
     T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;

@@ -31,14 +31,47 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// The activations after a product or a norm.  relu and leaky_relu are the operators' own (a NaN gives 0 and NaN).
-__device__ __forceinline__ float activate(float v, int activation, float leaky) {
-    switch (activation) {
-        case TSB_ACT_RELU: return v > 0.0f ? v : 0.0f;
-        case TSB_ACT_LEAKY_RELU: return v > 0.0f ? v : __fmul_rn(v, leaky);
-        case TSB_ACT_SILU: return __fdiv_rn(v, __fadd_rn(1.0f, expf(-v)));
-        case TSB_ACT_GELU: return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));
-        default: return v;
+// silu, v / (1 + exp(-v)), by the hardware's exp2 and reciprocal (relative errors of 2^-22 and 2^-23).
+// For fp32 results the rounding error of -v log2(e), which exp2 would turn into a relative error of |v| 2^-24, is computed by a fused
+// multiply-add and put back to first order: 8 half steps of the result in all.  Results of 16 bits, whose half step is 2^13 times that
+// of fp32 or more, go without.  (expf and a division take some 40 instructions a value: 25 M values of a product with 64 terms each took 126 us.)
+template <bool NARROW>
+__device__ __forceinline__ float silu(float v) {
+    float e;
+    if (NARROW) {
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(v, -1.44269504f)));
+    } else {
+        const float c = fminf(fmaxf(v, -200.0f), 200.0f);        // (exp2 is infinite or 0 at either end)
+        const float t = __fmul_rn(c, -1.44269502f);
+        const float r = fmaf(c, -1.92596303e-8f, fmaf(c, -1.44269502f, -t));   // log2(e) = 1.44269502 (fp32) + 1.92596303e-8
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+        e = __fmul_rn(e, fmaf(r, 0.693147182f, 1.0f));
+    }
+    float q;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(__fadd_rn(1.0f, e)));
+    return __fmul_rn(v, q);
+}
+__device__ __forceinline__ float gelu(float v) {
+    return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));
+}
+
+// The activation of N values that become results of type T (relu and leaky_relu are the operators' own: a NaN gives 0 and NaN).  One
+// branch for all of them: with the choice made value by value, the unrolled code of all five did not fit the instruction cache.
+template <typename T, int N>
+__device__ __forceinline__ void activate(float (&v)[N], int activation, float leaky) {
+    if (activation == TSB_ACT_NONE) return;
+    if (activation == TSB_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+    } else if (activation == TSB_ACT_LEAKY_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? v[i] : __fmul_rn(v[i], leaky);
+    } else if (activation == TSB_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = silu<sizeof(T) == 2>(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = gelu(v[i]);
     }
 }
 
