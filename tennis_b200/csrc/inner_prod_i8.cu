@@ -123,10 +123,11 @@ int check_args(const tsb_inner_prod_args *a) {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 int64_t rows_pitch(int64_t k) { return (k + 15) / 16 * 16; }
 
-int run(const InnerProdParams &p, int y_type, int kernel, cudaStream_t stream) {
+int run(const InnerProdParams &p, int y_type, int kernel, int early, cudaStream_t stream) {
     const char *why = "";
     const bool tc_can = tc::inner_prod_can(p, &why);
     if (kernel == TSB_KERNEL_TCGEN05 && !tc_can) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: no tensor-core kernel: %s", why);
+    if (kernel == TSB_KERNEL_AUTO && tc_can && p.m <= few::kMaxTokens) return few::inner_prod(p, y_type, early, stream);
     if (kernel == TSB_KERNEL_TCGEN05 || (kernel == TSB_KERNEL_AUTO && tc_can)) return tc::inner_prod(p, y_type, stream);
     switch (y_type) {
         case TSB_TYPE_F32: return launch_direct<float>(p, stream);
@@ -135,19 +136,7 @@ int run(const InnerProdParams &p, int y_type, int kernel, cudaStream_t stream) {
     }
 }
 
-}  // namespace
-
-int quantize_rows_i8(const void *, int, int64_t, int8_t *, int64_t, float *, int64_t, int64_t, cudaStream_t);
-
-// Workspace of floating rows: the rows as int8 (16-byte pitch), then their scales.
-size_t inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *a) {
-    if (check_args(a) != TSB_OK || a->m == 0 || a->n == 0 || a->x_type == TSB_TYPE_I8) return 0;
-    return align256((size_t)(a->m * rows_pitch(a->k))) + align256((size_t)a->m * 4);
-}
-
-int inner_prod_i8(const tsb_inner_prod_args *a, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
-    int st = check_args(a);
-    if (st != TSB_OK || a->m == 0 || a->n == 0) return st;
+InnerProdParams params_of(const tsb_inner_prod_args *a) {
     InnerProdParams p = {};
     p.x = static_cast<const int8_t *>(a->x);
     p.x_pitch = a->m > 1 ? a->x_pitch : 0;      // (of a single row, never stepped by)
@@ -167,20 +156,48 @@ int inner_prod_i8(const tsb_inner_prod_args *a, void *workspace, size_t workspac
     p.activation = a->activation;
     p.leaky = a->leaky_scale;
     p.residual_after = a->residual && a->residual_after_activation ? 1 : 0;
-    if (a->x_type != TSB_TYPE_I8) {
-        const size_t need = inner_prod_i8_workspace_bytes(a);
-        if (!workspace || workspace_bytes < need) return fail(TSB_ERR_WORKSPACE_TOO_SMALL, "inner_prod_i8: %zu bytes of workspace, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
-        if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TSB_ERR_INVALID_ARGUMENT, "inner_prod_i8: the workspace must be 256-byte aligned");
-        int8_t *q = static_cast<int8_t *>(workspace);
-        float *s = reinterpret_cast<float *>(q + align256((size_t)(a->m * rows_pitch(a->k))));
-        st = quantize_rows_i8(a->x, a->x_type, a->x_pitch, q, rows_pitch(a->k), s, a->m, a->k, stream);
-        if (st != TSB_OK) return st;
-        p.x = q;
-        p.x_pitch = rows_pitch(a->k);
-        p.x_scales = s;
-        p.xs_stride = 1;
-    }
-    return run(p, a->y_type, a->kernel, stream);
+    return p;
+}
+
+// Whether floating rows are quantized by the kernel that multiplies them.
+bool quantizes_inside(const tsb_inner_prod_args *a, const InnerProdParams &p) {
+    return a->kernel == TSB_KERNEL_AUTO && tc::weights_fit(p) && few::can_quantize(p, a->x_type, a->y_type);
+}
+
+// Workspace of floating rows: the rows as int8 (16-byte pitch), then their scales.
+size_t workspace_of(const tsb_inner_prod_args *a, const InnerProdParams &p) {
+    if (a->x_type == TSB_TYPE_I8 || quantizes_inside(a, p)) return 0;
+    return align256((size_t)(a->m * rows_pitch(a->k))) + align256((size_t)a->m * 4);
+}
+
+}  // namespace
+
+int quantize_rows_i8(const void *, int, int64_t, int8_t *, int64_t, float *, int64_t, int64_t, cudaStream_t);
+
+size_t inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *a) {
+    return check_args(a) != TSB_OK || a->m == 0 || a->n == 0 ? 0 : workspace_of(a, params_of(a));
+}
+
+int inner_prod_i8(const tsb_inner_prod_args *a, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    int st = check_args(a);
+    if (st != TSB_OK || a->m == 0 || a->n == 0) return st;
+    InnerProdParams p = params_of(a);
+    if (a->x_type == TSB_TYPE_I8) return run(p, a->y_type, a->kernel, 0, stream);
+    if (quantizes_inside(a, p)) return few::inner_prod_quantize(p, a->y_type, stream);
+    const size_t need = workspace_of(a, p);
+    if (!workspace || workspace_bytes < need) return fail(TSB_ERR_WORKSPACE_TOO_SMALL, "inner_prod_i8: %zu bytes of workspace, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
+    if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TSB_ERR_INVALID_ARGUMENT, "inner_prod_i8: the workspace must be 256-byte aligned");
+    int8_t *q = static_cast<int8_t *>(workspace);
+    float *s = reinterpret_cast<float *>(q + align256((size_t)(a->m * rows_pitch(a->k))));
+    st = quantize_rows_i8(a->x, a->x_type, a->x_pitch, q, rows_pitch(a->k), s, a->m, a->k, stream);
+    if (st != TSB_OK) return st;
+    p.x = q;
+    p.x_pitch = rows_pitch(a->k);
+    p.x_scales = s;
+    p.xs_stride = 1;
+    // The weights may be read early: quantize_rows lets the next kernel start only after all in front of it, and so whatever
+    // wrote the weights, has completed.
+    return run(p, a->y_type, a->kernel, 1, stream);
 }
 
 }  // namespace tsb

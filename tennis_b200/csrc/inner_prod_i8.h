@@ -42,9 +42,18 @@ __device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, cons
 
 // inner_prod_tc.cu: the tensor-core kernel
 namespace tc {
-bool inner_prod_can(const InnerProdParams &p, const char **why);     // whether it takes these operands, and if not, why
+bool inner_prod_can(const InnerProdParams &p, const char **why);     // whether it (and the one below) takes these operands, and if not, why
+bool weights_fit(const InnerProdParams &p);                           // the part of that that concerns w
 int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream);
 int inner_prod_status(cudaStream_t stream);
 }  // namespace tc
+
+// inner_prod_few.cu: the kernel of few tokens
+namespace few {
+constexpr int kMaxTokens = 32;
+int inner_prod(const InnerProdParams &p, int y_type, int early, cudaStream_t stream);      // early: weights may be read before the kernel in front is done
+bool can_quantize(const InnerProdParams &p, int x_type, int y_type);                       // whether the next one takes these floating rows
+int inner_prod_quantize(const InnerProdParams &p, int y_type, cudaStream_t stream);
+}  // namespace few
 
 }  // namespace tsb

@@ -66,57 +66,6 @@ __device__ __forceinline__ uint32_t staged(int r, int u) {
     return (uint32_t)(r * UNITS * 16 + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4));
 }
 
-template <typename T> struct Vec16;        // 16 bytes of a type as fp32 values, and back
-template <> struct Vec16<float> {
-    static constexpr int kN = 4;
-    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[4]) {
-        v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
-    }
-    static __device__ __forceinline__ uint4 put(const float (&v)[4]) {
-        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    }
-};
-template <> struct Vec16<__half> {
-    static constexpr int kN = 8;
-    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            v[2 * i] = f.x; v[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-template <> struct Vec16<__nv_bfloat16> {
-    static constexpr int kN = 8;
-    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-
 // CH channels (32 or 64) of a warp's 32 tokens: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel.
 template <typename T, int CH>
 __device__ __forceinline__ void epilogue_chunk(const InnerProdParams &p, uint32_t taddr, int64_t m0, int c0, float xs, uint8_t *rows, float *table, bool y_vec, bool res_vec) {
@@ -363,11 +312,16 @@ int pick(const InnerProdParams &p, cudaStream_t stream) {
 
 }  // namespace
 
+namespace {
+bool operand_fits(const int8_t *at, int64_t rows, int64_t pitch, int k) {
+    return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows == 1 || (pitch % 16 == 0 && pitch >= k && pitch < (int64_t)1 << 40));
+}
+}  // namespace
+
+bool weights_fit(const InnerProdParams &p) { return operand_fits(p.w, p.n, p.w_pitch, p.k); }
+
 bool inner_prod_can(const InnerProdParams &p, const char **why) {
-    auto operand = [](const int8_t *at, int64_t rows, int64_t pitch, int k) {
-        return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (rows == 1 || (pitch % 16 == 0 && pitch >= k && pitch < (int64_t)1 << 40));
-    };
-    if (!operand(p.x, p.m, p.x_pitch, p.k) || !operand(p.w, p.n, p.w_pitch, p.k)) { *why = "an operand's address or pitch is no multiple of 16 bytes, or its rows overlap"; return false; }
+    if (!operand_fits(p.x, p.m, p.x_pitch, p.k) || !weights_fit(p)) { *why = "an operand's address or pitch is no multiple of 16 bytes, or its rows overlap"; return false; }
     if (ceil_div64(p.m, kBM) * ceil_div(p.n, 64) > INT32_MAX / 2) { *why = "too many tiles"; return false; }
     return true;
 }

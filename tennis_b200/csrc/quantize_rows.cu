@@ -6,13 +6,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// The largest magnitude of a row as the bits of an fp32 value: magnitudes order as their bits do, infinity lies above every number
-// and NaN above infinity, so an integer maximum carries both through to the scale.
-__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-
-// Rows below 2^-100 count as zero: the factor 127 / a stays a finite number and the scale a / 127 a normal one.
-__device__ __forceinline__ bool counts_as_zero(float largest) { return largest < 7.888609052210118e-31f; }
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restrict__ y, int64_t y_pitch, float *__restrict__ scales,
@@ -30,12 +23,10 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restric
 #pragma unroll
         for (int i = 0; i < kThreads / 32; ++i) m = max(m, part[i]);
         __syncthreads();
-        const float largest = __uint_as_float(m);
-        const bool zero = counts_as_zero(largest);
-        const float by = zero ? 0.0f : __fdiv_rn(127.0f, largest);
-        if (threadIdx.x == 0) scales[r] = zero ? 0.0f : __fdiv_rn(largest, 127.0f);
+        const RowScale row(m);
+        if (threadIdx.x == 0) scales[r] = row.scale;
         int8_t *yr = y + r * y_pitch;
-        for (int c = threadIdx.x; c < cols; c += kThreads) yr[c] = (int8_t)q8_half_even(__fmul_rn(to_f32(xr[c]), by));
+        for (int c = threadIdx.x; c < cols; c += kThreads) yr[c] = (int8_t)row(to_f32(xr[c]));
     }
 }
 

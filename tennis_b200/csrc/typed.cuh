@@ -31,6 +31,73 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+template <typename T> struct Vec16;        // 16 bytes of a type as fp32 values, and back
+template <> struct Vec16<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[4]) {
+        v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+};
+template <> struct Vec16<__half> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Vec16<__nv_bfloat16> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void get(const uint4 &q, float (&v)[8]) {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 put(const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// ---- int8 rows with a scale taken from the row
+// The largest magnitude of a row as the bits of an fp32 value: magnitudes order as their bits do, infinity lies above every number
+// and NaN above infinity, so an integer maximum carries both through to the scale.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// Rows below 2^-100 count as zero: the factor 127 / a stays a finite number and the scale a / 127 a normal one.
+struct RowScale {
+    float by, scale;
+    __device__ __forceinline__ explicit RowScale(uint32_t largest_bits) {
+        const float a = __uint_as_float(largest_bits);
+        const bool zero = a < 7.888609052210118e-31f;
+        by = zero ? 0.0f : __fdiv_rn(127.0f, a);
+        scale = zero ? 0.0f : __fdiv_rn(a, 127.0f);
+    }
+    __device__ __forceinline__ int operator()(float v) const { return q8_half_even(__fmul_rn(v, by)); }
+};
+
 // silu, v / (1 + exp(-v)), by the hardware's exp2 and reciprocal (relative errors of 2^-22 and 2^-23).
 // For fp32 results the rounding error of -v log2(e), which exp2 would turn into a relative error of |v| 2^-24, is computed by a fused
 // multiply-add and put back to first order: 8 half steps of the result in all.  Results of 16 bits, whose half step is 2^13 times that
