@@ -83,6 +83,22 @@ __device__ __forceinline__ void pdl_sync() {
 }
 #endif
 
+// Something that is done once for each device (an attribute of a kernel, which is the device's own): first() until done().
+class DeviceOnce {
+public:
+    bool first() {
+        int dev = 0;
+        return cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || !(devices_.load(std::memory_order_acquire) >> dev & 1);
+    }
+    void done() {
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) devices_.fetch_or(1ull << dev, std::memory_order_release);
+    }
+
+private:
+    std::atomic<uint64_t> devices_{0};
+};
+
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int round_up(int a, int b) { return ceil_div(a, b) * b; }

@@ -1,194 +1,248 @@
 // The int8 inner product of few tokens: the weights' bytes are the work, each is read once.
 //
-//   block      MT * 16 output channels and all of K; its warps take blocks of 128 bytes of K in turn, and their int32 sums meet in
-//              shared memory.  16 channels' rows of 4096 bytes fit the registers of eight warps, so all of a block's loads are in flight at once.
-//   product    mma.sync m16n8k32 on bytes that go from memory straight to registers: a thread's 16 bytes of a weight row and of a token's
-//              row are the operands of two MMAs, which so take the 64 bytes of four threads in an order of K of their own -- the same
-//              one for both operands, which is all that a sum needs.  (With up to 32 tokens the MMAs of a block take a fraction of its loads' time,
-//              tcgen05 would only add its set-up.)
-//   tokens     int8 rows, read like the weights; or floating rows of which every block quantizes all in shared memory, while its
-//              weights are on their way
+//   block      16 output channels and all of K; its warps take blocks of 128 bytes of K in turn, and their int32 sums meet in shared memory
+//   loads      cp.async into a ring of the warp's own, kDepth blocks of K ahead; a thread reads back what it loaded itself, so a ring needs
+//              no barrier.  The blocks on a multiprocessor have 128 KB of weights under way, whatever their number of warps
+//   product    mma.sync m16n8k32: a thread's 16 bytes of a weight row and of a token's row are the operands of two MMAs, which so take
+//              the 64 bytes of four threads in an order of K of their own -- the same one for both operands, which is all that a sum
+//              needs.  (The MMAs of up to 32 tokens take a fraction of the loads' time; tcgen05 would only add its set-up.)
+//   tokens     int8 rows, read like the weights; or one floating row, which every block quantizes in shared memory while its weights
+//              are on their way (two rows or more are quantized sooner by quantize_rows, a block each)
 #include "inner_prod_i8.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tsb {
 namespace few {
 namespace {
+
+constexpr int kMaxQuantized = 32768;      // bytes of a quantized row that a block keeps
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Bytes [k, k + 16) of a row of `cols` bytes; those behind its end are zero.
-__device__ __forceinline__ uint4 load16(const int8_t *row, int k, int cols) {
-    if (k + 16 <= cols) return __ldg(reinterpret_cast<const uint4 *>(row + k));
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll 1
-    for (int i = 0; i < cols - k; ++i) w[i >> 2] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+// 16 bytes to shared memory, of which `size` come from memory and the rest are zero
+__device__ __forceinline__ void load16(uint32_t to, const int8_t *from, int size) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(size) : "memory");
+}
+__device__ __forceinline__ uint4 read16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
 }
 
-template <int NT, int MT>
+// NT: groups of eight tokens; X: int8_t, or the type of one floating row
+template <typename X, int NT>
 struct Shape {
-    static constexpr int kTokens = 8 * NT, kChannels = 16 * MT;
-    static constexpr int kPitch = kChannels + 4;             // words between two tokens' sums: a warp's writes meet 32 banks
-    static constexpr int kAhead = NT * MT <= 2 ? 4 : 2;      // blocks of 128 bytes a warp loads before it multiplies
+    static constexpr bool kQuantize = sizeof(X) > 1;
+    static constexpr int kTokens = 8 * NT, kChannels = 16;
+    static constexpr int kPitch = kChannels + 4;                  // words between two tokens' sums: a warp's writes meet 32 banks
+    static constexpr int kSlots = 4 + (kQuantize ? 0 : 2 * NT);   // 16-byte pieces a thread loads for a block of K
+    static constexpr int kDepth = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+    static constexpr uint32_t kRing = kDepth * kSlots * 512;      // a warp's; its sums lie there afterwards
+    static_assert(kTokens * kPitch * 4 <= kRing, "the sums fit the ring");
 };
 
-// Quantizes the block's M floating rows into shared memory, `pitch` bytes apart and zero up to there.
-template <typename X>
-__device__ void quantize_tokens(const InnerProdParams &p, const X *x, int8_t *rows, int pitch, float *scales, uint32_t *part) {
-    constexpr int kN = Vec16<X>::kN;
-    const int threads = blockDim.x;
-    for (int m = 0; m < (int)p.m; ++m) {
-        const X *row = x + m * p.x_pitch;
-        const bool vec = reinterpret_cast<uintptr_t>(row) % 16 == 0;
-        const int whole = vec ? p.k / kN : 0;
+// Quantizes the one floating row into shared memory, zero up to `pitch`: held in registers between the maximum and the rounding as far
+// as it fits eight vectors a thread.  start() loads, finish() ends with a barrier.
+template <typename X, int W>
+struct TokenQuantizer {
+    static constexpr int kN = Vec16<X>::kN, kHeld = 8;
+    const X *row;
+    int k, whole;                 // whole: 16-byte vectors that are read as such
+    uint4 held[kHeld];
+
+    __device__ __forceinline__ TokenQuantizer(const InnerProdParams &p) : row(reinterpret_cast<const X *>(p.x)), k(p.k) {
+        whole = reinterpret_cast<uintptr_t>(row) % 16 == 0 ? k / kN : 0;
+    }
+    __device__ __forceinline__ uint4 vector(int u) const { return __ldg(reinterpret_cast<const uint4 *>(row) + u); }
+    __device__ __forceinline__ void start() {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int u = threadIdx.x + i * 32 * W;
+            held[i] = u < whole ? vector(u) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ float finish(int8_t *out, int pitch, uint32_t *part) {
         uint32_t most = 0;
-        for (int u = threadIdx.x; u < whole; u += threads) {
+        auto take = [&](const uint4 &q) {
             float v[kN];
-            Vec16<X>::get(__ldg(reinterpret_cast<const uint4 *>(row) + u), v);
+            Vec16<X>::get(q, v);
 #pragma unroll
             for (int i = 0; i < kN; ++i) most = max(most, magnitude(v[i]));
-        }
-        for (int c = whole * kN + threadIdx.x; c < p.k; c += threads) most = max(most, magnitude(to_f32(row[c])));
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) take(held[i]);
+        for (int u = threadIdx.x + kHeld * 32 * W; u < whole; u += 32 * W) take(vector(u));
+        for (int c = whole * kN + threadIdx.x; c < k; c += 32 * W) most = max(most, magnitude(to_f32(row[c])));
         most = __reduce_max_sync(0xffffffffu, most);
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
         __syncthreads();
         most = 0;
-        for (int i = 0; i < threads / 32; ++i) most = max(most, part[i]);
-        const RowScale q(most);
-        if (threadIdx.x == 0) scales[m] = q.scale;
-        int8_t *out = rows + m * pitch;
-        for (int u = threadIdx.x; u < whole; u += threads) {
-            float v[kN];
-            Vec16<X>::get(__ldg(reinterpret_cast<const uint4 *>(row) + u), v);
-            uint32_t w[kN / 4];
 #pragma unroll
-            for (int i = 0; i < kN / 4; ++i)
-                w[i] = (uint32_t)(uint8_t)q(v[4 * i]) | (uint32_t)(uint8_t)q(v[4 * i + 1]) << 8 | (uint32_t)(uint8_t)q(v[4 * i + 2]) << 16 | (uint32_t)(uint8_t)q(v[4 * i + 3]) << 24;
+        for (int i = 0; i < W; ++i) most = max(most, part[i]);
+        const RowScale q(most);
+        auto put = [&](const uint4 &from, int u) {
+            uint32_t w[kN / 4];
+            quantize16<X>(q, from, w);
 #pragma unroll
             for (int i = 0; i < kN / 4; ++i) reinterpret_cast<uint32_t *>(out)[u * (kN / 4) + i] = w[i];
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const int u = threadIdx.x + i * 32 * W;
+            if (u < whole) put(held[i], u);
         }
-        for (int c = whole * kN + threadIdx.x; c < pitch; c += threads) out[c] = c < p.k ? (int8_t)q(to_f32(row[c])) : (int8_t)0;
+        for (int u = threadIdx.x + kHeld * 32 * W; u < whole; u += 32 * W) put(vector(u), u);
+        for (int c = whole * kN + threadIdx.x; c < pitch; c += 32 * W) out[c] = c < k ? (int8_t)q(to_f32(row[c])) : (int8_t)0;
         __syncthreads();
+        return q.scale;
     }
-}
+};
 
-// X: the type of floating rows, or int8_t.  early: the weights may be read before the kernel in front has completed.
-template <typename T, typename X, int NT, int MT, int W>
+// early: the weights may be read before the kernel in front has completed.
+template <typename T, typename X, int NT, int W>
 __global__ void __launch_bounds__(32 * W)
-inner_prod_i8_few_kernel(const __grid_constant__ InnerProdParams p, int early, int x_rows_pitch) {
-    using S = Shape<NT, MT>;
-    constexpr bool kQuantize = sizeof(X) > 1;
-    constexpr int kAhead = S::kAhead;
+inner_prod_i8_few_kernel(const __grid_constant__ InnerProdParams p, int early, int x_row_bytes) {
+    using S = Shape<X, NT>;
     extern __shared__ __align__(16) uint8_t smem[];
-    int *sums = reinterpret_cast<int *>(smem);                                    // [warp][token][channel]
-    float *scales = reinterpret_cast<float *>(smem + W * S::kTokens * S::kPitch * 4);
-    uint32_t *part = reinterpret_cast<uint32_t *>(scales + S::kTokens);
-    int8_t *x_rows = reinterpret_cast<int8_t *>(part + W);
+    int8_t *x_rows = reinterpret_cast<int8_t *>(smem + W * S::kRing);              // floating rows: quantized
+    uint32_t *part = reinterpret_cast<uint32_t *>(x_rows + (S::kQuantize ? x_row_bytes : 0));
+    float scale = 0.0f;                                                            // of the floating row
     if (!early) pdl_sync();
+    TokenQuantizer<std::conditional_t<S::kQuantize, X, float>, W> quantizer(p);
+    if constexpr (S::kQuantize) quantizer.start();
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * S::kChannels;
-    const int8_t *w[MT][2];
+    const int8_t *w[2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int h = 0; h < 2; ++h) w[h] = p.w + (int64_t)min(n0 + h * 8 + g, p.n - 1) * p.w_pitch;   // (channels behind the last are not written)
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * S::kRing + lane * 16;
+    const int blocks = (p.k + 127) / 128, mine = blocks > warp ? (blocks - warp + W - 1) / W : 0;   // this warp's blocks of K: warp, warp + W, ...
+    auto load_weights = [&](int i) {
+        const uint32_t to = ring + (uint32_t)(i % S::kDepth) * (S::kSlots * 512);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) w[i][h] = p.w + (int64_t)min(n0 + i * 16 + h * 8 + g, p.n - 1) * p.w_pitch;   // (channels behind the last are not written)
-    int acc[MT][NT][4] = {};
-    uint4 a[kAhead][MT][2][2];
-    auto load_weights = [&](int k0) {
-#pragma unroll
-        for (int b = 0; b < kAhead; ++b)
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const int k = k0 + b * W * 128 + s * 64 + t * 16;
-                        a[b][i][h][s] = k < p.k ? load16(w[i][h], k, p.k) : make_uint4(0, 0, 0, 0);
-                    }
+        for (int s = 0; s < 2; ++s) {
+            const int k = (warp + i * W) * 128 + s * 64 + t * 16, size = max(0, min(16, p.k - k)), at = size ? k : 0;
+            load16(to + (s * 2 + 0) * 512, w[0] + at, size);
+            load16(to + (s * 2 + 1) * 512, w[1] + at, size);
+        }
     };
-    load_weights(warp * 128);
-    if (early) pdl_sync();
-    if constexpr (kQuantize) quantize_tokens<X>(p, reinterpret_cast<const X *>(p.x), x_rows, x_rows_pitch, scales, part);
-
-    for (int k0 = warp * 128; k0 < p.k; k0 += kAhead * W * 128) {
-        if (k0 > warp * 128) load_weights(k0);
-        uint4 x[kAhead][NT][2];
+    auto load_tokens = [&](int i) {
+        if constexpr (!S::kQuantize) {
+            const uint32_t to = ring + (uint32_t)(i % S::kDepth) * (S::kSlots * 512) + 4 * 512;
 #pragma unroll
-        for (int b = 0; b < kAhead; ++b)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j) {
+                const int m = j * 8 + g;
+                const int8_t *row = p.x + (m < p.m ? m : 0) * p.x_pitch;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const int k = k0 + b * W * 128 + s * 64 + t * 16, m = j * 8 + g;
-                    x[b][j][s] = make_uint4(0, 0, 0, 0);
-                    if (m < p.m && k < p.k) {
-                        if constexpr (kQuantize) x[b][j][s] = *reinterpret_cast<const uint4 *>(x_rows + m * x_rows_pitch + k);
-                        else x[b][j][s] = load16(p.x + m * p.x_pitch, k, p.k);
-                    }
+                    const int k = (warp + i * W) * 128 + s * 64 + t * 16, size = m < p.m ? max(0, min(16, p.k - k)) : 0;
+                    load16(to + (j * 2 + s) * 512, row + (size ? k : 0), size);
                 }
+            }
+        }
+    };
+    auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+    // A group of loads a block of K: block i is there once no more than kDepth - 1 younger groups are under way.  (Weights that are
+    // loaded early, ahead of the kernel in front, all belong to the first group.)
+    if (early) {
 #pragma unroll
-        for (int b = 0; b < kAhead; ++b)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const uint4 r0 = a[b][i][0][s], r1 = a[b][i][1][s];
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const uint4 v = x[b][j][s];
-                        mma_s8(acc[i][j], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
-                        mma_s8(acc[i][j], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
-                    }
-                }
+        for (int i = 0; i < S::kDepth; ++i)
+            if (i < mine) load_weights(i);
+        pdl_sync();
     }
+#pragma unroll
+    for (int i = 0; i < S::kDepth; ++i) {
+        if (i < mine) {
+            if (!early) load_weights(i);
+            load_tokens(i);
+        }
+        commit();
+    }
+    if constexpr (S::kQuantize) scale = quantizer.finish(x_rows, x_row_bytes, part);
 
-    int *mine = sums + warp * S::kTokens * S::kPitch;
+    int acc[NT][4] = {};
+    for (int i = 0; i < mine; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::kDepth - 1) : "memory");
+        const uint32_t at = ring + (uint32_t)(i % S::kDepth) * (S::kSlots * 512);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int s = 0; s < 2; ++s) {
+            const uint4 r0 = read16(at + (s * 2 + 0) * 512), r1 = read16(at + (s * 2 + 1) * 512);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if constexpr (S::kQuantize) {
+                    if (g == 0) v = *reinterpret_cast<const uint4 *>(x_rows + (warp + i * W) * 128 + s * 64 + t * 16);
+                } else {
+                    v = read16(at + (4 + j * 2 + s) * 512);
+                }
+                mma_s8(acc[j], r0.x, r1.x, r0.y, r1.y, v.x, v.y);
+                mma_s8(acc[j], r0.z, r1.z, r0.w, r1.w, v.z, v.w);
+            }
+        }
+        if (i + S::kDepth < mine) {
+            load_weights(i + S::kDepth);
+            load_tokens(i + S::kDepth);
+        }
+        commit();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // a warp's sums [token][channel] where its ring was (every lane's reads and loads are done)
+    __syncwarp();
+    int *sums = reinterpret_cast<int *>(smem + warp * S::kRing);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) mine[(j * 8 + t * 2 + (q & 1)) * S::kPitch + i * 16 + (q >> 1) * 8 + g] = acc[i][j][q];
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sums[(j * 8 + t * 2 + (q & 1)) * S::kPitch + (q >> 1) * 8 + g] = acc[j][q];
     __syncthreads();
     for (int o = threadIdx.x; o < S::kTokens * S::kChannels; o += 32 * W) {
         const int m = o / S::kChannels, c = o % S::kChannels, n = n0 + c;
         if (m >= p.m || n >= p.n) continue;
         int sum[1] = {0};
 #pragma unroll
-        for (int i = 0; i < W; ++i) sum[0] += sums[(i * S::kTokens + m) * S::kPitch + c];
+        for (int i = 0; i < W; ++i) sum[0] += reinterpret_cast<const int *>(smem + i * S::kRing)[m * S::kPitch + c];
         float v[1];
-        inner_prod_values<T>(p, sum, kQuantize ? scales[m] : p.x_scales[m * p.xs_stride], [&](int) { return p.w_scales[n]; }, [&](int) { return p.bias ? p.bias[n] : 0.0f; },
+        inner_prod_values<T>(p, sum, S::kQuantize ? scale : p.x_scales[m * p.xs_stride], [&](int) { return p.w_scales[n]; }, [&](int) { return p.bias ? p.bias[n] : 0.0f; },
                              [&](int) { return to_f32(static_cast<const T *>(p.residual)[m * p.residual_pitch + n]); }, v);
         static_cast<T *>(p.y)[m * p.y_pitch + n] = from_f32<T>(v[0]);
     }
 }
 
-template <typename T, typename X, int NT, int MT, int W>
+template <typename T, typename X, int NT, int W>
 int launch(const InnerProdParams &p, int early, cudaStream_t stream) {
-    using S = Shape<NT, MT>;
-    const int pitch = round_up(p.k, 128) + 64;      // (64 bytes more: two tokens' reads fall into different banks)
-    const size_t smem = (size_t)W * S::kTokens * S::kPitch * 4 + S::kTokens * 4 + W * 4 + (sizeof(X) > 1 ? (size_t)p.m * pitch : 0);
-    TSB_CUDA(launch_pdl(inner_prod_i8_few_kernel<T, X, NT, MT, W>, dim3(ceil_div(p.n, S::kChannels)), dim3(32 * W), smem, stream, p, early, pitch));
+    using S = Shape<X, NT>;
+    const int x_row_bytes = round_up(p.k, 128);
+    const size_t smem = W * S::kRing + (S::kQuantize ? x_row_bytes : 0) + W * 4;
+    auto kernel = inner_prod_i8_few_kernel<T, X, NT, W>;
+    static DeviceOnce raised;
+    if (raised.first()) {
+        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(W * S::kRing + kMaxQuantized + W * 4)));
+        raised.done();
+    }
+    TSB_CUDA(launch_pdl(kernel, dim3(ceil_div(p.n, S::kChannels)), dim3(32 * W), smem, stream, p, early, x_row_bytes));
     TSB_LAUNCHED("inner_prod_i8_few_kernel");
     return TSB_OK;
 }
 
-template <typename T>
-int pick(const InnerProdParams &p, int early, cudaStream_t stream) {
-    if (p.m <= 8) return launch<T, int8_t, 1, 1, 8>(p, early, stream);
-    if (p.m <= 16) return launch<T, int8_t, 2, 1, 8>(p, early, stream);
-    return launch<T, int8_t, 4, 1, 8>(p, early, stream);
+template <typename T, typename X, int NT>
+int pick_warps(const InnerProdParams &p, int early, cudaStream_t stream) {
+    // Two blocks of eight warps a multiprocessor, or four of four where there are more blocks than that (8192 channels x 2048: 6.3 us
+    // by eights, 5.5 by fours; 2048 x 8192: 5.3 and 6.4).
+    return ceil_div(p.n, 16) > 2 * 148 ? launch<T, X, NT, 4>(p, early, stream) : launch<T, X, NT, 8>(p, early, stream);
 }
 
 template <typename T>
-int pick_float(const InnerProdParams &p, cudaStream_t stream) { return launch<T, T, 1, 1, 8>(p, 0, stream); }
+int pick(const InnerProdParams &p, int early, cudaStream_t stream) {
+    if (p.m <= 8) return pick_warps<T, int8_t, 1>(p, early, stream);
+    if (p.m <= 16) return pick_warps<T, int8_t, 2>(p, early, stream);
+    return pick_warps<T, int8_t, 4>(p, early, stream);
+}
 
 }  // namespace
 
@@ -201,14 +255,14 @@ int inner_prod(const InnerProdParams &p, int y_type, int early, cudaStream_t str
     }
 }
 
-bool can_quantize(const InnerProdParams &p, int x_type, int y_type) { return x_type == y_type && p.m <= 8 && p.m * (round_up(p.k, 128) + 64) <= 32768; }
+bool can_quantize(const InnerProdParams &p, int x_type, int y_type) { return x_type == y_type && p.m == 1 && p.k <= kMaxQuantized; }
 
-// Up to 8 tokens of floating rows, of y's type, 32 KB of int8 rows.
+// One floating row of y's type.
 int inner_prod_quantize(const InnerProdParams &p, int y_type, cudaStream_t stream) {
     switch (y_type) {
-        case TSB_TYPE_F32: return pick_float<float>(p, stream);
-        case TSB_TYPE_F16: return pick_float<__half>(p, stream);
-        default: return pick_float<__nv_bfloat16>(p, stream);
+        case TSB_TYPE_F32: return pick_warps<float, float, 1>(p, 0, stream);
+        case TSB_TYPE_F16: return pick_warps<__half, __half, 1>(p, 0, stream);
+        default: return pick_warps<__nv_bfloat16, __nv_bfloat16, 1>(p, 0, stream);
     }
 }
 

@@ -16,7 +16,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <atomic>
 
 namespace tsb {
 namespace tc {
@@ -285,14 +284,11 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
     int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
     if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, BN);
     if (st != TSB_OK) return st;
-    static std::atomic<uint64_t> configured{0};      // devices that this kernel's shared-memory limit was raised on
     auto kernel = inner_prod_i8_tc_kernel<T, BN>;
-    int dev = 0;
-    TSB_CUDA(cudaGetDevice(&dev));
-    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
-    if (!(configured.load(std::memory_order_acquire) & bit)) {
+    static DeviceOnce raised;
+    if (raised.first()) {
         TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
-        configured.fetch_or(bit, std::memory_order_release);
+        raised.done();
     }
     TcParams t = {p, (int)ceil_div64(p.m, kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
     const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;

@@ -1,42 +1,128 @@
 // quantize with a scale for each row that is taken from the row (no counterpart in the reference, whose scales are attributes).
+//
+// Bound by memory: a row is read once, held in registers while its largest magnitude is found, and written as int8.  A thread holds up
+// to four 16-byte vectors; a row belongs to a warp, or to a block of as many warps as it needs -- of many rows, few threads with
+// four vectors each (loads in flight), of few rows, many threads with one (a short way from load to store).
 #include "typed.cuh"
+
+#include <algorithm>
 
 namespace tsb {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarpRowThreads = 256;      // rows of a warp each: threads of a block
+constexpr int kMost = 1024;               // threads of a row, at most
+
+// Vector u of a row: one 16-byte load, or value by value where rows do not start on 16 bytes and at the row's end (zeros behind it,
+// which change neither the maximum nor what is written).
+template <typename T>
+__device__ __forceinline__ uint4 load_vector(const T *row, int u, int cols, bool aligned) {
+    constexpr int kN = Vec16<T>::kN;
+    if (aligned && u * kN + kN <= cols) return __ldg(reinterpret_cast<const uint4 *>(row) + u);
+    uint4 out = make_uint4(0, 0, 0, 0);
+    T *v = reinterpret_cast<T *>(&out);
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+        if (u * kN + i < cols) v[i] = row[u * kN + i];
+    return out;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restrict__ y, int64_t y_pitch, float *__restrict__ scales,
-                     int64_t rows, int cols) {
-    __shared__ uint32_t part[kThreads / 32];
-    pdl_sync();
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const T *xr = x + r * x_pitch;
-        uint32_t m = 0;
-        for (int c = threadIdx.x; c < cols; c += kThreads) m = max(m, magnitude(to_f32(xr[c])));
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-        __syncthreads();
-        m = 0;
+__device__ __forceinline__ uint32_t largest_of(const uint4 &q) {
+    float v[Vec16<T>::kN];
+    Vec16<T>::get(q, v);
+    uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) m = max(m, part[i]);
-        __syncthreads();
-        const RowScale row(m);
-        if (threadIdx.x == 0) scales[r] = row.scale;
+    for (int i = 0; i < Vec16<T>::kN; ++i) m = max(m, magnitude(v[i]));
+    return m;
+}
+
+// Vector u as int8, in one store where the row starts on a multiple of its bytes.
+template <typename T>
+__device__ __forceinline__ void store_vector(const RowScale &scale, const uint4 &q, int8_t *row, int u, int cols, bool aligned) {
+    constexpr int kN = Vec16<T>::kN;
+    uint32_t w[kN / 4];
+    quantize16<T>(scale, q, w);
+    int8_t *to = row + u * kN;
+    if (aligned && u * kN + kN <= cols) {
+        if constexpr (kN == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t *>(to) = w[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (u * kN + i < cols) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+// V: vectors a thread holds; 0: any number, read a second time.  WARP: a row belongs to a warp, else to the block.
+template <typename T, int V, bool WARP>
+__global__ void __launch_bounds__(WARP ? kWarpRowThreads : kMost)
+quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restrict__ y, int64_t y_pitch, float *__restrict__ scales,
+                     int64_t rows, int cols, int x_aligned, int y_aligned) {
+    __shared__ uint32_t part[kMost / 32];
+    pdl_sync();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int at = WARP ? lane : threadIdx.x, step = WARP ? 32 : blockDim.x;
+    const int vectors = (cols + Vec16<T>::kN - 1) / Vec16<T>::kN;
+    const int64_t first = WARP ? (int64_t)blockIdx.x * warps + warp : blockIdx.x, stride = WARP ? (int64_t)gridDim.x * warps : gridDim.x;
+    for (int64_t r = first; r < rows; r += stride) {
+        const T *xr = x + r * x_pitch;
         int8_t *yr = y + r * y_pitch;
-        for (int c = threadIdx.x; c < cols; c += kThreads) yr[c] = (int8_t)row(to_f32(xr[c]));
+        uint4 held[V > 0 ? V : 1];
+        uint32_t most = 0;
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                held[i] = make_uint4(0, 0, 0, 0);
+                if (at + i * step < vectors) held[i] = load_vector(xr, at + i * step, cols, x_aligned);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) most = max(most, largest_of<T>(held[i]));
+        } else {
+#pragma unroll 4
+            for (int u = at; u < vectors; u += step) most = max(most, largest_of<T>(load_vector(xr, u, cols, x_aligned)));
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if constexpr (!WARP) {
+            if (lane == 0) part[warp] = most;
+            __syncthreads();
+            most = __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0);
+        }
+        const RowScale scale(most);
+        if (at == 0) scales[r] = scale.scale;
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (at + i * step < vectors) store_vector<T>(scale, held[i], yr, at + i * step, cols, y_aligned);
+        } else {
+#pragma unroll 4
+            for (int u = at; u < vectors; u += step) store_vector<T>(scale, load_vector(xr, u, cols, x_aligned), yr, u, cols, y_aligned);
+        }
+        if constexpr (!WARP) __syncthreads();      // (the next row's maxima)
     }
 }
 
 template <typename T>
 int launch(const void *x, int64_t x_pitch, int8_t *y, int64_t y_pitch, float *scales, int64_t rows, int cols, cudaStream_t stream) {
-    const int grid = (int)(rows < 148 * 64 ? rows : 148 * 64);
-    TSB_CUDA(launch_pdl(quantize_rows_kernel<T>, dim3(grid), dim3(kThreads), 0, stream, static_cast<const T *>(x), x_pitch, y, y_pitch, scales, rows,
-                        cols));
-    TSB_LAUNCHED("quantize_rows_kernel");
-    return TSB_OK;
+    constexpr int kN = Vec16<T>::kN;
+    const int x_aligned = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (x_pitch * (int64_t)sizeof(T)) % 16 == 0;
+    const int y_aligned = reinterpret_cast<uintptr_t>(y) % kN == 0 && y_pitch % kN == 0;
+    const int vectors = ceil_div(cols, kN);
+    auto go = [&](auto kernel, int64_t blocks, int threads) {
+        TSB_CUDA(launch_pdl(kernel, dim3((int)std::min<int64_t>(blocks, 148 * 64)), dim3(threads), 0, stream, static_cast<const T *>(x), x_pitch, y, y_pitch,
+                            scales, rows, cols, x_aligned, y_aligned));
+        TSB_LAUNCHED("quantize_rows_kernel");
+        return TSB_OK;
+    };
+    // a warp a row: of many short rows (of few, a block each is done sooner)
+    if (vectors <= 32 || (vectors <= 128 && rows > 148 * 8)) {
+        const int64_t blocks = ceil_div64(rows, kWarpRowThreads / 32);
+        if (vectors <= 32) return go(quantize_rows_kernel<T, 1, true>, blocks, kWarpRowThreads);
+        return go(quantize_rows_kernel<T, 4, true>, blocks, kWarpRowThreads);
+    }
+    if (vectors <= kMost && rows <= 148 * 2) return go(quantize_rows_kernel<T, 1, false>, rows, round_up(vectors, 32));
+    if (vectors <= 4 * kMost) return go(quantize_rows_kernel<T, 4, false>, rows, round_up(ceil_div(vectors, 4), 32));
+    return go(quantize_rows_kernel<T, 0, false>, rows, kMost);
 }
 
 }  // namespace

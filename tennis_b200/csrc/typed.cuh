@@ -98,6 +98,17 @@ struct RowScale {
     __device__ __forceinline__ int operator()(float v) const { return q8_half_even(__fmul_rn(v, by)); }
 };
 
+// 16 bytes of a floating row as int8
+template <typename X>
+__device__ __forceinline__ void quantize16(const RowScale &q, const uint4 &from, uint32_t *to) {
+    constexpr int kN = Vec16<X>::kN;
+    float v[kN];
+    Vec16<X>::get(from, v);
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i)
+        to[i] = (uint32_t)(uint8_t)q(v[4 * i]) | (uint32_t)(uint8_t)q(v[4 * i + 1]) << 8 | (uint32_t)(uint8_t)q(v[4 * i + 2]) << 16 | (uint32_t)(uint8_t)q(v[4 * i + 3]) << 24;
+}
+
 // silu, v / (1 + exp(-v)), by the hardware's exp2 and reciprocal (relative errors of 2^-22 and 2^-23).
 // For fp32 results the rounding error of -v log2(e), which exp2 would turn into a relative error of |v| 2^-24, is computed by a fused
 // multiply-add and put back to first order: 8 half steps of the result in all.  Results of 16 bits, whose half step is 2^13 times that
