@@ -522,16 +522,30 @@ def repack_nhwc_to_nchw(x, channels, stream=None):
 # ---- int8 layers with scales per token: quantize_rows, inner_prod_quantized, group_norm_nhwc --------------------------------
 # These three work on the device that their tensors are on, on its current stream or on `stream`; what they allocate (outputs,
 # workspace) belongs to that stream.  Memory of an input that another stream allocated is the caller's to keep until the work is done.
+# A kernel of theirs can be done in 2 us, so the host's way to it counts: a check is a comparison whose text is made only when it
+# fails, and empty_strided with lists of sizes and strides takes 1.5 us where empty takes 2.3.
 _TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16, torch.int8: _lib.TYPE_I8}
-_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_FLOATS = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+_FLOAT_NAMES = "float32, float16 or bfloat16, not %s"
+_int8, _float32 = torch.int8, torch.float32
+_empty_strided = torch.empty_strided
 
 
-def _on(x, stream):
-    """A context on x's device and on `stream`, or None where the program is there already."""
+def _refuse(text, *values):
+    raise EjectionException("Check failed: (%s)." % (text % values if values else text))
+
+
+def _elsewhere(call, x, stream, *args):
+    """call(x, *args) with x's device and `stream` as the current ones."""
+    if not x.is_cuda:
+        _refuse("x.is_cuda")
     if stream is None:
-        return None if x.get_device() == _current_device() else torch.cuda.device(x.device)
-    _auto_check(stream.device == x.device, "stream.device == x.device")
-    return torch.cuda.stream(stream)
+        with torch.cuda.device(x.device):
+            return call(x, *args)
+    if stream.device != x.device:
+        _refuse("stream.device == x.device")
+    with torch.cuda.stream(stream):
+        return call(x, *args)
 
 
 def _rows_of(t):
@@ -541,9 +555,19 @@ def _rows_of(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-def _check_vector(t, size, x, name):
-    _auto_check(t.dtype == torch.float32 and t.numel() == size and t.is_contiguous() and t.device == x.device,
-                "%s: %d contiguous float32 values on x's device" % (name, size))
+def _rows_to(out):
+    """The rows of an output as a view."""
+    if out.dim() == 2:
+        return out
+    try:
+        return out.view(-1, out.shape[-1])
+    except RuntimeError:
+        _refuse("out: its rows lie a fixed step apart")
+
+
+def _check_vector(t, size, device, name):
+    if t.dtype is not _float32 or t.numel() != size or t.get_device() != device or not t.is_contiguous():
+        _refuse("%s: %d contiguous float32 values on x's device", name, size)
 
 
 def quantize_rows(x, out=None, scales=None, stream=None):
@@ -553,31 +577,33 @@ def quantize_rows(x, out=None, scales=None, stream=None):
     q is [..., k]; its rows start a multiple of 16 bytes apart, the way inner_prod_quantized reads them fastest.  The rows of x are
     tokens of an activation, or output channels of a weight tensor.  ``out`` (int8, x's shape, values of a row next to each other)
     and ``scales`` take the results where they are given."""
-    _auto_check(x.is_cuda, "x.is_cuda")
-    there = _on(x, stream)
-    if there is not None:
-        with there:
-            return quantize_rows(x, out, scales)
-    _auto_check(x.dtype in _FLOATS, "x.dtype: float32, float16 or bfloat16, not %s" % x.dtype)
-    _auto_check(x.dim() >= 1 and x.shape[-1] > 0, "x_tensor.size(-1) > 0")
-    shape, k = x.shape, x.shape[-1]
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(quantize_rows, x, stream, out, scales)
+    kind = _FLOATS.get(x.dtype)
+    if kind is None:
+        _refuse("x.dtype: " + _FLOAT_NAMES, x.dtype)
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        _refuse("x_tensor.size(-1) > 0")
     rows = _rows_of(x)
+    m, k = rows.shape
     if out is None:
-        out = torch.empty(shape[:-1] + ((k + 15) // 16 * 16,), dtype=torch.int8, device=x.device)[..., :k]
-    else:
-        _auto_check(out.dtype == torch.int8 and out.shape == shape and out.device == x.device and (out.stride(-1) == 1 or k == 1),
-                    "out: int8 of x's shape on x's device, values of a row next to each other")
-    # (a view: an `out` whose rows lie no fixed step apart is refused, as it could only be written through a copy)
-    try:
-        q = out if out.dim() == 2 else out.view(-1, k)
-    except RuntimeError:
-        raise EjectionException("out: its rows lie no fixed step apart")
+        pitch = (k + 15) // 16 * 16
+        q = _empty_strided((m, k), (pitch, 1), dtype=_int8, device=x.device)
+        out = q if len(shape) == 2 else q.view(shape) if k == pitch else torch.empty(shape[:-1] + (pitch,), dtype=_int8, device=x.device)[..., :k]
+    elif out.dtype is not _int8 or out.shape != shape or out.get_device() != device or (out.stride(-1) != 1 and k > 1):
+        _refuse("out: int8 of x's shape on x's device, values of a row next to each other")
+    if out.numel():
+        q = _rows_to(out)
     if scales is None:
-        scales = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+        scales = _empty_strided((m,), (1,), dtype=_float32, device=x.device)
+        if len(shape) != 2:
+            scales = scales.view(shape[:-1])
     else:
-        _check_vector(scales, rows.shape[0], x, "scales")
-    status = _lib.load().tsb_quantize_rows_i8(rows.data_ptr(), _TYPE[x.dtype], rows.stride(0), q.data_ptr(), q.stride(0), scales.data_ptr(),
-                                              rows.shape[0], k, _stream_ptr())
+        _check_vector(scales, m, device, "scales")
+    status = _lib.load().tsb_quantize_rows_i8(rows.data_ptr(), kind, rows.stride(0), q.data_ptr(), q.stride(0), scales.data_ptr(), m, k,
+                                              _current_raw_stream(device))
     if status:
         check(status)
     return out, scales
@@ -588,60 +614,71 @@ def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, act
     """x [..., k] times w [n, k] transposed, in int8 with int32 sums, a scale per token and per output channel:
     ``activation(sum * w_scales * x_scales + bias + residual)`` (or ``activation(...) + residual``), [..., n].
 
-    x is int8 with ``x_scales`` (one per row, or one value for all), as quantize_rows gives them, or floating with ``x_scales=None``: then its rows are
-    quantized in the call.  w int8 and w_scales [n] are what quantize_rows makes of a float weight tensor.  ``residual``
+    x is int8 with ``x_scales`` (one per row, or one value for all), as quantize_rows gives them, or floating with ``x_scales=None``: then
+    its rows are quantized in the call.  w int8 and w_scales [n] are what quantize_rows makes of a float weight tensor.  ``residual``
     has the output's type and shape.  ``out_dtype`` is x's type (of int8 rows: float32) unless given; ``out`` takes the result where
     it is given (it may be ``residual``, and no other operand)."""
-    _auto_check(x.is_cuda, "x.is_cuda")
-    there = _on(x, stream)
-    if there is not None:
-        with there:
-            return inner_prod_quantized(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, out, residual_after_activation, kernel)
-    dynamic = x_scales is None
-    dev = x.device
-    _auto_check(x.dtype in _FLOATS if dynamic else x.dtype == torch.int8,
-                "x.dtype: int8 with x_scales; float32, float16 or bfloat16 without; not %s" % x.dtype)
-    _auto_check(w.dtype == torch.int8 and w.dim() == 2 and w.device == dev, "w: an int8 matrix on x's device")
-    _auto_check(x.dim() >= 1 and x.shape[-1] == w.shape[1], "w_tensor.size(1) == x_tensor.size(-1)")
-    lead, n = x.shape[:-1], w.shape[0]
-    rows = _rows_of(x)
-    m, k = rows.shape
-    w = _rows_of(w)
-    _check_vector(w_scales, n, x, "w_scales")
-    if not dynamic:
-        _check_vector(x_scales, 1 if x_scales.numel() == 1 else m, x, "x_scales")
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(inner_prod_quantized, x, stream, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, out,
+                          residual_after_activation, kernel)
+    x_dtype, shape = x.dtype, x.shape
+    if x_scales is None:
+        if x_dtype not in _FLOATS:
+            _refuse("x.dtype: int8 with x_scales, without " + _FLOAT_NAMES, x_dtype)
+    elif x_dtype is not _int8:
+        _refuse("x.dtype: int8 with x_scales, not %s", x_dtype)
+    if w.dtype is not _int8 or w.dim() != 2 or w.get_device() != device:
+        _refuse("w: an int8 matrix on x's device")
+    n, k = w.shape
+    if not shape or shape[-1] != k:
+        _refuse("w_tensor.size(1) == x_tensor.size(-1)")
+    if k < 1:
+        _refuse("x_tensor.size(-1) > 0")
+    rows, w = _rows_of(x), _rows_of(w)
+    m = rows.shape[0]
+    _check_vector(w_scales, n, device, "w_scales")
+    scales_at = scales_step = 0
+    if x_scales is not None:
+        one = x_scales.numel() == 1
+        _check_vector(x_scales, 1 if one else m, device, "x_scales")
+        scales_at, scales_step = x_scales.data_ptr(), 0 if one else 1
+    bias_at = 0
     if bias is not None:
-        _check_vector(bias, n, x, "bias")
+        _check_vector(bias, n, device, "bias")
+        bias_at = bias.data_ptr()
+    dtype = out_dtype if out_dtype is not None else out.dtype if out is not None else x_dtype if x_scales is None else _float32
+    kind = _FLOATS.get(dtype)
+    if kind is None:
+        _refuse("out_dtype: " + _FLOAT_NAMES, dtype)
+    want = (m, n) if len(shape) == 2 else shape[:-1] + (n,)
     if out is None:
-        dtype = out_dtype if out_dtype is not None else (x.dtype if dynamic else torch.float32)
-        _auto_check(dtype in _FLOATS, "out_dtype: float32, float16 or bfloat16, not %s" % dtype)
-        out = torch.empty(lead + (n,), dtype=dtype, device=dev)
+        y = _empty_strided((m, n), (n, 1), dtype=dtype, device=x.device)
+        out = y if len(shape) == 2 else y.view(want)
     else:
-        dtype = out.dtype
-        _auto_check(dtype in _FLOATS and out_dtype in (None, dtype) and out.shape == lead + (n,) and out.device == dev and (n <= 1 or out.stride(-1) == 1),
-                    "out: a floating [..., n] on x's device, values of a row next to each other")
+        if out.dtype is not dtype or out.shape != want or out.get_device() != device or (out.stride(-1) != 1 and n > 1):
+            _refuse("out: of out_dtype, [..., n] on x's device, values of a row next to each other")
+        y = _rows_to(out) if out.numel() else out
+    residual_at = residual_step = 0
     if residual is not None:
-        _auto_check(residual.dtype == dtype and residual.shape == lead + (n,) and residual.device == dev, "residual: of the output's type and shape on x's device")
-    if not out.numel():
+        if residual.dtype is not dtype or residual.shape != want or residual.get_device() != device:
+            _refuse("residual: of the output's type and shape on x's device")
+    if not (m and n):
         return out
-    try:
-        y = out if out.dim() == 2 else out.view(-1, n)
-    except RuntimeError:
-        raise EjectionException("out: its rows lie no fixed step apart")
     if residual is not None:
         residual = _rows_of(residual)
+        residual_at, residual_step = residual.data_ptr(), residual.stride(0)
     lib = _lib.load()
-    args = _lib.INNER_PROD_ARGS.pack(m, n, k, rows.data_ptr(), rows.stride(0), 0 if dynamic else x_scales.data_ptr(),
-                                     0 if dynamic or x_scales.numel() == 1 else 1, w.data_ptr(), w.stride(0), w_scales.data_ptr(),
-                                     0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(),
-                                     0 if residual is None else residual.stride(0), y.data_ptr(), y.stride(0), _TYPE[x.dtype], _TYPE[dtype],
-                                     activation, leaky, 1 if residual_after_activation else 0, kernel)
-    workspace, size = None, 0
-    if dynamic:
+    args = _lib.INNER_PROD_ARGS.pack(m, n, k, rows.data_ptr(), rows.stride(0), scales_at, scales_step, w.data_ptr(), w.stride(0), w_scales.data_ptr(),
+                                     bias_at, residual_at, residual_step, y.data_ptr(), y.stride(0), _TYPE[x_dtype], kind, activation, leaky,
+                                     1 if residual_after_activation else 0, kernel)
+    workspace = size = 0
+    if x_scales is None:
         size = lib.tsb_inner_prod_i8_workspace_bytes(args)
         if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=dev)
-    status = lib.tsb_inner_prod_i8(args, _ptr(workspace), size, _stream_ptr())
+            room = _empty_strided((size,), (1,), dtype=torch.uint8, device=x.device)
+            workspace = room.data_ptr()
+    status = lib.tsb_inner_prod_i8(args, workspace, size, _current_raw_stream(device))
     if status:
         check(status)
     return out
@@ -659,45 +696,62 @@ def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_N
     """Group norm and activation of a channels-last x [n, ..., channels] (fp32, fp16 or bf16): mean and variance of each image's
     ``groups`` equal runs of channels over all its pixels, ``activation((x - mean) / sqrt(variance + eps) * gamma + beta)``.
 
-    The result has x's type and shape (``out`` takes it where it is given; it may be x).  ``out_dtype=torch.int8`` with ``requant_scales`` (one, or one per image)
-    gives ``quantize`` of it as NHWC_PAD [n, ..., padded_channels(channels)] instead, what a convolution plan reads."""
-    _auto_check(x.is_cuda, "x.is_cuda")
-    there = _on(x, stream)
-    if there is not None:
-        with there:
-            return group_norm_nhwc(x, groups, gamma, beta, eps, activation, leaky, out_dtype, requant_scales, out)
-    _auto_check(x.dtype in _FLOATS, "x.dtype: float32, float16 or bfloat16, not %s" % x.dtype)
-    _auto_check(x.dim() >= 3, "x_tensor.dims() >= 3")
-    dtype = out_dtype if out_dtype is not None else (x.dtype if out is None else out.dtype)
-    _auto_check(dtype == x.dtype or dtype == torch.int8, "out_dtype: x's type or int8, not %s" % dtype)
-    shape, n, c = x.shape, x.shape[0], x.shape[-1]
-    _auto_check(c > 0, "x_tensor.size(-1) > 0")
+    The result has x's type and shape (``out`` takes it where it is given; it may be x).  ``out_dtype=torch.int8`` with
+    ``requant_scales`` (one, or one per image) gives ``quantize`` of it as NHWC_PAD [n, ..., padded_channels(channels)] instead, what
+    a convolution plan reads."""
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(group_norm_nhwc, x, stream, groups, gamma, beta, eps, activation, leaky, out_dtype, requant_scales, out)
+    kind, shape = _FLOATS.get(x.dtype), x.shape
+    if kind is None:
+        _refuse("x.dtype: " + _FLOAT_NAMES, x.dtype)
+    if len(shape) < 3:
+        _refuse("x_tensor.dims() >= 3")
+    n, c = shape[0], shape[-1]
+    if c < 1:
+        _refuse("x_tensor.size(-1) > 0")
+    dtype = out_dtype if out_dtype is not None else x.dtype if out is None else out.dtype
+    if dtype is not x.dtype and dtype is not _int8:
+        _refuse("out_dtype: x's type or int8, not %s", dtype)
     pixels = x.numel() // (n * c) if n else 0
-    for v, name in ((gamma, "gamma"), (beta, "beta")):
-        if v is not None:
-            _check_vector(v, c, x, name)
-    scales, n_scales = None, 0
-    if dtype == torch.int8:
-        _auto_check(requant_scales is not None, "out_dtype int8 comes with requant_scales")
+    gamma_at = beta_at = 0
+    if gamma is not None:
+        _check_vector(gamma, c, device, "gamma")
+        gamma_at = gamma.data_ptr()
+    if beta is not None:
+        _check_vector(beta, c, device, "beta")
+        beta_at = beta.data_ptr()
+    lib = _lib.load()
+    scales_at = n_scales = 0
+    if dtype is _int8:
+        if requant_scales is None:
+            _refuse("out_dtype int8 comes with requant_scales")
         scales = _scales_of(requant_scales)
-        n_scales = len(scales)
+        scales_at, n_scales = ctypes.addressof(scales), len(scales)
+        want = shape[:-1] + (lib.tsb_padded_channels(c),)
+    else:
+        want = shape
     x_step = _pixel_step(x)
     if x_step is None:
         x, x_step = x.contiguous(), c
-    want = shape[:-1] + (padded_channels(c),) if scales is not None else shape
+    y_image = y_step = 0
     if out is None:
-        out = torch.empty(want, dtype=dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format) if want is shape else torch.empty(want, dtype=dtype, device=x.device)
+        y_image, y_step = pixels * c, c
     else:
-        _auto_check(out.dtype == dtype and out.shape == want and out.device == x.device, "out: x's shape (int8: NHWC_PAD) and the output's type on x's device")
-    y_step = _pixel_step(out)
-    _auto_check(y_step is not None and (scales is None or out.is_contiguous()), "out: pixels of an image a fixed step apart, channels next to each other")
-    lib = _lib.load()
-    desc = _lib.GROUP_NORM_DESC.pack(n, pixels, c, groups, x.data_ptr(), x_step, x.stride(0), out.data_ptr(), y_step, out.stride(0),
-                                     0 if gamma is None else gamma.data_ptr(), 0 if beta is None else beta.data_ptr(), eps,
-                                     0 if scales is None else ctypes.addressof(scales), n_scales, _TYPE[x.dtype], _TYPE[dtype], activation, leaky)
+        if out.dtype is not dtype or out.shape != want or out.get_device() != device:
+            _refuse("out: x's shape (int8: NHWC_PAD) and the output's type on x's device")
+        y_image, y_step = out.stride(0), _pixel_step(out)
+        if y_step is None or (dtype is _int8 and not out.is_contiguous()):
+            _refuse("out: pixels of an image a fixed step apart, channels next to each other (int8: contiguous)")
+    desc = _lib.GROUP_NORM_DESC.pack(n, pixels, c, groups, x.data_ptr(), x_step, x.stride(0), out.data_ptr(), y_step, y_image, gamma_at, beta_at, eps,
+                                     scales_at, n_scales, kind, _TYPE[dtype], activation, leaky)
     size = lib.tsb_group_norm_workspace_bytes(desc)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    status = lib.tsb_group_norm_nhwc(desc, _ptr(workspace), size, _stream_ptr())
+    workspace = 0
+    if size:
+        room = _empty_strided((size,), (1,), dtype=torch.uint8, device=x.device)
+        workspace = room.data_ptr()
+    status = lib.tsb_group_norm_nhwc(desc, workspace, size, _current_raw_stream(device))
     if status:
         check(status)
     return out
