@@ -1,4 +1,15 @@
 // Group norm with an activation on channels-last tensors (no counterpart in the reference).
+//
+// Bound by memory: each value is read once and written once, if what lies between -- the statistics of its whole group -- is had
+// without reading it again from HBM.
+//
+//   sums       in 64 bits: with 53 bits the difference of the mean square and the squared mean keeps 32-bit accuracy for means up to
+//              10^4 deviations, in one pass over the data, and no order of summation shows in the rounded mean and deviation
+//   threads    a thread owns one 16-byte vector of channels (or one channel, where vectors do not fit) and walks over pixels: loads of
+//              neighbouring threads are neighbours, its channels' gamma, beta and statistics stay in registers
+//   resident   an image's run of groups is held in the shared memory of a cluster of up to eight blocks: loaded once, summed on the
+//              way, the blocks' sums exchanged through distributed shared memory, normalized from shared memory.  One launch
+//   sweep      larger images: a launch sums images j + 1 while it normalizes images j, which the L2 still holds
 #include "typed.cuh"
 
 #include <algorithm>
@@ -8,7 +19,10 @@ namespace tsb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxSplits = 64;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;                  // the portable limit
+constexpr int kMaxGroups = 256;                 // groups of a run of channels
+constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
 struct GroupNormParams {
     const void *x;
@@ -17,103 +31,338 @@ struct GroupNormParams {
     const float *gamma, *beta;                    // or NULL
     int n, channels, groups, per;                 // per = channels of a group
     int64_t pixels;
-    int splits;
+    int run_groups, runs;                         // groups of a run of channels, runs of an image
+    int cols;                                     // vectors of a run that the block's threads own at a time
+    int64_t tile;                                 // pixels of a block's tile
+    int tiles;                                    // ... and tiles of an image
     double eps;
     int activation;
     float leaky;
     int out_channels;                             // channels written: int8 outputs are padded with zeros
     int64_t rne_limit;                            // int8: values below this (in channel-major order) round half to even
+    int tail;                                     // ... and there are values at or above it that do not
     int nscales;
     float scales[TSB_MAX_REQUANT_SCALES];
 };
 
-// sums[image][split][group] = {sum, sum of squares} of the split's pixels.  Both in 64 bits: with 53 bits the difference of the mean
-// square and the squared mean keeps 32-bit accuracy for means up to 10^4 deviations, in one pass and any order of summation.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-group_norm_sums_kernel(GroupNormParams p, double2 *__restrict__ sums) {
-    __shared__ double2 part[kThreads];
-    pdl_sync();
-    const int split = blockIdx.x % p.splits, image = blockIdx.x / p.splits;
-    const int64_t p0 = p.pixels * split / p.splits, p1 = p.pixels * (split + 1) / p.splits;
-    const int lanes = min(p.channels, kThreads), rows = kThreads / lanes;
-    const int lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
-    double2 *out = sums + ((int64_t)image * p.splits + split) * p.groups;
-    for (int g = threadIdx.x; g < p.groups; g += kThreads) out[g] = make_double2(0.0, 0.0);
-    for (int c0 = 0; c0 < p.channels; c0 += lanes) {
-        double s = 0.0, ss = 0.0;
-        if (c0 + lane < p.channels && row < rows) {
-            const T *col = static_cast<const T *>(p.x) + image * p.x_image + c0 + lane;
-            for (int64_t q = p0 + row; q < p1; q += rows) {
-                const double v = (double)to_f32(col[q * p.x_pixel]);
-                s += v;
-                ss = fma(v, v, ss);
-            }
-        }
-        __syncthreads();
-        part[threadIdx.x] = make_double2(s, ss);
-        __syncthreads();
-        // a group's channels in this block of channels, by the one thread that owns the group
-        const int c1 = min(c0 + lanes, p.channels);
-        for (int g = threadIdx.x; g < p.groups; g += kThreads) {
-            const int a = max(c0, g * p.per), b = min(c1, (g + 1) * p.per);
-            double2 t = out[g];
-            for (int c = a; c < b; ++c)
-                for (int r = 0; r < rows; ++r) {
-                    t.x += part[r * lanes + c - c0].x;
-                    t.y += part[r * lanes + c - c0].y;
-                }
-            out[g] = t;
-        }
-    }
+// A block's part of the work: channels [c0, c0 + width) of an image, pixels [p0, p1)
+struct Part {
+    int image, c0, width, g0, groups;
+    int64_t p0, p1;
+};
+__device__ __forceinline__ Part part_of(const GroupNormParams &p, int image, int run, int tile) {
+    Part t;
+    t.image = image;
+    t.g0 = run * p.run_groups;
+    t.groups = min(p.run_groups, p.groups - t.g0);
+    t.c0 = t.g0 * p.per;
+    t.width = t.groups * p.per;
+    t.p0 = min((int64_t)tile * p.tile, p.pixels);
+    t.p1 = min(t.p0 + p.tile, p.pixels);
+    return t;
 }
 
-// stats[image][group] = {mean, 1 / sqrt(variance + eps)}, each rounded once
-__global__ void __launch_bounds__(kThreads)
-group_norm_stats_kernel(GroupNormParams p, const double2 *__restrict__ sums, float2 *__restrict__ stats) {
-    pdl_sync();
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (i >= (int64_t)p.n * p.groups) return;
-    const int64_t image = i / p.groups, g = i % p.groups;
-    double s = 0.0, ss = 0.0;
-    for (int k = 0; k < p.splits; ++k) {
-        const double2 t = sums[(image * p.splits + k) * p.groups + g];
-        s += t.x;
-        ss += t.y;
+// VEC values of a type, as they lie in memory
+template <typename T, int VEC> struct Raw { using type = uint4; };
+template <typename T> struct Raw<T, 1> { using type = T; };
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const typename Raw<T, VEC>::type &q, float (&v)[VEC]) {
+    if constexpr (VEC == 1) v[0] = to_f32(q);
+    else Vec16<T>::get(q, v);
+}
+
+// Sums of a thread's channels; ONE: all channels of a vector belong to one group, and one pair of sums serves them.
+template <int VEC, bool ONE>
+struct Sums {
+    static constexpr int kN = ONE ? 1 : VEC;
+    double s[kN], ss[kN];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) s[i] = ss[i] = 0.0;
     }
+    __device__ __forceinline__ void add(const float (&v)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const double d = (double)v[i];
+            s[ONE ? 0 : i] += d;
+            ss[ONE ? 0 : i] = fma(d, d, ss[ONE ? 0 : i]);
+        }
+    }
+};
+
+// Adds the threads' sums of channels [b0, b1) of the run to the groups' sums in shared memory, in a fixed order: a warp takes a group,
+// its lanes the group's entries in turn.  Thread (row, col) of `rows` x `cols` owns vector b0 / VEC + col.
+template <int VEC, bool ONE>
+__device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scratch, double2 *group_sums, int b0, int b1, int per, int groups, int rows, int cols) {
+    constexpr int kN = Sums<VEC, ONE>::kN, kStep = VEC / kN;     // entries of a vector, channels of an entry
+#pragma unroll
+    for (int i = 0; i < kN; ++i) scratch[i * kThreads + threadIdx.x] = make_double2(sums.s[i], sums.ss[i]);
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    for (int g = b0 / per + (threadIdx.x >> 5); g < groups && g * per < b1; g += kWarps) {
+        const int a = max(g * per, b0) - b0, b = min((g + 1) * per, b1) - b0;      // the group's channels within the block of columns
+        const int entries = (b - a) / kStep, first = a / kStep;
+        double s = 0.0, ss = 0.0;
+        for (int e = lane; e < entries * rows; e += 32) {
+            const int row = e / entries, entry = first + e - row * entries;
+            const double2 t = scratch[(kN == 1 ? 0 : entry % kN) * kThreads + row * cols + entry / kN];
+            s += t.x;
+            ss += t.y;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_down_sync(0xffffffffu, s, o);
+            ss += __shfl_down_sync(0xffffffffu, ss, o);
+        }
+        if (lane == 0) {
+            group_sums[g].x += s;
+            group_sums[g].y += ss;
+        }
+    }
+    __syncthreads();
+}
+
+// {mean, 1 / sqrt(variance + eps)} of a group, each rounded once
+__device__ __forceinline__ float2 statistics(const GroupNormParams &p, double s, double ss) {
     const double count = (double)p.pixels * p.per;
     const double mean = s / count;
-    double var = fma(-mean, mean, ss / count);
-    var = var < 0.0 ? 0.0 : var;
-    stats[i] = make_float2((float)mean, (float)(1.0 / sqrt(var + p.eps)));
+    const double raw = fma(-mean, mean, ss / count);
+    const double var = raw < 0.0 ? 0.0 : raw;            // (a NaN stays one)
+    return make_float2((float)mean, (float)(1.0 / sqrt(var + p.eps)));
 }
 
-template <typename T, typename Y>
-__global__ void __launch_bounds__(kThreads)
-group_norm_apply_kernel(GroupNormParams p, const float2 *__restrict__ stats) {
-    pdl_sync();
-    const int64_t total = (int64_t)p.n * p.pixels * p.out_channels;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const int c = (int)(i % p.out_channels);
-        const int64_t q = i / p.out_channels % p.pixels, image = i / p.out_channels / p.pixels;
-        Y *y = static_cast<Y *>(p.y) + image * p.y_image + q * p.y_pixel + c;
-        if (c >= p.channels) {
-            *y = Y(0);
-            continue;
+// What a thread applies to its channels: statistics, gamma, beta, activation, rounding.
+template <typename T, typename Y, int VEC, bool ONE>
+struct Apply {
+    static constexpr int kG = ONE ? 1 : VEC;
+    float mean[kG], rstd[kG], gamma[VEC], beta[VEC];
+    // c: the thread's first channel within the run
+    __device__ __forceinline__ void init(const GroupNormParams &p, const Part &t, const float2 *stats, int c) {
+#pragma unroll
+        for (int i = 0; i < kG; ++i) {
+            const float2 st = stats[(c + i) / p.per];
+            mean[i] = st.x;
+            rstd[i] = st.y;
         }
-        const float2 st = stats[image * p.groups + c / p.per];
-        float v = __fmul_rn(__fsub_rn(to_f32(static_cast<const T *>(p.x)[image * p.x_image + q * p.x_pixel + c]), st.x), st.y);
-        if (p.gamma) v = __fmul_rn(v, p.gamma[c]);
-        if (p.beta) v = __fadd_rn(v, p.beta[c]);
-        float one[1] = {v};
-        activate<Y>(one, p.activation, p.leaky);
-        v = one[0];
-        if constexpr (sizeof(Y) == 1) {
-            const int64_t at = (image * p.channels + c) * p.pixels + q;
-            *y = (Y)q8(v, p.scales[p.nscales == 1 ? 0 : image], at < p.rne_limit);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            gamma[i] = p.gamma ? __ldg(p.gamma + t.c0 + c + i) : 1.0f;      // (a product with 1 and a sum with -0 change nothing)
+            beta[i] = p.beta ? __ldg(p.beta + t.c0 + c + i) : -0.0f;
+        }
+    }
+    __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c) const {
+        float v[VEC];
+        unpack<T, VEC>(q, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__fsub_rn(v[i], mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]), gamma[i]), beta[i]);
+        activate<Y>(v, p.activation, p.leaky);
+        Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + pixel * p.y_pixel + t.c0 + c;
+        if constexpr (sizeof(Y) > 1) {
+            if constexpr (VEC == 1) *y = from_f32<Y>(v[0]);
+            else *reinterpret_cast<uint4 *>(y) = Vec16<Y>::put(v);
         } else {
-            *y = from_f32<Y>(v);
+            const float scale = p.scales[p.nscales == 1 ? 0 : t.image];
+            int r[VEC];
+            if (p.nscales == 1 && !p.tail) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) r[i] = q8(v[i], scale, true);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) r[i] = q8(v[i], scale, ((int64_t)t.image * p.channels + t.c0 + c + i) * p.pixels + pixel < p.rne_limit);
+            }
+            if constexpr (VEC == 1) {
+                *y = (int8_t)r[0];
+            } else {
+                uint32_t w[VEC / 4];
+#pragma unroll
+                for (int i = 0; i < VEC / 4; ++i)
+                    w[i] = (uint32_t)(uint8_t)r[4 * i] | (uint32_t)(uint8_t)r[4 * i + 1] << 8 | (uint32_t)(uint8_t)r[4 * i + 2] << 16 | (uint32_t)(uint8_t)r[4 * i + 3] << 24;
+                if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(y) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t *>(y) = w[0];
+            }
         }
+    }
+};
+
+// The zeros behind the last channel of an int8 output
+template <typename Y>
+__device__ __forceinline__ void pad_channels(const GroupNormParams &p, const Part &t) {
+    if (sizeof(Y) > 1 || t.g0 + t.groups < p.groups) return;
+    const int extra = p.out_channels - p.channels;
+    for (int64_t i = threadIdx.x; i < (t.p1 - t.p0) * extra; i += kThreads)
+        static_cast<int8_t *>(p.y)[t.image * p.y_image + (t.p0 + i / extra) * p.y_pixel + p.channels + i % extra] = 0;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ double2 load_of_rank(const double2 *mine, uint32_t rank) {
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
+    double2 v;
+    asm volatile("ld.shared::cluster.v2.f64 {%0, %1}, [%2];" : "=d"(v.x), "=d"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
+// ---- resident: a cluster of p.tiles blocks holds a run of an image's groups
+template <typename T, typename Y, int VEC, bool ONE>
+__global__ void __launch_bounds__(kThreads)
+group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
+    using R = typename Raw<T, VEC>::type;
+    extern __shared__ __align__(16) uint8_t smem[];
+    double2 *group_sums = reinterpret_cast<double2 *>(smem);
+    double2 *scratch = group_sums + p.run_groups;
+    float2 *stats = reinterpret_cast<float2 *>(scratch + Sums<VEC, ONE>::kN * kThreads);
+    R *held = reinterpret_cast<R *>(stats + (p.run_groups + 1) / 2 * 2);
+    const int tile = blockIdx.x % p.tiles, unit = blockIdx.x / p.tiles;
+    const Part t = part_of(p, unit / p.runs, unit % p.runs, tile);
+    const int cols = t.width / VEC, rows = kThreads / cols, row = threadIdx.x / cols, col = threadIdx.x % cols;
+    for (int g = threadIdx.x; g < t.groups; g += kThreads) group_sums[g] = make_double2(0.0, 0.0);
+    pdl_sync();
+
+    Sums<VEC, ONE> sums;
+    sums.clear();
+    const int count = (int)(t.p1 - t.p0);
+    if (row < rows) {
+        const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + t.p0 * p.x_pixel + t.c0 + col * VEC;
+        constexpr int kAhead = 8;
+        for (int q0 = row; q0 < count; q0 += kAhead * rows) {
+            R q[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (q0 + i * rows < count) q[i] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + i * rows) * p.x_pixel);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (q0 + i * rows < count) {
+                    float v[VEC];
+                    unpack<T, VEC>(q[i], v);
+                    sums.add(v);
+                    held[(q0 + i * rows) * cols + col] = q[i];
+                }
+        }
+    }
+    __syncthreads();
+    collect<VEC, ONE>(sums, scratch, group_sums, 0, t.width, p.per, t.groups, rows, cols);
+    if (p.tiles > 1) {
+        cluster_arrive();
+        cluster_wait();
+    }
+    for (int g = threadIdx.x; g < t.groups; g += kThreads) {
+        double s = 0.0, ss = 0.0;
+        for (int r = 0; r < p.tiles; ++r) {
+            const double2 v = p.tiles > 1 ? load_of_rank(group_sums + g, r) : group_sums[g];
+            s += v.x;
+            ss += v.y;
+        }
+        stats[g] = statistics(p, s, ss);
+    }
+    if (p.tiles > 1) cluster_arrive();       // this block has read the others' sums (they stay until all have: the wait at the end)
+    __syncthreads();
+    if (row < rows) {
+        Apply<T, Y, VEC, ONE> apply;
+        apply.init(p, t, stats, col * VEC);
+#pragma unroll 2
+        for (int q = row; q < count; q += rows) apply.run(p, t, held[q * cols + col], t.p0 + q, col * VEC);
+    }
+    pad_channels<Y>(p, t);
+    if (p.tiles > 1) cluster_wait();
+}
+
+// ---- sweep: sums of images [sum0, sum1) and outputs of images [out0, out1), whose sums an earlier launch left
+// sums[image][run][tile][group of the run], stats[image][group], arrived[image][run]
+template <typename T, typename Y, int VEC, bool ONE>
+__global__ void __launch_bounds__(kThreads)
+group_norm_sweep_kernel(const __grid_constant__ GroupNormParams p, double2 *__restrict__ all_sums, float2 *all_stats, unsigned *arrived, int sum0, int sum1, int out0, int out1) {
+    using R = typename Raw<T, VEC>::type;
+    extern __shared__ __align__(16) uint8_t smem[];
+    double2 *group_sums = reinterpret_cast<double2 *>(smem);
+    double2 *scratch = group_sums + p.run_groups;
+    __shared__ unsigned before;
+    pdl_sync();
+    const int per_image = p.runs * p.tiles;
+    const int64_t to_sum = (int64_t)(sum1 - sum0) * per_image, to_write = (int64_t)(out1 - out0) * per_image, both = 2 * min(to_sum, to_write);
+    for (int64_t w = blockIdx.x; w < to_sum + to_write; w += gridDim.x) {
+        // sums and outputs by turns, as long as there are both
+        const bool summing = w < both ? w % 2 == 0 : to_sum > to_write;
+        const int64_t i = w < both ? w / 2 : w - both / 2;
+        const int image = (int)(i / per_image) + (summing ? sum0 : out0), run = (int)(i % per_image) / p.tiles, tile = (int)(i % p.tiles);
+        const Part t = part_of(p, image, run, tile);
+        const int count = (int)(t.p1 - t.p0);
+        const int block_width = p.cols * VEC, rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
+        const T *x0 = static_cast<const T *>(p.x) + t.image * p.x_image + t.p0 * p.x_pixel + t.c0;
+        if (summing) {
+            for (int g = threadIdx.x; g < t.groups; g += kThreads) group_sums[g] = make_double2(0.0, 0.0);
+            for (int b0 = 0; b0 < t.width; b0 += block_width) {
+                const int b1 = min(b0 + block_width, t.width), c = b0 + col * VEC;
+                Sums<VEC, ONE> sums;
+                sums.clear();
+                if (row < rows && c < b1) {
+                    const T *x = x0 + c;
+                    constexpr int kAhead = 8;
+                    for (int q0 = row; q0 < count; q0 += kAhead * rows) {
+                        R q[kAhead];
+#pragma unroll
+                        for (int j = 0; j < kAhead; ++j)
+                            if (q0 + j * rows < count) q[j] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + j * rows) * p.x_pixel);
+#pragma unroll
+                        for (int j = 0; j < kAhead; ++j)
+                            if (q0 + j * rows < count) {
+                                float v[VEC];
+                                unpack<T, VEC>(q[j], v);
+                                sums.add(v);
+                            }
+                    }
+                }
+                __syncthreads();
+                collect<VEC, ONE>(sums, scratch, group_sums, b0, b1, p.per, t.groups, rows, p.cols);
+            }
+            double2 *mine = all_sums + (((int64_t)image * p.runs + run) * p.tiles + tile) * p.run_groups;
+            for (int g = threadIdx.x; g < t.groups; g += kThreads) mine[g] = group_sums[g];
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) before = atomicInc(arrived + (int64_t)image * p.runs + run, p.tiles - 1);
+            __syncthreads();
+            if (before == (unsigned)p.tiles - 1) {
+                // the last of the run's tiles: adds up all of them, in their order
+                __threadfence();
+                const double2 *first = all_sums + ((int64_t)image * p.runs + run) * p.tiles * p.run_groups;
+                const int lane = threadIdx.x & 31;
+                for (int g = threadIdx.x >> 5; g < t.groups; g += kWarps) {
+                    double s = 0.0, ss = 0.0;
+                    for (int k = lane; k < p.tiles; k += 32) {
+                        const double2 v = __ldcg(first + (int64_t)k * p.run_groups + g);
+                        s += v.x;
+                        ss += v.y;
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) {
+                        s += __shfl_down_sync(0xffffffffu, s, o);
+                        ss += __shfl_down_sync(0xffffffffu, ss, o);
+                    }
+                    if (lane == 0) all_stats[(int64_t)image * p.groups + t.g0 + g] = statistics(p, s, ss);
+                }
+            }
+        } else {
+            const float2 *stats = all_stats + (int64_t)image * p.groups + t.g0;
+            for (int b0 = 0; b0 < t.width; b0 += block_width) {
+                const int b1 = min(b0 + block_width, t.width), c = b0 + col * VEC;
+                if (row >= rows || c >= b1) continue;
+                const T *x = x0 + c;
+                Apply<T, Y, VEC, ONE> apply;
+                apply.init(p, t, stats, c);
+                constexpr int kAhead = 4;
+                for (int q0 = row; q0 < count; q0 += kAhead * rows) {
+                    R q[kAhead];
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        if (q0 + j * rows < count) q[j] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + j * rows) * p.x_pixel);
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        if (q0 + j * rows < count) apply.run(p, t, q[j], t.p0 + q0 + j * rows, c);
+                }
+            }
+            pad_channels<Y>(p, t);
+        }
+        __syncthreads();
     }
 }
 
@@ -147,40 +396,123 @@ int check_desc(const tsb_group_norm_desc *d) {
     return TSB_OK;
 }
 
-// Parts that an image's pixels are summed in: some four blocks a multiprocessor over the whole batch, 64 values a thread or more.
-int choose_splits(const tsb_group_norm_desc *d) {
-    const int64_t by_work = ceil_div64(d->pixels * d->channels, 64 * kThreads), by_blocks = ceil_div64(148 * 4, d->n);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({by_work, by_blocks, d->pixels, kMaxSplits}));
+size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+// How a call runs: by 16-byte vectors or value by value, resident or swept, in which runs of channels and tiles of pixels.
+struct Plan {
+    int vec;
+    bool one, resident;
+    int run_groups, runs, cols, tiles;
+    int64_t tile;
+    size_t smem, off_stats, off_arrived, bytes;    // of shared memory; of the workspace
+};
+
+size_t scratch_bytes(int vec, bool one, int run_groups) { return (size_t)run_groups * 16 + (size_t)(one ? 1 : vec) * kThreads * 16 + (size_t)(run_groups + 1) / 2 * 16; }
+
+Plan make_plan(const tsb_group_norm_desc *d) {
+    const int size = (int)type_bytes(d->x_type), per = (int)(d->channels / d->groups), groups = (int)d->groups, vectors = 16 / size;
+    auto fits = [&](const void *at, int64_t pixel, int64_t image) {
+        return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (d->pixels == 1 || pixel * size % 16 == 0) && (d->n == 1 || image * size % 16 == 0);
+    };
+    Plan q = {};
+    const bool wide = d->channels % vectors == 0 && fits(d->x, d->x_pixel_stride, d->x_image_stride) &&
+                      (d->y_type == TSB_TYPE_I8 || fits(d->y, d->y_pixel_stride, d->y_image_stride));
+    q.vec = wide ? vectors : 1;
+    q.one = per % q.vec == 0;
+    // groups that make whole vectors
+    int step = 1;
+    while (step * per % q.vec) ++step;
+    // Resident: the widest run and the smallest cluster that give two blocks a multiprocessor; rows of 128 bytes or more (or all
+    // channels), tiles of 16 KB or more.  Otherwise whichever has most blocks.
+    int64_t best = 0;
+    for (int rg = (groups + step - 1) / step * step; rg >= step; rg = rg > step ? std::max(step, rg / 2 / step * step) : 0) {
+        const int run = std::min(rg, groups), width = run * per;
+        if (run > kMaxGroups || width / q.vec > kThreads) continue;
+        if (width * size < 128 && rg < groups && best) break;
+        const int runs = ceil_div(groups, run);
+        for (int s = 1; s <= kMaxCluster; s *= 2) {
+            const int64_t tile = ceil_div64(d->pixels, s), bytes = tile * width * size, blocks = d->n * runs * s;
+            if (bytes + (int64_t)scratch_bytes(q.vec, q.one, run) > kLargeTile) continue;
+            if (best && (bytes < 16 * 1024 || best >= 2 * 148)) break;
+            if (blocks < best || (blocks == best && s >= q.tiles) || blocks > INT32_MAX) continue;      // (of as many blocks the smaller cluster)
+            best = blocks;
+            q.resident = true;
+            q.run_groups = run; q.runs = runs; q.tiles = s; q.tile = tile; q.cols = width / q.vec;
+            q.smem = scratch_bytes(q.vec, q.one, run) + (size_t)bytes;
+        }
+    }
+    if (q.resident) return q;
+    // Swept: runs of as many channels as the block's threads own vectors, tiles of some 32 KB
+    q.run_groups = std::max(step, std::min({groups, kMaxGroups, kThreads * q.vec / per}) / step * step);
+    q.run_groups = std::min(q.run_groups, groups);
+    q.runs = ceil_div(groups, q.run_groups);
+    const int width = q.run_groups * per;
+    q.cols = std::min(width / q.vec, kThreads);
+    q.tile = std::max<int64_t>(1, 32768 / ((int64_t)width * size));
+    q.tile = std::max(q.tile, ceil_div64(d->pixels, 4096));      // (the last tile of an image adds up all tiles' sums)
+    q.tiles = (int)ceil_div64(d->pixels, q.tile);
+    q.smem = scratch_bytes(q.vec, q.one, q.run_groups);
+    q.off_stats = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
+    q.off_arrived = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));
+    q.bytes = q.off_arrived + align256((size_t)d->n * q.runs * sizeof(unsigned));
+    return q;
 }
 
-size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
-size_t sums_bytes(const tsb_group_norm_desc *d) { return align256((size_t)d->n * choose_splits(d) * d->groups * sizeof(double2)); }
+template <typename T, typename Y, int VEC, bool ONE>
+int launch(const GroupNormParams &p, const Plan &q, char *workspace, cudaStream_t stream) {
+    if (q.resident) {
+        auto kernel = group_norm_resident_kernel<T, Y, VEC, ONE>;
+        static DeviceOnce raised;
+        if (raised.first()) {
+            TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLargeTile));
+            raised.done();
+        }
+        TSB_CUDA(launch_pdl_cluster(p.tiles, kernel, dim3(p.n * p.runs * p.tiles), dim3(kThreads), q.smem, stream, p));
+        TSB_LAUNCHED("group_norm_resident_kernel");
+        return TSB_OK;
+    }
+    double2 *sums = reinterpret_cast<double2 *>(workspace);
+    float2 *stats = reinterpret_cast<float2 *>(workspace + q.off_stats);
+    unsigned *arrived = reinterpret_cast<unsigned *>(workspace + q.off_arrived);
+    auto kernel = group_norm_sweep_kernel<T, Y, VEC, ONE>;
+    static DeviceOnce raised;
+    if (raised.first()) {
+        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
+        raised.done();
+    }
+    TSB_CUDA(cudaMemsetAsync(arrived, 0, (size_t)p.n * p.runs * sizeof(unsigned), stream));
+    // images of a launch: some 32 MB, so that the next ones' values, these ones' and what is written fit the L2 together
+    const int64_t image_bytes = std::max<int64_t>(1, p.pixels * p.channels * (int64_t)sizeof(T));
+    const int batch = (int)std::max<int64_t>(1, std::min<int64_t>(p.n, (32 << 20) / image_bytes));
+    for (int j = 0; j < p.n + batch; j += batch) {
+        const int sum0 = std::min(j, p.n), sum1 = std::min(j + batch, p.n), out0 = std::max(0, j - batch), out1 = std::min(j, p.n);
+        const int64_t items = (int64_t)((sum1 - sum0) + (out1 - out0)) * p.runs * p.tiles;
+        TSB_CUDA(launch_pdl(kernel, dim3((int)std::min<int64_t>(items, 148 * 6)), dim3(kThreads), q.smem, stream, p, sums, stats, arrived, sum0, sum1, out0, out1));
+        TSB_LAUNCHED("group_norm_sweep_kernel");
+    }
+    return TSB_OK;
+}
 
 template <typename T, typename Y>
-int launch(const GroupNormParams &p, double2 *sums, float2 *stats, cudaStream_t stream) {
-    TSB_CUDA(launch_pdl(group_norm_sums_kernel<T>, dim3(p.n * p.splits), dim3(kThreads), 0, stream, p, sums));
-    TSB_LAUNCHED("group_norm_sums_kernel");
-    TSB_CUDA(launch_pdl(group_norm_stats_kernel, dim3((int)ceil_div64((int64_t)p.n * p.groups, kThreads)), dim3(kThreads), 0, stream, p, sums, stats));
-    TSB_LAUNCHED("group_norm_stats_kernel");
-    const int64_t values = (int64_t)p.n * p.pixels * p.out_channels;
-    TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y>, dim3((int)std::min<int64_t>(ceil_div64(values, kThreads), 148 * 64)), dim3(kThreads), 0, stream, p, stats));
-    TSB_LAUNCHED("group_norm_apply_kernel");
-    return TSB_OK;
+int pick(const GroupNormParams &p, const Plan &q, char *workspace, cudaStream_t stream) {
+    if (q.vec == 1) return launch<T, Y, 1, true>(p, q, workspace, stream);
+    return q.one ? launch<T, Y, Vec16<T>::kN, true>(p, q, workspace, stream) : launch<T, Y, Vec16<T>::kN, false>(p, q, workspace, stream);
 }
 
 }  // namespace
 
 size_t group_norm_workspace_bytes(const tsb_group_norm_desc *d) {
-    if (check_desc(d) != TSB_OK || d->n == 0 || d->pixels == 0) return 0;
-    return sums_bytes(d) + align256((size_t)d->n * d->groups * sizeof(float2));
+    return check_desc(d) != TSB_OK || d->n == 0 || d->pixels == 0 ? 0 : make_plan(d).bytes;
 }
 
 int group_norm_nhwc(const tsb_group_norm_desc *d, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
     int st = check_desc(d);
     if (st != TSB_OK || d->n == 0 || d->pixels == 0) return st;
-    const size_t need = group_norm_workspace_bytes(d);
-    if (!workspace || workspace_bytes < need) return fail(TSB_ERR_WORKSPACE_TOO_SMALL, "group_norm: %zu bytes of workspace, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
-    if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TSB_ERR_INVALID_ARGUMENT, "group_norm: the workspace must be 256-byte aligned");
+    const Plan q = make_plan(d);
+    if (q.bytes) {
+        if (!workspace || workspace_bytes < q.bytes) return fail(TSB_ERR_WORKSPACE_TOO_SMALL, "group_norm: %zu bytes of workspace, %zu needed", workspace ? workspace_bytes : (size_t)0, q.bytes);
+        if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TSB_ERR_INVALID_ARGUMENT, "group_norm: the workspace must be 256-byte aligned");
+    }
     const bool i8 = d->y_type == TSB_TYPE_I8;
     GroupNormParams p = {};
     p.x = d->x;
@@ -194,7 +526,11 @@ int group_norm_nhwc(const tsb_group_norm_desc *d, void *workspace, size_t worksp
     p.groups = (int)d->groups;
     p.per = p.channels / p.groups;
     p.pixels = d->pixels;
-    p.splits = choose_splits(d);
+    p.run_groups = q.run_groups;
+    p.runs = q.runs;
+    p.cols = q.cols;
+    p.tile = q.tile;
+    p.tiles = q.tiles;
     p.eps = d->eps;
     p.activation = d->activation;
     p.leaky = d->leaky_scale;
@@ -204,14 +540,14 @@ int group_norm_nhwc(const tsb_group_norm_desc *d, void *workspace, size_t worksp
     if (i8) {
         p.nscales = d->n_requant_scales;
         p.rne_limit = p.nscales == 1 ? d->n * d->pixels * d->channels / 8 * 8 : 0;
+        p.tail = p.nscales == 1 && p.rne_limit < d->n * d->pixels * d->channels;
         for (int i = 0; i < p.nscales; ++i) p.scales[i] = d->requant_scales_host[i];
     }
-    double2 *sums = static_cast<double2 *>(workspace);
-    float2 *stats = reinterpret_cast<float2 *>(static_cast<char *>(workspace) + sums_bytes(d));
+    char *room = static_cast<char *>(workspace);
     switch (d->x_type) {
-        case TSB_TYPE_F32: return i8 ? launch<float, int8_t>(p, sums, stats, stream) : launch<float, float>(p, sums, stats, stream);
-        case TSB_TYPE_F16: return i8 ? launch<__half, int8_t>(p, sums, stats, stream) : launch<__half, __half>(p, sums, stats, stream);
-        default: return i8 ? launch<__nv_bfloat16, int8_t>(p, sums, stats, stream) : launch<__nv_bfloat16, __nv_bfloat16>(p, sums, stats, stream);
+        case TSB_TYPE_F32: return i8 ? pick<float, int8_t>(p, q, room, stream) : pick<float, float>(p, q, room, stream);
+        case TSB_TYPE_F16: return i8 ? pick<__half, int8_t>(p, q, room, stream) : pick<__half, __half>(p, q, room, stream);
+        default: return i8 ? pick<__nv_bfloat16, int8_t>(p, q, room, stream) : pick<__nv_bfloat16, __nv_bfloat16>(p, q, room, stream);
     }
 }
 
