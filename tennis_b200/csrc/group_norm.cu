@@ -9,11 +9,13 @@
 //              neighbouring threads are neighbours, its channels' gamma, beta and statistics stay in registers
 //   resident   an image's run of groups is held in the shared memory of a cluster of up to eight blocks: loaded once, summed on the
 //              way, the blocks' sums exchanged through distributed shared memory, normalized from shared memory.  One launch
-//   sweep      larger images: a launch sums images j + 1 while it normalizes images j, which the L2 still holds
+//   swept      larger images: a launch sums as many as the L2 holds, the next one normalizes them
 #include "typed.cuh"
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <cstdio>
 
 namespace tsb {
 namespace {
@@ -21,6 +23,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // the portable limit
+constexpr int kFold = 32;                        // tiles that are added up together
 constexpr int kMaxGroups = 256;                 // groups of a run of channels
 constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
@@ -62,6 +65,13 @@ __device__ __forceinline__ Part part_of(const GroupNormParams &p, int image, int
     return t;
 }
 
+// q8_half_even without a conversion (of which a multiprocessor does 16 a clock, the norm's sums take one a value): a sum with 1.5 * 2^23
+// rounds to a whole number, half to even, that its low bits hold.
+__device__ __forceinline__ int round_even(float v) {
+    const float in = fminf(fmaxf(v, -128.0f), 127.0f);
+    return fabsf(v) < 2147483648.0f ? __float_as_int(__fadd_rn(in, 12582912.0f)) : -128;      // (the caller keeps the low byte)
+}
+
 // VEC values of a type, as they lie in memory
 template <typename T, int VEC> struct Raw { using type = uint4; };
 template <typename T> struct Raw<T, 1> { using type = T; };
@@ -71,32 +81,68 @@ __device__ __forceinline__ void unpack(const typename Raw<T, VEC>::type &q, floa
     else Vec16<T>::get(q, v);
 }
 
+// An fp32 value in 64 bits without the conversion instruction, of which a multiprocessor does few a clock: its exponent and fraction put
+// where fp64 has them read as the value times 2^-896 -- subnormals and zeros too, both formats lay them out alike -- and a product with
+// 2^896 is exact.  (Infinities and NaN come out as numbers: Sums keeps a mark of its own for them.)
+__device__ __forceinline__ double widen(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return __dmul_rn(__hiloint2double((int)(((uint32_t)((int)u >> 3)) & 0x8fffffffu), (int)(u << 29)), __hiloint2double(0x77f00000, 0));
+}
+
 // Sums of a thread's channels; ONE: all channels of a vector belong to one group, and one pair of sums serves them.
+// Every value and square goes into the 64-bit sums as it is.
 template <int VEC, bool ONE>
 struct Sums {
     static constexpr int kN = ONE ? 1 : VEC;
     double s[kN], ss[kN];
+    float mark[kN];             // NaN once an infinity or a NaN was added, else a zero
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) s[i] = ss[i] = 0.0;
-    }
-    __device__ __forceinline__ void add(const float (&v)[VEC]) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const double d = (double)v[i];
-            s[ONE ? 0 : i] += d;
-            ss[ONE ? 0 : i] = fma(d, d, ss[ONE ? 0 : i]);
+        for (int i = 0; i < kN; ++i) {
+            s[i] = ss[i] = 0.0;
+            mark[i] = 0.0f;
         }
     }
+    __device__ __forceinline__ void add(const float (&v)[VEC]) {
+        double d[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            d[i] = widen(v[i]);
+            mark[ONE ? 0 : i] = fmaf(v[i], 0.0f, mark[ONE ? 0 : i]);
+        }
+        if constexpr (ONE && VEC > 1) {
+            // (two chains each, and sums of pairs: an addition takes longer than to issue the eight)
+            double a = d[0] + d[1], b = d[2] + d[3], e = d[0] * d[0], f = d[1] * d[1];
+#pragma unroll
+            for (int i = 4; i < VEC; i += 4) {
+                a += d[i] + d[i + 1];
+                b += d[i + 2] + d[i + 3];
+            }
+#pragma unroll
+            for (int i = 2; i < VEC; i += 2) {
+                e = fma(d[i], d[i], e);
+                f = fma(d[i + 1], d[i + 1], f);
+            }
+            s[0] += a + b;
+            ss[0] += e + f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                s[i] += d[i];
+                ss[i] = fma(d[i], d[i], ss[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ double2 pair(int i) const { return make_double2(s[i] + (double)mark[i], ss[i]); }
 };
 
 // Adds the threads' sums of channels [b0, b1) of the run to the groups' sums in shared memory, in a fixed order: a warp takes a group,
 // its lanes the group's entries in turn.  Thread (row, col) of `rows` x `cols` owns vector b0 / VEC + col.
 template <int VEC, bool ONE>
 __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scratch, double2 *group_sums, int b0, int b1, int per, int groups, int rows, int cols) {
-    constexpr int kN = Sums<VEC, ONE>::kN, kStep = VEC / kN;     // entries of a vector, channels of an entry
+    constexpr int kN = ONE ? 1 : VEC, kStep = VEC / kN;     // entries of a vector, channels of an entry
 #pragma unroll
-    for (int i = 0; i < kN; ++i) scratch[i * kThreads + threadIdx.x] = make_double2(sums.s[i], sums.ss[i]);
+    for (int i = 0; i < kN; ++i) scratch[i * kThreads + threadIdx.x] = sums.pair(i);
     __syncthreads();
     const int lane = threadIdx.x & 31;
     for (int g = b0 / per + (threadIdx.x >> 5); g < groups && g * per < b1; g += kWarps) {
@@ -122,6 +168,36 @@ __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scr
     __syncthreads();
 }
 
+// A thread's pixels row, row + rows, ... of a tile of `count`: into `sums`, and to seen(pixel, values) as they lie in memory.
+template <typename T, int VEC, bool ONE, typename Seen>
+__device__ __forceinline__ void sums_of_pixels(const GroupNormParams &p, const Part &t, int c, int row, int rows, int count, Sums<VEC, ONE> &sums, const Seen &seen) {
+    using R = typename Raw<T, VEC>::type;
+    const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c;
+    const int64_t step = rows * p.x_pixel;
+    constexpr int kAhead = 8;
+    int q = row;
+    auto take = [&](int pixel, const R &raw) {
+        float v[VEC];
+        unpack<T, VEC>(raw, v);
+        sums.add(v);
+        seen(pixel, raw);
+    };
+    for (; q + (kAhead - 1) * rows < count; q += kAhead * rows) {
+        R held[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i, x += step) held[i] = *reinterpret_cast<const R *>(x);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) take(q + i * rows, held[i]);
+    }
+    R held[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i, x += step)
+        if (q + i * rows < count) held[i] = *reinterpret_cast<const R *>(x);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (q + i * rows < count) take(q + i * rows, held[i]);
+}
+
 // {mean, 1 / sqrt(variance + eps)} of a group, each rounded once
 __device__ __forceinline__ float2 statistics(const GroupNormParams &p, double s, double ss) {
     const double count = (double)p.pixels * p.per;
@@ -131,32 +207,36 @@ __device__ __forceinline__ float2 statistics(const GroupNormParams &p, double s,
     return make_float2((float)mean, (float)(1.0 / sqrt(var + p.eps)));
 }
 
-// What a thread applies to its channels: statistics, gamma, beta, activation, rounding.
+// What a thread applies to its channels: statistics, gamma, beta, activation, rounding.  Results of 16 bits, whose half step is 2^13
+// times that of fp32 or more, take gamma into the reciprocal deviation and the product and the sum with beta as one operation.
 template <typename T, typename Y, int VEC, bool ONE>
 struct Apply {
+    static constexpr bool kShort = sizeof(Y) == 2;
     static constexpr int kG = ONE ? 1 : VEC;
-    float mean[kG], rstd[kG], gamma[VEC], beta[VEC];
+    float mean[kG], rstd[kShort ? 1 : kG], gamma[VEC], beta[VEC];
     // c: the thread's first channel within the run
     __device__ __forceinline__ void init(const GroupNormParams &p, const Part &t, const float2 *stats, int c) {
 #pragma unroll
-        for (int i = 0; i < kG; ++i) {
-            const float2 st = stats[(c + i) / p.per];
-            mean[i] = st.x;
-            rstd[i] = st.y;
-        }
-#pragma unroll
         for (int i = 0; i < VEC; ++i) {
+            const float2 st = stats[(c + (ONE ? 0 : i)) / p.per];
+            if (i < kG) mean[i] = st.x;
             gamma[i] = p.gamma ? __ldg(p.gamma + t.c0 + c + i) : 1.0f;      // (a product with 1 and a sum with -0 change nothing)
             beta[i] = p.beta ? __ldg(p.beta + t.c0 + c + i) : -0.0f;
+            if (kShort) gamma[i] = __fmul_rn(st.y, gamma[i]);
+            else if (i < kG) rstd[i] = st.y;
         }
     }
-    __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c) const {
+    // y: where the thread's channels of `pixel` go
+    template <int ACT>
+    __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c, Y *y) const {
         float v[VEC];
         unpack<T, VEC>(q, v);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__fsub_rn(v[i], mean[ONE ? 0 : i]), rstd[ONE ? 0 : i]), gamma[i]), beta[i]);
-        activate<Y>(v, p.activation, p.leaky);
-        Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + pixel * p.y_pixel + t.c0 + c;
+        for (int i = 0; i < VEC; ++i) {
+            const float d = __fsub_rn(v[i], mean[ONE ? 0 : i]);
+            v[i] = kShort ? fmaf(d, gamma[i], beta[i]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[ONE || kShort ? 0 : i]), gamma[i]), beta[i]);
+        }
+        activate<ACT, Y>(v, p.leaky);
         if constexpr (sizeof(Y) > 1) {
             if constexpr (VEC == 1) *y = from_f32<Y>(v[0]);
             else *reinterpret_cast<uint4 *>(y) = Vec16<Y>::put(v);
@@ -165,7 +245,7 @@ struct Apply {
             int r[VEC];
             if (p.nscales == 1 && !p.tail) {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) r[i] = q8(v[i], scale, true);
+                for (int i = 0; i < VEC; ++i) r[i] = round_even(__fmul_rn(v[i], scale));
             } else {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) r[i] = q8(v[i], scale, ((int64_t)t.image * p.channels + t.c0 + c + i) * p.pixels + pixel < p.rne_limit);
@@ -205,13 +285,13 @@ __device__ __forceinline__ double2 load_of_rank(const double2 *mine, uint32_t ra
 
 // ---- resident: a cluster of p.tiles blocks holds a run of an image's groups
 template <typename T, typename Y, int VEC, bool ONE>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 3)
 group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
     double2 *group_sums = reinterpret_cast<double2 *>(smem);
     double2 *scratch = group_sums + p.run_groups;
-    float2 *stats = reinterpret_cast<float2 *>(scratch + Sums<VEC, ONE>::kN * kThreads);
+    float2 *stats = reinterpret_cast<float2 *>(scratch + (ONE ? 1 : VEC) * kThreads);
     R *held = reinterpret_cast<R *>(stats + (p.run_groups + 1) / 2 * 2);
     const int tile = blockIdx.x % p.tiles, unit = blockIdx.x / p.tiles;
     const Part t = part_of(p, unit / p.runs, unit % p.runs, tile);
@@ -222,26 +302,9 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     Sums<VEC, ONE> sums;
     sums.clear();
     const int count = (int)(t.p1 - t.p0);
-    if (row < rows) {
-        const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + t.p0 * p.x_pixel + t.c0 + col * VEC;
-        constexpr int kAhead = 8;
-        for (int q0 = row; q0 < count; q0 += kAhead * rows) {
-            R q[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                if (q0 + i * rows < count) q[i] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + i * rows) * p.x_pixel);
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i)
-                if (q0 + i * rows < count) {
-                    float v[VEC];
-                    unpack<T, VEC>(q[i], v);
-                    sums.add(v);
-                    held[(q0 + i * rows) * cols + col] = q[i];
-                }
-        }
-    }
+    if (row < rows) sums_of_pixels<T, VEC, ONE>(p, t, col * VEC, row, rows, count, sums, [&](int pixel, const R &raw) { held[pixel * cols + col] = raw; });
     __syncthreads();
-    collect<VEC, ONE>(sums, scratch, group_sums, 0, t.width, p.per, t.groups, rows, cols);
+    collect(sums, scratch, group_sums, 0, t.width, p.per, t.groups, rows, cols);
     if (p.tiles > 1) {
         cluster_arrive();
         cluster_wait();
@@ -260,110 +323,115 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     if (row < rows) {
         Apply<T, Y, VEC, ONE> apply;
         apply.init(p, t, stats, col * VEC);
-#pragma unroll 2
-        for (int q = row; q < count; q += rows) apply.run(p, t, held[q * cols + col], t.p0 + q, col * VEC);
+        Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + (t.p0 + row) * p.y_pixel + t.c0 + col * VEC;
+        const R *from = held + row * cols + col;
+        by_activation(p.activation, [&](auto act) {
+#pragma unroll 4
+            for (int q = row; q < count; q += rows, from += rows * cols, y += rows * p.y_pixel)
+                apply.template run<decltype(act)::value>(p, t, *from, t.p0 + q, col * VEC, y);
+        });
     }
     pad_channels<Y>(p, t);
     if (p.tiles > 1) cluster_wait();
 }
 
-// ---- sweep: sums of images [sum0, sum1) and outputs of images [out0, out1), whose sums an earlier launch left
-// sums[image][run][tile][group of the run], stats[image][group], arrived[image][run]
-template <typename T, typename Y, int VEC, bool ONE>
-__global__ void __launch_bounds__(kThreads)
-group_norm_sweep_kernel(const __grid_constant__ GroupNormParams p, double2 *__restrict__ all_sums, float2 *all_stats, unsigned *arrived, int sum0, int sum1, int out0, int out1) {
+// Whether this block is the last of `count` to come here, with what they wrote before in sight.
+__device__ __forceinline__ bool last_of(unsigned *arrived, int count, unsigned *before) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) *before = atomicInc(arrived, count - 1);
+    __syncthreads();
+    const bool last = *before == (unsigned)count - 1;
+    __threadfence();
+    return last;
+}
+// Sums of `count` (at most 32) tiles' group sums: a warp takes a group, a lane a tile.
+template <typename Put>
+__device__ __forceinline__ void add_up(const double2 *first, int count, int pitch, int groups, const Put &put) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 4
+    for (int g = threadIdx.x >> 5; g < groups; g += kWarps) {
+        double2 v = lane < count ? __ldcg(first + (int64_t)lane * pitch + g) : make_double2(0.0, 0.0);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            v.x += __shfl_down_sync(0xffffffffu, v.x, o);
+            v.y += __shfl_down_sync(0xffffffffu, v.y, o);
+        }
+        if (lane == 0) put(g, v.x, v.y);
+    }
+}
+
+// ---- swept: the sums of images [image0, ...), a block a tile
+// all_sums[image][run][tile][group of the run], fold_sums[image][run][tile / kFold][group of the run], all_stats[image][group],
+// arrived[image][run][1 + kFold]
+template <typename T, int VEC, bool ONE>
+__global__ void __launch_bounds__(kThreads, 4)
+group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, double2 *all_sums, double2 *fold_sums, float2 *all_stats, unsigned *arrived) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
     double2 *group_sums = reinterpret_cast<double2 *>(smem);
     double2 *scratch = group_sums + p.run_groups;
     __shared__ unsigned before;
+    const int tile = blockIdx.x % p.tiles, unit0 = blockIdx.x / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
+    const Part t = part_of(p, image, run, tile);
+    const int count = (int)(t.p1 - t.p0);
+    const int rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
+    for (int g = threadIdx.x; g < t.groups; g += kThreads) group_sums[g] = make_double2(0.0, 0.0);
     pdl_sync();
-    const int per_image = p.runs * p.tiles;
-    const int64_t to_sum = (int64_t)(sum1 - sum0) * per_image, to_write = (int64_t)(out1 - out0) * per_image, both = 2 * min(to_sum, to_write);
-    for (int64_t w = blockIdx.x; w < to_sum + to_write; w += gridDim.x) {
-        // sums and outputs by turns, as long as there are both
-        const bool summing = w < both ? w % 2 == 0 : to_sum > to_write;
-        const int64_t i = w < both ? w / 2 : w - both / 2;
-        const int image = (int)(i / per_image) + (summing ? sum0 : out0), run = (int)(i % per_image) / p.tiles, tile = (int)(i % p.tiles);
-        const Part t = part_of(p, image, run, tile);
-        const int count = (int)(t.p1 - t.p0);
-        const int block_width = p.cols * VEC, rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
-        const T *x0 = static_cast<const T *>(p.x) + t.image * p.x_image + t.p0 * p.x_pixel + t.c0;
-        if (summing) {
-            for (int g = threadIdx.x; g < t.groups; g += kThreads) group_sums[g] = make_double2(0.0, 0.0);
-            for (int b0 = 0; b0 < t.width; b0 += block_width) {
-                const int b1 = min(b0 + block_width, t.width), c = b0 + col * VEC;
-                Sums<VEC, ONE> sums;
-                sums.clear();
-                if (row < rows && c < b1) {
-                    const T *x = x0 + c;
-                    constexpr int kAhead = 8;
-                    for (int q0 = row; q0 < count; q0 += kAhead * rows) {
-                        R q[kAhead];
-#pragma unroll
-                        for (int j = 0; j < kAhead; ++j)
-                            if (q0 + j * rows < count) q[j] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + j * rows) * p.x_pixel);
-#pragma unroll
-                        for (int j = 0; j < kAhead; ++j)
-                            if (q0 + j * rows < count) {
-                                float v[VEC];
-                                unpack<T, VEC>(q[j], v);
-                                sums.add(v);
-                            }
-                    }
-                }
-                __syncthreads();
-                collect<VEC, ONE>(sums, scratch, group_sums, b0, b1, p.per, t.groups, rows, p.cols);
-            }
-            double2 *mine = all_sums + (((int64_t)image * p.runs + run) * p.tiles + tile) * p.run_groups;
-            for (int g = threadIdx.x; g < t.groups; g += kThreads) mine[g] = group_sums[g];
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) before = atomicInc(arrived + (int64_t)image * p.runs + run, p.tiles - 1);
-            __syncthreads();
-            if (before == (unsigned)p.tiles - 1) {
-                // the last of the run's tiles: adds up all of them, in their order
-                __threadfence();
-                const double2 *first = all_sums + ((int64_t)image * p.runs + run) * p.tiles * p.run_groups;
-                const int lane = threadIdx.x & 31;
-                for (int g = threadIdx.x >> 5; g < t.groups; g += kWarps) {
-                    double s = 0.0, ss = 0.0;
-                    for (int k = lane; k < p.tiles; k += 32) {
-                        const double2 v = __ldcg(first + (int64_t)k * p.run_groups + g);
-                        s += v.x;
-                        ss += v.y;
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        s += __shfl_down_sync(0xffffffffu, s, o);
-                        ss += __shfl_down_sync(0xffffffffu, ss, o);
-                    }
-                    if (lane == 0) all_stats[(int64_t)image * p.groups + t.g0 + g] = statistics(p, s, ss);
-                }
-            }
-        } else {
-            const float2 *stats = all_stats + (int64_t)image * p.groups + t.g0;
-            for (int b0 = 0; b0 < t.width; b0 += block_width) {
-                const int b1 = min(b0 + block_width, t.width), c = b0 + col * VEC;
-                if (row >= rows || c >= b1) continue;
-                const T *x = x0 + c;
-                Apply<T, Y, VEC, ONE> apply;
-                apply.init(p, t, stats, c);
-                constexpr int kAhead = 4;
-                for (int q0 = row; q0 < count; q0 += kAhead * rows) {
-                    R q[kAhead];
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j)
-                        if (q0 + j * rows < count) q[j] = *reinterpret_cast<const R *>(x + (int64_t)(q0 + j * rows) * p.x_pixel);
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j)
-                        if (q0 + j * rows < count) apply.run(p, t, q[j], t.p0 + q0 + j * rows, c);
-                }
-            }
-            pad_channels<Y>(p, t);
-        }
+    for (int b0 = 0; b0 < t.width; b0 += p.cols * VEC) {
+        const int b1 = min(b0 + p.cols * VEC, t.width), c = b0 + col * VEC;
+        Sums<VEC, ONE> sums;
+        sums.clear();
+        if (row < rows && c < b1) sums_of_pixels<T, VEC, ONE>(p, t, c, row, rows, count, sums, [](int, const R &) {});
         __syncthreads();
+        collect(sums, scratch, group_sums, b0, b1, p.per, t.groups, rows, p.cols);
     }
+    // The last of every kFold neighbouring tiles to arrive adds up theirs, the last of those their sums: each time in the order of the
+    // tiles, so no order of arrival shows.
+    const int64_t unit = (int64_t)image * p.runs + run;
+    const int folds = (p.tiles + kFold - 1) / kFold, fold = tile / kFold, in_fold = min(kFold, p.tiles - fold * kFold);
+    double2 *mine = all_sums + (unit * p.tiles + tile) * p.run_groups, *folded = fold_sums + unit * folds * p.run_groups;
+    for (int g = threadIdx.x; g < t.groups; g += kThreads) mine[g] = group_sums[g];
+    if (!last_of(arrived + unit * (kFold + 1) + 1 + fold, in_fold, &before)) return;
+    add_up(all_sums + (unit * p.tiles + fold * kFold) * p.run_groups, in_fold, p.run_groups, t.groups,
+           [&](int g, double s, double ss) { folded[fold * p.run_groups + g] = make_double2(s, ss); });
+    if (!last_of(arrived + unit * (kFold + 1), folds, &before)) return;
+    add_up(folded, folds, p.run_groups, t.groups, [&](int g, double s, double ss) { all_stats[(int64_t)image * p.groups + t.g0 + g] = statistics(p, s, ss); });
+}
+
+// ---- swept: the outputs, last tile first (what the sums read last is in the L2 for certain)
+template <typename T, typename Y, int VEC, bool ONE>
+__global__ void __launch_bounds__(kThreads, 4)
+group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, int image0, const float2 *__restrict__ all_stats) {
+    using R = typename Raw<T, VEC>::type;
+    const int item = gridDim.x - 1 - blockIdx.x, tile = item % p.tiles, unit0 = item / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
+    const Part t = part_of(p, image, run, tile);
+    const int count = (int)(t.p1 - t.p0);
+    const int rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
+    pdl_sync();
+    const float2 *stats = all_stats + (int64_t)image * p.groups + t.g0;
+    for (int c = col * VEC; c < t.width; c += p.cols * VEC) {
+        if (row >= rows) break;
+        Apply<T, Y, VEC, ONE> apply;
+        apply.init(p, t, stats, c);
+        const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c;
+        Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + (t.p0 + row) * p.y_pixel + t.c0 + c;
+        const int64_t x_step = rows * p.x_pixel, y_step = rows * p.y_pixel;
+        by_activation(p.activation, [&](auto act) {
+            constexpr int kAhead = VEC == 1 ? 8 : 4;
+            int q = row;
+            for (; q + (kAhead - 1) * rows < count; q += kAhead * rows) {
+                R held[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j, x += x_step) held[j] = *reinterpret_cast<const R *>(x);
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j, y += y_step) apply.template run<decltype(act)::value>(p, t, held[j], t.p0 + q + j * rows, c, y);
+            }
+            for (; q < count; q += rows, x += x_step, y += y_step)
+                apply.template run<decltype(act)::value>(p, t, *reinterpret_cast<const R *>(x), t.p0 + q, c, y);
+        });
+    }
+    pad_channels<Y>(p, t);
 }
 
 int check_desc(const tsb_group_norm_desc *d) {
@@ -403,8 +471,9 @@ struct Plan {
     int vec;
     bool one, resident;
     int run_groups, runs, cols, tiles;
+    int batch;                                     // images of a pair of launches
     int64_t tile;
-    size_t smem, off_stats, off_arrived, bytes;    // of shared memory; of the workspace
+    size_t smem, off_folds, off_stats, off_arrived, bytes;    // of shared memory; of the workspace
 };
 
 size_t scratch_bytes(int vec, bool one, int run_groups) { return (size_t)run_groups * 16 + (size_t)(one ? 1 : vec) * kThreads * 16 + (size_t)(run_groups + 1) / 2 * 16; }
@@ -415,6 +484,8 @@ Plan make_plan(const tsb_group_norm_desc *d) {
         return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (d->pixels == 1 || pixel * size % 16 == 0) && (d->n == 1 || image * size % 16 == 0);
     };
     Plan q = {};
+    const char *force = getenv("GN");
+    int f_run = 0, f_s = 0; if (force) sscanf(force, "%d,%d", &f_run, &f_s);
     const bool wide = d->channels % vectors == 0 && fits(d->x, d->x_pixel_stride, d->x_image_stride) &&
                       (d->y_type == TSB_TYPE_I8 || fits(d->y, d->y_pixel_stride, d->y_image_stride));
     q.vec = wide ? vectors : 1;
@@ -427,10 +498,12 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     int64_t best = 0;
     for (int rg = (groups + step - 1) / step * step; rg >= step; rg = rg > step ? std::max(step, rg / 2 / step * step) : 0) {
         const int run = std::min(rg, groups), width = run * per;
+        if (f_run && run != f_run) continue;
         if (run > kMaxGroups || width / q.vec > kThreads) continue;
-        if (width * size < 128 && rg < groups && best) break;
+        if (width * size < (best ? 128 : 64) && run < groups) break;
         const int runs = ceil_div(groups, run);
         for (int s = 1; s <= kMaxCluster; s *= 2) {
+            if (f_s && s != f_s) continue;
             const int64_t tile = ceil_div64(d->pixels, s), bytes = tile * width * size, blocks = d->n * runs * s;
             if (bytes + (int64_t)scratch_bytes(q.vec, q.one, run) > kLargeTile) continue;
             if (best && (bytes < 16 * 1024 || best >= 2 * 148)) break;
@@ -448,13 +521,16 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     q.runs = ceil_div(groups, q.run_groups);
     const int width = q.run_groups * per;
     q.cols = std::min(width / q.vec, kThreads);
-    q.tile = std::max<int64_t>(1, 32768 / ((int64_t)width * size));
-    q.tile = std::max(q.tile, ceil_div64(d->pixels, 4096));      // (the last tile of an image adds up all tiles' sums)
+    const int64_t image_bytes = std::max<int64_t>(1, d->pixels * d->channels * size);
+    q.batch = (int)std::max<int64_t>(1, std::min<int64_t>(d->n, (48 << 20) / image_bytes));
+    const int64_t blocks = std::max<int64_t>(1, 148 * 4 / ((int64_t)q.batch * q.runs));
+    q.tile = std::max(ceil_div64(d->pixels, std::min<int64_t>(blocks, kFold * kFold)), std::max<int64_t>(1, 16384 / ((int64_t)width * size)));
     q.tiles = (int)ceil_div64(d->pixels, q.tile);
     q.smem = scratch_bytes(q.vec, q.one, q.run_groups);
-    q.off_stats = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
+    q.off_folds = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
+    q.off_stats = q.off_folds + align256((size_t)d->n * q.runs * ceil_div(q.tiles, kFold) * q.run_groups * sizeof(double2));
     q.off_arrived = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));
-    q.bytes = q.off_arrived + align256((size_t)d->n * q.runs * sizeof(unsigned));
+    q.bytes = q.off_arrived + align256((size_t)d->n * q.runs * (kFold + 1) * sizeof(unsigned));
     return q;
 }
 
@@ -472,23 +548,16 @@ int launch(const GroupNormParams &p, const Plan &q, char *workspace, cudaStream_
         return TSB_OK;
     }
     double2 *sums = reinterpret_cast<double2 *>(workspace);
+    double2 *folds = reinterpret_cast<double2 *>(workspace + q.off_folds);
     float2 *stats = reinterpret_cast<float2 *>(workspace + q.off_stats);
     unsigned *arrived = reinterpret_cast<unsigned *>(workspace + q.off_arrived);
-    auto kernel = group_norm_sweep_kernel<T, Y, VEC, ONE>;
-    static DeviceOnce raised;
-    if (raised.first()) {
-        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024));
-        raised.done();
-    }
-    TSB_CUDA(cudaMemsetAsync(arrived, 0, (size_t)p.n * p.runs * sizeof(unsigned), stream));
-    // images of a launch: some 32 MB, so that the next ones' values, these ones' and what is written fit the L2 together
-    const int64_t image_bytes = std::max<int64_t>(1, p.pixels * p.channels * (int64_t)sizeof(T));
-    const int batch = (int)std::max<int64_t>(1, std::min<int64_t>(p.n, (32 << 20) / image_bytes));
-    for (int j = 0; j < p.n + batch; j += batch) {
-        const int sum0 = std::min(j, p.n), sum1 = std::min(j + batch, p.n), out0 = std::max(0, j - batch), out1 = std::min(j, p.n);
-        const int64_t items = (int64_t)((sum1 - sum0) + (out1 - out0)) * p.runs * p.tiles;
-        TSB_CUDA(launch_pdl(kernel, dim3((int)std::min<int64_t>(items, 148 * 6)), dim3(kThreads), q.smem, stream, p, sums, stats, arrived, sum0, sum1, out0, out1));
-        TSB_LAUNCHED("group_norm_sweep_kernel");
+    TSB_CUDA(cudaMemsetAsync(arrived, 0, (size_t)p.n * p.runs * (kFold + 1) * sizeof(unsigned), stream));
+    for (int i = 0; i < p.n; i += q.batch) {
+        const dim3 grid((unsigned)(std::min(q.batch, p.n - i) * p.runs * p.tiles));
+        TSB_CUDA(launch_pdl(group_norm_sums_kernel<T, VEC, ONE>, grid, dim3(kThreads), q.smem, stream, p, i, sums, folds, stats, arrived));
+        TSB_LAUNCHED("group_norm_sums_kernel");
+        TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y, VEC, ONE>, grid, dim3(kThreads), 0, stream, p, i, stats));
+        TSB_LAUNCHED("group_norm_apply_kernel");
     }
     return TSB_OK;
 }

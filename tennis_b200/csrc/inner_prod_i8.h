@@ -32,7 +32,7 @@ __device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, cons
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
     }
-    activate<T>(v, p.activation, p.leaky);
+    by_activation(p.activation, [&](auto act) { activate<decltype(act)::value, T>(v, p.leaky); });
     if (p.residual && p.residual_after) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));

@@ -133,23 +133,28 @@ __device__ __forceinline__ float gelu(float v) {
     return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));
 }
 
-// The activation of N values that become results of type T (relu and leaky_relu are the operators' own: a NaN gives 0 and NaN).  One
-// branch for all of them: with the choice made value by value, the unrolled code of all five did not fit the instruction cache.
-template <typename T, int N>
-__device__ __forceinline__ void activate(float (&v)[N], int activation, float leaky) {
-    if (activation == TSB_ACT_NONE) return;
-    if (activation == TSB_ACT_RELU) {
+// The activation of N values that become results of type T (relu and leaky_relu are the operators' own: a NaN gives 0 and NaN).
+template <int ACT, typename T, int N>
+__device__ __forceinline__ void activate(float (&v)[N], float leaky) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
-    } else if (activation == TSB_ACT_LEAKY_RELU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? v[i] : __fmul_rn(v[i], leaky);
-    } else if (activation == TSB_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = silu<sizeof(T) == 2>(v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = gelu(v[i]);
+    for (int i = 0; i < N; ++i) {
+        if (ACT == TSB_ACT_RELU) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
+        if (ACT == TSB_ACT_LEAKY_RELU) v[i] = v[i] > 0.0f ? v[i] : __fmul_rn(v[i], leaky);
+        if (ACT == TSB_ACT_SILU) v[i] = silu<sizeof(T) == 2>(v[i]);
+        if (ACT == TSB_ACT_GELU) v[i] = gelu(v[i]);
+    }
+}
+// body(a constant of the activation's number): one branch for all values of a loop.  (With the choice made value by value, the unrolled
+// code of all five did not fit the instruction cache.)
+template <int ACT> struct Activation { static constexpr int value = ACT; };
+template <typename Body>
+__device__ __forceinline__ void by_activation(int activation, const Body &body) {
+    switch (activation) {
+        case TSB_ACT_NONE: body(Activation<TSB_ACT_NONE>()); break;
+        case TSB_ACT_RELU: body(Activation<TSB_ACT_RELU>()); break;
+        case TSB_ACT_LEAKY_RELU: body(Activation<TSB_ACT_LEAKY_RELU>()); break;
+        case TSB_ACT_SILU: body(Activation<TSB_ACT_SILU>()); break;
+        default: body(Activation<TSB_ACT_GELU>());
     }
 }
 
