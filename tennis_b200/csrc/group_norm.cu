@@ -23,7 +23,6 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // the portable limit
-constexpr int kFold = 32;                        // tiles that are added up together
 constexpr int kMaxGroups = 256;                 // groups of a run of channels
 constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
@@ -81,35 +80,20 @@ __device__ __forceinline__ void unpack(const typename Raw<T, VEC>::type &q, floa
     else Vec16<T>::get(q, v);
 }
 
-// An fp32 value in 64 bits without the conversion instruction, of which a multiprocessor does few a clock: its exponent and fraction put
-// where fp64 has them read as the value times 2^-896 -- subnormals and zeros too, both formats lay them out alike -- and a product with
-// 2^896 is exact.  (Infinities and NaN come out as numbers: Sums keeps a mark of its own for them.)
-__device__ __forceinline__ double widen(float v) {
-    const uint32_t u = __float_as_uint(v);
-    return __dmul_rn(__hiloint2double((int)(((uint32_t)((int)u >> 3)) & 0x8fffffffu), (int)(u << 29)), __hiloint2double(0x77f00000, 0));
-}
-
 // Sums of a thread's channels; ONE: all channels of a vector belong to one group, and one pair of sums serves them.
 // Every value and square goes into the 64-bit sums as it is.
 template <int VEC, bool ONE>
 struct Sums {
     static constexpr int kN = ONE ? 1 : VEC;
     double s[kN], ss[kN];
-    float mark[kN];             // NaN once an infinity or a NaN was added, else a zero
     __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            s[i] = ss[i] = 0.0;
-            mark[i] = 0.0f;
-        }
+        for (int i = 0; i < kN; ++i) s[i] = ss[i] = 0.0;
     }
     __device__ __forceinline__ void add(const float (&v)[VEC]) {
         double d[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            d[i] = widen(v[i]);
-            mark[ONE ? 0 : i] = fmaf(v[i], 0.0f, mark[ONE ? 0 : i]);
-        }
+        for (int i = 0; i < VEC; ++i) d[i] = (double)v[i];
         if constexpr (ONE && VEC > 1) {
             // (two chains each, and sums of pairs: an addition takes longer than to issue the eight)
             double a = d[0] + d[1], b = d[2] + d[3], e = d[0] * d[0], f = d[1] * d[1];
@@ -133,34 +117,38 @@ struct Sums {
             }
         }
     }
-    __device__ __forceinline__ double2 pair(int i) const { return make_double2(s[i] + (double)mark[i], ss[i]); }
 };
 
-// Adds the threads' sums of channels [b0, b1) of the run to the groups' sums in shared memory, in a fixed order: a warp takes a group,
-// its lanes the group's entries in turn.  Thread (row, col) of `rows` x `cols` owns vector b0 / VEC + col.
+// Adds the threads' sums of channels [b0, b1) of the run to the groups' sums in shared memory, in a fixed order: a few lanes take a
+// group, each its entries of some rows.  Thread (row, col) of `rows` x `cols` owns vector b0 / VEC + col.
 template <int VEC, bool ONE>
 __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scratch, double2 *group_sums, int b0, int b1, int per, int groups, int rows, int cols) {
     constexpr int kN = ONE ? 1 : VEC, kStep = VEC / kN;     // entries of a vector, channels of an entry
 #pragma unroll
-    for (int i = 0; i < kN; ++i) scratch[i * kThreads + threadIdx.x] = sums.pair(i);
+    for (int i = 0; i < kN; ++i) scratch[i * kThreads + threadIdx.x] = make_double2(sums.s[i], sums.ss[i]);
     __syncthreads();
-    const int lane = threadIdx.x & 31;
-    for (int g = b0 / per + (threadIdx.x >> 5); g < groups && g * per < b1; g += kWarps) {
-        const int a = max(g * per, b0) - b0, b = min((g + 1) * per, b1) - b0;      // the group's channels within the block of columns
-        const int entries = (b - a) / kStep, first = a / kStep;
+    // as many lanes a group (a power of two) as give every thread one
+    const int g0 = b0 / per, g1 = min(groups, (b1 + per - 1) / per);
+    const int lanes = g1 - g0 >= kThreads ? 1 : min(32, 1 << (31 - __clz(kThreads / (g1 - g0)))), lane = threadIdx.x & (lanes - 1);
+    for (int first_g = g0; first_g < g1; first_g += kThreads / lanes) {       // (all threads: shuffles)
+        const int g = first_g + threadIdx.x / lanes;
         double s = 0.0, ss = 0.0;
-        for (int e = lane; e < entries * rows; e += 32) {
-            const int row = e / entries, entry = first + e - row * entries;
-            const double2 t = scratch[(kN == 1 ? 0 : entry % kN) * kThreads + row * cols + entry / kN];
-            s += t.x;
-            ss += t.y;
+        if (g < g1) {
+            const int a = (max(g * per, b0) - b0) / kStep, b = (min((g + 1) * per, b1) - b0) / kStep;      // the group's entries of a row
+            for (int entry = a; entry < b; ++entry) {
+                const double2 *from = scratch + (kN == 1 ? 0 : entry % kN) * kThreads + entry / kN;
+                for (int row = lane; row < rows; row += lanes) {
+                    const double2 t = from[row * cols];
+                    s += t.x;
+                    ss += t.y;
+                }
+            }
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            s += __shfl_down_sync(0xffffffffu, s, o);
-            ss += __shfl_down_sync(0xffffffffu, ss, o);
+        for (int o = lanes / 2; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
-        if (lane == 0) {
+        if (g < g1 && lane == 0) {
             group_sums[g].x += s;
             group_sums[g].y += ss;
         }
@@ -168,34 +156,54 @@ __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scr
     __syncthreads();
 }
 
-// A thread's pixels row, row + rows, ... of a tile of `count`: into `sums`, and to seen(pixel, values) as they lie in memory.
-template <typename T, int VEC, bool ONE, typename Seen>
-__device__ __forceinline__ void sums_of_pixels(const GroupNormParams &p, const Part &t, int c, int row, int rows, int count, Sums<VEC, ONE> &sums, const Seen &seen) {
-    using R = typename Raw<T, VEC>::type;
-    const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c;
-    const int64_t step = rows * p.x_pixel;
-    constexpr int kAhead = 8;
-    int q = row;
-    auto take = [&](int pixel, const R &raw) {
-        float v[VEC];
-        unpack<T, VEC>(raw, v);
-        sums.add(v);
-        seen(pixel, raw);
-    };
-    for (; q + (kAhead - 1) * rows < count; q += kAhead * rows) {
-        R held[kAhead];
+// ---- a thread's vectors of a tile, one every `step` elements from x on, in turn to use(i, vector)
+// By asynchronous copies into slots of the thread's own, kDepth ahead of their use: a thread reads back what it loaded itself, so
+// neither registers nor barriers hold loads up.  slot: its first slot, in shared memory; slot_step: bytes to the next one; KEEP: every
+// vector has a slot of its own and stays there, otherwise the kDepth slots go round.
+constexpr int kDepth = 8;
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ uint4 read16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+template <typename T, int VEC, bool KEEP, typename Use>
+__device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t slot, uint32_t slot_step, const Use &use) {
+    if constexpr (VEC > 1) {
+        constexpr int kAhead = KEEP ? 4 * kDepth : kDepth;
+        const T *next = x;
+        uint32_t to = slot, at = slot;
+        const uint32_t end = slot + kAhead * slot_step;
+#pragma unroll 4
+        for (int i = 0; i < kAhead; ++i, next += step, to += slot_step) {
+            if (i < n) copy16(to, next);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        if (!KEEP) to = slot;
+#pragma unroll 2
+        for (int i = 0; i < n; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+            use(i, read16(at));
+            if (i + kAhead < n) copy16(to, next);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            next += step;
+            to += slot_step;
+            at += slot_step;
+            if (!KEEP && at == end) to = at = slot;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+        constexpr int kAhead = 8;
+        for (int i0 = 0; i0 < n; i0 += kAhead, x += kAhead * step) {
+            T v[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i, x += step) held[i] = *reinterpret_cast<const R *>(x);
+            for (int i = 0; i < kAhead; ++i)
+                if (i0 + i < n) v[i] = x[i * step];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) take(q + i * rows, held[i]);
+            for (int i = 0; i < kAhead; ++i)
+                if (i0 + i < n) use(i0 + i, v[i]);
+        }
     }
-    R held[kAhead];
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i, x += step)
-        if (q + i * rows < count) held[i] = *reinterpret_cast<const R *>(x);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-        if (q + i * rows < count) take(q + i * rows, held[i]);
 }
 
 // {mean, 1 / sqrt(variance + eps)} of a group, each rounded once
@@ -231,10 +239,20 @@ struct Apply {
     __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c, Y *y) const {
         float v[VEC];
         unpack<T, VEC>(q, v);
+        if constexpr (kShort && VEC > 1) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const float d = __fsub_rn(v[i], mean[ONE ? 0 : i]);
-            v[i] = kShort ? fmaf(d, gamma[i], beta[i]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[ONE || kShort ? 0 : i]), gamma[i]), beta[i]);
+            for (int i = 0; i < VEC; i += 2) {
+                const float2 d = add2(make_float2(v[i], v[i + 1]), make_float2(-mean[ONE ? 0 : i], -mean[ONE ? 0 : i + 1]));
+                const float2 r = fma2(d, make_float2(gamma[i], gamma[i + 1]), make_float2(beta[i], beta[i + 1]));
+                v[i] = r.x;
+                v[i + 1] = r.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float d = __fsub_rn(v[i], mean[ONE ? 0 : i]);
+                v[i] = kShort ? fmaf(d, gamma[i], beta[i]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[ONE || kShort ? 0 : i]), gamma[i]), beta[i]);
+            }
         }
         activate<ACT, Y>(v, p.leaky);
         if constexpr (sizeof(Y) > 1) {
@@ -302,7 +320,15 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     Sums<VEC, ONE> sums;
     sums.clear();
     const int count = (int)(t.p1 - t.p0);
-    if (row < rows) sums_of_pixels<T, VEC, ONE>(p, t, col * VEC, row, rows, count, sums, [&](int pixel, const R &raw) { held[pixel * cols + col] = raw; });
+    const int mine = row < rows && row < count ? (count - row + rows - 1) / rows : 0;      // this thread's pixels: row, row + rows, ...
+    R *slots = held + row * cols + col;
+    stream<T, VEC, true>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + col * VEC, rows * p.x_pixel, mine,
+                         (uint32_t)__cvta_generic_to_shared(slots), rows * cols * sizeof(R), [&](int i, const R &raw) {
+                             float v[VEC];
+                             unpack<T, VEC>(raw, v);
+                             sums.add(v);
+                             if (VEC == 1) slots[i * rows * cols] = raw;
+                         });
     __syncthreads();
     collect(sums, scratch, group_sums, 0, t.width, p.per, t.groups, rows, cols);
     if (p.tiles > 1) {
@@ -320,58 +346,29 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     }
     if (p.tiles > 1) cluster_arrive();       // this block has read the others' sums (they stay until all have: the wait at the end)
     __syncthreads();
-    if (row < rows) {
+    if (mine > 0) {
         Apply<T, Y, VEC, ONE> apply;
         apply.init(p, t, stats, col * VEC);
         Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + (t.p0 + row) * p.y_pixel + t.c0 + col * VEC;
-        const R *from = held + row * cols + col;
+        const R *from = slots;
         by_activation(p.activation, [&](auto act) {
 #pragma unroll 4
-            for (int q = row; q < count; q += rows, from += rows * cols, y += rows * p.y_pixel)
-                apply.template run<decltype(act)::value>(p, t, *from, t.p0 + q, col * VEC, y);
+            for (int i = 0; i < mine; ++i, from += rows * cols, y += rows * p.y_pixel)
+                apply.template run<decltype(act)::value>(p, t, *from, t.p0 + row + i * rows, col * VEC, y);
         });
     }
     pad_channels<Y>(p, t);
     if (p.tiles > 1) cluster_wait();
 }
 
-// Whether this block is the last of `count` to come here, with what they wrote before in sight.
-__device__ __forceinline__ bool last_of(unsigned *arrived, int count, unsigned *before) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) *before = atomicInc(arrived, count - 1);
-    __syncthreads();
-    const bool last = *before == (unsigned)count - 1;
-    __threadfence();
-    return last;
-}
-// Sums of `count` (at most 32) tiles' group sums: a warp takes a group, a lane a tile.
-template <typename Put>
-__device__ __forceinline__ void add_up(const double2 *first, int count, int pitch, int groups, const Put &put) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll 4
-    for (int g = threadIdx.x >> 5; g < groups; g += kWarps) {
-        double2 v = lane < count ? __ldcg(first + (int64_t)lane * pitch + g) : make_double2(0.0, 0.0);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            v.x += __shfl_down_sync(0xffffffffu, v.x, o);
-            v.y += __shfl_down_sync(0xffffffffu, v.y, o);
-        }
-        if (lane == 0) put(g, v.x, v.y);
-    }
-}
-
-// ---- swept: the sums of images [image0, ...), a block a tile
-// all_sums[image][run][tile][group of the run], fold_sums[image][run][tile / kFold][group of the run], all_stats[image][group],
-// arrived[image][run][1 + kFold]
+// ---- swept: the sums of images [image0, ...), a block a tile, to sums[image][run][tile][group of the run]
 template <typename T, int VEC, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4)
-group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, double2 *all_sums, double2 *fold_sums, float2 *all_stats, unsigned *arrived) {
+group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, double2 *all_sums) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
     double2 *group_sums = reinterpret_cast<double2 *>(smem);
     double2 *scratch = group_sums + p.run_groups;
-    __shared__ unsigned before;
     const int tile = blockIdx.x % p.tiles, unit0 = blockIdx.x / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
     const Part t = part_of(p, image, run, tile);
     const int count = (int)(t.p1 - t.p0);
@@ -382,28 +379,51 @@ group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, do
         const int b1 = min(b0 + p.cols * VEC, t.width), c = b0 + col * VEC;
         Sums<VEC, ONE> sums;
         sums.clear();
-        if (row < rows && c < b1) sums_of_pixels<T, VEC, ONE>(p, t, c, row, rows, count, sums, [](int, const R &) {});
+        if (row < rows && row < count && c < b1)
+            stream<T, VEC, false>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c, rows * p.x_pixel, (count - row + rows - 1) / rows,
+                                  (uint32_t)__cvta_generic_to_shared(scratch) + threadIdx.x * 16, kThreads * 16, [&](int, const R &raw) {
+                                      float v[VEC];
+                                      unpack<T, VEC>(raw, v);
+                                      sums.add(v);
+                                  });
         __syncthreads();
         collect(sums, scratch, group_sums, b0, b1, p.per, t.groups, rows, p.cols);
     }
-    // The last of every kFold neighbouring tiles to arrive adds up theirs, the last of those their sums: each time in the order of the
-    // tiles, so no order of arrival shows.
-    const int64_t unit = (int64_t)image * p.runs + run;
-    const int folds = (p.tiles + kFold - 1) / kFold, fold = tile / kFold, in_fold = min(kFold, p.tiles - fold * kFold);
-    double2 *mine = all_sums + (unit * p.tiles + tile) * p.run_groups, *folded = fold_sums + unit * folds * p.run_groups;
+    double2 *mine = all_sums + (((int64_t)image * p.runs + run) * p.tiles + tile) * p.run_groups;
     for (int g = threadIdx.x; g < t.groups; g += kThreads) mine[g] = group_sums[g];
-    if (!last_of(arrived + unit * (kFold + 1) + 1 + fold, in_fold, &before)) return;
-    add_up(all_sums + (unit * p.tiles + fold * kFold) * p.run_groups, in_fold, p.run_groups, t.groups,
-           [&](int g, double s, double ss) { folded[fold * p.run_groups + g] = make_double2(s, ss); });
-    if (!last_of(arrived + unit * (kFold + 1), folds, &before)) return;
-    add_up(folded, folds, p.run_groups, t.groups, [&](int g, double s, double ss) { all_stats[(int64_t)image * p.groups + t.g0 + g] = statistics(p, s, ss); });
+}
+
+// ---- swept: the statistics of the groups from `first` on, a warp a group; its tiles' sums in a fixed order
+__global__ void __launch_bounds__(kThreads)
+group_norm_stats_kernel(const __grid_constant__ GroupNormParams p, int64_t first, int64_t end, const double2 *all_sums, float2 *all_stats) {
+    pdl_sync();
+    const int lane = threadIdx.x & 31;
+    const int64_t i = first + (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (i >= end) return;
+    const int64_t image = i / p.groups;
+    const int group = (int)(i - image * p.groups), run = group / p.run_groups;
+    const double2 *from = all_sums + (image * p.runs + run) * p.tiles * p.run_groups + (group - run * p.run_groups);
+    double s = 0.0, ss = 0.0;
+#pragma unroll 4
+    for (int k = lane; k < p.tiles; k += 32) {
+        const double2 v = from[(int64_t)k * p.run_groups];
+        s += v.x;
+        ss += v.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    }
+    if (lane == 0) all_stats[i] = statistics(p, s, ss);
 }
 
 // ---- swept: the outputs, last tile first (what the sums read last is in the L2 for certain)
 template <typename T, typename Y, int VEC, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4)
-group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, int image0, const float2 *__restrict__ all_stats) {
+group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, int image0, const float2 *all_stats) {
     using R = typename Raw<T, VEC>::type;
+    extern __shared__ __align__(16) uint8_t smem[];
     const int item = gridDim.x - 1 - blockIdx.x, tile = item % p.tiles, unit0 = item / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
     const Part t = part_of(p, image, run, tile);
     const int count = (int)(t.p1 - t.p0);
@@ -411,24 +431,16 @@ group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, int image0, c
     pdl_sync();
     const float2 *stats = all_stats + (int64_t)image * p.groups + t.g0;
     for (int c = col * VEC; c < t.width; c += p.cols * VEC) {
-        if (row >= rows) break;
+        if (row >= rows || row >= count) break;
         Apply<T, Y, VEC, ONE> apply;
         apply.init(p, t, stats, c);
-        const T *x = static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c;
         Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + (t.p0 + row) * p.y_pixel + t.c0 + c;
-        const int64_t x_step = rows * p.x_pixel, y_step = rows * p.y_pixel;
         by_activation(p.activation, [&](auto act) {
-            constexpr int kAhead = VEC == 1 ? 8 : 4;
-            int q = row;
-            for (; q + (kAhead - 1) * rows < count; q += kAhead * rows) {
-                R held[kAhead];
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j, x += x_step) held[j] = *reinterpret_cast<const R *>(x);
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j, y += y_step) apply.template run<decltype(act)::value>(p, t, held[j], t.p0 + q + j * rows, c, y);
-            }
-            for (; q < count; q += rows, x += x_step, y += y_step)
-                apply.template run<decltype(act)::value>(p, t, *reinterpret_cast<const R *>(x), t.p0 + q, c, y);
+            stream<T, VEC, false>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c, rows * p.x_pixel, (count - row + rows - 1) / rows,
+                                  (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16, kThreads * 16, [&](int i, const R &raw) {
+                                      apply.template run<decltype(act)::value>(p, t, raw, t.p0 + row + i * rows, c, y);
+                                      y += rows * p.y_pixel;
+                                  });
         });
     }
     pad_channels<Y>(p, t);
@@ -473,7 +485,7 @@ struct Plan {
     int run_groups, runs, cols, tiles;
     int batch;                                     // images of a pair of launches
     int64_t tile;
-    size_t smem, off_folds, off_stats, off_arrived, bytes;    // of shared memory; of the workspace
+    size_t smem, off_stats, bytes;    // of shared memory; of the workspace
 };
 
 size_t scratch_bytes(int vec, bool one, int run_groups) { return (size_t)run_groups * 16 + (size_t)(one ? 1 : vec) * kThreads * 16 + (size_t)(run_groups + 1) / 2 * 16; }
@@ -522,15 +534,13 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     const int width = q.run_groups * per;
     q.cols = std::min(width / q.vec, kThreads);
     const int64_t image_bytes = std::max<int64_t>(1, d->pixels * d->channels * size);
-    q.batch = (int)std::max<int64_t>(1, std::min<int64_t>(d->n, (48 << 20) / image_bytes));
-    const int64_t blocks = std::max<int64_t>(1, 148 * 4 / ((int64_t)q.batch * q.runs));
-    q.tile = std::max(ceil_div64(d->pixels, std::min<int64_t>(blocks, kFold * kFold)), std::max<int64_t>(1, 16384 / ((int64_t)width * size)));
+    q.batch = (int)std::max<int64_t>(1, std::min<int64_t>(d->n, ((getenv("GNB") ? atoll(getenv("GNB")) : 48) << 20) / image_bytes));
+    const int64_t blocks = std::max<int64_t>(1, 148 * (getenv("GNT") ? atoi(getenv("GNT")) : 4) / ((int64_t)q.batch * q.runs));
+    q.tile = std::max(ceil_div64(d->pixels, blocks), std::max<int64_t>(1, 16384 / ((int64_t)width * size)));
     q.tiles = (int)ceil_div64(d->pixels, q.tile);
-    q.smem = scratch_bytes(q.vec, q.one, q.run_groups);
-    q.off_folds = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
-    q.off_stats = q.off_folds + align256((size_t)d->n * q.runs * ceil_div(q.tiles, kFold) * q.run_groups * sizeof(double2));
-    q.off_arrived = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));
-    q.bytes = q.off_arrived + align256((size_t)d->n * q.runs * (kFold + 1) * sizeof(unsigned));
+    q.smem = (size_t)q.run_groups * 16 + (size_t)kDepth * kThreads * 16;      // (at least collect's scratch: a vector has at most eight pairs of sums)
+    q.off_stats = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
+    q.bytes = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));
     return q;
 }
 
@@ -548,15 +558,16 @@ int launch(const GroupNormParams &p, const Plan &q, char *workspace, cudaStream_
         return TSB_OK;
     }
     double2 *sums = reinterpret_cast<double2 *>(workspace);
-    double2 *folds = reinterpret_cast<double2 *>(workspace + q.off_folds);
     float2 *stats = reinterpret_cast<float2 *>(workspace + q.off_stats);
-    unsigned *arrived = reinterpret_cast<unsigned *>(workspace + q.off_arrived);
-    TSB_CUDA(cudaMemsetAsync(arrived, 0, (size_t)p.n * p.runs * (kFold + 1) * sizeof(unsigned), stream));
     for (int i = 0; i < p.n; i += q.batch) {
-        const dim3 grid((unsigned)(std::min(q.batch, p.n - i) * p.runs * p.tiles));
-        TSB_CUDA(launch_pdl(group_norm_sums_kernel<T, VEC, ONE>, grid, dim3(kThreads), q.smem, stream, p, i, sums, folds, stats, arrived));
+        const int images = std::min(q.batch, p.n - i);
+        const dim3 grid((unsigned)(images * p.runs * p.tiles));
+        const int64_t first = (int64_t)i * p.groups, end = first + (int64_t)images * p.groups;
+        TSB_CUDA(launch_pdl(group_norm_sums_kernel<T, VEC, ONE>, grid, dim3(kThreads), q.smem, stream, p, i, sums));
         TSB_LAUNCHED("group_norm_sums_kernel");
-        TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y, VEC, ONE>, grid, dim3(kThreads), 0, stream, p, i, stats));
+        TSB_CUDA(launch_pdl(group_norm_stats_kernel, dim3((unsigned)ceil_div64(end - first, kWarps)), dim3(kThreads), 0, stream, p, first, end, sums, stats));
+        TSB_LAUNCHED("group_norm_stats_kernel");
+        TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y, VEC, ONE>, grid, dim3(kThreads), (size_t)kDepth * kThreads * 16, stream, p, i, stats));
         TSB_LAUNCHED("group_norm_apply_kernel");
     }
     return TSB_OK;

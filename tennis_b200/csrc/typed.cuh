@@ -109,25 +109,54 @@ __device__ __forceinline__ void quantize16(const RowScale &q, const uint4 &from,
         to[i] = (uint32_t)(uint8_t)q(v[4 * i]) | (uint32_t)(uint8_t)q(v[4 * i + 1]) << 8 | (uint32_t)(uint8_t)q(v[4 * i + 2]) << 16 | (uint32_t)(uint8_t)q(v[4 * i + 3]) << 24;
 }
 
-// silu, v / (1 + exp(-v)), by the hardware's exp2 and reciprocal (relative errors of 2^-22 and 2^-23).
-// For fp32 results the rounding error of -v log2(e), which exp2 would turn into a relative error of |v| 2^-24, is computed by a fused
-// multiply-add and put back to first order: 8 half steps of the result in all.  Results of 16 bits, whose half step is 2^13 times that
-// of fp32 or more, go without.  (expf and a division take some 40 instructions a value: 25 M values of a product with 64 terms each took 126 us.)
-template <bool NARROW>
-__device__ __forceinline__ float silu(float v) {
+// ---- two fp32 values in one instruction (each half is rounded by itself)
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float exp2_approx(float t) {
     float e;
-    if (NARROW) {
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(v, -1.44269504f)));
-    } else {
-        const float c = fminf(fmaxf(v, -200.0f), 200.0f);        // (exp2 is infinite or 0 at either end)
-        const float t = __fmul_rn(c, -1.44269502f);
-        const float r = fmaf(c, -1.92596303e-8f, fmaf(c, -1.44269502f, -t));   // log2(e) = 1.44269502 (fp32) + 1.92596303e-8
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-        e = __fmul_rn(e, fmaf(r, 0.693147182f, 1.0f));
-    }
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    return e;
+}
+__device__ __forceinline__ float reciprocal_approx(float v) {
     float q;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(__fadd_rn(1.0f, e)));
-    return __fmul_rn(v, q);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(v));
+    return q;
+}
+
+// silu, v / (1 + exp(-v)), by the hardware's exp2 and reciprocal (relative errors of 2^-22 and 2^-23).  For fp32 results the rounding
+// error of -v log2(e), which exp2 would turn into a relative error of |v| 2^-24, is computed by a fused multiply-add and put back
+// to first order: 8 half steps of the result in all.  (expf and a division take some 40 instructions a value.)
+__device__ __forceinline__ float silu(float v) {
+    const float c = fminf(fmaxf(v, -200.0f), 200.0f);        // (exp2 is infinite or 0 at either end)
+    const float t = __fmul_rn(c, -1.44269502f);
+    const float r = fmaf(c, -1.92596303e-8f, fmaf(c, -1.44269502f, -t));   // log2(e) = 1.44269502 (fp32) + 1.92596303e-8
+    return __fmul_rn(v, reciprocal_approx(__fadd_rn(1.0f, __fmul_rn(exp2_approx(t), fmaf(r, 0.693147182f, 1.0f)))));
+}
+// Two values that become results of 16 bits, whose half step is 2^13 times that of fp32 or more: without that correction, and with one
+// reciprocal for both (a multiprocessor does 16 of these functions a clock, and eight times as many products): 1 / a = b (1 / ab).
+// exp2's argument is kept below 63, so that ab stays a number: below v = -43.7 the result is v 2^-63.
+__device__ __forceinline__ float2 silu_short(float2 v) {
+    const float2 t = mul2(v, make_float2(-1.44269504f, -1.44269504f));
+    const float2 a = add2(make_float2(exp2_approx(fminf(t.x, 63.0f)), exp2_approx(fminf(t.y, 63.0f))), make_float2(1.0f, 1.0f));
+    const float r = reciprocal_approx(__fmul_rn(a.x, a.y));
+    return mul2(v, mul2(make_float2(a.y, a.x), make_float2(r, r)));
 }
 __device__ __forceinline__ float gelu(float v) {
     return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));
@@ -136,11 +165,20 @@ __device__ __forceinline__ float gelu(float v) {
 // The activation of N values that become results of type T (relu and leaky_relu are the operators' own: a NaN gives 0 and NaN).
 template <int ACT, typename T, int N>
 __device__ __forceinline__ void activate(float (&v)[N], float leaky) {
+    if constexpr (ACT == TSB_ACT_SILU && sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 y = silu_short(make_float2(v[i], i + 1 < N ? v[i + (i + 1 < N)] : 0.0f));
+            v[i] = y.x;
+            if (i + 1 < N) v[i + (i + 1 < N)] = y.y;
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (ACT == TSB_ACT_RELU) v[i] = v[i] > 0.0f ? v[i] : 0.0f;
         if (ACT == TSB_ACT_LEAKY_RELU) v[i] = v[i] > 0.0f ? v[i] : __fmul_rn(v[i], leaky);
-        if (ACT == TSB_ACT_SILU) v[i] = silu<sizeof(T) == 2>(v[i]);
+        if (ACT == TSB_ACT_SILU) v[i] = silu(v[i]);
         if (ACT == TSB_ACT_GELU) v[i] = gelu(v[i]);
     }
 }
