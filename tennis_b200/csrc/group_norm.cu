@@ -9,13 +9,14 @@
 //              neighbouring threads are neighbours, its channels' gamma, beta and statistics stay in registers
 //   resident   an image's run of groups is held in the shared memory of a cluster of up to eight blocks: loaded once, summed on the
 //              way, the blocks' sums exchanged through distributed shared memory, normalized from shared memory.  One launch
-//   swept      larger images: a launch sums as many as the L2 holds, the next one normalizes them
+//   swept      larger images: one launch sums, a small one makes the statistics, the third reads again and normalizes, in the reverse
+//              order, so that it finds in the L2 what the first read last.  (Batch by batch, each small enough for the L2, the
+//              launches' beginnings and ends cost more than the reads of HBM that they save: 8 x 256 x 256 x 256 bf16 152 us in one
+//              batch, 176 in batches of two images, 266 image by image)
 #include "typed.cuh"
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
-#include <cstdio>
 
 namespace tsb {
 namespace {
@@ -24,6 +25,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // the portable limit
 constexpr int kMaxGroups = 256;                 // groups of a run of channels
+constexpr int kResidentBlocks = 3;               // resident blocks a multiprocessor, by their registers
 constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
 struct GroupNormParams {
@@ -37,7 +39,7 @@ struct GroupNormParams {
     int cols;                                     // vectors of a run that the block's threads own at a time
     int64_t tile;                                 // pixels of a block's tile
     int tiles;                                    // ... and tiles of an image
-    double eps;
+    double eps, one_over_count;                   // of a group's values: a product with it is off by half a step of 64 bits more than a quotient
     int activation;
     float leaky;
     int out_channels;                             // channels written: int8 outputs are padded with zeros
@@ -208,9 +210,8 @@ __device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t
 
 // {mean, 1 / sqrt(variance + eps)} of a group, each rounded once
 __device__ __forceinline__ float2 statistics(const GroupNormParams &p, double s, double ss) {
-    const double count = (double)p.pixels * p.per;
-    const double mean = s / count;
-    const double raw = fma(-mean, mean, ss / count);
+    const double mean = s * p.one_over_count;
+    const double raw = fma(-mean, mean, ss * p.one_over_count);
     const double var = raw < 0.0 ? 0.0 : raw;            // (a NaN stays one)
     return make_float2((float)mean, (float)(1.0 / sqrt(var + p.eps)));
 }
@@ -303,7 +304,7 @@ __device__ __forceinline__ double2 load_of_rank(const double2 *mine, uint32_t ra
 
 // ---- resident: a cluster of p.tiles blocks holds a run of an image's groups
 template <typename T, typename Y, int VEC, bool ONE>
-__global__ void __launch_bounds__(kThreads, 3)
+__global__ void __launch_bounds__(kThreads, kResidentBlocks)
 group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -336,13 +337,17 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
         cluster_wait();
     }
     for (int g = threadIdx.x; g < t.groups; g += kThreads) {
-        double s = 0.0, ss = 0.0;
-        for (int r = 0; r < p.tiles; ++r) {
-            const double2 v = p.tiles > 1 ? load_of_rank(group_sums + g, r) : group_sums[g];
-            s += v.x;
-            ss += v.y;
-        }
-        stats[g] = statistics(p, s, ss);
+        double2 v[kMaxCluster];
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r) v[r] = r >= p.tiles ? make_double2(0.0, 0.0) : p.tiles > 1 ? load_of_rank(group_sums + g, r) : group_sums[g];
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o *= 2)
+#pragma unroll
+            for (int r = 0; r + o < kMaxCluster; r += 2 * o) {
+                v[r].x += v[r + o].x;
+                v[r].y += v[r + o].y;
+            }
+        stats[g] = statistics(p, v[0].x, v[0].y);
     }
     if (p.tiles > 1) cluster_arrive();       // this block has read the others' sums (they stay until all have: the wait at the end)
     __syncthreads();
@@ -361,15 +366,15 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     if (p.tiles > 1) cluster_wait();
 }
 
-// ---- swept: the sums of images [image0, ...), a block a tile, to sums[image][run][tile][group of the run]
+// ---- swept: the sums, a block a tile, to sums[image][run][tile][group of the run]
 template <typename T, int VEC, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4)
-group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, double2 *all_sums) {
+group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, double2 *all_sums) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
     double2 *group_sums = reinterpret_cast<double2 *>(smem);
     double2 *scratch = group_sums + p.run_groups;
-    const int tile = blockIdx.x % p.tiles, unit0 = blockIdx.x / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
+    const int tile = blockIdx.x % p.tiles, unit0 = blockIdx.x / p.tiles, run = unit0 % p.runs, image = unit0 / p.runs;
     const Part t = part_of(p, image, run, tile);
     const int count = (int)(t.p1 - t.p0);
     const int rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
@@ -393,13 +398,13 @@ group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, int image0, do
     for (int g = threadIdx.x; g < t.groups; g += kThreads) mine[g] = group_sums[g];
 }
 
-// ---- swept: the statistics of the groups from `first` on, a warp a group; its tiles' sums in a fixed order
+// ---- swept: the statistics, a warp a group; its tiles' sums in a fixed order
 __global__ void __launch_bounds__(kThreads)
-group_norm_stats_kernel(const __grid_constant__ GroupNormParams p, int64_t first, int64_t end, const double2 *all_sums, float2 *all_stats) {
+group_norm_stats_kernel(const __grid_constant__ GroupNormParams p, const double2 *all_sums, float2 *all_stats) {
     pdl_sync();
     const int lane = threadIdx.x & 31;
-    const int64_t i = first + (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (i >= end) return;
+    const int64_t i = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (i >= (int64_t)p.n * p.groups) return;
     const int64_t image = i / p.groups;
     const int group = (int)(i - image * p.groups), run = group / p.run_groups;
     const double2 *from = all_sums + (image * p.runs + run) * p.tiles * p.run_groups + (group - run * p.run_groups);
@@ -421,10 +426,10 @@ group_norm_stats_kernel(const __grid_constant__ GroupNormParams p, int64_t first
 // ---- swept: the outputs, last tile first (what the sums read last is in the L2 for certain)
 template <typename T, typename Y, int VEC, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4)
-group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, int image0, const float2 *all_stats) {
+group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, const float2 *all_stats) {
     using R = typename Raw<T, VEC>::type;
     extern __shared__ __align__(16) uint8_t smem[];
-    const int item = gridDim.x - 1 - blockIdx.x, tile = item % p.tiles, unit0 = item / p.tiles, run = unit0 % p.runs, image = image0 + unit0 / p.runs;
+    const int item = gridDim.x - 1 - blockIdx.x, tile = item % p.tiles, unit0 = item / p.tiles, run = unit0 % p.runs, image = unit0 / p.runs;
     const Part t = part_of(p, image, run, tile);
     const int count = (int)(t.p1 - t.p0);
     const int rows = kThreads / p.cols, row = threadIdx.x / p.cols, col = threadIdx.x % p.cols;
@@ -483,7 +488,6 @@ struct Plan {
     int vec;
     bool one, resident;
     int run_groups, runs, cols, tiles;
-    int batch;                                     // images of a pair of launches
     int64_t tile;
     size_t smem, off_stats, bytes;    // of shared memory; of the workspace
 };
@@ -496,8 +500,6 @@ Plan make_plan(const tsb_group_norm_desc *d) {
         return reinterpret_cast<uintptr_t>(at) % 16 == 0 && (d->pixels == 1 || pixel * size % 16 == 0) && (d->n == 1 || image * size % 16 == 0);
     };
     Plan q = {};
-    const char *force = getenv("GN");
-    int f_run = 0, f_s = 0; if (force) sscanf(force, "%d,%d", &f_run, &f_s);
     const bool wide = d->channels % vectors == 0 && fits(d->x, d->x_pixel_stride, d->x_image_stride) &&
                       (d->y_type == TSB_TYPE_I8 || fits(d->y, d->y_pixel_stride, d->y_image_stride));
     q.vec = wide ? vectors : 1;
@@ -505,37 +507,37 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     // groups that make whole vectors
     int step = 1;
     while (step * per % q.vec) ++step;
-    // Resident: the widest run and the smallest cluster that give two blocks a multiprocessor; rows of 128 bytes or more (or all
-    // channels), tiles of 16 KB or more.  Otherwise whichever has most blocks.
+    // Resident: as many blocks as run at the same time (a second round of them waits for the first to be through all of its steps:
+    // 16 x 56 x 56 x 256 bf16 in 256 blocks of 100 KB 20 us, in 512 of 50 KB 25), of as many the smaller cluster; rows of 64
+    // bytes or more, tiles of 16 KB or more where there is a choice.  Images that do not fit so are swept (4 x 128 x 128 x 128 fp32: 22 us,
+    // resident in two rounds 33).
     int64_t best = 0;
     for (int rg = (groups + step - 1) / step * step; rg >= step; rg = rg > step ? std::max(step, rg / 2 / step * step) : 0) {
         const int run = std::min(rg, groups), width = run * per;
-        if (f_run && run != f_run) continue;
         if (run > kMaxGroups || width / q.vec > kThreads) continue;
-        if (width * size < (best ? 128 : 64) && run < groups) break;
+        if (width * size < 64 && run < groups) break;
         const int runs = ceil_div(groups, run);
         for (int s = 1; s <= kMaxCluster; s *= 2) {
-            if (f_s && s != f_s) continue;
-            const int64_t tile = ceil_div64(d->pixels, s), bytes = tile * width * size, blocks = d->n * runs * s;
-            if (bytes + (int64_t)scratch_bytes(q.vec, q.one, run) > kLargeTile) continue;
-            if (best && (bytes < 16 * 1024 || best >= 2 * 148)) break;
-            if (blocks < best || (blocks == best && s >= q.tiles) || blocks > INT32_MAX) continue;      // (of as many blocks the smaller cluster)
+            const int64_t tile = ceil_div64(d->pixels, s), bytes = tile * width * size, smem = bytes + (int64_t)scratch_bytes(q.vec, q.one, run);
+            if (smem > kLargeTile) continue;
+            if (best && bytes < 16 * 1024) break;
+            const int64_t blocks = d->n * runs * s, at_once = 148 * std::min<int64_t>(kResidentBlocks, (227 * 1024) / (smem + 1024));
+            if (blocks > at_once && !(s == 1 && smem <= kLargeTile / 4)) continue;      // (single blocks do not wait for one another)
+            if (blocks < best || (blocks == best && s >= q.tiles) || blocks > INT32_MAX) continue;
             best = blocks;
             q.resident = true;
             q.run_groups = run; q.runs = runs; q.tiles = s; q.tile = tile; q.cols = width / q.vec;
-            q.smem = scratch_bytes(q.vec, q.one, run) + (size_t)bytes;
+            q.smem = (size_t)smem;
         }
     }
     if (q.resident) return q;
-    // Swept: runs of as many channels as the block's threads own vectors, tiles of some 32 KB
+    // Swept: runs of as many channels as the block's threads own vectors, of 16 KB or more
     q.run_groups = std::max(step, std::min({groups, kMaxGroups, kThreads * q.vec / per}) / step * step);
     q.run_groups = std::min(q.run_groups, groups);
     q.runs = ceil_div(groups, q.run_groups);
     const int width = q.run_groups * per;
     q.cols = std::min(width / q.vec, kThreads);
-    const int64_t image_bytes = std::max<int64_t>(1, d->pixels * d->channels * size);
-    q.batch = (int)std::max<int64_t>(1, std::min<int64_t>(d->n, ((getenv("GNB") ? atoll(getenv("GNB")) : 48) << 20) / image_bytes));
-    const int64_t blocks = std::max<int64_t>(1, 148 * (getenv("GNT") ? atoi(getenv("GNT")) : 4) / ((int64_t)q.batch * q.runs));
+    const int64_t blocks = std::max<int64_t>(1, 148 * 4 / (d->n * q.runs));      // four blocks a multiprocessor, all at once
     q.tile = std::max(ceil_div64(d->pixels, blocks), std::max<int64_t>(1, 16384 / ((int64_t)width * size)));
     q.tiles = (int)ceil_div64(d->pixels, q.tile);
     q.smem = (size_t)q.run_groups * 16 + (size_t)kDepth * kThreads * 16;      // (at least collect's scratch: a vector has at most eight pairs of sums)
@@ -559,17 +561,14 @@ int launch(const GroupNormParams &p, const Plan &q, char *workspace, cudaStream_
     }
     double2 *sums = reinterpret_cast<double2 *>(workspace);
     float2 *stats = reinterpret_cast<float2 *>(workspace + q.off_stats);
-    for (int i = 0; i < p.n; i += q.batch) {
-        const int images = std::min(q.batch, p.n - i);
-        const dim3 grid((unsigned)(images * p.runs * p.tiles));
-        const int64_t first = (int64_t)i * p.groups, end = first + (int64_t)images * p.groups;
-        TSB_CUDA(launch_pdl(group_norm_sums_kernel<T, VEC, ONE>, grid, dim3(kThreads), q.smem, stream, p, i, sums));
-        TSB_LAUNCHED("group_norm_sums_kernel");
-        TSB_CUDA(launch_pdl(group_norm_stats_kernel, dim3((unsigned)ceil_div64(end - first, kWarps)), dim3(kThreads), 0, stream, p, first, end, sums, stats));
-        TSB_LAUNCHED("group_norm_stats_kernel");
-        TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y, VEC, ONE>, grid, dim3(kThreads), (size_t)kDepth * kThreads * 16, stream, p, i, stats));
-        TSB_LAUNCHED("group_norm_apply_kernel");
-    }
+    const int64_t blocks = (int64_t)p.n * p.runs * p.tiles, groups = (int64_t)p.n * p.groups;
+    if (blocks > INT32_MAX) return fail(TSB_ERR_UNSUPPORTED, "group_norm: more than 2^31 tiles");
+    TSB_CUDA(launch_pdl(group_norm_sums_kernel<T, VEC, ONE>, dim3((unsigned)blocks), dim3(kThreads), q.smem, stream, p, sums));
+    TSB_LAUNCHED("group_norm_sums_kernel");
+    TSB_CUDA(launch_pdl(group_norm_stats_kernel, dim3((unsigned)ceil_div64(groups, kWarps)), dim3(kThreads), 0, stream, p, sums, stats));
+    TSB_LAUNCHED("group_norm_stats_kernel");
+    TSB_CUDA(launch_pdl(group_norm_apply_kernel<T, Y, VEC, ONE>, dim3((unsigned)blocks), dim3(kThreads), (size_t)kDepth * kThreads * 16, stream, p, stats));
+    TSB_LAUNCHED("group_norm_apply_kernel");
     return TSB_OK;
 }
 
@@ -612,6 +611,7 @@ int group_norm_nhwc(const tsb_group_norm_desc *d, void *workspace, size_t worksp
     p.tile = q.tile;
     p.tiles = q.tiles;
     p.eps = d->eps;
+    p.one_over_count = 1.0 / ((double)d->pixels * p.per);
     p.activation = d->activation;
     p.leaky = d->leaky_scale;
     p.out_channels = i8 ? tsb_padded_channels(p.channels) : p.channels;
