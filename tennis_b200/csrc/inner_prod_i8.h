@@ -3,6 +3,8 @@
 
 #include "typed.cuh"
 
+#include <type_traits>
+
 namespace tsb {
 
 struct InnerProdParams {
@@ -22,12 +24,36 @@ struct InnerProdParams {
 };
 
 #ifdef __CUDACC__
+// A sum as fp32.  SHORT: sums of at most 255 products, below 2^22 in magnitude, by an addition to the bits of 1.5 * 2^23 (the
+// conversion instruction is done 16 times a clock on a multiprocessor, an eighth as often).
+constexpr int kShortSum = 255;
+template <bool SHORT>
+__device__ __forceinline__ float sum_to_f32(int acc) {
+    return SHORT ? __fadd_rn(__int_as_float(acc + 0x4b400000), -12582912.0f) : __int2float_rn(acc);
+}
+
 // N values of a token: sum -> fp32, times the output channel's scale, times the token's, + bias (a missing one is 0), + residual,
 // activation (+ residual); every step is rounded by itself, so the values do not depend on which kernel computed them.
 template <typename T, int N, typename Ws, typename Bias, typename Res>
 __device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, const int (&acc)[N], float xs, Ws ws, Bias bias, Res res, float (&v)[N]) {
+    auto scale = [&](auto is_short) {
+        constexpr bool kShort = decltype(is_short)::value;
+        if constexpr (N % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(acc[i]), ws(i)), xs), bias(i));
+            for (int i = 0; i < N; i += 2) {
+                const float2 f = make_float2(sum_to_f32<kShort>(acc[i]), sum_to_f32<kShort>(acc[i + 1]));
+                // (products by twos, sums one by one: the assembler makes fused operations of a packed product and a packed sum)
+                const float2 r = mul2(mul2(f, make_float2(ws(i), ws(i + 1))), make_float2(xs, xs));
+                v[i] = __fadd_rn(r.x, bias(i));
+                v[i + 1] = __fadd_rn(r.y, bias(i + 1));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(sum_to_f32<kShort>(acc[i]), ws(i)), xs), bias(i));
+        }
+    };
+    if (N >= 16 && p.k <= kShortSum) scale(std::true_type());
+    else scale(std::false_type());
     if (p.residual && !p.residual_after) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));

@@ -2,9 +2,10 @@
 //
 //   tile       128 tokens x BN output channels, 128 bytes of K a stage: two TMA boxes (128-byte swizzle; rows and columns behind the
 //              matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums in tensor memory, two buffers of them
-//   roles      warp 0 loads, warp 1 issues the MMAs, eight warps turn finished sums into outputs while the next tile is computed
-//   epilogue   a thread owns a token: tcgen05.ld gives it 32 channels, the rows of a warp go through 4 KB of shared memory so that
-//              residuals are read and outputs written as whole 128-byte lines
+//   roles      warp 0 loads, warp 1 issues the MMAs, sixteen warps (eight of narrow tiles) turn finished sums into outputs while the next
+//              tile is computed
+//   epilogue   a thread owns a token: tcgen05.ld gives it 64 bytes' worth of channels, the rows of a warp go through 2 KB of shared
+//              memory so that residuals are read and outputs written in runs of 64 bytes
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
 //
@@ -22,12 +23,10 @@ namespace tc {
 namespace {
 
 constexpr int kKBytes = 128;                 // bytes of K a stage
-constexpr int kEpiWarps = 8;
-constexpr int kWarps = 2 + kEpiWarps;
 constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
 constexpr uint32_t kABytes = kBM * kKBytes;
-constexpr uint32_t kStageRow = 128;          // bytes of a staged output row, at most
-constexpr uint32_t kTableFloats = 128;       // a warp's scales and biases: 64 channels each
+constexpr uint32_t kStageRow = 64;           // bytes of a staged output row: 32 channels of 2 bytes, 16 of 4
+constexpr uint32_t kTableFloats = 64;        // a warp's scales and biases of as many channels
 constexpr uint32_t kSmem = 227 * 1024;
 constexpr int kMaxStages = 8;
 
@@ -41,6 +40,8 @@ struct TcParams {
 
 template <int BN>
 struct Layout {
+    static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
+    static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr uint32_t kBBytes = BN * kKBytes;
     static constexpr uint32_t kStage = kABytes + kBBytes;
     static constexpr uint32_t kOut = kEpiWarps * 32 * kStageRow;                  // staged output rows
@@ -59,81 +60,69 @@ __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, i
     m_tile = g * kGroupM + r - n_tile * rows;
 }
 
-// The 16-byte unit u of row r of a warp's staged rows: the units of eight neighbouring rows lie in different banks.
-template <int UNITS>
-__device__ __forceinline__ uint32_t staged(int r, int u) {
-    return (uint32_t)(r * UNITS * 16 + ((u ^ (UNITS == 8 ? r & 7 : (r >> 1) & 3)) << 4));
-}
+// The 16-byte unit u of row r of a warp's staged rows (four units): the units of eight neighbouring rows lie in different banks.
+__device__ __forceinline__ uint32_t staged(int r, int u) { return (uint32_t)(r * kStageRow + ((u ^ ((r >> 1) & 3)) << 4)); }
 
-// CH channels (32 or 64) of a warp's 32 tokens: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel.
-template <typename T, int CH>
+// CH = 64 bytes of channels of a warp's 32 tokens: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel.
+template <typename T>
 __device__ __forceinline__ void epilogue_chunk(const InnerProdParams &p, uint32_t taddr, int64_t m0, int c0, float xs, uint8_t *rows, float *table, bool y_vec, bool res_vec) {
-    constexpr int kN = Vec16<T>::kN, kUnits = CH / kN;        // values of a 16-byte unit, units of a row: 8 (or 4 of 2-byte values, CH = 32)
-    static_assert(kUnits == 8 || kUnits == 4, "rows of 64 or 128 bytes");
+    constexpr int kN = Vec16<T>::kN, CH = kStageRow / sizeof(T);        // values of a 16-byte unit, of a row
     const int lane = threadIdx.x & 31;
     const int live = (int)min((int64_t)32, p.m - m0), cols = min(CH, p.n - c0);
-#pragma unroll
-    for (int i = 0; i < CH / 32; ++i) {
-        const int c = c0 + i * 32 + lane;
-        table[i * 32 + lane] = c < p.n ? __ldg(p.w_scales + c) : 0.0f;
-        table[64 + i * 32 + lane] = c < p.n && p.bias ? __ldg(p.bias + c) : 0.0f;
+    if (lane < CH) {
+        table[lane] = c0 + lane < p.n ? __ldg(p.w_scales + c0 + lane) : 0.0f;
+        table[CH + lane] = c0 + lane < p.n && p.bias ? __ldg(p.bias + c0 + lane) : 0.0f;
     }
+    int acc[CH];
+    if constexpr (CH == 32) tmem_ld32(taddr, acc);
+    else tmem_ld16(taddr, acc);
     if (p.residual) {
         const T *res = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0;
+        if (res_vec && cols == CH) {
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-            const int r = i * (32 / kUnits) + lane / kUnits, u = lane % kUnits;
-            if (r >= live || u * kN >= cols) continue;
-            const T *at = res + r * p.residual_pitch + u * kN;
-            uint8_t *to = rows + staged<kUnits>(r, u);
-            if (res_vec && u * kN + kN <= cols) {
-                *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kN; ++j)
-                    if (u * kN + j < cols) reinterpret_cast<T *>(to)[j] = at[j];
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + lane / 4, u = lane % 4;
+                if (r < live) *reinterpret_cast<uint4 *>(rows + staged(r, u)) = *reinterpret_cast<const uint4 *>(res + r * p.residual_pitch + u * kN);
             }
+        } else {
+            // value by value, neighbouring lanes neighbouring channels
+            constexpr int kRows = 32 / CH;
+            const int c = lane % CH;
+#pragma unroll 4
+            for (int r = lane / CH; r < live; r += kRows)
+                if (c < cols) reinterpret_cast<T *>(rows + staged(r, c / kN))[c % kN] = res[r * p.residual_pitch + c];
         }
     }
     __syncwarp();
+    float v[CH], res[CH];
+    if (p.residual) {
 #pragma unroll
-    for (int h = 0; h < CH / 32; ++h) {
-        int acc[32];
-        tmem_ld32(taddr + h * 32, acc);
-        tmem_ld_wait();
-        float v[32], res[32];
-        if (p.residual) {
-#pragma unroll
-            for (int u = 0; u < 32 / kN; ++u)
-                Vec16<T>::get(*reinterpret_cast<const uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u)), *reinterpret_cast<float (*)[kN]>(&res[u * kN]));
-        }
-        inner_prod_values<T>(p, acc, xs, [&](int j) { return table[h * 32 + j]; }, [&](int j) { return table[64 + h * 32 + j]; },
-                             [&](int j) { return res[j]; }, v);
-#pragma unroll
-        for (int u = 0; u < 32 / kN; ++u)
-            *reinterpret_cast<uint4 *>(rows + staged<kUnits>(lane, h * (32 / kN) + u)) = Vec16<T>::put(*reinterpret_cast<float (*)[kN]>(&v[u * kN]));
+        for (int u = 0; u < 4; ++u) Vec16<T>::get(*reinterpret_cast<const uint4 *>(rows + staged(lane, u)), *reinterpret_cast<float (*)[kN]>(&res[u * kN]));
     }
+    tmem_ld_wait();
+    inner_prod_values<T>(p, acc, xs, [&](int j) { return table[j]; }, [&](int j) { return table[CH + j]; }, [&](int j) { return res[j]; }, v);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4 *>(rows + staged(lane, u)) = Vec16<T>::put(*reinterpret_cast<float (*)[kN]>(&v[u * kN]));
     __syncwarp();
     T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;
+    if (y_vec && cols == CH) {
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-        const int r = i * (32 / kUnits) + lane / kUnits, u = lane % kUnits;
-        if (r >= live || u * kN >= cols) continue;
-        T *to = y + r * p.y_pitch + u * kN;
-        const uint8_t *at = rows + staged<kUnits>(r, u);
-        if (y_vec && u * kN + kN <= cols) {
-            *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kN; ++j)
-                if (u * kN + j < cols) to[j] = reinterpret_cast<const T *>(at)[j];
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + lane / 4, u = lane % 4;
+            if (r < live) *reinterpret_cast<uint4 *>(y + r * p.y_pitch + u * kN) = *reinterpret_cast<const uint4 *>(rows + staged(r, u));
         }
+    } else {
+        constexpr int kRows = 32 / CH;
+        const int c = lane % CH;
+#pragma unroll 4
+        for (int r = lane / CH; r < live; r += kRows)
+            if (c < cols) y[r * p.y_pitch + c] = reinterpret_cast<const T *>(rows + staged(r, c / kN))[c % kN];
     }
     __syncwarp();
 }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(32 * kWarps, 1)
+__global__ void __launch_bounds__(Layout<BN>::kThreads, 1)
 inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TcParams t,
                         int y_vec, int res_vec) {
     using L = Layout<BN>;
@@ -156,7 +145,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
         if (lane < 2) {
             mbar_init(bar_tfull + 8 * lane, 1);
-            mbar_init(bar_tempty + 8 * lane, kEpiWarps);
+            mbar_init(bar_tempty + 8 * lane, L::kEpiWarps);
         }
         if (lane == 0) {
             *abort_flag = 0;
@@ -217,8 +206,9 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             }
         }
     } else {
-        const int e = warp - 2, quarter = warp & 3, half = e >> 2;      // tensor memory lanes of this warp: 32 * (warp % 4); channels: half of the tile
-        constexpr int kCh = BN / 2 >= 64 && sizeof(T) == 2 ? 64 : 32;
+        const int e = warp - 2, quarter = warp & 3;      // tensor memory lanes of this warp: 32 * (warp % 4)
+        constexpr int kShare = BN / (L::kEpiWarps / 4), kCh = kStageRow / sizeof(T);
+        const int share = e / 4 * kShare;                // its channels of the tile
         uint8_t *rows = out_rows + e * 32 * kStageRow;
         float *table = tables + e * kTableFloats;
         uint32_t n = 0;
@@ -231,8 +221,8 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
             if (m0 < t.p.m)
-                for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && nt * BN + c < t.p.n; c += kCh)
-                    epilogue_chunk<T, kCh>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32) << 16) + c, m0, nt * BN + c, xs, rows, table, y_vec != 0, res_vec != 0);
+                for (int c = share; c < share + kShare && nt * BN + c < t.p.n; c += kCh)
+                    epilogue_chunk<T>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32) << 16) + c, m0, nt * BN + c, xs, rows, table, y_vec != 0, res_vec != 0);
             tc_fence_before();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
             __syncwarp();
@@ -294,7 +284,7 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
     const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
     const int y_vec = aligned16(p.y, p.y_pitch, type), res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     const int grid = (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148);
-    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(32 * kWarps), L::kBytes, stream, mx, mw, t, y_vec, res_vec));
+    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, t, y_vec, res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");
     return TSB_OK;
 }
