@@ -208,7 +208,8 @@ inner_prod_i8_few_kernel(const __grid_constant__ InnerProdParams p, int early, i
 #pragma unroll
         for (int i = 0; i < W; ++i) sum[0] += reinterpret_cast<const int *>(smem + i * S::kRing)[m * S::kPitch + c];
         float v[1];
-        inner_prod_values<T>(p, sum, S::kQuantize ? scale : p.x_scales[m * p.xs_stride], [&](int) { return p.w_scales[n]; }, [&](int) { return p.bias ? p.bias[n] : 0.0f; },
+        const float xs = S::kQuantize ? scale : p.x_scales[m * p.xs_stride];
+        inner_prod_values<T>(p, sum, [&](int) { return PairScales{make_float2(p.w_scales[n], 0.0f), xs, make_float2(p.bias ? p.bias[n] : 0.0f, 0.0f)}; },
                              [&](int) { return to_f32(static_cast<const T *>(p.residual)[m * p.residual_pitch + n]); }, v);
         static_cast<T *>(p.y)[m * p.y_pitch + n] = from_f32<T>(v[0]);
     }

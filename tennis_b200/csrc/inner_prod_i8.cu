@@ -74,7 +74,12 @@ inner_prod_i8_direct_kernel(InnerProdParams p, int vec_x, int vec_w) {
             const int last = p.n - 1;
             auto at = [&](int j) { return min(n0 + tn + 16 * j, last); };
             float v[4];
-            inner_prod_values<T>(p, acc[i], p.x_scales[m * p.xs_stride], [&](int j) { return p.w_scales[at(j)]; }, [&](int j) { return p.bias ? p.bias[at(j)] : 0.0f; },
+            const float xs = p.x_scales[m * p.xs_stride];
+            inner_prod_values<T>(p, acc[i],
+                                 [&](int j) {
+                                     return PairScales{make_float2(p.w_scales[at(j)], p.w_scales[at(j + 1)]), xs,
+                                                       p.bias ? make_float2(p.bias[at(j)], p.bias[at(j + 1)]) : make_float2(0.0f, 0.0f)};
+                                 },
                                  [&](int j) { return to_f32(static_cast<const T *>(p.residual)[m * p.residual_pitch + at(j)]); }, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j)

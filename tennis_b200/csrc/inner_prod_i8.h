@@ -32,24 +32,30 @@ __device__ __forceinline__ float sum_to_f32(int acc) {
     return SHORT ? __fadd_rn(__int_as_float(acc + 0x4b400000), -12582912.0f) : __int2float_rn(acc);
 }
 
-// N values of a token: sum -> fp32, times the output channel's scale, times the token's, + bias (a missing one is 0), + residual,
-// activation (+ residual); every step is rounded by itself, so the values do not depend on which kernel computed them.
-template <typename T, int N, typename Ws, typename Bias, typename Res>
-__device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, const int (&acc)[N], float xs, Ws ws, Bias bias, Res res, float (&v)[N]) {
+// N values: sum -> fp32, times the output channel's scale, times the token's, + bias (a missing one is 0), + residual, activation
+// (+ residual); every step is rounded by itself, so the values do not depend on which kernel computed them.
+// of(i): values i and i + 1's scales of their channels (one value: .x alone), their token's scale, their biases, their residuals.
+struct PairScales {
+    float2 ws;
+    float xs;
+    float2 bias;
+};
+template <typename T, int N, typename Of, typename Res>
+__device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, const int (&acc)[N], const Of &of, const Res &res, float (&v)[N]) {
     auto scale = [&](auto is_short) {
         constexpr bool kShort = decltype(is_short)::value;
-        if constexpr (N % 2 == 0) {
+        if constexpr (N > 1) {
 #pragma unroll
             for (int i = 0; i < N; i += 2) {
-                const float2 f = make_float2(sum_to_f32<kShort>(acc[i]), sum_to_f32<kShort>(acc[i + 1]));
                 // (products by twos, sums one by one: the assembler makes fused operations of a packed product and a packed sum)
-                const float2 r = mul2(mul2(f, make_float2(ws(i), ws(i + 1))), make_float2(xs, xs));
-                v[i] = __fadd_rn(r.x, bias(i));
-                v[i + 1] = __fadd_rn(r.y, bias(i + 1));
+                const PairScales s = of(i);
+                const float2 r = mul2(mul2(make_float2(sum_to_f32<kShort>(acc[i]), sum_to_f32<kShort>(acc[i + 1])), s.ws), make_float2(s.xs, s.xs));
+                v[i] = __fadd_rn(r.x, s.bias.x);
+                v[i + 1] = __fadd_rn(r.y, s.bias.y);
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = __fadd_rn(__fmul_rn(__fmul_rn(sum_to_f32<kShort>(acc[i]), ws(i)), xs), bias(i));
+            const PairScales s = of(0);
+            v[0] = __fadd_rn(__fmul_rn(__fmul_rn(sum_to_f32<kShort>(acc[0]), s.ws.x), s.xs), s.bias.x);
         }
     };
     if (N >= 16 && p.k <= kShortSum) scale(std::true_type());

@@ -4,8 +4,9 @@
 //              matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums in tensor memory, two buffers of them
 //   roles      warp 0 loads, warp 1 issues the MMAs, sixteen warps (eight of narrow tiles) turn finished sums into outputs while the next
 //              tile is computed
-//   epilogue   a thread owns a token: tcgen05.ld gives it 64 bytes' worth of channels, the rows of a warp go through 2 KB of shared
-//              memory so that residuals are read and outputs written in runs of 64 bytes
+//   epilogue   sums come in fragments, so that a lane has the same few channels of many tokens and keeps their scales in registers (a lane
+//              that has one token and all channels reads every channel's scales from shared memory, which then bounds the epilogue);
+//              16 rows of a warp go through 2 KB of shared memory: residuals are read and outputs written as whole lines
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
 //
@@ -25,8 +26,7 @@ namespace {
 constexpr int kKBytes = 128;                 // bytes of K a stage
 constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
 constexpr uint32_t kABytes = kBM * kKBytes;
-constexpr uint32_t kStageRow = 64;           // bytes of a staged output row: 32 channels of 2 bytes, 16 of 4
-constexpr uint32_t kTableFloats = 64;        // a warp's scales and biases of as many channels
+constexpr uint32_t kStageBytes = 2048;       // a warp's staged outputs: 16 tokens x 128 bytes
 constexpr uint32_t kSmem = 227 * 1024;
 constexpr int kMaxStages = 8;
 
@@ -44,12 +44,11 @@ struct Layout {
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr uint32_t kBBytes = BN * kKBytes;
     static constexpr uint32_t kStage = kABytes + kBBytes;
-    static constexpr uint32_t kOut = kEpiWarps * 32 * kStageRow;                  // staged output rows
-    static constexpr uint32_t kTables = kEpiWarps * kTableFloats * 4;
+    static constexpr uint32_t kOut = kEpiWarps * kStageBytes;
     static constexpr uint32_t kBars = 256;
-    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kTables - kBars) / kStage) < kMaxStages
-                                       ? (int)((kSmem - 1024 - kOut - kTables - kBars) / kStage) : kMaxStages;
-    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kTables + kBars;
+    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kBars) / kStage) < kMaxStages
+                                       ? (int)((kSmem - 1024 - kOut - kBars) / kStage) : kMaxStages;
+    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kBars;
 };
 
 __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, int &n_tile) {
@@ -60,63 +59,90 @@ __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, i
     m_tile = g * kGroupM + r - n_tile * rows;
 }
 
-// The 16-byte unit u of row r of a warp's staged rows (four units): the units of eight neighbouring rows lie in different banks.
-__device__ __forceinline__ uint32_t staged(int r, int u) { return (uint32_t)(r * kStageRow + ((u ^ ((r >> 1) & 3)) << 4)); }
+// A warp's staged outputs: 16 rows of UNITS 16-byte units.  Unit u of row r lies where neither the fragments' writes (eight rows at a time,
+// of 2-byte values a unit each, of 4-byte values half a unit to a lane) nor the rows' reads meet a bank twice.
+template <int SIZE, int UNITS>
+__device__ __forceinline__ uint32_t staged(int r, int u) {
+    const int with = UNITS == 4 ? (r >> 1) & 3 : SIZE == 2 ? r & 7 : (r & 3) << 1 | (r >> 2 & 1);
+    return (uint32_t)(r * UNITS * 16 + ((u ^ with) << 4));
+}
 
-// CH = 64 bytes of channels of a warp's 32 tokens: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel.
-template <typename T>
-__device__ __forceinline__ void epilogue_chunk(const InnerProdParams &p, uint32_t taddr, int64_t m0, int c0, float xs, uint8_t *rows, float *table, bool y_vec, bool res_vec) {
-    constexpr int kN = Vec16<T>::kN, CH = kStageRow / sizeof(T);        // values of a 16-byte unit, of a row
-    const int lane = threadIdx.x & 31;
-    const int live = (int)min((int64_t)32, p.m - m0), cols = min(CH, p.n - c0);
-    if (lane < CH) {
-        table[lane] = c0 + lane < p.n ? __ldg(p.w_scales + c0 + lane) : 0.0f;
-        table[CH + lane] = c0 + lane < p.n && p.bias ? __ldg(p.bias + c0 + lane) : 0.0f;
-    }
-    int acc[CH];
-    if constexpr (CH == 32) tmem_ld32(taddr, acc);
-    else tmem_ld16(taddr, acc);
-    if (p.residual) {
-        const T *res = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0;
-        if (res_vec && cols == CH) {
+// A lane's channels of a tile: 8 j + 2 (lane % 4) and the next one, for every j; zeros for channels that do not exist.
+template <int CH>
+struct Channels {
+    float2 ws[CH / 8], bias[CH / 8];
+    __device__ __forceinline__ void load(const InnerProdParams &p, int c0) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = i * 8 + lane / 4, u = lane % 4;
-                if (r < live) *reinterpret_cast<uint4 *>(rows + staged(r, u)) = *reinterpret_cast<const uint4 *>(res + r * p.residual_pitch + u * kN);
-            }
+        for (int j = 0; j < CH / 8; ++j) {
+            const int c = c0 + 8 * j + 2 * (threadIdx.x & 3);
+            ws[j] = make_float2(c < p.n ? __ldg(p.w_scales + c) : 0.0f, c + 1 < p.n ? __ldg(p.w_scales + c + 1) : 0.0f);
+            bias[j] = make_float2(p.bias && c < p.n ? __ldg(p.bias + c) : 0.0f, p.bias && c + 1 < p.n ? __ldg(p.bias + c + 1) : 0.0f);
+        }
+    }
+};
+
+// CH channels of 16 tokens, of which `live` exist: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel; xs: the
+// scales of tokens m0 + lane / 4 and the eighth behind it.
+template <typename T, int CH>
+__device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, uint32_t taddr, int64_t m0, int live, int c0, const Channels<CH> &ch, float2 xs, uint8_t *rows, bool y_vec,
+                                              bool res_vec) {
+    constexpr int kN = Vec16<T>::kN, kUnits = CH / kN, kPieces = kUnits / 2;      // units of a row; units that a lane moves
+    static_assert(kUnits == 8 || kUnits == 4, "rows of 64 or 128 bytes");
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bool whole = c0 + CH <= p.n;
+    auto at = [&](int r, int c) { return reinterpret_cast<T *>(rows + staged<sizeof(T), kUnits>(r, c / kN)) + c % kN; };
+    int acc[CH / 2];
+    tmem_ld_rows16(taddr, acc);
+    const int r0 = lane / kUnits, u0 = lane % kUnits;
+    constexpr int kStep = 32 / kUnits;
+    if (p.residual) {
+        if (res_vec && whole) {
+            const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
+            const int64_t step = kStep * p.residual_pitch;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i, from += step)
+                if (i * kStep + r0 < live) *reinterpret_cast<uint4 *>(at(i * kStep + r0, u0 * kN)) = *reinterpret_cast<const uint4 *>(from);
         } else {
             // value by value, neighbouring lanes neighbouring channels
-            constexpr int kRows = 32 / CH;
-            const int c = lane % CH;
-#pragma unroll 4
-            for (int r = lane / CH; r < live; r += kRows)
-                if (c < cols) reinterpret_cast<T *>(rows + staged(r, c / kN))[c % kN] = res[r * p.residual_pitch + c];
+            const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0;
+            for (int r = 0; r < live; ++r)
+#pragma unroll
+                for (int c = lane; c < CH; c += 32)
+                    if (c0 + c < p.n) *at(r, c) = from[r * p.residual_pitch + c];
         }
+        __syncwarp();
     }
-    __syncwarp();
-    float v[CH], res[CH];
+    float v[CH / 2], res[CH / 2];
     if (p.residual) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) Vec16<T>::get(*reinterpret_cast<const uint4 *>(rows + staged(lane, u)), *reinterpret_cast<float (*)[kN]>(&res[u * kN]));
+        for (int i = 0; i < CH / 2; ++i) res[i] = to_f32(*at(g + (i & 2) * 4, 8 * (i / 4) + 2 * t + (i & 1)));
     }
     tmem_ld_wait();
-    inner_prod_values<T>(p, acc, xs, [&](int j) { return table[j]; }, [&](int j) { return table[CH + j]; }, [&](int j) { return res[j]; }, v);
+    inner_prod_values<T>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4], i & 2 ? xs.y : xs.x, ch.bias[i / 4]}; }, [&](int i) { return res[i]; }, v);
+    if (p.residual) __syncwarp();
 #pragma unroll
-    for (int u = 0; u < 4; ++u) *reinterpret_cast<uint4 *>(rows + staged(lane, u)) = Vec16<T>::put(*reinterpret_cast<float (*)[kN]>(&v[u * kN]));
-    __syncwarp();
-    T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;
-    if (y_vec && cols == CH) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + lane / 4, u = lane % 4;
-            if (r < live) *reinterpret_cast<uint4 *>(y + r * p.y_pitch + u * kN) = *reinterpret_cast<const uint4 *>(rows + staged(r, u));
+    for (int i = 0; i < CH / 2; i += 2) {
+        T *to = at(g + (i & 2) * 4, 8 * (i / 4) + 2 * t);
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float2 *>(to) = make_float2(v[i], v[i + 1]);
+        } else {
+            const T pair[2] = {from_f32<T>(v[i]), from_f32<T>(v[i + 1])};
+            *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(pair);
         }
+    }
+    __syncwarp();
+    if (y_vec && whole) {
+        T *to = static_cast<T *>(p.y) + (m0 + r0) * p.y_pitch + c0 + u0 * kN;
+        const int64_t step = kStep * p.y_pitch;
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i, to += step)
+            if (i * kStep + r0 < live) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at(i * kStep + r0, u0 * kN));
     } else {
-        constexpr int kRows = 32 / CH;
-        const int c = lane % CH;
-#pragma unroll 4
-        for (int r = lane / CH; r < live; r += kRows)
-            if (c < cols) y[r * p.y_pitch + c] = reinterpret_cast<const T *>(rows + staged(r, c / kN))[c % kN];
+        T *to = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;
+        for (int r = 0; r < live; ++r)
+#pragma unroll
+            for (int c = lane; c < CH; c += 32)
+                if (c0 + c < p.n) to[r * p.y_pitch + c] = *at(r, c);
     }
     __syncwarp();
 }
@@ -130,8 +156,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t *out_rows = smem_raw + (base - raw) + L::kStages * L::kStage;
-    float *tables = reinterpret_cast<float *>(out_rows + L::kOut);
-    uint8_t *bars_ptr = out_rows + L::kOut + L::kTables;
+    uint8_t *bars_ptr = out_rows + L::kOut;
     const uint32_t bar_full = smem_u32(bars_ptr), bar_empty = bar_full + 8 * kMaxStages, bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars_ptr + 8 * (2 * kMaxStages + 4));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bars_ptr + 8 * (2 * kMaxStages + 4) + 4);
@@ -207,22 +232,49 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
     } else {
         const int e = warp - 2, quarter = warp & 3;      // tensor memory lanes of this warp: 32 * (warp % 4)
-        constexpr int kShare = BN / (L::kEpiWarps / 4), kCh = kStageRow / sizeof(T);
+        constexpr int kShare = BN / (L::kEpiWarps / 4), kCh = 32;
         const int share = e / 4 * kShare;                // its channels of the tile
-        uint8_t *rows = out_rows + e * 32 * kStageRow;
-        float *table = tables + e * kTableFloats;
+        uint8_t *rows = out_rows + e * kStageBytes;
         uint32_t n = 0;
+        int mt, nt, channels_of = -1;
+        Channels<kCh> channels[kShare / kCh];
+        // the scales of this lane's tokens: lane / 4 and every eighth behind it
+        auto scales_of = [&](int m_tile, float2 (&s)[2]) {
+            const int64_t m = (int64_t)m_tile * kBM + quarter * 32 + (lane >> 2);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                s[i] = make_float2(m + 16 * i < t.p.m ? t.p.x_scales[(m + 16 * i) * t.p.xs_stride] : 0.0f, m + 16 * i + 8 < t.p.m ? t.p.x_scales[(m + 16 * i + 8) * t.p.xs_stride] : 0.0f);
+        };
+        tile_of(t, blockIdx.x, mt, nt);
+        float2 xs[2], next_xs[2];
+        scales_of(mt, xs);
         for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
-            int mt, nt;
-            tile_of(t, i, mt, nt);
             const uint32_t acc = n & 1;
-            const int64_t m0 = (int64_t)mt * kBM + quarter * 32;
-            const float xs = m0 + lane < t.p.m ? t.p.x_scales[(m0 + lane) * t.p.xs_stride] : 0.0f;
+            if (nt != channels_of) {
+#pragma unroll
+                for (int c = 0; c < kShare / kCh; ++c) channels[c].load(t.p, nt * BN + share + c * kCh);
+            }
+            channels_of = nt;
+            // the next tile, and its tokens' scales, while this one is worked on
+            int next_mt = mt, next_nt = nt;
+            if (i + (int)gridDim.x < tiles) tile_of(t, i + gridDim.x, next_mt, next_nt);
+            scales_of(next_mt, next_xs);
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
-            if (m0 < t.p.m)
-                for (int c = share; c < share + kShare && nt * BN + c < t.p.n; c += kCh)
-                    epilogue_chunk<T>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32) << 16) + c, m0, nt * BN + c, xs, rows, table, y_vec != 0, res_vec != 0);
+#pragma unroll
+            for (int c = 0; c < kShare / kCh; ++c)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + h * 16;
+                    const int live = (int)max((int64_t)0, min((int64_t)16, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
+                    if (live > 0 && c0 < t.p.n)
+                        epilogue_rows<T, kCh>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32 + h * 16) << 16) + share + c * kCh, m0, live, c0, channels[c], xs[h], rows, y_vec != 0,
+                                              res_vec != 0);
+                }
+            mt = next_mt;
+            nt = next_nt;
+            xs[0] = next_xs[0];
+            xs[1] = next_xs[1];
             tc_fence_before();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
             __syncwarp();
