@@ -6,7 +6,8 @@
 //              tile is computed
 //   epilogue   sums come in fragments, so that a lane has the same few channels of many tokens and keeps their scales in registers (a lane
 //              that has one token and all channels reads every channel's scales from shared memory, which then bounds the epilogue);
-//              16 rows of a warp go through 2 KB of shared memory: residuals are read and outputs written as whole lines
+//              2 KB of a warp's at a time go through shared memory: residuals are read in whole pieces, outputs written by tensor-map
+//              copies (value by value where y does not lie on 16 bytes)
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
 //
@@ -26,7 +27,7 @@ namespace {
 constexpr int kKBytes = 128;                 // bytes of K a stage
 constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
 constexpr uint32_t kABytes = kBM * kKBytes;
-constexpr uint32_t kStageBytes = 2048;       // a warp's staged outputs: 16 tokens x 128 bytes
+constexpr int kCh = 32;                      // channels of a step of the epilogue
 constexpr uint32_t kSmem = 227 * 1024;
 constexpr int kMaxStages = 8;
 
@@ -38,13 +39,14 @@ struct TcParams {
     int tiles_m, tiles_n, kblocks, stages;
 };
 
-template <int BN>
+template <typename T, int BN>
 struct Layout {
+    static constexpr uint32_t kOutWarp = 2048;                                    // a warp's staged outputs
     static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr uint32_t kBBytes = BN * kKBytes;
     static constexpr uint32_t kStage = kABytes + kBBytes;
-    static constexpr uint32_t kOut = kEpiWarps * kStageBytes;
+    static constexpr uint32_t kOut = kEpiWarps * kOutWarp;
     static constexpr uint32_t kBars = 256;
     static constexpr int kStages = (int)((kSmem - 1024 - kOut - kBars) / kStage) < kMaxStages
                                        ? (int)((kSmem - 1024 - kOut - kBars) / kStage) : kMaxStages;
@@ -59,13 +61,15 @@ __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, i
     m_tile = g * kGroupM + r - n_tile * rows;
 }
 
-// A warp's staged outputs: 16 rows of UNITS 16-byte units.  Unit u of row r lies where neither the fragments' writes (eight rows at a time,
-// of 2-byte values a unit each, of 4-byte values half a unit to a lane) nor the rows' reads meet a bank twice.
-template <int SIZE, int UNITS>
-__device__ __forceinline__ uint32_t staged(int r, int u) {
-    const int with = UNITS == 4 ? (r >> 1) & 3 : SIZE == 2 ? r & 7 : (r & 3) << 1 | (r >> 2 & 1);
-    return (uint32_t)(r * UNITS * 16 + ((u ^ with) << 4));
-}
+// A warp's staged outputs, rows of kCh channels: in the order of a tensor map's 64- or 128-byte swizzle, so that the fragments' writes (eight
+// rows at a time, a 16-byte unit each or half a unit to a lane) and the rows' reads meet a bank once or twice.
+template <typename T>
+struct Staged {
+    static constexpr int kRowBytes = kCh * sizeof(T), kUnits = kRowBytes / 16;
+    static constexpr int kRows = 2048 / kRowBytes;            // tokens of a step: 32 of 2-byte values, 16 of 4-byte ones
+    static __device__ __forceinline__ uint32_t unit(int r, int u) { return (uint32_t)(r * kRowBytes + ((u ^ (kUnits == 4 ? (r >> 1) & 3 : r & 7)) << 4)); }
+    static __device__ __forceinline__ uint32_t value(int r, int c) { return unit(r, c * (int)sizeof(T) / 16) + c * (uint32_t)sizeof(T) % 16; }
+};
 
 // A lane's channels of a tile: 8 j + 2 (lane % 4) and the next one, for every j; zeros for channels that do not exist.
 template <int CH>
@@ -81,77 +85,77 @@ struct Channels {
     }
 };
 
-// CH channels of 16 tokens, of which `live` exist: sums in tensor memory at `taddr` -> y.  m0, c0: the first token and channel; xs: the
-// scales of tokens m0 + lane / 4 and the eighth behind it.
-template <typename T, int CH>
-__device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, uint32_t taddr, int64_t m0, int live, int c0, const Channels<CH> &ch, float2 xs, uint8_t *rows, bool y_vec,
-                                              bool res_vec) {
-    constexpr int kN = Vec16<T>::kN, kUnits = CH / kN, kPieces = kUnits / 2;      // units of a row; units that a lane moves
-    static_assert(kUnits == 8 || kUnits == 4, "rows of 64 or 128 bytes");
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const bool whole = c0 + CH <= p.n;
-    auto at = [&](int r, int c) { return reinterpret_cast<T *>(rows + staged<sizeof(T), kUnits>(r, c / kN)) + c % kN; };
-    int acc[CH / 2];
-    tmem_ld_rows16(taddr, acc);
-    const int r0 = lane / kUnits, u0 = lane % kUnits;
-    constexpr int kStep = 32 / kUnits;
+// kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
+// m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
+// the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of its own accord that is under way when this returns, else by the lanes.
+template <typename T>
+__device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CUtensorMap *map_y, uint32_t taddr, int64_t m0, int live, int c0, const Channels<kCh> &ch, const float *xs,
+                                              uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec) {
+    using S = Staged<T>;
+    constexpr int kN = Vec16<T>::kN, kHalves = S::kRows / 16, kValues = kHalves * kCh / 2;     // values of a unit; runs of 16 rows; values of a lane
+    const int lane = threadIdx.x & 31;
+    // value i of a lane: channels 8 j + 2 (lane % 4) + i % 2 of j = i / 4 % 4, of the row lane / 4, plus 8 for i & 2, plus 16 a half
+    int acc[kValues];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16), *reinterpret_cast<int (*)[kCh / 2]>(&acc[h * kCh / 2]));
+    auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
+    float v[kValues], res[kValues];
     if (p.residual) {
-        if (res_vec && whole) {
+        if (lane == 0) bulk_wait_read();       // (the copy that reads these rows last)
+        __syncwarp();
+        if (res_vec && c0 + kCh <= p.n) {
+            const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
+            constexpr int kStep = 32 / S::kUnits;
             const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
             const int64_t step = kStep * p.residual_pitch;
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i, from += step)
-                if (i * kStep + r0 < live) *reinterpret_cast<uint4 *>(at(i * kStep + r0, u0 * kN)) = *reinterpret_cast<const uint4 *>(from);
+            for (int r = 0; r < S::kRows; r += kStep, from += step)
+                if (r + r0 < live) *reinterpret_cast<uint4 *>(rows + S::unit(r + r0, u0)) = *reinterpret_cast<const uint4 *>(from);
         } else {
             // value by value, neighbouring lanes neighbouring channels
-            const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0;
-            for (int r = 0; r < live; ++r)
-#pragma unroll
-                for (int c = lane; c < CH; c += 32)
-                    if (c0 + c < p.n) *at(r, c) = from[r * p.residual_pitch + c];
+            const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
+            for (int r = 0; r < live; ++r, from += p.residual_pitch)
+                if (c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r, lane)) = *from;
         }
         __syncwarp();
-    }
-    float v[CH / 2], res[CH / 2];
-    if (p.residual) {
 #pragma unroll
-        for (int i = 0; i < CH / 2; ++i) res[i] = to_f32(*at(g + (i & 2) * 4, 8 * (i / 4) + 2 * t + (i & 1)));
+        for (int i = 0; i < kValues; ++i) res[i] = to_f32(reinterpret_cast<const T *>(at(i))[i & 1]);
     }
     tmem_ld_wait();
-    inner_prod_values<T>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4], i & 2 ? xs.y : xs.x, ch.bias[i / 4]}; }, [&](int i) { return res[i]; }, v);
-    if (p.residual) __syncwarp();
+    inner_prod_values<T>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4 % (kCh / 8)], xs[i / (kCh / 2) * 2 + (i >> 1 & 1)], ch.bias[i / 4 % (kCh / 8)]}; },
+                         [&](int i) { return res[i]; }, v);
+    if (!p.residual && lane == 0) bulk_wait_read();
+    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < CH / 2; i += 2) {
-        T *to = at(g + (i & 2) * 4, 8 * (i / 4) + 2 * t);
+    for (int i = 0; i < kValues; i += 2) {
         if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float2 *>(to) = make_float2(v[i], v[i + 1]);
+            *reinterpret_cast<float2 *>(at(i)) = make_float2(v[i], v[i + 1]);
         } else {
             const T pair[2] = {from_f32<T>(v[i]), from_f32<T>(v[i + 1])};
-            *reinterpret_cast<uint32_t *>(to) = *reinterpret_cast<const uint32_t *>(pair);
+            *reinterpret_cast<uint32_t *>(at(i)) = *reinterpret_cast<const uint32_t *>(pair);
         }
     }
-    __syncwarp();
-    if (y_vec && whole) {
-        T *to = static_cast<T *>(p.y) + (m0 + r0) * p.y_pitch + c0 + u0 * kN;
-        const int64_t step = kStep * p.y_pitch;
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i, to += step)
-            if (i * kStep + r0 < live) *reinterpret_cast<uint4 *>(to) = *reinterpret_cast<const uint4 *>(at(i * kStep + r0, u0 * kN));
+    if (tile_store && (c0 + kCh <= p.n || p.n % kN == 0)) {      // (such a copy stops at 16 bytes, not at the value, where y ends)
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map_y, smem_u32(rows), c0, (int)m0);    // (what lies outside y is not written)
+            bulk_commit();
+        }
     } else {
-        T *to = static_cast<T *>(p.y) + m0 * p.y_pitch + c0;
-        for (int r = 0; r < live; ++r)
-#pragma unroll
-            for (int c = lane; c < CH; c += 32)
-                if (c0 + c < p.n) to[r * p.y_pitch + c] = *at(r, c);
+        __syncwarp();
+        T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0 + lane;
+        for (int r = 0; r < live; ++r, y += p.y_pitch)
+            if (c0 + lane < p.n) *y = *reinterpret_cast<const T *>(rows + S::value(r, lane));
+        __syncwarp();
     }
-    __syncwarp();
 }
 
 template <typename T, int BN>
-__global__ void __launch_bounds__(Layout<BN>::kThreads, 1)
-inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TcParams t,
-                        int y_vec, int res_vec) {
-    using L = Layout<BN>;
+__global__ void __launch_bounds__(Layout<T, BN>::kThreads, 1)
+inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
+                        const __grid_constant__ TcParams t, int tile_store, int res_vec) {
+    using L = Layout<T, BN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -232,21 +236,22 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
     } else {
         const int e = warp - 2, quarter = warp & 3;      // tensor memory lanes of this warp: 32 * (warp % 4)
-        constexpr int kShare = BN / (L::kEpiWarps / 4), kCh = 32;
+        constexpr int kShare = BN / (L::kEpiWarps / 4);
         const int share = e / 4 * kShare;                // its channels of the tile
-        uint8_t *rows = out_rows + e * kStageBytes;
-        uint32_t n = 0;
+        uint8_t *rows = out_rows + e * L::kOutWarp;
+        uint32_t n = 0, to[kCh / 8];
+#pragma unroll
+        for (int j = 0; j < kCh / 8; ++j) to[j] = Staged<T>::value(lane >> 2, 8 * j + 2 * (lane & 3));
         int mt, nt, channels_of = -1;
         Channels<kCh> channels[kShare / kCh];
         // the scales of this lane's tokens: lane / 4 and every eighth behind it
-        auto scales_of = [&](int m_tile, float2 (&s)[2]) {
+        auto scales_of = [&](int m_tile, float (&s)[4]) {
             const int64_t m = (int64_t)m_tile * kBM + quarter * 32 + (lane >> 2);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                s[i] = make_float2(m + 16 * i < t.p.m ? t.p.x_scales[(m + 16 * i) * t.p.xs_stride] : 0.0f, m + 16 * i + 8 < t.p.m ? t.p.x_scales[(m + 16 * i + 8) * t.p.xs_stride] : 0.0f);
+            for (int i = 0; i < 4; ++i) s[i] = m + 8 * i < t.p.m ? t.p.x_scales[(m + 8 * i) * t.p.xs_stride] : 0.0f;
         };
         tile_of(t, blockIdx.x, mt, nt);
-        float2 xs[2], next_xs[2];
+        float xs[4], next_xs[4];
         scales_of(mt, xs);
         for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
             const uint32_t acc = n & 1;
@@ -261,26 +266,28 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             scales_of(next_mt, next_xs);
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
+            constexpr int kRows = Staged<T>::kRows;
 #pragma unroll
             for (int c = 0; c < kShare / kCh; ++c)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + h * 16;
-                    const int live = (int)max((int64_t)0, min((int64_t)16, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
+                for (int r = 0; r < 32; r += kRows) {
+                    const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
+                    const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
                     if (live > 0 && c0 < t.p.n)
-                        epilogue_rows<T, kCh>(t.p, tmem + acc * BN + ((uint32_t)(quarter * 32 + h * 16) << 16) + share + c * kCh, m0, live, c0, channels[c], xs[h], rows, y_vec != 0,
-                                              res_vec != 0);
+                        epilogue_rows<T>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, m0, live, c0, channels[c], xs + r / 8, rows, to,
+                                         tile_store != 0, res_vec != 0);
                 }
             mt = next_mt;
             nt = next_nt;
-            xs[0] = next_xs[0];
-            xs[1] = next_xs[1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) xs[j] = next_xs[j];
             tc_fence_before();
             if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
             __syncwarp();
         }
     }
 done:
+    if (warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // this warp's outputs are written
     if (*abort_flag) {
         // copies that may still be in flight get time to land before shared memory is released
         const long long t0 = clock64();
@@ -319,13 +326,31 @@ int encode(CUtensorMap *map, const int8_t *at, int64_t rows, int cols, int64_t p
     return TSB_OK;
 }
 
+// The boxes that a warp writes
+template <typename T>
+int encode_output(CUtensorMap *map, const InnerProdParams &p) {
+    const auto fn = encode_tiled();
+    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
+    cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m};
+    cuuint64_t strides[1] = {(cuuint64_t)(p.m > 1 ? p.y_pitch * (int64_t)sizeof(T) : ((int64_t)p.n * (int64_t)sizeof(T) + 15) / 16 * 16)};
+    cuuint32_t box[2] = {kCh, Staged<T>::kRows}, estr[2] = {1, 1};
+    const CUresult r = fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: cuTensorMapEncodeTiled(y) failed with %d", (int)r);
+    return TSB_OK;
+}
+
 template <typename T, int BN>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
-    using L = Layout<BN>;
-    CUtensorMap mx, mw;
+    using L = Layout<T, BN>;
+    CUtensorMap mx, mw, my;
     int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
     if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, BN);
     if (st != TSB_OK) return st;
+    const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
+    const bool tile_store = aligned16(p.y, p.y_pitch, type) && p.y_pitch < (int64_t)1 << 37, res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
+    if (!tile_store) my = mx;
+    else if ((st = encode_output<T>(&my, p)) != TSB_OK) return st;
     auto kernel = inner_prod_i8_tc_kernel<T, BN>;
     static DeviceOnce raised;
     if (raised.first()) {
@@ -333,10 +358,8 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
         raised.done();
     }
     TcParams t = {p, (int)ceil_div64(p.m, kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
-    const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
-    const int y_vec = aligned16(p.y, p.y_pitch, type), res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     const int grid = (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148);
-    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, t, y_vec, res_vec));
+    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");
     return TSB_OK;
 }
