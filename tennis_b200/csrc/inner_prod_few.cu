@@ -67,17 +67,12 @@ struct TokenQuantizer {
         }
     }
     __device__ __forceinline__ float finish(int8_t *out, int pitch, uint32_t *part) {
-        uint32_t most = 0;
-        auto take = [&](const uint4 &q) {
-            float v[kN];
-            Vec16<X>::get(q, v);
+        Largest<X> largest;
 #pragma unroll
-            for (int i = 0; i < kN; ++i) most = max(most, magnitude(v[i]));
-        };
-#pragma unroll
-        for (int i = 0; i < kHeld; ++i) take(held[i]);
-        for (int u = threadIdx.x + kHeld * 32 * W; u < whole; u += 32 * W) take(vector(u));
-        for (int c = whole * kN + threadIdx.x; c < k; c += 32 * W) most = max(most, magnitude(to_f32(row[c])));
+        for (int i = 0; i < kHeld; ++i) largest.add(held[i]);
+        for (int u = threadIdx.x + kHeld * 32 * W; u < whole; u += 32 * W) largest.add(vector(u));
+        for (int c = whole * kN + threadIdx.x; c < k; c += 32 * W) largest.add(row[c]);
+        uint32_t most = largest.bits();
         most = __reduce_max_sync(0xffffffffu, most);
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
         __syncthreads();

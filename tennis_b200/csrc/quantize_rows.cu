@@ -1,8 +1,8 @@
 // quantize with a scale for each row that is taken from the row (no counterpart in the reference, whose scales are attributes).
 //
-// Bound by memory: a row is read once, held in registers while its largest magnitude is found, and written as int8.  A thread holds up
-// to four 16-byte vectors; a row belongs to a warp, or to a block of as many warps as it needs -- of many rows, few threads with
-// four vectors each (loads in flight), of few rows, many threads with one (a short way from load to store).
+// Bound by memory: a row is read once, held in registers while its largest magnitude is found, and written as int8.  A row belongs to
+// a warp, whose lanes hold up to two 16-byte vectors and need no barrier; or, where it is longer, to a block of as many warps as
+// it needs -- of many rows, threads with four vectors each (loads in flight), of few, more threads with one (a short way from load to store).
 #include "typed.cuh"
 
 #include <algorithm>
@@ -10,7 +10,7 @@
 namespace tsb {
 namespace {
 
-constexpr int kWarpRowThreads = 256;      // rows of a warp each: threads of a block
+constexpr int kWarpRowThreads = 128;      // rows of a warp each: threads of a block
 constexpr int kMost = 1024;               // threads of a row, at most
 
 // Vector u of a row: one 16-byte load, or value by value where rows do not start on 16 bytes and at the row's end (zeros behind it,
@@ -25,16 +25,6 @@ __device__ __forceinline__ uint4 load_vector(const T *row, int u, int cols, bool
     for (int i = 0; i < kN; ++i)
         if (u * kN + i < cols) v[i] = row[u * kN + i];
     return out;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t largest_of(const uint4 &q) {
-    float v[Vec16<T>::kN];
-    Vec16<T>::get(q, v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < Vec16<T>::kN; ++i) m = max(m, magnitude(v[i]));
-    return m;
 }
 
 // Vector u as int8, in one store where the row starts on a multiple of its bytes.
@@ -69,7 +59,7 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restric
         const T *xr = x + r * x_pitch;
         int8_t *yr = y + r * y_pitch;
         uint4 held[V > 0 ? V : 1];
-        uint32_t most = 0;
+        Largest<T> largest;
         if constexpr (V > 0) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -77,12 +67,12 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t x_pitch, int8_t *__restric
                 if (at + i * step < vectors) held[i] = load_vector(xr, at + i * step, cols, x_aligned);
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) most = max(most, largest_of<T>(held[i]));
+            for (int i = 0; i < V; ++i) largest.add(held[i]);
         } else {
 #pragma unroll 4
-            for (int u = at; u < vectors; u += step) most = max(most, largest_of<T>(load_vector(xr, u, cols, x_aligned)));
+            for (int u = at; u < vectors; u += step) largest.add(load_vector(xr, u, cols, x_aligned));
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+        uint32_t most = __reduce_max_sync(0xffffffffu, largest.bits());
         if constexpr (!WARP) {
             if (lane == 0) part[warp] = most;
             __syncthreads();
@@ -114,12 +104,9 @@ int launch(const void *x, int64_t x_pitch, int8_t *y, int64_t y_pitch, float *sc
         TSB_LAUNCHED("quantize_rows_kernel");
         return TSB_OK;
     };
-    // a warp a row: of many short rows (of few, a block each is done sooner)
-    if (vectors <= 32 || (vectors <= 128 && rows > 148 * 8)) {
-        const int64_t blocks = ceil_div64(rows, kWarpRowThreads / 32);
-        if (vectors <= 32) return go(quantize_rows_kernel<T, 1, true>, blocks, kWarpRowThreads);
-        return go(quantize_rows_kernel<T, 4, true>, blocks, kWarpRowThreads);
-    }
+    // A warp a row, which needs no barrier, where a row is two vectors a lane or less (262144 x 256 fp32 66 us, by blocks 74; of longer rows
+    // blocks are as fast or faster: 65536 x 1024 fp32 56 us, by warps 92, whose registers hold too few rows)
+    if (vectors <= 64) return go(quantize_rows_kernel<T, 2, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
     if (vectors <= kMost && rows <= 148 * 2) return go(quantize_rows_kernel<T, 1, false>, rows, round_up(vectors, 32));
     if (vectors <= 4 * kMost) return go(quantize_rows_kernel<T, 4, false>, rows, round_up(ceil_div(vectors, 4), 32));
     return go(quantize_rows_kernel<T, 0, false>, rows, kMost);

@@ -86,27 +86,62 @@ template <> struct Vec16<__nv_bfloat16> {
 // The largest magnitude of a row as the bits of an fp32 value: magnitudes order as their bits do, infinity lies above every number
 // and NaN above infinity, so an integer maximum carries both through to the scale.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The same of many values of type T, 16 bytes at a time (of 16-bit types by their own bits, two in one operation).
+template <typename T>
+class Largest {
+public:
+    __device__ __forceinline__ void add(const uint4 &q) {
+        if constexpr (sizeof(T) == 2) {
+            bits_ = __vimax3_u16x2(bits_, q.x & 0x7fff7fffu, q.y & 0x7fff7fffu);
+            bits_ = __vimax3_u16x2(bits_, q.z & 0x7fff7fffu, q.w & 0x7fff7fffu);
+        } else {
+            bits_ = max(bits_, max(max(q.x & 0x7fffffffu, q.y & 0x7fffffffu), max(q.z & 0x7fffffffu, q.w & 0x7fffffffu)));
+        }
+    }
+    __device__ __forceinline__ void add(T v) { single_ = max(single_, magnitude(to_f32(v))); }
+    __device__ __forceinline__ uint32_t bits() const {
+        if constexpr (sizeof(T) == 2) {
+            const uint16_t top = (uint16_t)max(bits_ & 0xffffu, bits_ >> 16);
+            return max(single_, magnitude(to_f32(*reinterpret_cast<const T *>(&top))));
+        } else {
+            return max(single_, bits_);
+        }
+    }
+
+private:
+    uint32_t bits_ = 0, single_ = 0;
+};
+
 // Rows below 2^-100 count as zero: the factor 127 / a stays a finite number and the scale a / 127 a normal one.
 struct RowScale {
     float by, scale;
+    bool finite;
     __device__ __forceinline__ explicit RowScale(uint32_t largest_bits) {
         const float a = __uint_as_float(largest_bits);
         const bool zero = a < 7.888609052210118e-31f;
         by = zero ? 0.0f : __fdiv_rn(127.0f, a);
         scale = zero ? 0.0f : __fdiv_rn(a, 127.0f);
+        finite = largest_bits < 0x7f800000u;
     }
     __device__ __forceinline__ int operator()(float v) const { return q8_half_even(__fmul_rn(v, by)); }
 };
-
-// 16 bytes of a floating row as int8
+// 16 bytes of a floating row as int8.  The products of a row of numbers are at most 127 (1 + 2^-23), so nothing is to be clamped, and a
+// sum with 1.5 * 2^23 rounds them, half to even, to whole numbers that its low byte holds (a conversion is done an eighth as often).
 template <typename X>
 __device__ __forceinline__ void quantize16(const RowScale &q, const uint4 &from, uint32_t *to) {
     constexpr int kN = Vec16<X>::kN;
     float v[kN];
     Vec16<X>::get(from, v);
+    uint32_t r[kN];
+    if (q.finite) {
 #pragma unroll
-    for (int i = 0; i < kN / 4; ++i)
-        to[i] = (uint32_t)(uint8_t)q(v[4 * i]) | (uint32_t)(uint8_t)q(v[4 * i + 1]) << 8 | (uint32_t)(uint8_t)q(v[4 * i + 2]) << 16 | (uint32_t)(uint8_t)q(v[4 * i + 3]) << 24;
+        for (int i = 0; i < kN; ++i) r[i] = __float_as_uint(__fadd_rn(__fmul_rn(v[i], q.by), 12582912.0f));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) r[i] = (uint32_t)q(v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kN / 4; ++i) to[i] = __byte_perm(__byte_perm(r[4 * i], r[4 * i + 1], 0x0040), __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x0040), 0x5410);
 }
 
 // ---- two fp32 values in one instruction (each half is rounded by itself)
