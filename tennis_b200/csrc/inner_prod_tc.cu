@@ -114,8 +114,15 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
         } else {
             // value by value, neighbouring lanes neighbouring channels
             const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
-            for (int r = 0; r < live; ++r, from += p.residual_pitch)
-                if (c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r, lane)) = *from;
+            T some[8];
+            for (int r = 0; r < live; r += 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i, from += p.residual_pitch)
+                    if (r + i < live && c0 + lane < p.n) some[i] = *from;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (r + i < live && c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, lane)) = some[i];
+            }
         }
         __syncwarp();
 #pragma unroll
@@ -145,6 +152,7 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     } else {
         __syncwarp();
         T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0 + lane;
+#pragma unroll 4
         for (int r = 0; r < live; ++r, y += p.y_pitch)
             if (c0 + lane < p.n) *y = *reinterpret_cast<const T *>(rows + S::value(r, lane));
         __syncwarp();
@@ -366,9 +374,15 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
 
 template <typename T>
 int pick(const InnerProdParams &p, cudaStream_t stream) {
-    if (p.n <= 64) return launch<T, 64>(p, stream);
-    if (p.n <= 128 || ceil_div64(p.m, kBM) * ceil_div(p.n, 256) < 148) return launch<T, 128>(p, stream);
-    return launch<T, 256>(p, stream);
+    // The tile's width by the clocks that its rounds take: a multiprocessor gets 64 bytes a clock, so a stage of 128 + BN rows of 128 bytes
+    // takes 2 (128 + BN); the epilogue some 9 BN.  (Measured, 64, 128 and 256 wide: 64 x 4096 x 4096 9.7, 11.0, 16.2 us, 2048 x 4096 x 4096
+    // 48.6, 35.4, 29.1, 2048 x 1000 x 2048 9.9, 8.1, 11.0.)
+    auto clocks = [&](int bn) {
+        return ceil_div64(ceil_div64(p.m, kBM) * ceil_div(p.n, bn), 148) * (ceil_div(p.k, kKBytes) * 2 * (128 + bn) + 9 * bn);
+    };
+    const int64_t c64 = clocks(64), c128 = clocks(128), c256 = clocks(256);
+    if (c64 <= c128 && c64 <= c256) return launch<T, 64>(p, stream);
+    return c128 <= c256 ? launch<T, 128>(p, stream) : launch<T, 256>(p, stream);
 }
 
 }  // namespace

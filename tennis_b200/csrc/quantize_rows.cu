@@ -104,8 +104,9 @@ int launch(const void *x, int64_t x_pitch, int8_t *y, int64_t y_pitch, float *sc
         TSB_LAUNCHED("quantize_rows_kernel");
         return TSB_OK;
     };
-    // A warp a row, which needs no barrier, where a row is two vectors a lane or less (262144 x 256 fp32 66 us, by blocks 74; of longer rows
-    // blocks are as fast or faster: 65536 x 1024 fp32 56 us, by warps 92, whose registers hold too few rows)
+    // A warp a row, which needs no barrier, where a row is two vectors a lane or less (262144 x 256 fp32 57 us, by blocks 74; of longer rows
+    // blocks are as fast or faster: 65536 x 1024 fp32 55 us, by warps 92, whose registers hold too few rows)
+    if (vectors <= 32) return go(quantize_rows_kernel<T, 1, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
     if (vectors <= 64) return go(quantize_rows_kernel<T, 2, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
     if (vectors <= kMost && rows <= 148 * 2) return go(quantize_rows_kernel<T, 1, false>, rows, round_up(vectors, 32));
     if (vectors <= 4 * kMost) return go(quantize_rows_kernel<T, 4, false>, rows, round_up(ceil_div(vectors, 4), 32));
