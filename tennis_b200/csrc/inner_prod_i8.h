@@ -40,7 +40,8 @@ struct PairScales {
     float xs;
     float2 bias;
 };
-template <typename T, int N, typename Of, typename Res>
+// RES: false where there is certainly no residual.
+template <typename T, bool RES = true, int N, typename Of, typename Res>
 __device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, const int (&acc)[N], const Of &of, const Res &res, float (&v)[N]) {
     auto scale = [&](auto is_short) {
         constexpr bool kShort = decltype(is_short)::value;
@@ -60,12 +61,12 @@ __device__ __forceinline__ void inner_prod_values(const InnerProdParams &p, cons
     };
     if (N >= 16 && p.k <= kShortSum) scale(std::true_type());
     else scale(std::false_type());
-    if (p.residual && !p.residual_after) {
+    if (RES && p.residual && !p.residual_after) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
     }
     by_activation(p.activation, [&](auto act) { activate<decltype(act)::value, T>(v, p.leaky); });
-    if (p.residual && p.residual_after) {
+    if (RES && p.residual && p.residual_after) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
     }

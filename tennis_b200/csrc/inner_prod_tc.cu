@@ -88,7 +88,7 @@ struct Channels {
 // kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
 // the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of its own accord that is under way when this returns, else by the lanes.
-template <typename T>
+template <typename T, bool RES>
 __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CUtensorMap *map_y, uint32_t taddr, int64_t m0, int live, int c0, const Channels<kCh> &ch, const float *xs,
                                               uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec) {
     using S = Staged<T>;
@@ -99,8 +99,8 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16), *reinterpret_cast<int (*)[kCh / 2]>(&acc[h * kCh / 2]));
     auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
-    float v[kValues], res[kValues];
-    if (p.residual) {
+    float v[kValues], res[RES ? kValues : 1];
+    if constexpr (RES) {
         if (lane == 0) bulk_wait_read();       // (the copy that reads these rows last)
         __syncwarp();
         if (res_vec && c0 + kCh <= p.n) {
@@ -129,9 +129,9 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
         for (int i = 0; i < kValues; ++i) res[i] = to_f32(reinterpret_cast<const T *>(at(i))[i & 1]);
     }
     tmem_ld_wait();
-    inner_prod_values<T>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4 % (kCh / 8)], xs[i / (kCh / 2) * 2 + (i >> 1 & 1)], ch.bias[i / 4 % (kCh / 8)]}; },
-                         [&](int i) { return res[i]; }, v);
-    if (!p.residual && lane == 0) bulk_wait_read();
+    inner_prod_values<T, RES>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4 % (kCh / 8)], xs[i / (kCh / 2) * 2 + (i >> 1 & 1)], ch.bias[i / 4 % (kCh / 8)]}; },
+                         [&](int i) { return res[RES ? i : 0]; }, v);
+    if (!RES && lane == 0) bulk_wait_read();
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kValues; i += 2) {
@@ -159,7 +159,7 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     }
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool RES>
 __global__ void __launch_bounds__(Layout<T, BN>::kThreads, 1)
 inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
                         const __grid_constant__ TcParams t, int tile_store, int res_vec) {
@@ -282,7 +282,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
                     const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
                     if (live > 0 && c0 < t.p.n)
-                        epilogue_rows<T>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, m0, live, c0, channels[c], xs + r / 8, rows, to,
+                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, m0, live, c0, channels[c], xs + r / 8, rows, to,
                                          tile_store != 0, res_vec != 0);
                 }
             mt = next_mt;
@@ -348,7 +348,7 @@ int encode_output(CUtensorMap *map, const InnerProdParams &p) {
     return TSB_OK;
 }
 
-template <typename T, int BN>
+template <typename T, int BN, bool RES>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
     using L = Layout<T, BN>;
     CUtensorMap mx, mw, my;
@@ -359,7 +359,7 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
     const bool tile_store = aligned16(p.y, p.y_pitch, type) && p.y_pitch < (int64_t)1 << 37, res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     if (!tile_store) my = mx;
     else if ((st = encode_output<T>(&my, p)) != TSB_OK) return st;
-    auto kernel = inner_prod_i8_tc_kernel<T, BN>;
+    auto kernel = inner_prod_i8_tc_kernel<T, BN, RES>;
     static DeviceOnce raised;
     if (raised.first()) {
         TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
@@ -372,7 +372,7 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
     return TSB_OK;
 }
 
-template <typename T>
+template <typename T, bool RES>
 int pick(const InnerProdParams &p, cudaStream_t stream) {
     // The tile's width by the clocks that its rounds take: a multiprocessor gets 64 bytes a clock, so a stage of 128 + BN rows of 128 bytes
     // takes 2 (128 + BN); the epilogue some 9 BN.  (Measured, 64, 128 and 256 wide: 64 x 4096 x 4096 9.7, 11.0, 16.2 us, 2048 x 4096 x 4096
@@ -381,8 +381,8 @@ int pick(const InnerProdParams &p, cudaStream_t stream) {
         return ceil_div64(ceil_div64(p.m, kBM) * ceil_div(p.n, bn), 148) * (ceil_div(p.k, kKBytes) * 2 * (128 + bn) + 9 * bn);
     };
     const int64_t c64 = clocks(64), c128 = clocks(128), c256 = clocks(256);
-    if (c64 <= c128 && c64 <= c256) return launch<T, 64>(p, stream);
-    return c128 <= c256 ? launch<T, 128>(p, stream) : launch<T, 256>(p, stream);
+    if (c64 <= c128 && c64 <= c256) return launch<T, 64, RES>(p, stream);
+    return c128 <= c256 ? launch<T, 128, RES>(p, stream) : launch<T, 256, RES>(p, stream);
 }
 
 }  // namespace
@@ -403,9 +403,9 @@ bool inner_prod_can(const InnerProdParams &p, const char **why) {
 
 int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream) {
     switch (y_type) {
-        case TSB_TYPE_F32: return pick<float>(p, stream);
-        case TSB_TYPE_F16: return pick<__half>(p, stream);
-        default: return pick<__nv_bfloat16>(p, stream);
+        case TSB_TYPE_F32: return p.residual ? pick<float, true>(p, stream) : pick<float, false>(p, stream);
+        case TSB_TYPE_F16: return p.residual ? pick<__half, true>(p, stream) : pick<__half, false>(p, stream);
+        default: return p.residual ? pick<__nv_bfloat16, true>(p, stream) : pick<__nv_bfloat16, false>(p, stream);
     }
 }
 
