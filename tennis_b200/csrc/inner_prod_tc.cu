@@ -1,6 +1,7 @@
 // The int8 inner product on the sm_100a tensor cores: y [m, n] = x [m, k] . w [n, k], both operands K-major as they lie in memory.
 //
-//   tile       128 tokens x BN output channels, 128 bytes of K a stage: two TMA boxes (128-byte swizzle; rows and columns behind the
+//   tile       128 tokens x BN output channels (or 256 x 256 of two CTAs, each with its half of both operands: a multiprocessor then reads
+//              32 instead of 48 KB for the same arithmetic, and its 64 bytes a clock no longer bound the MMAs), 128 bytes of K a stage: two TMA boxes (128-byte swizzle; rows and columns behind the
 //              matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums in tensor memory, two buffers of them
 //   roles      warp 0 loads, warp 1 issues the MMAs, sixteen warps (eight of narrow tiles) turn finished sums into outputs while the next
 //              tile is computed
@@ -39,12 +40,14 @@ struct TcParams {
     int tiles_m, tiles_n, kblocks, stages;
 };
 
-template <typename T, int BN>
+// PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory
+template <typename T, int BN, bool PAIR>
 struct Layout {
     static constexpr uint32_t kOutWarp = 2048;                                    // a warp's staged outputs
     static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
-    static constexpr uint32_t kBBytes = BN * kKBytes;
+    static constexpr int kBRows = PAIR ? BN / 2 : BN;
+    static constexpr uint32_t kBBytes = kBRows * kKBytes;
     static constexpr uint32_t kStage = kABytes + kBBytes;
     static constexpr uint32_t kOut = kEpiWarps * kOutWarp;
     static constexpr uint32_t kBars = 256;
@@ -159,11 +162,11 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     }
 }
 
-template <typename T, int BN, bool RES>
-__global__ void __launch_bounds__(Layout<T, BN>::kThreads, 1)
+template <typename T, int BN, bool RES, bool PAIR>
+__global__ void __launch_bounds__(Layout<T, BN, PAIR>::kThreads, 1)
 inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
                         const __grid_constant__ TcParams t, int tile_store, int res_vec) {
-    using L = Layout<T, BN>;
+    using L = Layout<T, BN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -174,6 +177,8 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bars_ptr + 8 * (2 * kMaxStages + 4) + 4);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int tiles = t.tiles_m * t.tiles_n;
+    const int rank = PAIR ? (int)cluster_rank() : 0, first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+    auto rows_of = [&](int m_tile) { return PAIR ? 2 * m_tile + rank : m_tile; };      // this CTA's 128 tokens of a tile
 
     if (warp == 0) {
         if (lane < L::kStages) {
@@ -182,7 +187,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
         if (lane < 2) {
             mbar_init(bar_tfull + 8 * lane, 1);
-            mbar_init(bar_tempty + 8 * lane, L::kEpiWarps);
+            mbar_init(bar_tempty + 8 * lane, PAIR ? 2 * L::kEpiWarps : L::kEpiWarps);
         }
         if (lane == 0) {
             *abort_flag = 0;
@@ -193,11 +198,21 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         fence_async_smem();
     }
     if (warp == 1) {
-        tmem_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
-        tmem_relinquish();
+        const uint32_t slot = smem_u32(const_cast<uint32_t *>(tmem_slot));
+        if constexpr (PAIR) {
+            pair_tmem_alloc(slot, 512);
+            pair_tmem_relinquish();
+        } else {
+            tmem_alloc(slot, 512);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) {                      // the other CTA's barriers and tensor memory are there too
+        cluster_arrive();
+        cluster_wait();
+    }
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_sync();
@@ -206,42 +221,66 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     };
 
     if (warp == 0) {
+        // Both CTAs of a pair load their halves; the bytes of both count at the even one's barrier.  Neither can be a round ahead: its
+        // own stage is free only when the MMAs that read both have completed.
         uint32_t s = 0;
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x) {
+        const uint32_t lead_full = PAIR ? map_to_rank(bar_full, 0) : bar_full;
+        for (int i = first; i < tiles; i += step) {
             int mt, nt;
             tile_of(t, i, mt, nt);
             for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
-                const uint32_t stage = s % L::kStages, round = s / L::kStages;
+                const uint32_t stage = s % L::kStages, round = s / L::kStages, at = base + stage * L::kStage;
                 if (!mbar_wait_warp(bar_empty + 8 * stage, (round & 1) ^ 1, abort_flag)) { give_up(1); goto done; }
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(bar_full + 8 * stage, L::kStage);
-                    tma_load_2d(base + stage * L::kStage, &map_x, bar_full + 8 * stage, kb * kKBytes, mt * kBM);
-                    tma_load_2d(base + stage * L::kStage + kABytes, &map_w, bar_full + 8 * stage, kb * kKBytes, nt * BN);
+                    if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, PAIR ? 2 * L::kStage : L::kStage);
+                    if constexpr (PAIR) {
+                        pair_tma_load_2d(at, &map_x, lead_full + 8 * stage, kb * kKBytes, rows_of(mt) * kBM);
+                        pair_tma_load_2d(at + kABytes, &map_w, lead_full + 8 * stage, kb * kKBytes, nt * BN + rank * L::kBRows);
+                    } else {
+                        tma_load_2d(at, &map_x, bar_full + 8 * stage, kb * kKBytes, rows_of(mt) * kBM);
+                        tma_load_2d(at + kABytes, &map_w, bar_full + 8 * stage, kb * kKBytes, nt * BN);
+                    }
                 }
                 __syncwarp();
             }
+        }
+        if constexpr (PAIR) {
+            // no arrival from the other CTA is to come when this one leaves
+            for (uint32_t back = min(s, (uint32_t)L::kStages); back > 0; --back)
+                if (!mbar_wait_warp(bar_empty + 8 * ((s - back) % L::kStages), (s - back) / L::kStages & 1, abort_flag)) { give_up(1); goto done; }
         }
     } else if (warp == 1) {
         uint32_t s = 0, n = 0;
         constexpr uint64_t kDescHi = smem_desc_hi<kKBytes>(8 * kKBytes);
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
-            const uint32_t acc = n & 1;
-            if (!mbar_wait_warp(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag)) { give_up(3); goto done; }
-            tc_fence_after();
-            for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
-                const uint32_t stage = s % L::kStages, round = s / L::kStages;
-                if (!mbar_wait_warp(bar_full + 8 * stage, round & 1, abort_flag)) { give_up(2); goto done; }
+        constexpr uint32_t kInstr = instr_desc<BN>() + (PAIR ? (uint32_t)(kBM >> 4) << 24 : 0);      // (M = 256)
+        if (rank == 0)
+            for (int i = first; i < tiles; i += step, ++n) {
+                const uint32_t acc = n & 1;
+                if (!(PAIR ? __all_sync(0xffffffffu, mbar_wait_cluster(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag))
+                           : mbar_wait_warp(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag))) { give_up(3); goto done; }
                 tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t a = kDescHi | ((base + stage * L::kStage) >> 4), b = kDescHi | ((base + stage * L::kStage + kABytes) >> 4);
+                for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
+                    const uint32_t stage = s % L::kStages, round = s / L::kStages;
+                    if (!mbar_wait_warp(bar_full + 8 * stage, round & 1, abort_flag)) { give_up(2); goto done; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t a = kDescHi | ((base + stage * L::kStage) >> 4), b = kDescHi | ((base + stage * L::kStage + kABytes) >> 4);
 #pragma unroll
-                    for (int q = 0; q < kKBytes / 32; ++q) mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, instr_desc<BN>(), kb > 0 || q > 0);
-                    tc_commit(bar_empty + 8 * stage);
-                    if (kb == t.kblocks - 1) tc_commit(bar_tfull + 8 * acc);
+                        for (int q = 0; q < kKBytes / 32; ++q) {
+                            if constexpr (PAIR) pair_mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > 0 || q > 0);
+                            else mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > 0 || q > 0);
+                        }
+                        if constexpr (PAIR) {
+                            pair_commit(bar_empty + 8 * stage);
+                            if (kb == t.kblocks - 1) pair_commit(bar_tfull + 8 * acc);
+                        } else {
+                            tc_commit(bar_empty + 8 * stage);
+                            if (kb == t.kblocks - 1) tc_commit(bar_tfull + 8 * acc);
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
-        }
     } else {
         const int e = warp - 2, quarter = warp & 3;      // tensor memory lanes of this warp: 32 * (warp % 4)
         constexpr int kShare = BN / (L::kEpiWarps / 4);
@@ -254,14 +293,15 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         Channels<kCh> channels[kShare / kCh];
         // the scales of this lane's tokens: lane / 4 and every eighth behind it
         auto scales_of = [&](int m_tile, float (&s)[4]) {
-            const int64_t m = (int64_t)m_tile * kBM + quarter * 32 + (lane >> 2);
+            const int64_t m = (int64_t)rows_of(m_tile) * kBM + quarter * 32 + (lane >> 2);
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] = m + 8 * i < t.p.m ? t.p.x_scales[(m + 8 * i) * t.p.xs_stride] : 0.0f;
         };
-        tile_of(t, blockIdx.x, mt, nt);
+        tile_of(t, first, mt, nt);
         float xs[4], next_xs[4];
         scales_of(mt, xs);
-        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++n) {
+        const uint32_t lead_tempty = PAIR ? map_to_rank(bar_tempty, 0) : bar_tempty;
+        for (int i = first; i < tiles; i += step, ++n) {
             const uint32_t acc = n & 1;
             if (nt != channels_of) {
 #pragma unroll
@@ -270,7 +310,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             channels_of = nt;
             // the next tile, and its tokens' scales, while this one is worked on
             int next_mt = mt, next_nt = nt;
-            if (i + (int)gridDim.x < tiles) tile_of(t, i + gridDim.x, next_mt, next_nt);
+            if (i + step < tiles) tile_of(t, i + step, next_mt, next_nt);
             scales_of(next_mt, next_xs);
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
@@ -279,7 +319,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             for (int c = 0; c < kShare / kCh; ++c)
 #pragma unroll
                 for (int r = 0; r < 32; r += kRows) {
-                    const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
+                    const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32 + r;
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
                     if (live > 0 && c0 < t.p.n)
                         epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, m0, live, c0, channels[c], xs + r / 8, rows, to,
@@ -290,7 +330,10 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
 #pragma unroll
             for (int j = 0; j < 4; ++j) xs[j] = next_xs[j];
             tc_fence_before();
-            if (lane == 0) mbar_arrive(bar_tempty + 8 * acc);
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(lead_tempty + 8 * acc);
+                else mbar_arrive(bar_tempty + 8 * acc);
+            }
             __syncwarp();
         }
     }
@@ -304,9 +347,14 @@ done:
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) {                      // nobody leaves while the other CTA may reach into its shared or tensor memory
+        cluster_arrive();
+        cluster_wait();
+    }
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        if constexpr (PAIR) pair_tmem_dealloc(tmem, 512);
+        else tmem_dealloc(tmem, 512);
     }
 }
 
@@ -348,39 +396,43 @@ int encode_output(CUtensorMap *map, const InnerProdParams &p) {
     return TSB_OK;
 }
 
-template <typename T, int BN, bool RES>
+template <typename T, int BN, bool RES, bool PAIR = false>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
-    using L = Layout<T, BN>;
+    using L = Layout<T, BN, PAIR>;
     CUtensorMap mx, mw, my;
     int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
-    if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, BN);
+    if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, L::kBRows);
     if (st != TSB_OK) return st;
     const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
     const bool tile_store = aligned16(p.y, p.y_pitch, type) && p.y_pitch < (int64_t)1 << 37, res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     if (!tile_store) my = mx;
     else if ((st = encode_output<T>(&my, p)) != TSB_OK) return st;
-    auto kernel = inner_prod_i8_tc_kernel<T, BN, RES>;
+    auto kernel = inner_prod_i8_tc_kernel<T, BN, RES, PAIR>;
     static DeviceOnce raised;
     if (raised.first()) {
         TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
         raised.done();
     }
-    TcParams t = {p, (int)ceil_div64(p.m, kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
-    const int grid = (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148);
-    TSB_CUDA(launch_pdl(kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
+    constexpr int kCtas = PAIR ? 2 : 1;
+    TcParams t = {p, (int)ceil_div64(p.m, kBM * kCtas), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
+    const int grid = kCtas * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148 / kCtas);
+    TSB_CUDA(launch_pdl_cluster(kCtas, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");
     return TSB_OK;
 }
 
 template <typename T, bool RES>
 int pick(const InnerProdParams &p, cudaStream_t stream) {
-    // The tile's width by the clocks that its rounds take: a multiprocessor gets 64 bytes a clock, so a stage of 128 + BN rows of 128 bytes
-    // takes 2 (128 + BN); the epilogue some 9 BN.  (Measured, 64, 128 and 256 wide: 64 x 4096 x 4096 9.7, 11.0, 16.2 us, 2048 x 4096 x 4096
-    // 48.6, 35.4, 29.1, 2048 x 1000 x 2048 9.9, 8.1, 11.0.)
-    auto clocks = [&](int bn) {
-        return ceil_div64(ceil_div64(p.m, kBM) * ceil_div(p.n, bn), 148) * (ceil_div(p.k, kKBytes) * 2 * (128 + bn) + 9 * bn);
+    // The tile by the clocks that its rounds take: a multiprocessor gets 64 bytes a clock, so a stage of 128 + BN rows of 128 bytes takes
+    // 2 (128 + BN); the epilogue some 9 BN; a pair's tile, of half the rows of w for each, 3500 more for what its CTAs wait for each other.
+    // (Measured, 64, 128, 256 wide and by pairs: 64 x 4096 x 4096 9.7, 11.0, 16.2 us; 2048 x 1000 x 2048 9.9, 8.1, 11.0, 11.4;
+    // 2048 x 4096 x 4096 48.6, 35.4, 29.1, 26.3; 8192^3 - , - , 359, 331; but 16384 x 8192 x 512 80 us 256 wide, 103 by pairs.)
+    auto clocks = [&](int bn, int ctas) {
+        const int64_t rounds = ceil_div64(ceil_div64(p.m, kBM * ctas) * ceil_div(p.n, bn), 148 / ctas);
+        return rounds * (ceil_div(p.k, kKBytes) * 2 * (int64_t)(128 + bn / ctas) + 9 * bn + (ctas - 1) * 3500);
     };
-    const int64_t c64 = clocks(64), c128 = clocks(128), c256 = clocks(256);
+    const int64_t c64 = clocks(64, 1), c128 = clocks(128, 1), c256 = clocks(256, 1), pair = clocks(256, 2);
+    if (pair < std::min({c64, c128, c256})) return launch<T, 256, RES, true>(p, stream);
     if (c64 <= c128 && c64 <= c256) return launch<T, 64, RES>(p, stream);
     return c128 <= c256 ? launch<T, 128, RES>(p, stream) : launch<T, 256, RES>(p, stream);
 }

@@ -78,6 +78,19 @@ def test_kernels_agree_bit_for_bit(m):
     assert torch.equal(got[m // 2:], ops.inner_prod_quantized(d["x"][m // 2:], d["xs"][m // 2:], *args[2:5], d["residual"][m // 2:], _lib.ACT_SILU))
 
 
+@pytest.mark.parametrize("m,n,k", [(4096, 2560, 2048), (2500, 2304, 4096), (9472, 256, 4096), (2049, 4097, 2176), (2430, 2432, 8192), (4097, 2080, 1920)])
+def test_large_products(m, n, k):
+    """Sizes of many tiles a multiprocessor, of one and of two CTAs: int32 sums do not depend on their order, so a product of doubles has the
+    very bits of what is left to do in fp32."""
+    from tennis_b200 import ops
+    d = case(m, n, k, torch.float32, m, residual=False)
+    want = (d["x"].double() @ d["w"].double().t()).float() * d["ws"] * d["xs"][:, None] + d["bias"]
+    for out in FLOATS:
+        got = ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], out_dtype=out)
+        assert torch.equal(got, want.to(out))
+    ops.inner_prod_status()
+
+
 @pytest.mark.parametrize("x_pitch,x_at,w_pitch,w_at", [(512, 0, 512, 0), (512, 0, 500, 0), (501, 0, 512, 0), (512, 1, 512, 0), (512, 0, 512, 4), (520, 8, 504, 8), (1024, 16, 640, 32)])
 @pytest.mark.parametrize("m", [1, 13, 50, 300])
 def test_layouts(m, x_pitch, x_at, w_pitch, w_at):
