@@ -449,7 +449,7 @@ bool weights_fit(const InnerProdParams &p) { return operand_fits(p.w, p.n, p.w_p
 
 bool inner_prod_can(const InnerProdParams &p, const char **why) {
     if (!operand_fits(p.x, p.m, p.x_pitch, p.k) || !weights_fit(p)) { *why = "an operand's address or pitch is no multiple of 16 bytes, or its rows overlap"; return false; }
-    if (ceil_div64(p.m, kBM) * ceil_div(p.n, 64) > INT32_MAX / 2) { *why = "too many tiles"; return false; }
+    if (p.m > INT32_MAX - 2 * kBM || ceil_div64(p.m, kBM) * ceil_div(p.n, 64) > INT32_MAX / 2) { *why = "too many rows or tiles"; return false; }
     return true;
 }
 

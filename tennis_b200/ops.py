@@ -740,6 +740,8 @@ def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_N
         scales_at, n_scales = ctypes.addressof(scales), len(scales)
         want = shape[:-1] + (lib.tsb_padded_channels(c),)
     else:
+        if requant_scales is not None:
+            _refuse("requant_scales come with out_dtype int8")
         want = shape
     x_step = _pixel_step(x)
     if x_step is None:

@@ -159,6 +159,19 @@ def test_streams_and_graphs():
             assert torch.equal(got, want[i:i + 1])
 
 
+def test_refusals():
+    from tennis_b200 import ops
+    x, gamma, beta = tensors((1, 4, 4, 16), torch.float32, 8)
+    for call in (lambda: ops.group_norm_nhwc(x, 4, requant_scales=[1.0]), lambda: ops.group_norm_nhwc(x, 4, out_dtype=torch.int8), lambda: ops.group_norm_nhwc(x[0, 0], 4),
+                 lambda: ops.group_norm_nhwc(x.double(), 4), lambda: ops.group_norm_nhwc(x, 4, gamma[:8]), lambda: ops.group_norm_nhwc(x, 4, gamma, beta.double()),
+                 lambda: ops.group_norm_nhwc(x, 4, out_dtype=torch.float16), lambda: ops.group_norm_nhwc(x, 4, out=x[..., :8]),
+                 lambda: ops.group_norm_nhwc(x, 4, out=torch.empty((1, 4, 4, 16, 2), device="cuda")[..., 0])):
+        with pytest.raises(ops.EjectionException, match="Check failed"):
+            call()
+    with pytest.raises(RuntimeError, match="do not make 5 groups"):
+        ops.group_norm_nhwc(x, 5)
+
+
 def test_empty():
     from tennis_b200 import ops
     for shape in ((0, 4, 4, 8), (2, 0, 4, 8)):

@@ -167,6 +167,32 @@ def test_floating_rows(dtype, m, n, k):
         assert m <= 2 or (torch.isnan(got[2]).all() and not torch.isnan(got[0]).any())
 
 
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("k", [24, 1000, 4096, 20000, 40000])
+def test_one_floating_row(dtype, k):
+    """The row that is quantized inside the product: ordinary, of zeros, with a NaN, with an infinity, near the type's largest, misaligned."""
+    from tennis_b200 import ops
+    d = case(1, 300, k, dtype, 7, residual=False)
+    g = torch.Generator(device="cuda").manual_seed(k)
+    room = torch.randn(k + 1, device="cuda", generator=g).to(dtype)
+    for at in (0, 1):
+        for spoil in (None, "zero", "nan", "inf", "large"):
+            x = room.clone()[at:at + k].view(1, k)
+            if spoil == "zero":
+                x.zero_()
+            elif spoil == "nan":
+                x[0, k // 2] = float("nan")
+            elif spoil == "inf":
+                x[0, k - 1] = -float("inf")
+            elif spoil == "large":
+                x.mul_(0.0).add_(torch.finfo(dtype).max)
+            q, s = ops.quantize_rows(x)
+            want = ops.inner_prod_quantized(q, s, d["w"], d["ws"], d["bias"], out_dtype=dtype)
+            got = ops.inner_prod_quantized(x, None, d["w"], d["ws"], d["bias"])
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(3.0), want.nan_to_num(3.0))
+            assert torch.isnan(got).all() == (spoil == "nan")
+
+
 def test_far_offsets():
     """Outputs and operands whose offsets pass 32 bits, of elements and of bytes."""
     from tennis_b200 import ops
@@ -215,6 +241,22 @@ def test_operands_that_the_tensor_cores_cannot_read():
     with pytest.raises(_lib.TsbError, match="16 bytes"):
         ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], kernel=_lib.KERNEL_TCGEN05)
     ops.inner_prod_status()
+
+
+def test_refusals():
+    from tennis_b200 import ops
+    d = case(6, 32, 64, torch.float32, 1)
+    x, xs, w, ws, bias, res = (d[v] for v in ("x", "xs", "w", "ws", "bias", "residual"))
+    call = ops.inner_prod_quantized
+    for bad in (lambda: call(x.float(), xs, w, ws), lambda: call(x, None, w, ws), lambda: call(x.double(), None, w, ws), lambda: call(x, xs, w.float(), ws),
+                lambda: call(x, xs, w[0], ws), lambda: call(x[:, :48], xs, w, ws), lambda: call(x, xs[:5], w, ws), lambda: call(x, xs.double(), w, ws),
+                lambda: call(x, xs, w, ws[:31]), lambda: call(x, xs, w, ws, bias[:31]), lambda: call(x, xs, w, ws, bias.half()), lambda: call(x, xs, w, ws, bias, res.half()),
+                lambda: call(x, xs, w, ws, bias, res[:, :31]), lambda: call(x, xs, w, ws, out_dtype=torch.int8), lambda: call(x, xs, w, ws, out=res.t()),
+                lambda: call(x, xs, w, ws, out=res, out_dtype=torch.float16), lambda: call(x, xs, w.cpu(), ws), lambda: call(x[:, :0], xs, w[:, :0], ws)):
+        with pytest.raises(ops.EjectionException, match="Check failed"):
+            bad()
+    with pytest.raises(RuntimeError, match="activation 9"):
+        call(x, xs, w, ws, activation=9)
 
 
 def test_empty():

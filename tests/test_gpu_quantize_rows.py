@@ -116,6 +116,17 @@ def test_streams_and_graphs():
         check(x, q, s)
 
 
+def test_refusals():
+    from tennis_b200 import ops
+    x = torch.ones((4, 8), device="cuda")
+    for call in (lambda: ops.quantize_rows(x.double()), lambda: ops.quantize_rows(x[:, :0]), lambda: ops.quantize_rows(x.new_ones(())),
+                 lambda: ops.quantize_rows(x, out=torch.empty((4, 8), device="cuda")), lambda: ops.quantize_rows(x, out=torch.empty((8, 4), dtype=torch.int8, device="cuda").t()),
+                 lambda: ops.quantize_rows(x, scales=torch.ones(3, device="cuda")), lambda: ops.quantize_rows(x, scales=torch.ones(8, device="cuda")[::2]),
+                 lambda: ops.quantize_rows(x.view(2, 2, 8), out=torch.empty((2, 3, 8), dtype=torch.int8, device="cuda")[:, :2])):
+        with pytest.raises(ops.EjectionException, match="Check failed"):
+            call()
+
+
 def test_empty():
     from tennis_b200 import ops
     q, s = ops.quantize_rows(torch.empty((0, 8), device="cuda"))

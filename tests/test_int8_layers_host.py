@@ -75,8 +75,12 @@ def norm(lib, n=2, pixels=9, channels=32, groups=4, x=P, x_pixel=32, x_image=288
     (dict(eps=float("inf")), -1, "eps"), (dict(y_type=3), -1, "requant_scales"), (dict(y_type=3, scales=[1.0] * 3), -1, "one per image"),
     (dict(y_type=3, n=129, scales=[1.0] * 129), -2, "128"), (dict(x=0), -1, "null"), (dict(y=0), -1, "null"), (dict(x=P + 2), -1, "aligned"), (dict(gamma=P + 1), -1, "aligned"),
     (dict(y_type=3, y=P + 8, scales=[1.0]), -1, "aligned"), (dict(x_pixel=-32), -1, "stride"), (dict(y_pixel=31), -1, "overlap"), (dict(y_image=287), -1, "overlap"),
-    (dict(x_image=1 << 61), -1, "address range"), (dict(workspace=None), -3, "workspace"), (dict(size=16), -3, "workspace"), (dict(workspace=P + 64), -1, "256-byte")])
+    (dict(x_image=1 << 61), -1, "address range"), (dict(large=True, workspace=None), -3, "workspace"), (dict(large=True, size=16), -3, "workspace"),
+    (dict(large=True, workspace=P + 64), -1, "256-byte")])
 def test_group_norm_refuses(lib, bad, status, text):
+    bad = dict(bad)
+    if bad.pop("large", False):      # an image that no cluster holds: its sums go through a workspace
+        bad = dict(pixels=1 << 20, channels=512, x_pixel=512, x_image=1 << 29, y_pixel=512, y_image=1 << 29, **bad)
     launched = lib.tsb_kernel_launch_count()
     assert norm(lib, **bad) == status and text in lib.tsb_last_error().decode() and lib.tsb_kernel_launch_count() == launched
 
