@@ -163,6 +163,7 @@ __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scr
 // neither registers nor barriers hold loads up.  slot: its first slot, in shared memory; slot_step: bytes to the next one; KEEP: every
 // vector has a slot of its own and stays there, otherwise the kDepth slots go round.
 constexpr int kDepth = 8;
+static_assert(kDepth >= 8, "the sums' scratch, up to eight pairs a thread, lies where the slots were");
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 __device__ __forceinline__ uint4 read16(uint32_t at) {
     uint4 v;
@@ -222,7 +223,7 @@ template <typename T, typename Y, int VEC, bool ONE>
 struct Apply {
     static constexpr bool kShort = sizeof(Y) == 2;
     static constexpr int kG = ONE ? 1 : VEC;
-    float mean[kG], rstd[kShort ? 1 : kG], gamma[VEC], beta[VEC];
+    float mean[kG], rstd[kG], gamma[VEC], beta[VEC];
     // c: the thread's first channel within the run
     __device__ __forceinline__ void init(const GroupNormParams &p, const Part &t, const float2 *stats, int c) {
 #pragma unroll
@@ -240,20 +241,25 @@ struct Apply {
     __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c, Y *y) const {
         float v[VEC];
         unpack<T, VEC>(q, v);
-        if constexpr (kShort && VEC > 1) {
+        if constexpr (VEC > 1) {
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
+                const float2 g = make_float2(gamma[i], gamma[i + 1]);
                 const float2 d = add2(make_float2(v[i], v[i + 1]), make_float2(-mean[ONE ? 0 : i], -mean[ONE ? 0 : i + 1]));
-                const float2 r = fma2(d, make_float2(gamma[i], gamma[i + 1]), make_float2(beta[i], beta[i + 1]));
-                v[i] = r.x;
-                v[i + 1] = r.y;
+                if constexpr (kShort) {
+                    const float2 r = fma2(d, g, make_float2(beta[i], beta[i + 1]));
+                    v[i] = r.x;
+                    v[i + 1] = r.y;
+                } else {
+                    // (products by twos, the sum one by one: the assembler makes fused operations of a packed product and a packed sum)
+                    const float2 r = mul2(mul2(d, make_float2(rstd[ONE ? 0 : i], rstd[ONE ? 0 : i + 1])), g);
+                    v[i] = __fadd_rn(r.x, beta[i]);
+                    v[i + 1] = __fadd_rn(r.y, beta[i + 1]);
+                }
             }
         } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = __fsub_rn(v[i], mean[ONE ? 0 : i]);
-                v[i] = kShort ? fmaf(d, gamma[i], beta[i]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[ONE || kShort ? 0 : i]), gamma[i]), beta[i]);
-            }
+            const float d = __fsub_rn(v[0], mean[0]);
+            v[0] = kShort ? fmaf(d, gamma[0], beta[0]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[0]), gamma[0]), beta[0]);
         }
         activate<ACT, Y>(v, p.leaky);
         if constexpr (sizeof(Y) > 1) {
