@@ -9,6 +9,8 @@
 //              that has one token and all channels reads every channel's scales from shared memory, which then bounds the epilogue);
 //              2 KB of a warp's at a time go through shared memory: residuals are read in whole pieces, outputs written by tensor-map
 //              copies (value by value where y does not lie on 16 bytes)
+//   split      of few tiles, two or four CTAs of a cluster share one: each multiplies a part of K, hands its sums of the others' 32 channels
+//              over through distributed shared memory (int32 sums are the same in any order) and writes its own 32
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
 //
@@ -41,7 +43,7 @@ struct TcParams {
 };
 
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory
-template <typename T, int BN, bool PAIR>
+template <typename T, int BN, bool PAIR, int SPLIT = 1>
 struct Layout {
     static constexpr uint32_t kOutWarp = 2048;                                    // a warp's staged outputs
     static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
@@ -50,10 +52,11 @@ struct Layout {
     static constexpr uint32_t kBBytes = kBRows * kKBytes;
     static constexpr uint32_t kStage = kABytes + kBBytes;
     static constexpr uint32_t kOut = kEpiWarps * kOutWarp;
+    static constexpr uint32_t kParts = (SPLIT - 1) * kBM * kCh * 4;               // the other CTAs' sums of this CTA's channels
     static constexpr uint32_t kBars = 256;
-    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kBars) / kStage) < kMaxStages
-                                       ? (int)((kSmem - 1024 - kOut - kBars) / kStage) : kMaxStages;
-    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kBars;
+    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) < kMaxStages
+                                       ? (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) : kMaxStages;
+    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kParts + kBars;
 };
 
 __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, int &n_tile) {
@@ -91,8 +94,9 @@ struct Channels {
 // kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
 // the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of its own accord that is under way when this returns, else by the lanes.
-template <typename T, bool RES>
-__device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CUtensorMap *map_y, uint32_t taddr, int64_t m0, int live, int c0, const Channels<kCh> &ch, const float *xs,
+// GIVEN: the sums are in `given` already.
+template <typename T, bool RES, bool GIVEN = false>
+__device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CUtensorMap *map_y, uint32_t taddr, const int *given, int64_t m0, int live, int c0, const Channels<kCh> &ch, const float *xs,
                                               uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec) {
     using S = Staged<T>;
     constexpr int kN = Vec16<T>::kN, kHalves = S::kRows / 16, kValues = kHalves * kCh / 2;     // values of a unit; runs of 16 rows; values of a lane
@@ -100,7 +104,12 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     // value i of a lane: channels 8 j + 2 (lane % 4) + i % 2 of j = i / 4 % 4, of the row lane / 4, plus 8 for i & 2, plus 16 a half
     int acc[kValues];
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16), *reinterpret_cast<int (*)[kCh / 2]>(&acc[h * kCh / 2]));
+    for (int h = 0; h < kHalves; ++h)
+        if (!GIVEN) tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16), *reinterpret_cast<int (*)[kCh / 2]>(&acc[h * kCh / 2]));
+    if (GIVEN) {
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) acc[i] = given[i];
+    }
     auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
     float v[kValues], res[RES ? kValues : 1];
     if constexpr (RES) {
@@ -131,7 +140,7 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
 #pragma unroll
         for (int i = 0; i < kValues; ++i) res[i] = to_f32(reinterpret_cast<const T *>(at(i))[i & 1]);
     }
-    tmem_ld_wait();
+    if (!GIVEN) tmem_ld_wait();
     inner_prod_values<T, RES>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4 % (kCh / 8)], xs[i / (kCh / 2) * 2 + (i >> 1 & 1)], ch.bias[i / 4 % (kCh / 8)]}; },
                          [&](int i) { return res[RES ? i : 0]; }, v);
     if (!RES && lane == 0) bulk_wait_read();
@@ -162,22 +171,26 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     }
 }
 
-template <typename T, int BN, bool RES, bool PAIR>
-__global__ void __launch_bounds__(Layout<T, BN, PAIR>::kThreads, 1)
+template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
+__global__ void __launch_bounds__(Layout<T, BN, PAIR, SPLIT>::kThreads, 1)
 inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
                         const __grid_constant__ TcParams t, int tile_store, int res_vec) {
-    using L = Layout<T, BN, PAIR>;
+    static_assert(SPLIT == 1 || (!PAIR && BN == kCh * SPLIT), "split: kCh channels of the tile for each CTA");
+    using L = Layout<T, BN, PAIR, SPLIT>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
     uint8_t *out_rows = smem_raw + (base - raw) + L::kStages * L::kStage;
-    uint8_t *bars_ptr = out_rows + L::kOut;
+    uint8_t *parts = out_rows + L::kOut, *bars_ptr = parts + L::kParts;
     const uint32_t bar_full = smem_u32(bars_ptr), bar_empty = bar_full + 8 * kMaxStages, bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars_ptr + 8 * (2 * kMaxStages + 4));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bars_ptr + 8 * (2 * kMaxStages + 4) + 4);
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int tiles = t.tiles_m * t.tiles_n;
-    const int rank = PAIR ? (int)cluster_rank() : 0, first = PAIR ? (int)blockIdx.x / 2 : (int)blockIdx.x, step = PAIR ? (int)gridDim.x / 2 : (int)gridDim.x;
+    constexpr int kCluster = PAIR ? 2 : SPLIT;
+    const int rank = kCluster > 1 ? (int)cluster_rank() : 0, first = (int)blockIdx.x / kCluster, step = (int)gridDim.x / kCluster;
+    // the blocks of K that this CTA multiplies (split: a part of its tile's)
+    const int kb0 = SPLIT > 1 ? t.kblocks * rank / SPLIT : 0, kb1 = SPLIT > 1 ? t.kblocks * (rank + 1) / SPLIT : t.kblocks;
     auto rows_of = [&](int m_tile) { return PAIR ? 2 * m_tile + rank : m_tile; };      // this CTA's 128 tokens of a tile
 
     if (warp == 0) {
@@ -209,12 +222,13 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
     }
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) {                      // the other CTA's barriers and tensor memory are there too
+    if constexpr (kCluster > 1) {              // the other CTAs' shared and tensor memory are there too
         cluster_arrive();
         cluster_wait();
     }
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    bool met = false;                          // split: this warp has been at the cluster's meeting
     pdl_sync();
     auto give_up = [&](int code) {
         if (!*abort_flag) { *abort_flag = 1; atomicExch(&g_status, code); }
@@ -228,11 +242,11 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         for (int i = first; i < tiles; i += step) {
             int mt, nt;
             tile_of(t, i, mt, nt);
-            for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
+            for (int kb = kb0; kb < kb1; ++kb, ++s) {
                 const uint32_t stage = s % L::kStages, round = s / L::kStages, at = base + stage * L::kStage;
                 if (!mbar_wait_warp(bar_empty + 8 * stage, (round & 1) ^ 1, abort_flag)) { give_up(1); goto done; }
                 if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, PAIR ? 2 * L::kStage : L::kStage);
+                    if (!PAIR || rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, PAIR ? 2 * L::kStage : L::kStage);
                     if constexpr (PAIR) {
                         pair_tma_load_2d(at, &map_x, lead_full + 8 * stage, kb * kKBytes, rows_of(mt) * kBM);
                         pair_tma_load_2d(at + kABytes, &map_w, lead_full + 8 * stage, kb * kKBytes, nt * BN + rank * L::kBRows);
@@ -253,13 +267,13 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         uint32_t s = 0, n = 0;
         constexpr uint64_t kDescHi = smem_desc_hi<kKBytes>(8 * kKBytes);
         constexpr uint32_t kInstr = instr_desc<BN>() + (PAIR ? (uint32_t)(kBM >> 4) << 24 : 0);      // (M = 256)
-        if (rank == 0)
+        if (!PAIR || rank == 0)
             for (int i = first; i < tiles; i += step, ++n) {
                 const uint32_t acc = n & 1;
                 if (!(PAIR ? __all_sync(0xffffffffu, mbar_wait_cluster(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag))
                            : mbar_wait_warp(bar_tempty + 8 * acc, ((n >> 1) & 1) ^ 1, abort_flag))) { give_up(3); goto done; }
                 tc_fence_after();
-                for (int kb = 0; kb < t.kblocks; ++kb, ++s) {
+                for (int kb = kb0; kb < kb1; ++kb, ++s) {
                     const uint32_t stage = s % L::kStages, round = s / L::kStages;
                     if (!mbar_wait_warp(bar_full + 8 * stage, round & 1, abort_flag)) { give_up(2); goto done; }
                     tc_fence_after();
@@ -267,15 +281,15 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
                         const uint64_t a = kDescHi | ((base + stage * L::kStage) >> 4), b = kDescHi | ((base + stage * L::kStage + kABytes) >> 4);
 #pragma unroll
                         for (int q = 0; q < kKBytes / 32; ++q) {
-                            if constexpr (PAIR) pair_mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > 0 || q > 0);
-                            else mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > 0 || q > 0);
+                            if constexpr (PAIR) pair_mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > kb0 || q > 0);
+                            else mma_i8(tmem + acc * BN, a + 2 * q, b + 2 * q, kInstr, kb > kb0 || q > 0);
                         }
                         if constexpr (PAIR) {
                             pair_commit(bar_empty + 8 * stage);
-                            if (kb == t.kblocks - 1) pair_commit(bar_tfull + 8 * acc);
+                            if (kb == kb1 - 1) pair_commit(bar_tfull + 8 * acc);
                         } else {
                             tc_commit(bar_empty + 8 * stage);
-                            if (kb == t.kblocks - 1) tc_commit(bar_tfull + 8 * acc);
+                            if (kb == kb1 - 1) tc_commit(bar_tfull + 8 * acc);
                         }
                     }
                     __syncwarp();
@@ -315,14 +329,57 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
             constexpr int kRows = Staged<T>::kRows;
+            if constexpr (SPLIT > 1) {
+                // The tile's channels kCh j are CTA j's: its sums come from the CTAs of the cluster, each with a part of K.  A lane's sums of a
+                // fragment travel as they are, to the same lane of the same quarter: parts[sender, in the order of ranks][quarter][16 bytes i][lane]
+                constexpr int kLane = kCh;                        // sums of a lane
+                const int owner = e / 4;
+                const bool any = (int64_t)mt * kBM + quarter * 32 < t.p.m;
+                int sum[kLane];
+                if (any) {
 #pragma unroll
-            for (int c = 0; c < kShare / kCh; ++c)
+                    for (int h = 0; h < 2; ++h)
+                        tmem_ld_rows16(tmem + acc * BN + ((uint32_t)(quarter * 32 + h * 16) << 16) + share, *reinterpret_cast<int (*)[kLane / 2]>(&sum[h * kLane / 2]));
+                    tmem_ld_wait();
+                    if (owner != rank) {
+                        const int slot = rank < owner ? rank : rank - 1;
+                        const uint32_t to_rank = map_to_rank(smem_u32(parts) + (slot * 4 + quarter) * (kLane * 32 * 4) + lane * 16, owner);
+#pragma unroll
+                        for (int i = 0; i < kLane / 4; ++i) sts128_cluster(to_rank + i * 512, sum[4 * i], sum[4 * i + 1], sum[4 * i + 2], sum[4 * i + 3]);
+                    }
+                }
+                cluster_arrive();
+                cluster_wait();
+                met = true;
+                if (any && owner == rank) {
+#pragma unroll
+                    for (int from = 0; from < SPLIT - 1; ++from)
+#pragma unroll
+                        for (int i = 0; i < kLane / 4; ++i) {
+                            const int4 v = *reinterpret_cast<const int4 *>(parts + (from * 4 + quarter) * (kLane * 32 * 4) + i * 512 + lane * 16);
+                            sum[4 * i] += v.x;
+                            sum[4 * i + 1] += v.y;
+                            sum[4 * i + 2] += v.z;
+                            sum[4 * i + 3] += v.w;
+                        }
+#pragma unroll
+                    for (int r = 0; r < 32; r += kRows) {
+                        const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
+                        const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share;
+                        if (live > 0 && c0 < t.p.n)
+                            epilogue_rows<T, RES, true>(t.p, &map_y, 0, sum + r / 16 * (kLane / 2), m0, live, c0, channels[0], xs + r / 8, rows, to, tile_store != 0, res_vec != 0);
+                    }
+                }
+                goto done;
+            }
+#pragma unroll
+            for (int c = 0; c < (SPLIT > 1 ? 0 : kShare / kCh); ++c)
 #pragma unroll
                 for (int r = 0; r < 32; r += kRows) {
                     const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32 + r;
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
                     if (live > 0 && c0 < t.p.n)
-                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, m0, live, c0, channels[c], xs + r / 8, rows, to,
+                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, nullptr, m0, live, c0, channels[c], xs + r / 8, rows, to,
                                          tile_store != 0, res_vec != 0);
                 }
             mt = next_mt;
@@ -345,11 +402,19 @@ done:
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
     }
     __syncwarp();
+    if constexpr (SPLIT > 1) {
+        // The epilogue warps have met those of the other CTAs above, for which every thread of the cluster has to arrive: the other warps, and
+        // one that gave up in front of that, do so here -- ahead of the block's own barrier, where the waiting warps are still missing.
+        if (!met) cluster_arrive();
+    }
     tc_fence_before();
     __syncthreads();
     if constexpr (PAIR) {                      // nobody leaves while the other CTA may reach into its shared or tensor memory
         cluster_arrive();
         cluster_wait();
+    }
+    if constexpr (SPLIT > 1) {
+        if (!met) cluster_wait();
     }
     if (warp == 1) {
         tc_fence_after();
@@ -396,9 +461,9 @@ int encode_output(CUtensorMap *map, const InnerProdParams &p) {
     return TSB_OK;
 }
 
-template <typename T, int BN, bool RES, bool PAIR = false>
+template <typename T, int BN, bool RES, bool PAIR = false, int SPLIT = 1>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
-    using L = Layout<T, BN, PAIR>;
+    using L = Layout<T, BN, PAIR, SPLIT>;
     CUtensorMap mx, mw, my;
     int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
     if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, L::kBRows);
@@ -407,16 +472,16 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
     const bool tile_store = aligned16(p.y, p.y_pitch, type) && p.y_pitch < (int64_t)1 << 37, res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     if (!tile_store) my = mx;
     else if ((st = encode_output<T>(&my, p)) != TSB_OK) return st;
-    auto kernel = inner_prod_i8_tc_kernel<T, BN, RES, PAIR>;
+    auto kernel = inner_prod_i8_tc_kernel<T, BN, RES, PAIR, SPLIT>;
     static DeviceOnce raised;
     if (raised.first()) {
         TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
         raised.done();
     }
-    constexpr int kCtas = PAIR ? 2 : 1;
-    TcParams t = {p, (int)ceil_div64(p.m, kBM * kCtas), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
-    const int grid = kCtas * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, 148 / kCtas);
-    TSB_CUDA(launch_pdl_cluster(kCtas, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
+    constexpr int kCluster = PAIR ? 2 : SPLIT;
+    TcParams t = {p, (int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
+    const int grid = kCluster * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, SPLIT > 1 ? INT32_MAX : 148 / kCluster);      // (split: a tile a cluster)
+    TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");
     return TSB_OK;
 }
@@ -432,6 +497,14 @@ int pick(const InnerProdParams &p, cudaStream_t stream) {
         return rounds * (ceil_div(p.k, kKBytes) * 2 * (int64_t)(128 + bn / ctas) + 9 * bn + (ctas - 1) * 3500);
     };
     const int64_t c64 = clocks(64, 1), c128 = clocks(128, 1), c256 = clocks(256, 1), pair = clocks(256, 2);
+    // Few tiles: two or four CTAs a tile, each with a part of K, and 2000 clocks for handing sums over.  (64 x 2048 x 8192 15.4 -> 9.6 us,
+    // 64 x 4096 x 4096 9.6 -> 8.1, 64 x 1000 x 2048 5.8 -> 4.9.)
+    auto split_clocks = [&](int ctas) {
+        const int64_t tiles = ceil_div64(p.m, kBM) * ceil_div(p.n, kCh * ctas), blocks = ceil_div(p.k, kKBytes);
+        return tiles * ctas > 148 || blocks < ctas ? INT64_MAX : ceil_div64(blocks, ctas) * 2 * (128 + kCh * ctas) + 9 * kCh * ctas + 2000;
+    };
+    const int64_t split2 = split_clocks(2), split4 = split_clocks(4), whole = std::min({c64, c128, c256, pair});
+    if (std::min(split2, split4) < whole) return split4 <= split2 ? launch<T, 128, RES, false, 4>(p, stream) : launch<T, 64, RES, false, 2>(p, stream);
     if (pair < std::min({c64, c128, c256})) return launch<T, 256, RES, true>(p, stream);
     if (c64 <= c128 && c64 <= c256) return launch<T, 64, RES>(p, stream);
     return c128 <= c256 ? launch<T, 128, RES>(p, stream) : launch<T, 256, RES>(p, stream);
