@@ -13,6 +13,8 @@
 //              order, so that it finds in the L2 what the first read last.  (Batch by batch, each small enough for the L2, the
 //              launches' beginnings and ends cost more than the reads of HBM that they save: 8 x 256 x 256 x 256 bf16 152 us in one
 //              batch, 176 in batches of two images, 266 image by image)
+// Measured: 16 x 56 x 56 x 256 bf16 to int8 20 us (resident; load, meeting and writing follow each other in its one round of blocks), 8 x 256 x 256 x 256
+// bf16 154 us (swept: 805 MB at 5.2 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.6 us.
 #include "typed.cuh"
 
 #include <algorithm>

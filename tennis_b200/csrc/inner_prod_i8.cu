@@ -9,7 +9,8 @@ namespace tsb {
 namespace {
 
 // ---- CUDA-core kernel: any alignment, any pitch -----------------------------------------------------------------------
-// A block computes 64 tokens x 64 output channels, 16 values a thread (4 x 4), 64 bytes of K at a time from shared memory.
+// A block computes 64 tokens x 64 output channels, 16 values a thread (4 x 4), 64 bytes of K at a time from shared memory.  Bound by dp4a and the
+// shared-memory reads that feed it (8192^3 10.5 ms, 0.1 POPS): for operands that the copies of the other kernels cannot read.
 constexpr int kTile = 64, kTileK = 64, kThreads = 256;
 constexpr int kRow = kTileK / 4 + 1;      // words of a staged row; odd, so that neighbouring rows lie in different banks
 

@@ -1,8 +1,9 @@
 // The int8 inner product on the sm_100a tensor cores: y [m, n] = x [m, k] . w [n, k], both operands K-major as they lie in memory.
 //
 //   tile       128 tokens x BN output channels (or 256 x 256 of two CTAs, each with its half of both operands: a multiprocessor then reads
-//              32 instead of 48 KB for the same arithmetic, and its 64 bytes a clock no longer bound the MMAs), 128 bytes of K a stage: two TMA boxes (128-byte swizzle; rows and columns behind the
-//              matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums in tensor memory, two buffers of them
+//              32 instead of 48 KB for the same arithmetic, and its 64 bytes a clock no longer bound the MMAs), 128 bytes of K a stage: two
+//              TMA boxes (128-byte swizzle; rows and columns behind the matrices' ends arrive as zeros) feed tcgen05.mma kind::i8, int32 sums
+//              in tensor memory, two buffers of them
 //   roles      warp 0 loads, warp 1 issues the MMAs, sixteen warps (eight of narrow tiles) turn finished sums into outputs while the next
 //              tile is computed
 //   epilogue   sums come in fragments, so that a lane has the same few channels of many tokens and keeps their scales in registers (a lane
@@ -13,6 +14,9 @@
 //              over through distributed shared memory (int32 sums are the same in any order) and writes its own 32
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
+//
+// Measured, bf16 out: 8192^3 331 us (3.3 POPS, tensor pipe 90 % active), 4096^3 48 us, 64 x 4096 x 4096 8.1 us; 100352 x 256 x 64 20 us, where
+// the epilogue bounds it (silu: 27).
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and
 // all roles go to the common exit.

