@@ -522,17 +522,28 @@ def repack_nhwc_to_nchw(x, channels, stream=None):
 # ---- int8 layers with scales per token: quantize_rows, inner_prod_quantized, group_norm_nhwc --------------------------------
 # These three work on the device that their tensors are on, on its current stream or on `stream`; what they allocate (outputs,
 # workspace) belongs to that stream.  Memory of an input that another stream allocated is the caller's to keep until the work is done.
-# A kernel of theirs can be done in 2 us, so the host's way to it counts: a check is a comparison whose text is made only when it
-# fails, and the allocation that compiled programs use takes 0.8 us where torch.empty takes 2.3 (empty_strided 1.5).
+# Ordinary calls go through native.cpp (4 us a call); the Python below them is the general way: every layout, outputs of the caller's,
+# other streams and devices, and the texts of refusals.
 _TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16, torch.int8: _lib.TYPE_I8}
 _FLOATS = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _FLOAT_NAMES = "float32, float16 or bfloat16, not %s"
 _int8, _float32 = torch.int8, torch.float32
-try:
-    from torch._C._dynamo.guards import _empty_strided_cuda as _room       # (sizes, strides, dtype), on the current device
-except ImportError:
-    def _room(size, stride, dtype):
-        return torch.empty_strided(size, stride, dtype=dtype, device="cuda")
+
+
+_native = None
+
+
+def _ordinary():
+    """The calls of native.cpp: an operator's result where tensors, layouts and arguments are the ordinary ones, else None."""
+    global _native
+    _lib.load()
+    try:
+        from . import _native as module
+    except ImportError as e:
+        raise RuntimeError("tennis_b200: the module _native has not been built (python -c 'import __graft_entry__ as g; g.build()' or make -C "
+                           "tennis_b200/csrc): %s" % e)
+    _native = module
+    return module
 
 
 def _refuse(text, *values):
@@ -581,6 +592,10 @@ def quantize_rows(x, out=None, scales=None, stream=None):
     q is [..., k]; its rows start a multiple of 16 bytes apart, the way inner_prod_quantized reads them fastest.  The rows of x are
     tokens of an activation, or output channels of a weight tensor.  ``out`` (int8, x's shape, values of a row next to each other)
     and ``scales`` take the results where they are given."""
+    if out is None and scales is None and stream is None:
+        done = (_native or _ordinary()).quantize_rows(x)
+        if done is not None:
+            return done
     device = x.get_device()
     if device < 0 or stream is not None or device != _current_device():
         return _elsewhere(quantize_rows, x, stream, out, scales)
@@ -594,14 +609,14 @@ def quantize_rows(x, out=None, scales=None, stream=None):
     m, k = rows.shape
     if out is None:
         pitch = (k + 15) // 16 * 16
-        q = _room((m, k), (pitch, 1), _int8)
+        q = torch.empty_strided((m, k), (pitch, 1), dtype=_int8, device=x.device)
         out = q if len(shape) == 2 else q.view(shape) if k == pitch else torch.empty(shape[:-1] + (pitch,), dtype=_int8, device=x.device)[..., :k]
     elif out.dtype is not _int8 or out.shape != shape or out.get_device() != device or (out.stride(-1) != 1 and k > 1):
         _refuse("out: int8 of x's shape on x's device, values of a row next to each other")
     if out.numel():
         q = _rows_to(out)
     if scales is None:
-        scales = _room((m,), (1,), _float32)
+        scales = torch.empty((m,), dtype=_float32, device=x.device)
         if len(shape) != 2:
             scales = scales.view(shape[:-1])
     else:
@@ -622,6 +637,10 @@ def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, act
     its rows are quantized in the call.  w int8 and w_scales [n] are what quantize_rows makes of a float weight tensor.  ``residual``
     has the output's type and shape.  ``out_dtype`` is x's type (of int8 rows: float32) unless given; ``out`` takes the result where
     it is given (it may be ``residual``, and no other operand)."""
+    if out is None and stream is None and kernel == KERNEL_AUTO:
+        done = (_native or _ordinary()).inner_prod(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, bool(residual_after_activation))
+        if done is not None:
+            return done
     device = x.get_device()
     if device < 0 or stream is not None or device != _current_device():
         return _elsewhere(inner_prod_quantized, x, stream, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, out,
@@ -657,7 +676,7 @@ def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, act
         _refuse("out_dtype: " + _FLOAT_NAMES, dtype)
     want = (m, n) if len(shape) == 2 else shape[:-1] + (n,)
     if out is None:
-        y = _room((m, n), (n, 1), dtype)
+        y = torch.empty((m, n), dtype=dtype, device=x.device)
         out = y if len(shape) == 2 else y.view(want)
     else:
         if out.dtype is not dtype or out.shape != want or out.get_device() != device or (out.stride(-1) != 1 and n > 1):
@@ -678,15 +697,9 @@ def inner_prod_quantized(x, x_scales, w, w_scales, bias=None, residual=None, act
                                      1 if residual_after_activation else 0, kernel)
     workspace = size = 0
     if x_scales is None:
-        if m == 1:                        # (quantized inside, mostly: no workspace)
-            status = lib.tsb_inner_prod_i8(args, 0, 0, _current_raw_stream(device))
-            if not status:
-                return out
-            if status != _lib.ERR_WORKSPACE_TOO_SMALL:
-                check(status)
         size = lib.tsb_inner_prod_i8_workspace_bytes(args)
         if size:
-            room = _room((size,), (1,), torch.uint8)
+            room = torch.empty((size,), dtype=torch.uint8, device=x.device)
             workspace = room.data_ptr()
     status = lib.tsb_inner_prod_i8(args, workspace, size, _current_raw_stream(device))
     if status:
@@ -709,6 +722,10 @@ def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_N
     The result has x's type and shape (``out`` takes it where it is given; it may be x).  ``out_dtype=torch.int8`` with
     ``requant_scales`` (one, or one per image) gives ``quantize`` of it as NHWC_PAD [n, ..., padded_channels(channels)] instead, what
     a convolution plan reads."""
+    if out is None and stream is None:
+        done = (_native or _ordinary()).group_norm(x, groups, gamma, beta, eps, activation, leaky, out_dtype, requant_scales)
+        if done is not None:
+            return done
     device = x.get_device()
     if device < 0 or stream is not None or device != _current_device():
         return _elsewhere(group_norm_nhwc, x, stream, groups, gamma, beta, eps, activation, leaky, out_dtype, requant_scales, out)
@@ -761,7 +778,7 @@ def group_norm_nhwc(x, groups, gamma=None, beta=None, eps=1e-5, activation=ACT_N
     size = lib.tsb_group_norm_workspace_bytes(desc)
     workspace = 0
     if size:
-        room = _room((size,), (1,), torch.uint8)
+        room = torch.empty((size,), dtype=torch.uint8, device=x.device)
         workspace = room.data_ptr()
     status = lib.tsb_group_norm_nhwc(desc, workspace, size, _current_raw_stream(device))
     if status:

@@ -243,6 +243,31 @@ def test_operands_that_the_tensor_cores_cannot_read():
     ops.inner_prod_status()
 
 
+@pytest.mark.parametrize("lead", [(5,), (2, 3), (1, 2, 2)])
+def test_ordinary_and_general_calls_agree(lead):
+    """The module for ordinary calls and the Python behind it give the same tensors, for each operator and type."""
+    from tennis_b200 import ops
+    here = dict(stream=torch.cuda.current_stream())
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for dtype in FLOATS:
+        x = torch.randn(lead + (96,), device="cuda", generator=g).to(dtype)
+        w, ws = ops.quantize_rows(torch.randn((40, 96), device="cuda", generator=g))
+        bias, res = torch.randn(40, device="cuda", generator=g), torch.randn(lead + (40,), device="cuda", generator=g)
+        for one, other in zip(ops.quantize_rows(x), ops.quantize_rows(x, **here)):
+            assert torch.equal(one, other) and one.stride() == other.stride()
+        q, s = ops.quantize_rows(x)
+        for args in ((x, None, w, ws), (x, None, w, ws, bias), (q, s, w, ws, bias, res, 3), (q, s.flatten()[:1].contiguous(), w, ws), (q, s, w, ws, None, None, 2, 0.1)):
+            one, other = ops.inner_prod_quantized(*args), ops.inner_prod_quantized(*args, **here)
+            assert torch.equal(one, other) and one.dtype == other.dtype and one.shape == other.shape == lead + (40,)
+        assert torch.equal(ops.inner_prod_quantized(q, s, w, ws, bias, res, 1, residual_after_activation=True),
+                           ops.inner_prod_quantized(q, s, w, ws, bias, res, 1, residual_after_activation=True, **here))
+        image = torch.randn((2, 6, 5, 48), device="cuda", generator=g).to(dtype)
+        gamma, beta = torch.randn(48, device="cuda", generator=g), torch.randn(48, device="cuda", generator=g)
+        for kw in (dict(), dict(gamma=gamma, beta=beta, eps=1e-3, activation=2, leaky=0.2), dict(out_dtype=torch.int8, requant_scales=[9.0, 11.0]), dict(out_dtype=dtype)):
+            one, other = ops.group_norm_nhwc(image, 6, **kw), ops.group_norm_nhwc(image, 6, **kw, **here)
+            assert torch.equal(one, other) and one.dtype == other.dtype
+
+
 def test_refusals():
     from tennis_b200 import ops
     d = case(6, 32, 64, torch.float32, 1)

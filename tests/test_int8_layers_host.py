@@ -130,6 +130,21 @@ def test_operators_refuse_host_tensors():
             call()
 
 
+def test_the_module_of_ordinary_calls(monkeypatch):
+    """It takes nothing that is not ordinary, and its absence is told."""
+    from tennis_b200 import ops
+    native = ops._ordinary()
+    assert native.quantize_rows(cpu((2, 8))) is None and native.quantize_rows("x") is None and native.quantize_rows() is None
+    assert native.inner_prod(*[None] * 10) is None and native.inner_prod(cpu((2, 8)), None, cpu((4, 8), torch.int8), cpu(4), None, None, 0, 0.0, None, False) is None
+    assert native.group_norm(*[None] * 9) is None and native.group_norm(cpu((1, 2, 2, 8)), 2, None, None, 1e-5, 0, 0.0, None, None) is None
+    import sys
+    monkeypatch.setattr(ops, "_native", None)
+    monkeypatch.delattr(__import__("tennis_b200"), "_native", raising=False)
+    monkeypatch.setitem(sys.modules, "tennis_b200._native", None)
+    with pytest.raises(RuntimeError, match="_native has not been built"):
+        ops.quantize_rows(cpu((2, 8)))
+
+
 def test_pixel_step():
     from tennis_b200.ops import _pixel_step
     x = cpu((2, 5, 6, 16))
