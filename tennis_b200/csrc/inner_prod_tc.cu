@@ -95,13 +95,44 @@ struct Channels {
     }
 };
 
+// The residual of such a step into `rows`, once the copy that reads these rows last has done so.
+template <typename T>
+__device__ __forceinline__ void fetch_residual(const InnerProdParams &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
+    using S = Staged<T>;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) bulk_wait_read();
+    __syncwarp();
+    if (res_vec && c0 + kCh <= p.n) {
+        constexpr int kN = Vec16<T>::kN, kStep = 32 / S::kUnits;
+        const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
+        const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
+        const int64_t step = kStep * p.residual_pitch;
+#pragma unroll
+        for (int r = 0; r < S::kRows; r += kStep, from += step)
+            if (r + r0 < live) *reinterpret_cast<uint4 *>(rows + S::unit(r + r0, u0)) = *reinterpret_cast<const uint4 *>(from);
+    } else {
+        // value by value, neighbouring lanes neighbouring channels
+        const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
+        T some[8];
+        for (int r = 0; r < live; r += 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i, from += p.residual_pitch)
+                if (r + i < live && c0 + lane < p.n) some[i] = *from;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (r + i < live && c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, lane)) = some[i];
+        }
+    }
+    __syncwarp();
+}
+
 // kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
 // the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of its own accord that is under way when this returns, else by the lanes.
-// GIVEN: the sums are in `given` already.
+// fetched: the residual is in `rows` already.  GIVEN: the sums are in `given` already.
 template <typename T, bool RES, bool GIVEN = false>
 __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CUtensorMap *map_y, uint32_t taddr, const int *given, int64_t m0, int live, int c0, const Channels<kCh> &ch, const float *xs,
-                                              uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec) {
+                                              uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec, bool fetched) {
     using S = Staged<T>;
     constexpr int kN = Vec16<T>::kN, kHalves = S::kRows / 16, kValues = kHalves * kCh / 2;     // values of a unit; runs of 16 rows; values of a lane
     const int lane = threadIdx.x & 31;
@@ -117,30 +148,7 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
     auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
     float v[kValues], res[RES ? kValues : 1];
     if constexpr (RES) {
-        if (lane == 0) bulk_wait_read();       // (the copy that reads these rows last)
-        __syncwarp();
-        if (res_vec && c0 + kCh <= p.n) {
-            const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
-            constexpr int kStep = 32 / S::kUnits;
-            const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
-            const int64_t step = kStep * p.residual_pitch;
-#pragma unroll
-            for (int r = 0; r < S::kRows; r += kStep, from += step)
-                if (r + r0 < live) *reinterpret_cast<uint4 *>(rows + S::unit(r + r0, u0)) = *reinterpret_cast<const uint4 *>(from);
-        } else {
-            // value by value, neighbouring lanes neighbouring channels
-            const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
-            T some[8];
-            for (int r = 0; r < live; r += 8) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i, from += p.residual_pitch)
-                    if (r + i < live && c0 + lane < p.n) some[i] = *from;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (r + i < live && c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, lane)) = some[i];
-            }
-        }
-        __syncwarp();
+        if (!fetched) fetch_residual<T>(p, m0, live, c0, rows, res_vec);
 #pragma unroll
         for (int i = 0; i < kValues; ++i) res[i] = to_f32(reinterpret_cast<const T *>(at(i))[i & 1]);
     }
@@ -330,9 +338,14 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             int next_mt = mt, next_nt = nt;
             if (i + step < tiles) tile_of(t, i + step, next_mt, next_nt);
             scales_of(next_mt, next_xs);
+            constexpr int kRows = Staged<T>::kRows;
+            if constexpr (RES) {                       // (the first step's, while the sums are not there yet)
+                const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32;
+                const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0));
+                if (live > 0 && nt * BN + share < t.p.n && (SPLIT == 1 || e / 4 == rank)) fetch_residual<T>(t.p, m0, live, nt * BN + share, rows, res_vec != 0);
+            }
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
-            constexpr int kRows = Staged<T>::kRows;
             if constexpr (SPLIT > 1) {
                 // The tile's channels kCh j are CTA j's: its sums come from the CTAs of the cluster, each with a part of K.  A lane's sums of a
                 // fragment travel as they are, to the same lane of the same quarter: parts[sender, in the order of ranks][quarter][16 bytes i][lane]
@@ -371,7 +384,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
                         const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
                         const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share;
                         if (live > 0 && c0 < t.p.n)
-                            epilogue_rows<T, RES, true>(t.p, &map_y, 0, sum + r / 16 * (kLane / 2), m0, live, c0, channels[0], xs + r / 8, rows, to, tile_store != 0, res_vec != 0);
+                            epilogue_rows<T, RES, true>(t.p, &map_y, 0, sum + r / 16 * (kLane / 2), m0, live, c0, channels[0], xs + r / 8, rows, to, tile_store != 0, res_vec != 0, RES && r == 0);
                     }
                 }
                 goto done;
@@ -384,7 +397,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
                     if (live > 0 && c0 < t.p.n)
                         epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, nullptr, m0, live, c0, channels[c], xs + r / 8, rows, to,
-                                         tile_store != 0, res_vec != 0);
+                                         tile_store != 0, res_vec != 0, RES && c == 0 && r == 0);
                 }
             mt = next_mt;
             nt = next_nt;
