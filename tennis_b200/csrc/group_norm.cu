@@ -14,7 +14,7 @@
 //              launches' beginnings and ends cost more than the reads of HBM that they save: 8 x 256 x 256 x 256 bf16 152 us in one
 //              batch, 176 in batches of two images, 266 image by image)
 // Measured: 16 x 56 x 56 x 256 bf16 to int8 20 us (resident; load, meeting and writing follow each other in its one round of blocks), 8 x 256 x 256 x 256
-// bf16 154 us (swept: 805 MB at 5.2 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.6 us.
+// bf16 151 us (swept: 805 MB at 5.3 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.6 us.
 #include "typed.cuh"
 
 #include <algorithm>
@@ -41,6 +41,7 @@ struct GroupNormParams {
     int cols;                                     // vectors of a run that the block's threads own at a time
     int64_t tile;                                 // pixels of a block's tile
     int tiles;                                    // ... and tiles of an image
+    int let_go;                                   // swept: tiles whose values are not kept in the L2 for the second reading, which starts with the last
     double eps, one_over_count;                   // of a group's values: a product with it is off by half a step of 64 bits more than a quotient
     int activation;
     float leaky;
@@ -166,14 +167,24 @@ __device__ __forceinline__ void collect(const Sums<VEC, ONE> &sums, double2 *scr
 // vector has a slot of its own and stays there, otherwise the kDepth slots go round.
 constexpr int kDepth = 8;
 static_assert(kDepth >= 8, "the sums' scratch, up to eight pairs a thread, lies where the slots were");
+// (policy: which values the L2 lets go of first)
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t l2_policy(bool first_out) {
+    uint64_t p;
+    if (first_out) asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    else asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
 __device__ __forceinline__ uint4 read16(uint32_t at) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
 }
 template <typename T, int VEC, bool KEEP, typename Use>
-__device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t slot, uint32_t slot_step, const Use &use) {
+__device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t slot, uint32_t slot_step, uint64_t policy, const Use &use) {
     if constexpr (VEC > 1) {
         constexpr int kAhead = KEEP ? 4 * kDepth : kDepth;
         const T *next = x;
@@ -181,7 +192,7 @@ __device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t
         const uint32_t end = slot + kAhead * slot_step;
 #pragma unroll 4
         for (int i = 0; i < kAhead; ++i, next += step, to += slot_step) {
-            if (i < n) copy16(to, next);
+            if (i < n) KEEP ? copy16(to, next) : copy16(to, next, policy);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
         if (!KEEP) to = slot;
@@ -189,7 +200,7 @@ __device__ __forceinline__ void stream(const T *x, int64_t step, int n, uint32_t
         for (int i = 0; i < n; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
             use(i, read16(at));
-            if (i + kAhead < n) copy16(to, next);
+            if (i + kAhead < n) KEEP ? copy16(to, next) : copy16(to, next, policy);
             asm volatile("cp.async.commit_group;" ::: "memory");
             next += step;
             to += slot_step;
@@ -238,9 +249,9 @@ struct Apply {
             else if (i < kG) rstd[i] = st.y;
         }
     }
-    // y: where the thread's channels of `pixel` go
+    // y: where the thread's channels of `pixel` go; first_out: they are the first that the L2 lets go of
     template <int ACT>
-    __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c, Y *y) const {
+    __device__ __forceinline__ void run(const GroupNormParams &p, const Part &t, const typename Raw<T, VEC>::type &q, int64_t pixel, int c, Y *y, bool first_out) const {
         float v[VEC];
         unpack<T, VEC>(q, v);
         if constexpr (VEC > 1) {
@@ -266,6 +277,7 @@ struct Apply {
         activate<ACT, Y>(v, p.leaky);
         if constexpr (sizeof(Y) > 1) {
             if constexpr (VEC == 1) *y = from_f32<Y>(v[0]);
+            else if (first_out) __stcs(reinterpret_cast<uint4 *>(y), Vec16<Y>::put(v));
             else *reinterpret_cast<uint4 *>(y) = Vec16<Y>::put(v);
         } else {
             const float scale = p.scales[p.nscales == 1 ? 0 : t.image];
@@ -332,7 +344,7 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
     const int mine = row < rows && row < count ? (count - row + rows - 1) / rows : 0;      // this thread's pixels: row, row + rows, ...
     R *slots = held + row * cols + col;
     stream<T, VEC, true>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + col * VEC, rows * p.x_pixel, mine,
-                         (uint32_t)__cvta_generic_to_shared(slots), rows * cols * sizeof(R), [&](int i, const R &raw) {
+                         (uint32_t)__cvta_generic_to_shared(slots), rows * cols * sizeof(R), 0, [&](int i, const R &raw) {
                              float v[VEC];
                              unpack<T, VEC>(raw, v);
                              sums.add(v);
@@ -367,7 +379,7 @@ group_norm_resident_kernel(const __grid_constant__ GroupNormParams p) {
         by_activation(p.activation, [&](auto act) {
 #pragma unroll 4
             for (int i = 0; i < mine; ++i, from += rows * cols, y += rows * p.y_pixel)
-                apply.template run<decltype(act)::value>(p, t, *from, t.p0 + row + i * rows, col * VEC, y);
+                apply.template run<decltype(act)::value>(p, t, *from, t.p0 + row + i * rows, col * VEC, y, false);
         });
     }
     pad_channels<Y>(p, t);
@@ -394,7 +406,7 @@ group_norm_sums_kernel(const __grid_constant__ GroupNormParams p, double2 *all_s
         sums.clear();
         if (row < rows && row < count && c < b1)
             stream<T, VEC, false>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c, rows * p.x_pixel, (count - row + rows - 1) / rows,
-                                  (uint32_t)__cvta_generic_to_shared(scratch) + threadIdx.x * 16, kThreads * 16, [&](int, const R &raw) {
+                                  (uint32_t)__cvta_generic_to_shared(scratch) + threadIdx.x * 16, kThreads * 16, l2_policy((int)blockIdx.x < p.let_go), [&](int, const R &raw) {
                                       float v[VEC];
                                       unpack<T, VEC>(raw, v);
                                       sums.add(v);
@@ -450,8 +462,8 @@ group_norm_apply_kernel(const __grid_constant__ GroupNormParams p, const float2 
         Y *y = static_cast<Y *>(p.y) + t.image * p.y_image + (t.p0 + row) * p.y_pixel + t.c0 + c;
         by_activation(p.activation, [&](auto act) {
             stream<T, VEC, false>(static_cast<const T *>(p.x) + t.image * p.x_image + (t.p0 + row) * p.x_pixel + t.c0 + c, rows * p.x_pixel, (count - row + rows - 1) / rows,
-                                  (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16, kThreads * 16, [&](int i, const R &raw) {
-                                      apply.template run<decltype(act)::value>(p, t, raw, t.p0 + row + i * rows, c, y);
+                                  (uint32_t)__cvta_generic_to_shared(smem) + threadIdx.x * 16, kThreads * 16, l2_policy(p.let_go > 0), [&](int i, const R &raw) {
+                                      apply.template run<decltype(act)::value>(p, t, raw, t.p0 + row + i * rows, c, y, p.let_go > 0);
                                       y += rows * p.y_pixel;
                                   });
         });
@@ -497,6 +509,7 @@ struct Plan {
     bool one, resident;
     int run_groups, runs, cols, tiles;
     int64_t tile;
+    int let_go;
     size_t smem, off_stats, bytes;    // of shared memory; of the workspace
 };
 
@@ -549,6 +562,9 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     q.tile = std::max(ceil_div64(d->pixels, blocks), std::max<int64_t>(1, 16384 / ((int64_t)width * size)));
     q.tiles = (int)ceil_div64(d->pixels, q.tile);
     q.smem = (size_t)q.run_groups * 16 + (size_t)kDepth * kThreads * 16;      // (at least collect's scratch: a vector has at most eight pairs of sums)
+    // Of a tensor beyond 80 MB the L2 is to keep that much, the end of it, for the second reading: what comes before, and the outputs, goes
+    // first (8 x 256 x 256 x 256 bf16 154 -> 151 us, 16 x 128 x 128 x 256 79 -> 73)
+    q.let_go = (int)std::max<int64_t>(0, std::min<int64_t>(INT32_MAX, d->n * q.runs * q.tiles - (80 << 20) / std::max<int64_t>(1, q.tile * width * size)));
     q.off_stats = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
     q.bytes = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));
     return q;
@@ -618,6 +634,7 @@ int group_norm_nhwc(const tsb_group_norm_desc *d, void *workspace, size_t worksp
     p.cols = q.cols;
     p.tile = q.tile;
     p.tiles = q.tiles;
+    p.let_go = q.let_go;
     p.eps = d->eps;
     p.one_over_count = 1.0 / ((double)d->pixels * p.per);
     p.activation = d->activation;
