@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // the portable limit
 constexpr int kMaxGroups = 256;                 // groups of a run of channels
-constexpr int kResidentBlocks = 3;               // resident blocks a multiprocessor, by their registers
+constexpr int kResidentBlocks = 4;               // resident blocks a multiprocessor, by their registers (2000 x 14 x 14 x 256 bf16 122 us, with three 131)
 constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
 struct GroupNormParams {
@@ -543,7 +543,7 @@ Plan make_plan(const tsb_group_norm_desc *d) {
             if (smem > kLargeTile) continue;
             if (best && bytes < 16 * 1024) break;
             const int64_t blocks = d->n * runs * s, at_once = 148 * std::min<int64_t>(kResidentBlocks, (227 * 1024) / (smem + 1024));
-            if (blocks > at_once && !(s == 1 && smem <= kLargeTile / 4)) continue;      // (single blocks do not wait for one another)
+            if (blocks > at_once && !(s == 1 && smem <= 113 * 1024)) continue;      // (blocks that meet no others may take turns, two a multiprocessor or more)
             if (blocks < best || (blocks == best && s >= q.tiles) || blocks > INT32_MAX) continue;
             best = blocks;
             q.resident = true;
