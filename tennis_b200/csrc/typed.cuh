@@ -186,12 +186,13 @@ __device__ __forceinline__ float silu(float v) {
 }
 // Two values that become results of 16 bits, whose half step is 2^13 times that of fp32 or more: without that correction, and with one
 // reciprocal for both (a multiprocessor does 16 of these functions a clock, and eight times as many products): 1 / a = b (1 / ab).
-// exp2's argument is kept below 63, so that ab stays a number: below v = -43.7 the result is v 2^-63.
+// exp2's argument is kept below 63, so that ab stays a number; beyond that, v < -43.6, the quotient of a result below 10^-17 counts as 0.
 __device__ __forceinline__ float2 silu_short(float2 v) {
     const float2 t = mul2(v, make_float2(-1.44269504f, -1.44269504f));
     const float2 a = add2(make_float2(exp2_approx(fminf(t.x, 63.0f)), exp2_approx(fminf(t.y, 63.0f))), make_float2(1.0f, 1.0f));
     const float r = reciprocal_approx(__fmul_rn(a.x, a.y));
-    return mul2(v, mul2(make_float2(a.y, a.x), make_float2(r, r)));
+    const float2 q = mul2(make_float2(a.y, a.x), make_float2(r, r));
+    return mul2(v, make_float2(t.x > 63.0f ? 0.0f : q.x, t.y > 63.0f ? 0.0f : q.y));
 }
 __device__ __forceinline__ float gelu(float v) {
     return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));

@@ -67,6 +67,25 @@ def test_activations(m, n, k, act, leaky):
             check(got, d, act, leaky, after)
 
 
+@pytest.mark.parametrize("m", [1, 12, 40, 150, 400])
+@pytest.mark.parametrize("act", [1, 3, 4])
+def test_activations_of_the_largest_values(m, act):
+    """Values to the ends of fp32, infinities and NaN, side by side: what is far below zero becomes zero (an infinity NaN, 0 times it, as
+    the formulas say), and none changes its neighbour.  Sums of zero leave the bias itself."""
+    from tennis_b200 import ops
+    ends = [-1e4, 3.0, -1e30, -3.3e38, -44.0, -43.0, float("nan"), -1.0, -float("inf"), -2.0, float("inf"), -90.0, 3.3e38, -200.0, 1e-30, -3.3e38]
+    for n in (16, 200):
+        bias = torch.tensor((ends * 13)[:n], device="cuda")
+        v = bias.double().cpu()
+        want = v.clamp(min=0.0).nan_to_num(nan=0.0, posinf=float("inf")) if act == 1 else v / (1.0 + torch.exp(-v)) if act == 3 else 0.5 * v * (1.0 + torch.erf(v * 0.5 ** 0.5))
+        for out in FLOATS:
+            d = case(m, n, 48, out, 3)
+            got = ops.inner_prod_quantized(torch.zeros_like(d["x"]), d["xs"], d["w"], d["ws"], bias, activation=act, out_dtype=out).cpu()
+            # fp32: silu by 8 half steps of its value, gelu by 24 of 1; one rounding to 16 bits; 10^-17 as plain.activation's quotient
+            torch.testing.assert_close(got.double(), want.to(out).double().expand(m, n), rtol=2 * torch.finfo(out).eps + 8 * plain.EPS32,
+                                       atol=24 * plain.EPS32 if act == 4 else 1e-17, equal_nan=True)
+
+
 @pytest.mark.parametrize("m", [1, 6, 30, 140, 700])
 def test_kernels_agree_bit_for_bit(m):
     """The result's bits depend neither on the kernel nor on the rows that are computed with a row."""
