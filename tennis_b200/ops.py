@@ -613,7 +613,7 @@ def quantize_rows(x, out=None, scales=None, stream=None):
         out = q if len(shape) == 2 else q.view(shape) if k == pitch else torch.empty(shape[:-1] + (pitch,), dtype=_int8, device=x.device)[..., :k]
     elif out.dtype is not _int8 or out.shape != shape or out.get_device() != device or (out.stride(-1) != 1 and k > 1):
         _refuse("out: int8 of x's shape on x's device, values of a row next to each other")
-    if out.numel():
+    if m:
         q = _rows_to(out)
     if scales is None:
         scales = torch.empty((m,), dtype=_float32, device=x.device)
@@ -621,6 +621,8 @@ def quantize_rows(x, out=None, scales=None, stream=None):
             scales = scales.view(shape[:-1])
     else:
         _check_vector(scales, m, device, "scales")
+    if not m:
+        return out, scales
     status = _lib.load().tsb_quantize_rows_i8(rows.data_ptr(), kind, rows.stride(0), q.data_ptr(), q.stride(0), scales.data_ptr(), m, k,
                                               _current_raw_stream(device))
     if status:

@@ -133,3 +133,11 @@ def test_empty():
     assert q.shape == (0, 8) and s.shape == (0,)
     q, s = ops.quantize_rows(torch.empty((3, 0, 8), device="cuda"))
     assert q.shape == (3, 0, 8) and s.shape == (3, 0)
+
+
+@pytest.mark.parametrize("shape", [(0, 8), (3, 0, 8), (0, 3, 5)])
+def test_empty_outputs_of_the_callers(shape):
+    from tennis_b200 import ops
+    out, scales = torch.empty(shape, dtype=torch.int8, device="cuda"), torch.empty(shape[:-1], device="cuda")
+    q, s = ops.quantize_rows(torch.empty(shape, device="cuda"), out=out, scales=scales)
+    assert q is out and s is scales
