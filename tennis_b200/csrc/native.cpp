@@ -70,6 +70,12 @@ bool rows_of(const Tensor &t, int64_t *rows, int64_t *pitch) {
     return true;
 }
 
+// An int argument; -1, which is none of the values that the C ABI takes, for numbers that an int does not hold
+int int_of(PyObject *o) {
+    const long v = PyLong_AsLong(o);
+    return v == (int)v ? (int)v : -1;
+}
+
 void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
 // The sizes of x with another last one
@@ -149,7 +155,7 @@ PyObject *inner_prod(PyObject *, PyObject *const *args, Py_ssize_t count) {
             Py_RETURN_NONE;
         a.residual = r->const_data_ptr();
     }
-    a.activation = (int)PyLong_AsLong(args[6]);
+    a.activation = int_of(args[6]);
     a.leaky_scale = (float)PyFloat_AsDouble(args[7]);
     if (PyErr_Occurred()) {
         PyErr_Clear();
@@ -202,7 +208,7 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
     }
     d.groups = PyLong_AsLongLong(args[1]);
     d.eps = PyFloat_AsDouble(args[4]);
-    d.activation = (int)PyLong_AsLong(args[5]);
+    d.activation = int_of(args[5]);
     d.leaky_scale = (float)PyFloat_AsDouble(args[6]);
     if (PyErr_Occurred()) {
         PyErr_Clear();

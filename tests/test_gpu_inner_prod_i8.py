@@ -1,4 +1,6 @@
 """inner_prod_quantized against the product in 64 bits, at sizes, layouts and epilogues where it can go wrong."""
+import struct
+
 import numpy as np
 import pytest
 import torch
@@ -301,6 +303,17 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError, match="activation 9"):
         call(x, xs, w, ws, activation=9)
+
+
+def test_numbers_beyond_an_argument():
+    """Numbers of which an int's 32 bits would be valid ones."""
+    from tennis_b200 import ops
+    d = case(6, 32, 64, torch.float32, 1)
+    for bad in (1 << 32, (1 << 32) + 1, -(1 << 32)):
+        with pytest.raises((struct.error, RuntimeError)):
+            ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], activation=bad)
+        with pytest.raises((struct.error, RuntimeError)):
+            ops.group_norm_nhwc(torch.ones((1, 2, 2, 16), device="cuda"), 4, activation=bad)
 
 
 def test_empty():
