@@ -4,7 +4,7 @@
 // without reading it again from HBM.
 //
 //   sums       in 64 bits: with 53 bits the difference of the mean square and the squared mean keeps 32-bit accuracy for means up to
-//              10^4 deviations, in one pass over the data, and no order of summation shows in the rounded mean and deviation
+//              10^4 deviations, in one pass over the data, and the order of summation shows in the rounded mean and deviation next to never
 //   threads    a thread owns one 16-byte vector of channels (or one channel, where vectors do not fit) and walks over pixels: loads of
 //              neighbouring threads are neighbours, its channels' gamma, beta and statistics stay in registers
 //   resident   an image's run of groups is held in the shared memory of a cluster of up to eight blocks: loaded once, summed on the
@@ -14,7 +14,7 @@
 //              launches' beginnings and ends cost more than the reads of HBM that they save: 8 x 256 x 256 x 256 bf16 152 us in one
 //              batch, 176 in batches of two images, 266 image by image)
 // Measured: 16 x 56 x 56 x 256 bf16 to int8 20 us (resident; load, meeting and writing follow each other in its one round of blocks), 8 x 256 x 256 x 256
-// bf16 151 us (swept: 805 MB at 5.3 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.6 us.
+// bf16 152 us (swept: 805 MB at 5.3 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.5 us.
 #include "typed.cuh"
 
 #include <algorithm>
