@@ -43,7 +43,9 @@ __device__ int g_status;
 
 struct TcParams {
     InnerProdParams p;
-    int tiles_m, tiles_n, kblocks, stages;
+    int tiles_m, tiles_n, kblocks;
+    int group_m;                  // token tiles that neighbouring CTAs share: a power of two
+    uint32_t per_group, inverse;  // tiles of such a group, 2^32 / that
 };
 
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory
@@ -64,11 +66,15 @@ struct Layout {
 };
 
 __device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, int &n_tile) {
-    const int per_group = kGroupM * t.tiles_n;
-    const int g = i / per_group, r = i - g * per_group;
-    const int rows = min(kGroupM, t.tiles_m - g * kGroupM);
-    n_tile = r / rows;
-    m_tile = g * kGroupM + r - n_tile * rows;
+    // (every warp of the epilogue does this for every tile: no division but in the last group)
+    int g = (int)__umulhi((uint32_t)i, t.inverse), r = i - g * (int)t.per_group;      // the quotient or one less
+    if (r >= (int)t.per_group) {
+        ++g;
+        r -= (int)t.per_group;
+    }
+    const int rows = t.tiles_m - g * t.group_m;
+    n_tile = rows >= t.group_m ? r >> (31 - __clz(t.group_m)) : r / rows;
+    m_tile = g * t.group_m + r - n_tile * min(rows, t.group_m);
 }
 
 // A warp's staged outputs, rows of kCh channels: in the order of a tensor map's 64- or 128-byte swizzle, so that the fragments' writes (eight
@@ -86,6 +92,15 @@ template <int CH>
 struct Channels {
     float2 ws[CH / 8], bias[CH / 8];
     __device__ __forceinline__ void load(const InnerProdParams &p, int c0) {
+        if (c0 + CH <= p.n) {
+            const float *w = p.w_scales + c0 + 2 * (threadIdx.x & 3), *b = p.bias + c0 + 2 * (threadIdx.x & 3);
+#pragma unroll
+            for (int j = 0; j < CH / 8; ++j) {
+                ws[j] = make_float2(__ldg(w + 8 * j), __ldg(w + 8 * j + 1));
+                bias[j] = p.bias ? make_float2(__ldg(b + 8 * j), __ldg(b + 8 * j + 1)) : make_float2(0.0f, 0.0f);
+            }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < CH / 8; ++j) {
             const int c = c0 + 8 * j + 2 * (threadIdx.x & 3);
@@ -319,9 +334,10 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         Channels<kCh> channels[kShare / kCh];
         // the scales of this lane's tokens: lane / 4 and every eighth behind it
         auto scales_of = [&](int m_tile, float (&s)[4]) {
-            const int64_t m = (int64_t)rows_of(m_tile) * kBM + quarter * 32 + (lane >> 2);
+            const int m = rows_of(m_tile) * kBM + quarter * 32 + (lane >> 2), left = (int)t.p.m - m, every = 8 * (int)t.p.xs_stride;
+            const float *from = t.p.x_scales + (t.p.xs_stride ? m : 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = m + 8 * i < t.p.m ? t.p.x_scales[(m + 8 * i) * t.p.xs_stride] : 0.0f;
+            for (int i = 0; i < 4; ++i) s[i] = left > 8 * i ? from[i * every] : 0.0f;
         };
         tile_of(t, first, mt, nt);
         float xs[4], next_xs[4];
@@ -496,7 +512,11 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
         raised.done();
     }
     constexpr int kCluster = PAIR ? 2 : SPLIT;
-    TcParams t = {p, (int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes), L::kStages};
+    TcParams t = {p, (int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes)};
+    // (of few output channels, tiles of the same tokens follow each other: then a CTA of an even grid stays with its channels)
+    t.group_m = t.tiles_n <= 4 ? 1 : kGroupM;
+    t.per_group = (uint32_t)(t.group_m * t.tiles_n);
+    t.inverse = (uint32_t)std::min<uint64_t>(UINT32_MAX, ((uint64_t)1 << 32) / t.per_group);
     const int grid = kCluster * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, SPLIT > 1 ? INT32_MAX : 148 / kCluster);      // (split: a tile a cluster)
     TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");
