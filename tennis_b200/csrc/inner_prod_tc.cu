@@ -8,8 +8,9 @@
 //              tile is computed
 //   epilogue   sums come in fragments, so that a lane has the same few channels of many tokens and keeps their scales in registers (a lane
 //              that has one token and all channels reads every channel's scales from shared memory, which then bounds the epilogue);
-//              2 KB of a warp's at a time go through shared memory: residuals are read in whole pieces, outputs written by tensor-map
-//              copies (value by value where y does not lie on 16 bytes)
+//              2 KB of a warp's at a time go through shared memory: residuals come by asynchronous copies while the step in front is worked on
+//              (100352 x 256 x 64 with a residual 46 -> 27 us, 4096^3 62 -> 54), outputs are written by tensor-map copies (both value by value
+//              where they do not lie on 16 bytes)
 //   split      of few tiles, two or four CTAs of a cluster share one: each multiplies a part of K, hands its sums of the others' 32 channels
 //              over through distributed shared memory (int32 sums are the same in any order) and writes its own 32
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
@@ -35,6 +36,7 @@ constexpr int kKBytes = 128;                 // bytes of K a stage
 constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
 constexpr uint32_t kABytes = kBM * kKBytes;
 constexpr int kCh = 32;                      // channels of a step of the epilogue
+constexpr uint32_t kOutRows = 2048;          // bytes of a step of a warp's
 constexpr uint32_t kSmem = 227 * 1024;
 constexpr int kMaxStages = 8;
 
@@ -49,9 +51,10 @@ struct TcParams {
 };
 
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory
-template <typename T, int BN, bool PAIR, int SPLIT = 1>
+template <typename T, int BN, bool RES, bool PAIR, int SPLIT = 1>
 struct Layout {
-    static constexpr uint32_t kOutWarp = 2048;                                    // a warp's staged outputs
+    static constexpr bool kAhead = RES && SPLIT == 1;                        // residuals of a step come while the one in front of it is worked on
+    static constexpr uint32_t kOutWarp = kAhead ? 2 * kOutRows : kOutRows;        // a warp's staged outputs (and the next step's residuals)
     static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
     static constexpr int kBRows = PAIR ? BN / 2 : BN;
@@ -141,6 +144,26 @@ __device__ __forceinline__ void fetch_residual(const InnerProdParams &p, int64_t
     __syncwarp();
 }
 
+// The same without waiting for it: whole pieces alone (whole_residual), by asynchronous copies, a group of them in any case.
+__device__ __forceinline__ bool whole_residual(const InnerProdParams &p, int c0, bool res_vec) { return res_vec && c0 + kCh <= p.n; }
+template <typename T>
+__device__ __forceinline__ void start_residual(const InnerProdParams &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
+    using S = Staged<T>;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) bulk_wait_read();
+    __syncwarp();
+    if (live > 0 && whole_residual(p, c0, res_vec)) {
+        constexpr int kStep = 32 / S::kUnits;
+        const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
+        const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * Vec16<T>::kN;
+        const int64_t step = kStep * p.residual_pitch;
+#pragma unroll
+        for (int r = 0; r < S::kRows; r += kStep, from += step)
+            if (r + r0 < live) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(rows + S::unit(r + r0, u0))), "l"(from) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
 // kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
 // the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of its own accord that is under way when this returns, else by the lanes.
@@ -161,15 +184,11 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
         for (int i = 0; i < kValues; ++i) acc[i] = given[i];
     }
     auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
-    float v[kValues], res[RES ? kValues : 1];
-    if constexpr (RES) {
-        if (!fetched) fetch_residual<T>(p, m0, live, c0, rows, res_vec);
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) res[i] = to_f32(reinterpret_cast<const T *>(at(i))[i & 1]);
-    }
+    float v[kValues];
+    if (RES && !fetched) fetch_residual<T>(p, m0, live, c0, rows, res_vec);
     if (!GIVEN) tmem_ld_wait();
     inner_prod_values<T, RES>(p, acc, [&](int i) { return PairScales{ch.ws[i / 4 % (kCh / 8)], xs[i / (kCh / 2) * 2 + (i >> 1 & 1)], ch.bias[i / 4 % (kCh / 8)]}; },
-                         [&](int i) { return res[RES ? i : 0]; }, v);
+                         [&](int i) { return to_f32(reinterpret_cast<const T *>(at(i))[i & 1]); }, v);      // (a lane's outputs go where its residuals were)
     if (!RES && lane == 0) bulk_wait_read();
     __syncwarp();
 #pragma unroll
@@ -199,11 +218,11 @@ __device__ __forceinline__ void epilogue_rows(const InnerProdParams &p, const CU
 }
 
 template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
-__global__ void __launch_bounds__(Layout<T, BN, PAIR, SPLIT>::kThreads, 1)
+__global__ void __launch_bounds__(Layout<T, BN, RES, PAIR, SPLIT>::kThreads, 1)
 inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_y,
                         const __grid_constant__ TcParams t, int tile_store, int res_vec) {
     static_assert(SPLIT == 1 || (!PAIR && BN == kCh * SPLIT), "split: kCh channels of the tile for each CTA");
-    using L = Layout<T, BN, PAIR, SPLIT>;
+    using L = Layout<T, BN, RES, PAIR, SPLIT>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -342,6 +361,11 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         tile_of(t, first, mt, nt);
         float xs[4], next_xs[4];
         scales_of(mt, xs);
+        uint32_t turn = 0;                               // which half of its staging a step takes
+        if constexpr (L::kAhead) {
+            const int64_t m0 = (int64_t)mt * kBM + quarter * 32;
+            start_residual<T>(t.p, m0, (int)max((int64_t)0, min((int64_t)Staged<T>::kRows, t.p.m - m0)), nt * BN + share, rows, res_vec != 0);
+        }
         const uint32_t lead_tempty = PAIR ? map_to_rank(bar_tempty, 0) : bar_tempty;
         for (int i = first; i < tiles; i += step, ++n) {
             const uint32_t acc = n & 1;
@@ -358,7 +382,8 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
             if constexpr (RES) {                       // (the first step's, while the sums are not there yet)
                 const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32;
                 const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0));
-                if (live > 0 && nt * BN + share < t.p.n && (SPLIT == 1 || e / 4 == rank)) fetch_residual<T>(t.p, m0, live, nt * BN + share, rows, res_vec != 0);
+                if (live > 0 && nt * BN + share < t.p.n && (SPLIT == 1 || e / 4 == rank) && !(L::kAhead && whole_residual(t.p, nt * BN + share, res_vec != 0)))
+                    fetch_residual<T>(t.p, m0, live, nt * BN + share, rows + (L::kAhead ? kOutRows * (turn & 1) : 0), res_vec != 0);
             }
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
@@ -411,9 +436,22 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
                 for (int r = 0; r < 32; r += kRows) {
                     const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32 + r;
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share + c * kCh;
+                    bool fetched = RES && c == 0 && r == 0;
+                    uint8_t *staged = rows;
+                    if constexpr (L::kAhead) {
+                        staged = rows + kOutRows * (turn++ & 1);
+                        const bool last = c == kShare / kCh - 1 && r + kRows == 32;       // of the tile: the next step is the next tile's first
+                        const int next_r = last ? 0 : (r + kRows) % 32, next_c = last ? 0 : c + (r + kRows) / 32;
+                        const int64_t next_m0 = (int64_t)rows_of(last ? next_mt : mt) * kBM + quarter * 32 + next_r;
+                        const int next_live = last && i + step >= tiles ? 0 : (int)max((int64_t)0, min((int64_t)kRows, t.p.m - next_m0));
+                        start_residual<T>(t.p, next_m0, next_live, (last ? next_nt : nt) * BN + share + next_c * kCh, rows + kOutRows * (turn & 1), res_vec != 0);
+                        asm volatile("cp.async.wait_group 1;" ::: "memory");              // this step's
+                        __syncwarp();
+                        fetched = fetched || whole_residual(t.p, c0, res_vec != 0);
+                    }
                     if (live > 0 && c0 < t.p.n)
-                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, nullptr, m0, live, c0, channels[c], xs + r / 8, rows, to,
-                                         tile_store != 0, res_vec != 0, RES && c == 0 && r == 0);
+                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * BN + ((uint32_t)(quarter * 32 + r) << 16) + share + c * kCh, nullptr, m0, live, c0, channels[c], xs + r / 8, staged, to,
+                                         tile_store != 0, res_vec != 0, fetched);
                 }
             mt = next_mt;
             nt = next_nt;
@@ -428,6 +466,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
     }
 done:
+    if (L::kAhead) asm volatile("cp.async.wait_all;" ::: "memory");
     if (warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // this warp's outputs are written
     if (*abort_flag) {
         // copies that may still be in flight get time to land before shared memory is released
@@ -496,7 +535,7 @@ int encode_output(CUtensorMap *map, const InnerProdParams &p) {
 
 template <typename T, int BN, bool RES, bool PAIR = false, int SPLIT = 1>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
-    using L = Layout<T, BN, PAIR, SPLIT>;
+    using L = Layout<T, BN, RES, PAIR, SPLIT>;
     CUtensorMap mx, mw, my;
     int st = encode(&mx, p.x, p.m, p.k, p.x_pitch, kBM);
     if (st == TSB_OK) st = encode(&mw, p.w, p.n, p.k, p.w_pitch, L::kBRows);
@@ -528,10 +567,12 @@ int pick(const InnerProdParams &p, cudaStream_t stream) {
     // The tile by the clocks that its rounds take: a multiprocessor gets 64 bytes a clock, so a stage of 128 + BN rows of 128 bytes takes
     // 2 (128 + BN); the epilogue some 9 BN; a pair's tile, of half the rows of w for each, 3500 more for what its CTAs wait for each other.
     // (Measured, 64, 128, 256 wide and by pairs: 64 x 4096 x 4096 9.7, 11.0, 16.2 us; 2048 x 1000 x 2048 9.9, 8.1, 11.0, 11.4;
-    // 2048 x 4096 x 4096 48.6, 35.4, 29.1, 26.3; 8192^3 - , - , 359, 331; but 16384 x 8192 x 512 80 us 256 wide, 103 by pairs.)
+    // 2048 x 4096 x 4096 48.6, 35.4, 29.1, 26.3; 8192^3 - , - , 359, 331; but 16384 x 8192 x 512 80 us 256 wide, 103 by pairs.
+    // With a residual the 64 channels of a warp of the widest tiles do not fit its registers, and they take 16 BN: 16384 x 8192 x 512 143 us 256
+    // wide, 123 in tiles of 128; 25088 x 1024 x 256 34.7 and 23.9.)
     auto clocks = [&](int bn, int ctas) {
         const int64_t rounds = ceil_div64(ceil_div64(p.m, kBM * ctas) * ceil_div(p.n, bn), 148 / ctas);
-        return rounds * (ceil_div(p.k, kKBytes) * 2 * (int64_t)(128 + bn / ctas) + 9 * bn + (ctas - 1) * 3500);
+        return rounds * (ceil_div(p.k, kKBytes) * 2 * (int64_t)(128 + bn / ctas) + (RES && bn == 256 ? 16 : 9) * bn + (ctas - 1) * 3500);
     };
     const int64_t c64 = clocks(64, 1), c128 = clocks(128, 1), c256 = clocks(256, 1), pair = clocks(256, 2);
     // Few tiles: two or four CTAs a tile, each with a part of K, and 2000 clocks for handing sums over.  (64 x 2048 x 8192 15.4 -> 9.6 us,
