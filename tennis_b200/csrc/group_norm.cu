@@ -529,7 +529,7 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     int step = 1;
     while (step * per % q.vec) ++step;
     // Resident: as many blocks as run at the same time (a second round of them waits for the first to be through all of its steps:
-    // 16 x 56 x 56 x 256 bf16 in 256 blocks of 100 KB 20 us, in 512 of 50 KB 25), of as many the smaller cluster; rows of 64
+    // 16 x 56 x 56 x 256 bf16 in 512 blocks of 50 KB, four a multiprocessor, 20 us; three, which makes two rounds, 25), of as many the smaller cluster; rows of 64
     // bytes or more, tiles of 16 KB or more where there is a choice.  Images that do not fit so are swept (4 x 128 x 128 x 128 fp32: 22 us,
     // resident in two rounds 33).
     int64_t best = 0;
