@@ -363,7 +363,7 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         scales_of(mt, xs);
         uint32_t turn = 0;                               // which half of its staging a step takes
         if constexpr (L::kAhead) {
-            const int64_t m0 = (int64_t)mt * kBM + quarter * 32;
+            const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32;
             start_residual<T>(t.p, m0, (int)max((int64_t)0, min((int64_t)Staged<T>::kRows, t.p.m - m0)), nt * BN + share, rows, res_vec != 0);
         }
         const uint32_t lead_tempty = PAIR ? map_to_rank(bar_tempty, 0) : bar_tempty;

@@ -112,6 +112,44 @@ def test_large_products(m, n, k):
     ops.inner_prod_status()
 
 
+def after_the_sums(d, acc, act, after):
+    """The fp32 steps behind the sums (whole numbers, exact in `acc`), one by one as the header lists them."""
+    v = acc.float() * d["ws"] * d["xs"][:, None] + d["bias"]
+    r = d["residual"].float()
+    if not after:
+        v = v + r
+    if act == 1:
+        v = v.clamp(min=0.0)
+    return v + r if after else v
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 4096), (4992, 2560, 2048), (2430, 2432, 8192), (3201, 2056, 4096), (1152, 4096, 4096), (4096, 2560, 2048), (2049, 4097, 2176)])
+@pytest.mark.parametrize("act,after", [(0, False), (1, False), (1, True)])
+def test_large_products_with_a_residual(m, n, k, act, after):
+    """Tiles of two CTAs (the first four: also an odd number of 128 tokens, tokens and channels that fill no tile) and of one, many a
+    multiprocessor: the very bits of a product of doubles and the fp32 steps behind it."""
+    from tennis_b200 import ops
+    for out in FLOATS:
+        d = case(m, n, k, out, m + act)
+        want = after_the_sums(d, d["x"].double() @ d["w"].double().t(), act, after).to(out)
+        got = ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], d["residual"], act, out_dtype=out, residual_after_activation=after)
+        assert torch.equal(got, want)
+    ops.inner_prod_status()
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 4096), (4992, 2560, 2048), (2049, 4097, 2176)])
+def test_large_products_onto_their_residual(m, n, k):
+    """The residual is the output: every element is read before it is written."""
+    from tennis_b200 import ops
+    for out in FLOATS:
+        d = case(m, n, k, out, m + 7)
+        want = after_the_sums(d, d["x"].double() @ d["w"].double().t(), 0, False).to(out)
+        y = d["residual"].clone()
+        assert ops.inner_prod_quantized(d["x"], d["xs"], d["w"], d["ws"], d["bias"], y, out=y) is y
+        assert torch.equal(y, want)
+    ops.inner_prod_status()
+
+
 @pytest.mark.parametrize("x_pitch,x_at,w_pitch,w_at", [(512, 0, 512, 0), (512, 0, 500, 0), (501, 0, 512, 0), (512, 1, 512, 0), (512, 0, 512, 4), (520, 8, 504, 8), (1024, 16, 640, 32)])
 @pytest.mark.parametrize("m", [1, 13, 50, 300])
 def test_layouts(m, x_pitch, x_at, w_pitch, w_at):
