@@ -184,15 +184,13 @@ __device__ __forceinline__ float silu(float v) {
     const float r = fmaf(c, -1.92596303e-8f, fmaf(c, -1.44269502f, -t));   // log2(e) = 1.44269502 (fp32) + 1.92596303e-8
     return __fmul_rn(v, reciprocal_approx(__fadd_rn(1.0f, __fmul_rn(exp2_approx(t), fmaf(r, 0.693147182f, 1.0f)))));
 }
-// Two values that become results of 16 bits, whose half step is 2^13 times that of fp32 or more: without that correction, and with one
-// reciprocal for both (a multiprocessor does 16 of these functions a clock, and eight times as many products): 1 / a = b (1 / ab).
-// exp2's argument is kept below 63, so that ab stays a number; beyond that, v < -43.6, the quotient of a result below 10^-17 counts as 0.
+// Two values that become results of 16 bits, whose half step is 2^13 times that of fp32 or more: without that correction.  Each is a function of
+// itself alone, so its bits do not depend on what it is paired with.  (One reciprocal for both, 1 / a = b (1 / ab), saves one of the four
+// functions, of which a multiprocessor does 16 a clock; but then they do.)
 __device__ __forceinline__ float2 silu_short(float2 v) {
     const float2 t = mul2(v, make_float2(-1.44269504f, -1.44269504f));
-    const float2 a = add2(make_float2(exp2_approx(fminf(t.x, 63.0f)), exp2_approx(fminf(t.y, 63.0f))), make_float2(1.0f, 1.0f));
-    const float r = reciprocal_approx(__fmul_rn(a.x, a.y));
-    const float2 q = mul2(make_float2(a.y, a.x), make_float2(r, r));
-    return mul2(v, make_float2(t.x > 63.0f ? 0.0f : q.x, t.y > 63.0f ? 0.0f : q.y));
+    const float2 a = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), make_float2(1.0f, 1.0f));
+    return mul2(v, make_float2(reciprocal_approx(a.x), reciprocal_approx(a.y)));
 }
 __device__ __forceinline__ float gelu(float v) {
     return __fmul_rn(__fmul_rn(0.5f, v), __fadd_rn(1.0f, erff(__fmul_rn(v, 0.70710678118654752f))));

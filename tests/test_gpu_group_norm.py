@@ -124,6 +124,19 @@ def test_layouts(dtype, hw):
                 assert torch.equal(view, got)
 
 
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("act", [3, 4])
+def test_bits_of_a_value_are_its_own(dtype, act):
+    """Activations give the same bits by vectors and value by value (a view that starts off 16 bytes), resident and swept."""
+    from tennis_b200 import ops
+    for shape in ((3, 30, 30, 72), (2, 200, 200, 136)):
+        x, gamma, beta = tensors(shape, dtype, 13)
+        c = shape[-1] - 8
+        gamma, beta = gamma[:c].contiguous(), beta[:c].contiguous()
+        odd = x[..., 5:5 + c]
+        assert torch.equal(ops.group_norm_nhwc(odd, 8, gamma, beta, activation=act), ops.group_norm_nhwc(odd.contiguous(), 8, gamma, beta, activation=act))
+
+
 def test_far_offsets():
     from tennis_b200 import ops
     step = (1 << 32) // 63 + 8

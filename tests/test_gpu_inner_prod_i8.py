@@ -99,6 +99,29 @@ def test_kernels_agree_bit_for_bit(m):
     assert torch.equal(got[m // 2:], ops.inner_prod_quantized(d["x"][m // 2:], d["xs"][m // 2:], *args[2:5], d["residual"][m // 2:], _lib.ACT_SILU))
 
 
+@pytest.mark.parametrize("out", FLOATS, ids=str)
+@pytest.mark.parametrize("act,leaky", [(0, 0.0), (1, 0.0), (2, 0.1), (3, 0.0), (4, 0.0)])
+def test_bits_of_a_value_are_its_own(out, act, leaky):
+    """They depend on a row of x, a row of w and what is added: not on the kernel, on the rows or channels beside it (on either side of the 32
+    rows at which kernels change), or on the call.  An odd number of channels: the last one has no neighbour."""
+    from tennis_b200 import _lib, ops
+    for m, n, k in ((900, 1001, 64), (300, 776, 1056)):
+        for after in (False, True):
+            d = case(m, n, k, out, act)
+
+            def call(rows=slice(None), channels=slice(None), **kw):
+                return ops.inner_prod_quantized(d["x"][rows], d["xs"][rows], d["w"][channels], d["ws"][channels], d["bias"][channels], d["residual"][rows, channels].contiguous(), act, leaky,
+                                                out, residual_after_activation=after, **kw)
+            got = call()
+            assert torch.equal(got, call(kernel=_lib.KERNEL_DIRECT))
+            for rows in (slice(0, 1), slice(5, 37), slice(5, 38), slice(40, 140), slice(m // 2, m)):
+                assert torch.equal(got[rows], call(rows))
+            assert torch.equal(got[:, 1:], call(channels=slice(1, n)))
+            assert torch.equal(got[7:39, 1:], call(slice(7, 39), slice(1, n)))
+            for _ in range(3):
+                assert torch.equal(got, call())
+
+
 @pytest.mark.parametrize("m,n,k", [(4096, 2560, 2048), (2500, 2304, 4096), (9472, 256, 4096), (2049, 4097, 2176), (2430, 2432, 8192), (4097, 2080, 1920)])
 def test_large_products(m, n, k):
     """Sizes of many tiles a multiprocessor, of one and of two CTAs: int32 sums do not depend on their order, so a product of doubles has the
