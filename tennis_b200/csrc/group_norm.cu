@@ -230,11 +230,10 @@ __device__ __forceinline__ float2 statistics(const GroupNormParams &p, double s,
     return make_float2((float)mean, (float)(1.0 / sqrt(var + p.eps)));
 }
 
-// What a thread applies to its channels: statistics, gamma, beta, activation, rounding.  Results of 16 bits, whose half step is 2^13
-// times that of fp32 or more, take gamma into the reciprocal deviation and the product and the sum with beta as one operation.
+// What a thread applies to its channels: statistics, gamma, beta, activation, rounding.  (Results of 16 bits could take gamma into the reciprocal
+// deviation and the sum with beta into the product; but that product may lie beyond fp32 where what it is multiplied with brings it back.)
 template <typename T, typename Y, int VEC, bool ONE>
 struct Apply {
-    static constexpr bool kShort = sizeof(Y) == 2;
     static constexpr int kG = ONE ? 1 : VEC;
     float mean[kG], rstd[kG], gamma[VEC], beta[VEC];
     // c: the thread's first channel within the run
@@ -242,11 +241,12 @@ struct Apply {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const float2 st = stats[(c + (ONE ? 0 : i)) / p.per];
-            if (i < kG) mean[i] = st.x;
+            if (i < kG) {
+                mean[i] = st.x;
+                rstd[i] = st.y;
+            }
             gamma[i] = p.gamma ? __ldg(p.gamma + t.c0 + c + i) : 1.0f;      // (a product with 1 and a sum with -0 change nothing)
             beta[i] = p.beta ? __ldg(p.beta + t.c0 + c + i) : -0.0f;
-            if (kShort) gamma[i] = __fmul_rn(st.y, gamma[i]);
-            else if (i < kG) rstd[i] = st.y;
         }
     }
     // y: where the thread's channels of `pixel` go; first_out: they are the first that the L2 lets go of
@@ -257,22 +257,14 @@ struct Apply {
         if constexpr (VEC > 1) {
 #pragma unroll
             for (int i = 0; i < VEC; i += 2) {
-                const float2 g = make_float2(gamma[i], gamma[i + 1]);
                 const float2 d = add2(make_float2(v[i], v[i + 1]), make_float2(-mean[ONE ? 0 : i], -mean[ONE ? 0 : i + 1]));
-                if constexpr (kShort) {
-                    const float2 r = fma2(d, g, make_float2(beta[i], beta[i + 1]));
-                    v[i] = r.x;
-                    v[i + 1] = r.y;
-                } else {
-                    // (products by twos, the sum one by one: the assembler makes fused operations of a packed product and a packed sum)
-                    const float2 r = mul2(mul2(d, make_float2(rstd[ONE ? 0 : i], rstd[ONE ? 0 : i + 1])), g);
-                    v[i] = __fadd_rn(r.x, beta[i]);
-                    v[i + 1] = __fadd_rn(r.y, beta[i + 1]);
-                }
+                // (products by twos, the sum one by one: the assembler makes fused operations of a packed product and a packed sum)
+                const float2 r = mul2(mul2(d, make_float2(rstd[ONE ? 0 : i], rstd[ONE ? 0 : i + 1])), make_float2(gamma[i], gamma[i + 1]));
+                v[i] = __fadd_rn(r.x, beta[i]);
+                v[i + 1] = __fadd_rn(r.y, beta[i + 1]);
             }
         } else {
-            const float d = __fsub_rn(v[0], mean[0]);
-            v[0] = kShort ? fmaf(d, gamma[0], beta[0]) : __fadd_rn(__fmul_rn(__fmul_rn(d, rstd[0]), gamma[0]), beta[0]);
+            v[0] = __fadd_rn(__fmul_rn(__fmul_rn(__fsub_rn(v[0], mean[0]), rstd[0]), gamma[0]), beta[0]);
         }
         activate<ACT, Y>(v, p.leaky);
         if constexpr (sizeof(Y) > 1) {

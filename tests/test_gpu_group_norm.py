@@ -69,6 +69,34 @@ def test_values_far_from_zero(shape, groups):
     check(ops.group_norm_nhwc(small, groups, gamma, beta, 0.0), small, groups, gamma, beta, 0.0)
 
 
+@pytest.mark.parametrize("dtype", FLOATS, ids=str)
+@pytest.mark.parametrize("shape,groups", [((2, 8, 8, 64), 8), ((2, 16, 8, 32), 8), ((1, 256, 256, 256), 32), ((1, 256, 256, 128), 32)])
+def test_steps_are_rounded_one_by_one(shape, groups, dtype):
+    """Whole numbers, of which every group has a power of two: sums, mean and variance are exact in 64 bits whatever their order, so the steps behind
+    mean and reciprocal deviation (each rounded to fp32) can be compared bit for bit."""
+    from tennis_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(groups)
+    _, gamma, beta = tensors(shape, dtype, 9)
+    x = torch.randint(-60, 100, shape, device="cuda", generator=g).to(dtype)
+    t = x.double().view(shape[0], -1, groups, shape[-1] // groups)
+    mean = t.mean((1, 3), keepdim=True)
+    rstd = 1.0 / ((t * t).mean((1, 3), keepdim=True) - mean * mean + 1e-5).sqrt()
+    v = ((t.float() - mean.float()) * rstd.float()).view(shape) * gamma + beta
+    assert torch.equal(ops.group_norm_nhwc(x, groups, gamma, beta), v.to(dtype))
+    assert torch.equal(ops.group_norm_nhwc(x, groups, gamma, beta, activation=1), v.clamp(min=0.0).to(dtype))
+
+
+def test_deviation_and_gamma_whose_product_no_number_holds():
+    """eps = 0, deviations of 10^-25 and gammas of 10^20: their quotient is beyond fp32, the results are not."""
+    from tennis_b200 import ops
+    for shape in ((2, 8, 8, 32), (2, 90, 90, 64), (1, 7, 9, 33)):
+        x, gamma, beta = tensors(shape, torch.float32, 4)
+        x, gamma = (x * 1e-25).to(torch.bfloat16), gamma * 1e20
+        got = ops.group_norm_nhwc(x, shape[-1] // (8 if shape[-1] % 8 == 0 else 11), gamma, beta, 0.0)
+        assert torch.isfinite(got).all()
+        check(got, x, shape[-1] // (8 if shape[-1] % 8 == 0 else 11), gamma, beta, 0.0)
+
+
 def test_nan_and_infinity_stay_in_their_group():
     from tennis_b200 import ops
     for shape in ((3, 8, 8, 32), (3, 80, 80, 32)):
