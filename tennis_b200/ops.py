@@ -522,8 +522,8 @@ def repack_nhwc_to_nchw(x, channels, stream=None):
 # ---- int8 layers with scales per token: quantize_rows, inner_prod_quantized, group_norm_nhwc --------------------------------
 # These three work on the device that their tensors are on, on its current stream or on `stream`; what they allocate (outputs,
 # workspace) belongs to that stream.  Memory of an input that another stream allocated is the caller's to keep until the work is done.
-# Ordinary calls go through native.cpp (4 us a call); the Python below them is the general way: every layout, outputs of the caller's,
-# other streams and devices, and the texts of refusals.
+# Ordinary calls go through native.cpp (4 us a call), those on another stream or device too once it is made the current one; the Python below them is the
+# general way: every layout, outputs of the caller's, and the texts of refusals.
 _TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16, torch.int8: _lib.TYPE_I8}
 _FLOATS = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _FLOAT_NAMES = "float32, float16 or bfloat16, not %s"

@@ -350,6 +350,63 @@ def test_ordinary_and_general_calls_agree(lead):
             assert torch.equal(one, other) and one.dtype == other.dtype
 
 
+class Nothing:
+    """In the place of the module of ordinary calls: takes no call, and counts those that come."""
+
+    def __init__(self):
+        self.calls = 0
+
+    def __getattr__(self, name):
+        def take(*args):
+            self.calls += 1
+        return take
+
+
+@pytest.mark.parametrize("lead", [(), (1,), (5,), (40,), (2, 3), (3, 1, 15), (1, 2, 2)])
+@pytest.mark.parametrize("k,n", [(96, 40), (33, 37), (16, 1)])
+def test_the_module_of_ordinary_calls_and_the_general_way(monkeypatch, lead, k, n):
+    """The same tensors by both, for each operator, type and number of dimensions; on a stream and with outputs of the caller's too."""
+    from tennis_b200 import ops
+    native, nothing = ops._ordinary(), Nothing()
+
+    def both(call, *args, **kw):
+        monkeypatch.setattr(ops, "_native", native)
+        one = call(*args, **kw)
+        monkeypatch.setattr(ops, "_native", nothing)
+        before = nothing.calls
+        other = call(*args, **kw)
+        assert nothing.calls == before + 1
+        elsewhere = call(*args, stream=torch.cuda.current_stream(), **kw)
+        assert nothing.calls == before + 2
+        for a, b, c in zip(*(v if isinstance(v, tuple) else (v,) for v in (one, other, elsewhere))):
+            assert torch.equal(a, b) and torch.equal(a, c) and a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() == c.stride()
+        return one
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for dtype in FLOATS:
+        x = torch.randn(lead + (k,), device="cuda", generator=g).to(dtype)
+        w, ws = both(ops.quantize_rows, torch.randn((n, k), device="cuda", generator=g))
+        bias = torch.randn(n, device="cuda", generator=g)
+        q, s = both(ops.quantize_rows, x)
+        one = s.flatten()[:1].contiguous()
+        for out in FLOATS:
+            res = torch.randn(lead + (n,), device="cuda", generator=g).to(out)
+            for args, kw in (((x, None, w, ws), {}), ((x, None, w, ws, bias, res), {}), ((q, s, w, ws, bias, res, 3), {}), ((q, one, w, ws), {}), ((q, s, w, ws, None, None, 2, 0.1), {}),
+                             ((q, s, w, ws, bias, res, 4), dict(residual_after_activation=True)), ((x, None, w.contiguous(), ws, bias), {})):
+                y = both(ops.inner_prod_quantized, *args, out_dtype=out, **kw)
+                assert y.dtype == out and y.shape == lead + (n,)
+                room = torch.empty_like(y)
+                assert ops.inner_prod_quantized(*args, out_dtype=out, out=room, **kw) is room and torch.equal(room, y)
+        assert both(ops.inner_prod_quantized, x, None, w, ws).dtype == dtype and both(ops.inner_prod_quantized, q, s, w, ws).dtype == torch.float32
+    for dtype in FLOATS:
+        image = torch.randn((2,) + lead + (5, 3 * n), device="cuda", generator=g).to(dtype)
+        gamma, beta = torch.randn(3 * n, device="cuda", generator=g), torch.randn(3 * n, device="cuda", generator=g)
+        for kw in (dict(), dict(gamma=gamma, beta=beta, eps=1e-3, activation=2, leaky=0.2), dict(out_dtype=torch.int8, requant_scales=[9.0, 11.0]),
+                   dict(gamma=gamma, out_dtype=torch.int8, requant_scales=[9.0]), dict(beta=beta, out_dtype=dtype, activation=3)):
+            y = both(ops.group_norm_nhwc, image, 3, **kw)
+            assert y.shape == image.shape[:-1] + (ops.padded_channels(3 * n) if "requant_scales" in kw else 3 * n,)
+
+
 def test_refusals():
     from tennis_b200 import ops
     d = case(6, 32, 64, torch.float32, 1)
