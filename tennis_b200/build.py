@@ -7,7 +7,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 
 
 def build(verbose=False):
-    cmd = ["make", "-C", os.path.join(_HERE, "csrc"), "-j8", "PYTHON=" + sys.executable]
+    cmd = ["make", "-C", os.path.join(_HERE, "csrc"), "-j8", "python", "PYTHON=" + sys.executable]
     out = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or out.returncode != 0:
         print(out.stdout)

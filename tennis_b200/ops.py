@@ -540,8 +540,8 @@ def _ordinary():
     try:
         from . import _native as module
     except ImportError as e:
-        raise RuntimeError("tennis_b200: the module _native has not been built (python -c 'import __graft_entry__ as g; g.build()' or make -C "
-                           "tennis_b200/csrc): %s" % e)
+        raise RuntimeError("tennis_b200: the module _native has not been built for this Python and PyTorch (python -c 'import __graft_entry__ as g; "
+                           "g.build()' or make -C tennis_b200/csrc python): %s" % e)
     _native = module
     return module
 

@@ -2,6 +2,8 @@
 plain forms that their GPU tests compare with."""
 import ctypes
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -143,6 +145,30 @@ def test_the_module_of_ordinary_calls(monkeypatch):
     monkeypatch.setitem(sys.modules, "tennis_b200._native", None)
     with pytest.raises(RuntimeError, match="_native has not been built"):
         ops.quantize_rows(cpu((2, 8)))
+
+
+def make(*goals):
+    """What make would run, and its status."""
+    done = subprocess.run(["make", "-n", "-C", ROOT + "/tennis_b200/csrc"] + list(goals), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    return done.returncode, done.stdout
+
+
+def test_the_c_library_is_built_without_python(tmp_path):
+    status, text = make("-B", "PYTHON=" + str(tmp_path / "none"))
+    assert status == 0 and "libtennis_b200.so" in text and "native" not in text
+    status, text = make("python", "PYTHON=" + str(tmp_path / "none"))
+    assert status != 0 and "no PyTorch" in text
+
+
+def test_the_module_is_built_again_for_another_pytorch(lib, tmp_path):
+    """(lib: built just now for this one.)"""
+    status, text = make("python", "PYTHON=" + sys.executable)
+    assert status == 0 and "native.cpp" not in text
+    other = tmp_path / "python"
+    other.write_text("#!/bin/sh\necho another\n")
+    other.chmod(0o755)
+    status, text = make("python", "PYTHON=" + str(other))
+    assert status == 0 and "native.cpp" in text
 
 
 def test_pixel_step():
