@@ -408,10 +408,12 @@ TSB_API size_t tsb_inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *args
 TSB_API int tsb_inner_prod_i8(const tsb_inner_prod_args *args, void *workspace, size_t workspace_bytes, void *stream);
 /*
  * Failure detection, as tsb_conv2d_i8_status: every wait inside the tensor-core kernel is bounded, and one that runs out
- * leaves a code in a word that the library keeps on each GPU.  Waits for the stream, then TSB_OK, or TSB_ERR_DEVICE_TIMEOUT
- * where a call on the current GPU gave up since the last check (tsb_last_error names the wait); the word is cleared.
+ * leaves a code (1..4, which wait) in a word that the library keeps on each GPU.  Waits for the stream, then TSB_OK, or
+ * TSB_ERR_DEVICE_TIMEOUT where a call on the current GPU gave up since the last check (tsb_last_error names the wait); the word is cleared.
+ * _decode: what a word stands for, as a status and a message; needs no GPU.
  */
 TSB_API int tsb_inner_prod_i8_status(void *stream);
+TSB_API int tsb_inner_prod_i8_status_decode(int status_word);
 
 /*
  * Group norm with an activation on channels-last tensors: x [n, pixels, channels], channels in `groups` equal runs.

@@ -101,6 +101,7 @@ SYMBOLS = {
     "tsb_inner_prod_i8_workspace_bytes": (_sz, [ctypes.c_char_p]),
     "tsb_inner_prod_i8": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
     "tsb_inner_prod_i8_status": (_i, [_vp]),
+    "tsb_inner_prod_i8_status_decode": (_i, [_i]),
     "tsb_group_norm_workspace_bytes": (_sz, [ctypes.c_char_p]),
     "tsb_group_norm_nhwc": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
     "tsb_kernel_launch_count": (_i64, []),

@@ -35,7 +35,10 @@ int concat_i8_nhwc(const int8_t *, int, const int8_t *, int, int8_t *, int64_t, 
 int quantize_rows_i8(const void *, int, int64_t, int8_t *, int64_t, float *, int64_t, int64_t, cudaStream_t);
 size_t inner_prod_i8_workspace_bytes(const tsb_inner_prod_args *);
 int inner_prod_i8(const tsb_inner_prod_args *, void *, size_t, cudaStream_t);
-namespace tc { int inner_prod_status(cudaStream_t); }
+namespace tc {
+int inner_prod_status(cudaStream_t);
+int inner_prod_status_decode(int);
+}
 size_t group_norm_workspace_bytes(const tsb_group_norm_desc *);
 int group_norm_nhwc(const tsb_group_norm_desc *, void *, size_t, cudaStream_t);
 
@@ -150,6 +153,7 @@ int tsb_inner_prod_i8(const tsb_inner_prod_args *args, void *workspace, size_t w
     return inner_prod_i8(args, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 int tsb_inner_prod_i8_status(void *stream) { return tc::inner_prod_status((cudaStream_t)stream); }
+int tsb_inner_prod_i8_status_decode(int status_word) { return tc::inner_prod_status_decode(status_word); }
 size_t tsb_group_norm_workspace_bytes(const tsb_group_norm_desc *desc) { return group_norm_workspace_bytes(desc); }
 int tsb_group_norm_nhwc(const tsb_group_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream) {
     return group_norm_nhwc(desc, workspace, workspace_bytes, (cudaStream_t)stream);

@@ -79,6 +79,7 @@ bool inner_prod_can(const InnerProdParams &p, const char **why);     // whether 
 bool weights_fit(const InnerProdParams &p);                           // the part of that that concerns w
 int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream);
 int inner_prod_status(cudaStream_t stream);
+int inner_prod_status_decode(int word);
 }  // namespace tc
 
 // inner_prod_few.cu: the kernel of few tokens

@@ -466,6 +466,15 @@ inner_prod_i8_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_
         }
     }
 done:
+    // Every role of every CTA comes here, whether its work is done or a wait ran out, and meets the others once:
+    //   one CTA   the block's barrier; then warp 1 frees the tensor memory
+    //   pair      the block's barrier, then a phase of the cluster's in which all threads of both CTAs arrive and wait: what one CTA's MMAs, copies and
+    //             arrivals reach in the other is there until both are through.  A wait that runs out in one CTA is not told to the other, whose own waits for
+    //             it run out by themselves
+    //   split     one phase of the cluster's behind the one at the start, in which each thread arrives once: the epilogue warps in their one tile (a
+    //             cluster has one tile, so its loop is entered once and left for here: met), all other warps, and epilogue warps that
+    //             gave up in front of that, below.  Warps that have not met arrive ahead of the block's barrier and wait for the phase behind it; those that have met are
+    //             through it when they come here.  Either way each thread arrives once and waits once, and sums are written to another CTA ahead of the arrival only
     if (L::kAhead) asm volatile("cp.async.wait_all;" ::: "memory");
     if (warp >= 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");      // this warp's outputs are written
     if (*abort_flag) {
@@ -612,6 +621,14 @@ int inner_prod(const InnerProdParams &p, int y_type, cudaStream_t stream) {
     }
 }
 
+// What a status word stands for.
+int inner_prod_status_decode(int word) {
+    if (word == 0) return TSB_OK;
+    static const char *const kWaits[] = {"a stage to be free", "a stage to be loaded", "sums to be read", "sums to be complete"};
+    return fail(TSB_ERR_DEVICE_TIMEOUT, "inner_prod_i8: the wait for %s ran out; results since the last check are not to be used",
+                word >= 1 && word <= 4 ? kWaits[word - 1] : "an unknown event");
+}
+
 // The device's status word: waits for the stream, reads and clears it.
 int inner_prod_status(cudaStream_t stream) {
     int word = 0, zero = 0;
@@ -622,9 +639,7 @@ int inner_prod_status(cudaStream_t stream) {
     if (word == 0) return TSB_OK;
     TSB_CUDA(cudaMemcpyAsync(at, &zero, sizeof(zero), cudaMemcpyHostToDevice, stream));
     TSB_CUDA(cudaStreamSynchronize(stream));
-    static const char *const kWaits[] = {"a stage to be free", "a stage to be loaded", "sums to be read", "sums to be complete"};
-    return fail(TSB_ERR_DEVICE_TIMEOUT, "inner_prod_i8: the wait for %s ran out; results since the last check are not to be used",
-                word >= 1 && word <= 4 ? kWaits[word - 1] : "an unknown event");
+    return inner_prod_status_decode(word);
 }
 
 }  // namespace tc
