@@ -304,8 +304,9 @@ __device__ __forceinline__ void pad_channels(const GroupNormParams &p, const Par
         static_cast<int8_t *>(p.y)[t.image * p.y_image + (t.p0 + i / extra) * p.y_pixel + p.channels + i % extra] = 0;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// (not the aligned forms, for which all threads of a warp have to come at once: here they come from loops of different lengths)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 __device__ __forceinline__ double2 load_of_rank(const double2 *mine, uint32_t rank) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(mine)), "r"(rank));
