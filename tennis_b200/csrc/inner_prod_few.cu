@@ -2,7 +2,8 @@
 //
 //   block      16 output channels and all of K; its warps take blocks of 128 bytes of K in turn, and their int32 sums meet in shared memory
 //   loads      cp.async into a ring of the warp's own, kDepth blocks of K ahead; a thread reads back what it loaded itself, so a ring needs
-//              no barrier.  The blocks on a multiprocessor have 128 KB of weights under way, whatever their number of warps
+//              no barrier.  The sixteen warps on a multiprocessor have 128 KB of weights under way for up to 8 tokens, 96 KB for up to 16, 64 KB for
+//              up to 32, whose own loads take the rest of the rings
 //   product    mma.sync m16n8k32: a thread's 16 bytes of a weight row and of a token's row are the operands of two MMAs, which so take
 //              the 64 bytes of four threads in an order of K of their own -- the same one for both operands, which is all that a sum
 //              needs.  (The MMAs of up to 32 tokens take a fraction of the loads' time; tcgen05 would only add its set-up.)

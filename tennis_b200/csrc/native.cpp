@@ -35,7 +35,7 @@ Tensor room(at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType type,
 }
 Tensor bytes(int64_t n, c10::Device device) { return room({n}, {1}, at::kByte, device); }
 
-// A tensor argument on `device` (-1: any CUDA device that is the current one); NULL with *bad for what is none
+// A tensor argument on `device` (-1: any CUDA device that is the current one); NULL for anything else
 const Tensor *tensor(PyObject *o, int device) {
     if (!THPVariable_Check(o)) return nullptr;
     const Tensor &t = THPVariable_Unpack(o);
