@@ -39,8 +39,8 @@ extern "C" {
 #define TSB_ACT_RELU 1       /* src/kernels/cpu/relu.cpp:30-52 */
 #define TSB_ACT_LEAKY_RELU 2 /* src/kernels/cpu/leaky_relu.cpp:39-67, attribute "scale" */
 /* ... and, beyond the convolutions' three, after tsb_inner_prod_i8 and tsb_group_norm_nhwc */
-#define TSB_ACT_SILU 3       /* v / (1 + exp(-v)) */
-#define TSB_ACT_GELU 4       /* v / 2 * (1 + erf(v / sqrt(2))) */
+#define TSB_ACT_SILU 3       /* v / (1 + exp(-v)); 0 below v = -87, where that is less than 10^-35 */
+#define TSB_ACT_GELU 4       /* v / 2 * (1 + erf(v / sqrt(2))), in fp32 steps: far below zero the sum's rounding shows, up to |v| 2^-24 */
 
 /* element types of the operators that take more than one */
 #define TSB_TYPE_F32 0
@@ -419,9 +419,12 @@ TSB_API int tsb_inner_prod_i8_status_decode(int status_word);
  * Group norm with an activation on channels-last tensors: x [n, pixels, channels], channels in `groups` equal runs.
  *   mean, variance (biased) of an image's group over its pixels and channels, summed in 64 bits
  *   v = (x - mean) * (1 / sqrt(variance + eps)) * gamma[c] + beta[c];  y = activation(v)
- * mean and reciprocal deviation are rounded to fp32 once; the steps behind are separately rounded fp32 operations.
+ * mean and reciprocal deviation are rounded to fp32 once; the steps behind are separately rounded fp32 operations.  The variance is the mean square less
+ * the squared mean, in 64 bits: its relative error is some (mean / deviation)^2 2^-52 (10^-8 at means of 10^4 deviations, 10^-4 at 10^6, where the
+ * rounded mean alone is off by hundredths of a deviation).
  *   - x: fp32, fp16 or bf16, channels next to each other, pixels and images any number of elements apart.
- *   - y of x's type, pixels and images apart likewise; it may be x itself (same address and strides), else they do not overlap.
+ *   - y of x's type, pixels apart likewise, images one behind the other (TSB_ERR_INVALID_ARGUMENT where they interleave); it may be x itself (same
+ *     address and strides), else they do not overlap.
  *   - y of TSB_TYPE_I8: quantize(v) with the rules of tsb_quantize_f32_i8 on the channel-major element index and one
  *     requantize scale for the batch or one per image, written as NHWC_PAD (dense, padding channels zero; y's strides
  *     are not looked at): what tsb_conv2d_i8_run takes as TSB_LAYOUT_NHWC_PAD and tsb_inner_prod_i8 as int8 rows of one scale.

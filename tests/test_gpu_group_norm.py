@@ -69,6 +69,17 @@ def test_values_far_from_zero(shape, groups):
     check(ops.group_norm_nhwc(small, groups, gamma, beta, 0.0), small, groups, gamma, beta, 0.0)
 
 
+@pytest.mark.parametrize("mean", [1e4, -1e6, 1e7])
+@pytest.mark.parametrize("shape,groups", [((2, 11, 11, 64), 8), ((1, 90, 90, 96), 32), ((1, 9, 9, 15), 3)])
+def test_means_of_many_deviations(shape, groups, mean):
+    """The variance's relative error, (mean / deviation)^2 2^-52 or a small multiple of it (counted here with 2^-49), beside the rounded mean's."""
+    from tennis_b200 import ops
+    x, gamma, beta = tensors(shape, torch.float32, 3, shift=0.0)
+    x = x + mean
+    want, bound = plain.group_norm(numbers(x), groups, numbers(gamma), numbers(beta))
+    plain.assert_close(ops.group_norm_nhwc(x, groups, gamma, beta), want, bound + np.abs(want - numbers(beta)) * (mean / 0.5) ** 2 * 2.0 ** -49, torch.float32)
+
+
 @pytest.mark.parametrize("dtype", FLOATS, ids=str)
 @pytest.mark.parametrize("shape,groups", [((2, 8, 8, 64), 8), ((2, 16, 8, 32), 8), ((1, 256, 256, 256), 32), ((1, 256, 256, 128), 32)])
 def test_steps_are_rounded_one_by_one(shape, groups, dtype):
