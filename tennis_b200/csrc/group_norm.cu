@@ -12,9 +12,9 @@
 //   swept      larger images: one launch sums, a small one makes the statistics, the third reads again and normalizes, in the reverse
 //              order, so that it finds in the L2 what the first read last.  (Batch by batch, each small enough for the L2, the
 //              launches' beginnings and ends cost more than the reads of HBM that they save: 8 x 256 x 256 x 256 bf16 152 us in one
-//              batch, 176 in batches of two images, 266 image by image)
+//              batch when that was tried, 176 in batches of two images, 266 image by image)
 // Measured: 16 x 56 x 56 x 256 bf16 to int8 20 us (resident; load, meeting and writing follow each other in its one round of blocks), 8 x 256 x 256 x 256
-// bf16 152 us (swept: 805 MB at 5.3 TB/s, the rate of a copy), 16 x 16 x 128 fp32 3.5 us.
+// bf16 with silu 147 us (swept: 805 MB at 5.5 TB/s, near the rate of a copy), 16 x 16 x 128 fp32 3.5 us.
 #include "typed.cuh"
 
 #include <algorithm>
@@ -27,7 +27,7 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;                  // the portable limit
 constexpr int kMaxGroups = 256;                 // groups of a run of channels
-constexpr int kResidentBlocks = 4;               // resident blocks a multiprocessor, by their registers (2000 x 14 x 14 x 256 bf16 122 us, with three 131)
+constexpr int kResidentBlocks = 4;               // resident blocks a multiprocessor, by their registers (2000 x 14 x 14 x 256 bf16 with silu 128 us; with three 131, against 122 at the time)
 constexpr int64_t kLargeTile = 200 * 1024;      // shared memory of a resident block, at most
 
 struct GroupNormParams {
@@ -556,7 +556,7 @@ Plan make_plan(const tsb_group_norm_desc *d) {
     q.tiles = (int)ceil_div64(d->pixels, q.tile);
     q.smem = (size_t)q.run_groups * 16 + (size_t)kDepth * kThreads * 16;      // (at least collect's scratch: a vector has at most eight pairs of sums)
     // Of a tensor beyond 80 MB the L2 is to keep that much, the end of it, for the second reading: what comes before, and the outputs, goes
-    // first (8 x 256 x 256 x 256 bf16 154 -> 151 us, 16 x 128 x 128 x 256 79 -> 73)
+    // first (8 x 256 x 256 x 256 bf16 154 -> 151 us, 16 x 128 x 128 x 256 79 -> 73 when it came; 147 and 76 now)
     q.let_go = (int)std::max<int64_t>(0, std::min<int64_t>(INT32_MAX, d->n * q.runs * q.tiles - (80 << 20) / std::max<int64_t>(1, q.tile * width * size)));
     q.off_stats = align256((size_t)d->n * q.runs * q.tiles * q.run_groups * sizeof(double2));
     q.bytes = q.off_stats + align256((size_t)d->n * groups * sizeof(float2));

@@ -16,8 +16,8 @@
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of kGroupM token tiles, whose operands
 //              the L2 then serves
 //
-// Measured, bf16 out: 8192^3 331 us (3.3 POPS, tensor pipe 90 % active), 4096^3 48 us, 64 x 4096 x 4096 8.1 us; 100352 x 256 x 64 20 us, where
-// the epilogue bounds it (silu: 28).
+// Measured, bf16 out: 8192^3 331 us (3.3 POPS, tensor pipe 90 % active; with a residual 353), 4096^3 49 us (54), 64 x 4096 x 4096 8.1 us;
+// 100352 x 256 x 64 20 us (27), where the epilogue bounds it (silu: 27.6).
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and
 // all roles go to the common exit.
