@@ -47,6 +47,7 @@ extern "C" {
 #define TSB_TYPE_F16 1
 #define TSB_TYPE_BF16 2
 #define TSB_TYPE_I8 3
+#define TSB_TYPE_MXFP4 4       /* 4-bit floating point, a scale for every 32 values of a row: see tsb_quantize_rows_mxfp4 */
 
 /* memory layouts of activations */
 #define TSB_LAYOUT_NCHW 0     /* the operator-visible layout of TenniS tensors */
@@ -447,6 +448,94 @@ typedef struct tsb_group_norm_desc {
 /* Scratch of a call, as for tsb_inner_prod_i8. */
 TSB_API size_t tsb_group_norm_workspace_bytes(const tsb_group_norm_desc *desc);
 TSB_API int tsb_group_norm_nhwc(const tsb_group_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Rows in microscaled 4-bit floating point (the OCP microscaling format MXFP4; like the three operators above, without a counterpart in
+ * the reference).  32 neighbouring values of a row, a group, share a power of two:
+ *   a = max |x| of the group;  e = max(floor(log2 a) - 2, -127);  code = e2m1(x / 2^e);  2^e * code stands for x
+ *   - Codes: sign, two bits of exponent, one of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, rounded to nearest, ties to the
+ *     even code, beyond 6 to 6; the sign of a zero is kept.  Two codes a byte, the lower half first; a row is tsb_mxfp4_row_bytes(cols) =
+ *     16 ceil(cols / 32) bytes, zeros behind its last value.
+ *   - Scales: a byte e + 127 a group (E8M0), in tiles of 128 rows x 4 groups, the order that the tensor cores read: row r's group g is byte
+ *       (r / 128 * ceil(cols / 128) + g / 4) * 512 + r % 32 * 16 + r % 128 / 32 * 4 + g % 4
+ *     of tsb_mxfp4_scale_bytes(rows, cols) = ceil(rows / 128) * ceil(cols / 128) * 512, all of which are written (zero where there is no group).
+ *   - A group of zeros has the scale 2^-127.  A NaN or an infinity in a group makes its scale NaN (byte 255), and with it all its values.
+ *   - x: fp32, fp16 or bf16, rows x_pitch elements apart (0: the same row again);  q: rows q_pitch bytes apart.  Nothing overlaps.  What starts at a
+ *     multiple of 16 bytes (scales and q, and a q_pitch that is one) is what tsb_inner_prod_mxfp4 reads fastest.
+ * _dequantize: y[r][c] = 2^e * code, rounded once to y's type (fp32 and bf16 hold it exactly, but for the ends of their ranges).
+ */
+TSB_API int64_t tsb_mxfp4_row_bytes(int64_t cols);
+TSB_API int64_t tsb_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+TSB_API int tsb_quantize_rows_mxfp4(const void *x, int x_type, int64_t x_pitch, void *q, int64_t q_pitch, void *scales, int64_t rows,
+                                    int64_t cols, void *stream);
+TSB_API int tsb_dequantize_rows_mxfp4(const void *q, int64_t q_pitch, const void *scales, void *y, int y_type, int64_t y_pitch,
+                                      int64_t rows, int64_t cols, void *stream);
+
+/*
+ * inner product on 4-bit rows: y[m][n] = activation(sum_k x[m][k] * w[n][k] (+ bias[n]) (+ residual[m][n])) of the values that codes
+ * and scales stand for.
+ *   - Products are exact, sums are held in fp32; their order, and with it the last bits, depend on the kernel that the sizes choose, but not on the
+ *     values, the call or the rows of other tiles: the same call gives the same bits.  Steps behind the sum as in tsb_inner_prod_i8.
+ *   - x: 4-bit rows with x_scales, or floating rows without: those are quantized as tsb_quantize_rows_mxfp4 does it.
+ *   - w, w_scales: n rows of k values, as tsb_quantize_rows_mxfp4 lays out a weight tensor.  Rows are read to the end of their last
+ *     group, where zeros lie behind the k values.
+ *   - Any pitch and alignment is right; 4-bit operands at multiples of 16 bytes run on the tensor cores.
+ *   - y does not overlap the other tensors, but may be the residual itself (same address and pitch).
+ *   - m = 0 or n = 0: nothing is done.
+ */
+typedef struct tsb_inner_prod_mxfp4_args {
+    int64_t m, n, k;                 /* y [m, n] = x [m, k] . w [n, k] */
+    const void *x;
+    int64_t x_pitch;                 /* of 4-bit rows bytes, of floating ones elements */
+    const void *x_scales;            /* device; NULL with a floating x */
+    const void *w;
+    int64_t w_pitch;                 /* bytes */
+    const void *w_scales;
+    const float *bias;               /* [n] device or NULL */
+    const void *residual;            /* device or NULL, of y's type */
+    int64_t residual_pitch;          /* elements, here and below */
+    void *y;
+    int64_t y_pitch;
+    int x_type;                      /* TSB_TYPE_MXFP4, or a floating type */
+    int y_type;                      /* TSB_TYPE_F32, F16 or BF16 */
+    int activation;                  /* TSB_ACT_* */
+    float leaky_scale;
+    int residual_after_activation;   /* 0: act(v + residual); 1: act(v) + residual */
+    int kernel;                      /* TSB_KERNEL_AUTO; another one is tests' (TSB_ERR_UNSUPPORTED where it cannot) */
+} tsb_inner_prod_mxfp4_args;
+
+/* Scratch of a call with floating rows, as for tsb_inner_prod_i8. */
+TSB_API size_t tsb_inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *args);
+TSB_API int tsb_inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *args, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Root-mean-square norm of rows, with the addition of a residual in front of it and rows quantized for a product behind it.
+ *   h = x (+ residual, one fp32 addition rounded to x's type);  s = fp32(1 / sqrt(sum h^2 / cols + eps)), sum and root in 64 bits
+ *   v = (h * s) * gamma[c], two separately rounded fp32 products
+ *   y_type x_type             y = v, rounded to that type
+ *   y_type TSB_TYPE_I8        y and scales as tsb_quantize_rows_i8 makes them of v (scales: float [rows])
+ *   y_type TSB_TYPE_MXFP4     y and scales as tsb_quantize_rows_mxfp4 makes them of v
+ *   - x, residual: fp32, fp16 or bf16 of one type, rows any number of elements apart (0: the same row again).
+ *   - sum: h of every row, or NULL where it is not wanted; without a residual it has to be NULL.  It may be x or residual itself (same address and pitch).
+ *   - y of x_type may be x or residual itself where sum is not the same tensor.  Else nothing overlaps.
+ */
+typedef struct tsb_rms_norm_desc {
+    int64_t rows, cols;
+    const void *x;
+    int64_t x_pitch;                 /* elements between rows, here and below (y in 4 bits: bytes) */
+    const void *residual;            /* or NULL */
+    int64_t residual_pitch;
+    void *sum;                       /* or NULL */
+    int64_t sum_pitch;
+    const float *gamma;              /* [cols] device, or NULL: 1 */
+    void *y;
+    int64_t y_pitch;
+    void *scales;                    /* int8 and 4-bit y */
+    double eps;
+    int x_type, y_type;
+} tsb_rms_norm_desc;
+
+TSB_API int tsb_rms_norm(const tsb_rms_norm_desc *desc, void *stream);
 
 #ifdef TSB_ENABLE_TRACE
 /* Profiling builds only (compile the library with -DTSB_ENABLE_TRACE; release builds carry neither this symbol nor the

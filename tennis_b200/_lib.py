@@ -17,7 +17,7 @@ ERR_WORKSPACE_TOO_SMALL = -3
 ERR_DEVICE_TIMEOUT = -4
 
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4
-TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8 = 0, 1, 2, 3
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_I8, TYPE_MXFP4 = 0, 1, 2, 3, 4
 LAYOUT_NCHW, LAYOUT_NHWC_PAD, LAYOUT_STAGED = 0, 1, 2
 KERNEL_AUTO, KERNEL_DIRECT, KERNEL_TCGEN05 = 0, 1, 2
 TUNE_AUTO, TUNE_OFF, TUNE_ON = 0, 1, 2
@@ -52,9 +52,11 @@ class ConvEpilogue(ctypes.Structure):
     ]
 
 
-# tsb_inner_prod_args and tsb_group_norm_desc, packed field by field (both have their wide fields first)
+# tsb_inner_prod_args, tsb_group_norm_desc, tsb_inner_prod_mxfp4_args and tsb_rms_norm_desc, packed field by field (all have their wide fields first)
 INNER_PROD_ARGS = struct.Struct("@3q P q P q P q P P P q P q i i i f i i")
 GROUP_NORM_DESC = struct.Struct("@4q P 2q P 2q P P d P i i i i f 0q")
+INNER_PROD_MXFP4_ARGS = struct.Struct("@3q P q P P q P P P q P q i i i f i i")
+RMS_NORM_DESC = struct.Struct("@2q P q P q P q P P q P d i i")
 
 
 # name -> (restype, argtypes); every symbol include/tennis_b200.h declares
@@ -104,6 +106,13 @@ SYMBOLS = {
     "tsb_inner_prod_i8_status_decode": (_i, [_i]),
     "tsb_group_norm_workspace_bytes": (_sz, [ctypes.c_char_p]),
     "tsb_group_norm_nhwc": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
+    "tsb_mxfp4_row_bytes": (_i64, [_i64]),
+    "tsb_mxfp4_scale_bytes": (_i64, [_i64, _i64]),
+    "tsb_quantize_rows_mxfp4": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "tsb_dequantize_rows_mxfp4": (_i, [_vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _vp]),
+    "tsb_inner_prod_mxfp4_workspace_bytes": (_sz, [ctypes.c_char_p]),
+    "tsb_inner_prod_mxfp4": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
+    "tsb_rms_norm": (_i, [ctypes.c_char_p, _vp]),
     "tsb_kernel_launch_count": (_i64, []),
 }
 

@@ -41,6 +41,14 @@ int inner_prod_status_decode(int);
 }
 size_t group_norm_workspace_bytes(const tsb_group_norm_desc *);
 int group_norm_nhwc(const tsb_group_norm_desc *, void *, size_t, cudaStream_t);
+// quantize_mxfp4.cu, inner_prod_mxfp4.cu, rms_norm.cu
+int quantize_rows_mxfp4(const void *, int, int64_t, void *, int64_t, void *, int64_t, int64_t, cudaStream_t);
+int dequantize_rows_mxfp4(const void *, int64_t, const void *, void *, int, int64_t, int64_t, int64_t, cudaStream_t);
+int64_t mxfp4_row_bytes(int64_t);
+int64_t mxfp4_scale_bytes(int64_t, int64_t);
+size_t inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *);
+int inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *, void *, size_t, cudaStream_t);
+int rms_norm(const tsb_rms_norm_desc *, cudaStream_t);
 
 namespace {
 
@@ -158,6 +166,19 @@ size_t tsb_group_norm_workspace_bytes(const tsb_group_norm_desc *desc) { return 
 int tsb_group_norm_nhwc(const tsb_group_norm_desc *desc, void *workspace, size_t workspace_bytes, void *stream) {
     return group_norm_nhwc(desc, workspace, workspace_bytes, (cudaStream_t)stream);
 }
+int64_t tsb_mxfp4_row_bytes(int64_t cols) { return mxfp4_row_bytes(cols); }
+int64_t tsb_mxfp4_scale_bytes(int64_t rows, int64_t cols) { return mxfp4_scale_bytes(rows, cols); }
+int tsb_quantize_rows_mxfp4(const void *x, int x_type, int64_t x_pitch, void *q, int64_t q_pitch, void *scales, int64_t rows, int64_t cols, void *stream) {
+    return quantize_rows_mxfp4(x, x_type, x_pitch, q, q_pitch, scales, rows, cols, (cudaStream_t)stream);
+}
+int tsb_dequantize_rows_mxfp4(const void *q, int64_t q_pitch, const void *scales, void *y, int y_type, int64_t y_pitch, int64_t rows, int64_t cols, void *stream) {
+    return dequantize_rows_mxfp4(q, q_pitch, scales, y, y_type, y_pitch, rows, cols, (cudaStream_t)stream);
+}
+size_t tsb_inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *args) { return inner_prod_mxfp4_workspace_bytes(args); }
+int tsb_inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *args, void *workspace, size_t workspace_bytes, void *stream) {
+    return inner_prod_mxfp4(args, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+int tsb_rms_norm(const tsb_rms_norm_desc *desc, void *stream) { return rms_norm(desc, (cudaStream_t)stream); }
 
 int tsb_pool_out_dim(int x, int pad_lo, int pad_hi, int k, int stride) {
     if (x < 1 || k < 1 || stride < 1 || pad_lo < 0 || pad_hi < 0) return fail(TSB_ERR_INVALID_ARGUMENT, "pool_out_dim: bad geometry");

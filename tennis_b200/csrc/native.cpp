@@ -1,5 +1,5 @@
-// The ordinary calls of ops.quantize_rows, inner_prod_quantized and group_norm_nhwc, from Python straight to the C ABI: tensors on the
-// current device and stream, rows and images that lie one after the other, outputs that are allocated.  A kernel of these can be done in
+// The ordinary calls of ops.quantize_rows, inner_prod_quantized, group_norm_nhwc, quantize_rows_mxfp4, inner_prod_mxfp4 and rms_norm, from Python
+// straight to the C ABI: tensors on the current device and stream, rows and images that lie one after the other, outputs that are allocated.  A kernel of these can be done in
 // 2 us, where the checks, the allocations and the call take some 8 us in Python and half of that here.
 //
 // Each function returns its result, or None for any call that is not an ordinary one, wrong ones among them: ops.py then makes the same call
@@ -225,12 +225,173 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- 4 bits
+constexpr at::ScalarType kFp4 = at::ScalarType::Float4_e2m1fn_x2, kE8m0 = at::ScalarType::Float8_e8m0fnu;
+int64_t row_bytes(int64_t k) { return (k + 31) / 32 * 16; }
+
+// Room for the scales of m rows of k values
+Tensor scale_tiles(int64_t m, int64_t k, c10::Device device) {
+    const int64_t tiles = (k + 127) / 128;
+    return room({(m + 127) / 128, tiles, 32, 4, 4}, {tiles * 512, 512, 16, 4, 1}, kE8m0, device);
+}
+
+// A 4-bit matrix's scales; false for anything else
+bool scales_of(PyObject *o, int64_t m, int64_t k, int device, const void **at) {
+    const Tensor *t = tensor(o, device);
+    if (!t || (t->scalar_type() != kE8m0 && t->scalar_type() != at::kByte) || t->dim() != 5 || t->size(0) != (m + 127) / 128 || t->size(1) != (k + 127) / 128 || t->size(2) != 32 ||
+        t->size(3) != 4 || t->size(4) != 4 || !t->is_contiguous())
+        return false;
+    *at = t->const_data_ptr();
+    return true;
+}
+bool is_fp4(const Tensor &t) { return (t.scalar_type() == kFp4 || t.scalar_type() == at::kByte) && t.dim() >= 1 && t.size(-1) > 0 && t.size(-1) % 16 == 0; }
+
+PyObject *tuple_of(std::initializer_list<Tensor> all) {
+    PyObject *t = PyTuple_New((Py_ssize_t)all.size());
+    if (!t) return nullptr;
+    Py_ssize_t i = 0;
+    for (const Tensor &v : all) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(v));
+    return t;
+}
+
+// quantize_rows_mxfp4(x) -> (q, scales)
+PyObject *quantize_rows_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = count == 1 ? tensor(args[0], -1) : nullptr;
+    int type;
+    int64_t rows, pitch;
+    if (!x || !type_of(x->scalar_type(), &type) || !rows_of(*x, &rows, &pitch)) Py_RETURN_NONE;
+    const int64_t k = x->size(-1);
+    const Tensor q = dense(*x, row_bytes(k), kFp4), s = scale_tiles(rows, k, x->device());
+    if (tsb_quantize_rows_mxfp4(x->const_data_ptr(), type, pitch, q.mutable_data_ptr(), row_bytes(k), s.mutable_data_ptr(), rows, k, stream_of(x->get_device())) != TSB_OK) Py_RETURN_NONE;
+    return tuple_of({q, s});
+    END_HANDLE_TH_ERRORS
+}
+
+// inner_prod_mxfp4(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, residual_after) -> y
+PyObject *inner_prod_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = count == 10 ? tensor(args[0], -1) : nullptr;
+    if (!x) Py_RETURN_NONE;
+    const int device = x->get_device();
+    const Tensor *w = tensor(args[2], device);
+    tsb_inner_prod_mxfp4_args a = {};
+    if (!w || !is_fp4(*w) || w->dim() != 2 || w->stride(1) != 1 || !rows_of(*x, &a.m, &a.x_pitch)) Py_RETURN_NONE;
+    a.n = w->size(0);
+    a.k = 2 * w->size(1);
+    if (a.m < 1 || a.n < 1) Py_RETURN_NONE;
+    a.w_pitch = w->stride(0);
+    at::ScalarType out = at::kFloat;
+    if (args[1] == Py_None) {
+        if (!type_of(x->scalar_type(), &a.x_type) || row_bytes(x->size(-1)) != w->size(1)) Py_RETURN_NONE;
+        a.k = x->size(-1);
+        out = x->scalar_type();
+    } else {
+        if (!is_fp4(*x) || x->size(-1) != w->size(1) || !scales_of(args[1], a.m, a.k, device, &a.x_scales)) Py_RETURN_NONE;
+        a.x_type = TSB_TYPE_MXFP4;
+    }
+    if (args[8] != Py_None) {
+        if (!THPDtype_Check(args[8])) Py_RETURN_NONE;
+        out = reinterpret_cast<THPDtype *>(args[8])->scalar_type;
+    }
+    if (!type_of(out, &a.y_type) || !scales_of(args[3], a.n, a.k, device, &a.w_scales) || !vector(args[4], a.n, device, &a.bias)) Py_RETURN_NONE;
+    if (args[5] != Py_None) {
+        const Tensor *r = tensor(args[5], device);
+        int64_t rows;
+        if (!r || r->scalar_type() != out || r->dim() != x->dim() || r->size(-1) != a.n || !rows_of(*r, &rows, &a.residual_pitch) || rows != a.m ||
+            r->sizes().slice(0, r->dim() - 1) != x->sizes().slice(0, x->dim() - 1))
+            Py_RETURN_NONE;
+        a.residual = r->const_data_ptr();
+    }
+    a.activation = int_of(args[6]);
+    a.leaky_scale = (float)PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    a.residual_after_activation = args[9] == Py_True;
+    a.x = x->const_data_ptr();
+    a.w = w->const_data_ptr();
+    const Tensor y = dense(*x, a.n, out);
+    a.y = y.mutable_data_ptr();
+    a.y_pitch = a.n;
+    const size_t size = a.x_type == TSB_TYPE_MXFP4 ? 0 : tsb_inner_prod_mxfp4_workspace_bytes(&a);
+    Tensor workspace;
+    if (size) workspace = bytes((int64_t)size, x->device());
+    if (tsb_inner_prod_mxfp4(&a, size ? workspace.mutable_data_ptr() : nullptr, size, stream_of(device)) != TSB_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm(x, gamma, residual, eps, out_dtype) -> y, or (q, scales); with a residual the sum as one result more
+PyObject *rms_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    const Tensor *x = count == 5 ? tensor(args[0], -1) : nullptr;
+    tsb_rms_norm_desc d = {};
+    if (!x || !type_of(x->scalar_type(), &d.x_type) || !rows_of(*x, &d.rows, &d.x_pitch) || d.rows < 1) Py_RETURN_NONE;
+    const int device = x->get_device();
+    d.cols = x->size(-1);
+    if (!vector(args[1], d.cols, device, &d.gamma)) Py_RETURN_NONE;
+    Tensor sum;
+    if (args[2] != Py_None) {
+        const Tensor *r = tensor(args[2], device);
+        int64_t rows;
+        if (!r || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes() || !rows_of(*r, &rows, &d.residual_pitch) || rows != d.rows) Py_RETURN_NONE;
+        d.residual = r->const_data_ptr();
+    }
+    d.eps = PyFloat_AsDouble(args[3]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    at::ScalarType out = x->scalar_type();
+    if (args[4] != Py_None) {
+        if (!THPDtype_Check(args[4])) Py_RETURN_NONE;
+        out = reinterpret_cast<THPDtype *>(args[4])->scalar_type;
+    }
+    Tensor y, scales;
+    if (out == x->scalar_type()) {
+        d.y_type = d.x_type;
+        d.y_pitch = d.cols;
+        y = dense(*x, d.cols, out);
+    } else if (out == at::kChar) {
+        d.y_type = TSB_TYPE_I8;
+        d.y_pitch = (d.cols + 15) / 16 * 16;
+        if (x->dim() != 2 && (x->dim() == 1 || d.y_pitch != d.cols)) Py_RETURN_NONE;
+        y = x->dim() == 2 ? room({d.rows, d.cols}, {d.y_pitch, 1}, at::kChar, x->device()) : dense(*x, d.cols, at::kChar);
+        scales = room({d.rows}, {1}, at::kFloat, x->device());
+        if (x->dim() != 2) scales = scales.view(x->sizes().slice(0, x->dim() - 1));
+    } else if (out == kFp4) {
+        d.y_type = TSB_TYPE_MXFP4;
+        d.y_pitch = row_bytes(d.cols);
+        y = dense(*x, d.y_pitch, kFp4);
+        scales = scale_tiles(d.rows, d.cols, x->device());
+    } else {
+        Py_RETURN_NONE;
+    }
+    if (d.residual) {
+        sum = dense(*x, d.cols, x->scalar_type());
+        d.sum = sum.mutable_data_ptr();
+        d.sum_pitch = d.cols;
+    }
+    d.x = x->const_data_ptr();
+    d.y = y.mutable_data_ptr();
+    d.scales = scales.defined() ? scales.mutable_data_ptr() : nullptr;
+    if (tsb_rms_norm(&d, stream_of(device)) != TSB_OK) Py_RETURN_NONE;
+    if (scales.defined()) return d.residual ? tuple_of({y, scales, sum}) : tuple_of({y, scales});
+    return d.residual ? tuple_of({y, sum}) : THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef kMethods[] = {
     {"quantize_rows", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(quantize_rows)), METH_FASTCALL, nullptr},
     {"inner_prod", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(inner_prod)), METH_FASTCALL, nullptr},
     {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(group_norm)), METH_FASTCALL, nullptr},
+    {"quantize_rows_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(quantize_rows_mxfp4)), METH_FASTCALL, nullptr},
+    {"inner_prod_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(inner_prod_mxfp4)), METH_FASTCALL, nullptr},
+    {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rms_norm)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "The ordinary calls of the int8 layers.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "The ordinary calls of the int8 and 4-bit layers.", -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

@@ -528,6 +528,7 @@ _TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloa
 _FLOATS = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _FLOAT_NAMES = "float32, float16 or bfloat16, not %s"
 _int8, _float32 = torch.int8, torch.float32
+_mxfp4, _e8m0, _uint8 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu, torch.uint8
 
 
 _native = None
@@ -805,3 +806,259 @@ def _pixel_step(x):
                 return None
             step = stride * size
     return c if first is None else first
+
+
+# ---- layers in 4 bits: quantize_rows_mxfp4, dequantize_rows_mxfp4, inner_prod_mxfp4; rms_norm, in front of products in 8 or 4 bits ----------
+# Devices, streams, and which calls go through native.cpp: as above.  A 4-bit matrix [m, k] is a tensor of torch.float4_e2m1fn_x2 (two
+# values an element), [m, 16 * ceil(k / 32)], and its scales are one of torch.float8_e8m0fnu, [ceil(m / 128), ceil(k / 128), 32, 4, 4] in the order that the
+# tensor cores read (mxfp4_scale_tiles makes it of scales row by row); uint8 tensors of the same bytes are taken too.
+def _row_bytes(k):
+    return (k + 31) // 32 * 16
+
+
+def _scale_shape(m, k):
+    return ((m + 127) // 128, (k + 127) // 128, 32, 4, 4)
+
+
+def _check_mxfp4(t, device, name):
+    if (t.dtype is not _mxfp4 and t.dtype is not _uint8) or t.get_device() != device:
+        _refuse("%s: float4_e2m1fn_x2 (or its bytes as uint8) on x's device, not %s", name, t.dtype)
+    if not t.dim() or t.shape[-1] % 16 or not t.shape[-1]:
+        _refuse("%s.size(-1): 16 bytes for every 32 values", name)
+
+
+def _check_scales(t, m, k, device, name):
+    if (t.dtype is not _e8m0 and t.dtype is not _uint8) or t.shape != _scale_shape(m, k) or t.get_device() != device or not t.is_contiguous():
+        _refuse("%s: contiguous float8_e8m0fnu (or its bytes as uint8) of %s on x's device", name, list(_scale_shape(m, k)))
+
+
+def mxfp4_scale_tiles(scales, out=None):
+    """Scales of a 4-bit matrix as other programs hold them, [m, ceil(k / 32)] row by row (float8_e8m0fnu or uint8), in the order of
+    quantize_rows_mxfp4's: [ceil(m / 128), ceil(groups / 4), 32, 4, 4], zero where there is no row or group.  For weights, once."""
+    if scales.dim() != 2 or (scales.dtype is not _e8m0 and scales.dtype is not _uint8):
+        _refuse("scales: float8_e8m0fnu or uint8 [m, groups], not %s", scales.dtype)
+    m, groups = scales.shape
+    room = torch.zeros(((m + 127) // 128 * 128, (groups + 3) // 4 * 4), dtype=_uint8, device=scales.device)
+    room[:m, :groups] = scales.view(_uint8)
+    tiles = room.view(-1, 4, 32, room.shape[1] // 4, 4).permute(0, 3, 2, 1, 4)
+    if out is None:
+        return tiles.contiguous().view(_e8m0)
+    _check_scales(out, m, 32 * groups, scales.get_device(), "out")
+    out.view(_uint8).copy_(tiles)
+    return out
+
+
+def quantize_rows_mxfp4(x, out=None, scales=None, stream=None):
+    """4-bit values of x [..., k] (fp32, fp16 or bf16) with a power of two for every 32 of a row: (q, scales), as tsb_quantize_rows_mxfp4 says.
+
+    q is [..., 16 * ceil(k / 32)] float4_e2m1fn_x2, scales [ceil(m / 128), ceil(k / 128), 32, 4, 4] float8_e8m0fnu over the m rows of x.  The
+    rows are tokens of an activation, or output channels of a weight tensor.  ``out`` and ``scales`` take the results where they are given."""
+    if out is None and scales is None and stream is None:
+        done = (_native or _ordinary()).quantize_rows_mxfp4(x)
+        if done is not None:
+            return done
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(quantize_rows_mxfp4, x, stream, out, scales)
+    kind, shape = _FLOATS.get(x.dtype), x.shape
+    if kind is None:
+        _refuse("x.dtype: " + _FLOAT_NAMES, x.dtype)
+    if not shape or shape[-1] < 1:
+        _refuse("x_tensor.size(-1) > 0")
+    rows = _rows_of(x)
+    m, k = rows.shape
+    want = shape[:-1] + (_row_bytes(k),)
+    if out is None:
+        out = torch.empty(want, dtype=_mxfp4, device=x.device)
+    elif (out.dtype is not _mxfp4 and out.dtype is not _uint8) or out.shape != want or out.get_device() != device or out.stride(-1) != 1:
+        _refuse("out: float4_e2m1fn_x2 %s on x's device, bytes of a row next to each other", list(want))
+    if scales is None:
+        scales = torch.empty(_scale_shape(m, k), dtype=_e8m0, device=x.device)
+    else:
+        _check_scales(scales, m, k, device, "scales")
+    if m:
+        q = _rows_to(out)
+        status = _lib.load().tsb_quantize_rows_mxfp4(rows.data_ptr(), kind, rows.stride(0), q.data_ptr(), q.stride(0), scales.data_ptr(), m, k, _current_raw_stream(device))
+        if status:
+            check(status)
+    return out, scales
+
+
+def dequantize_rows_mxfp4(q, scales, k=None, dtype=torch.float32, out=None, stream=None):
+    """The values [..., k] that 4-bit rows q [..., 16 * ceil(k / 32)] with these scales stand for, rounded once to ``dtype`` (``out`` takes
+    them where it is given, and says their type).  k: twice q's last size unless given."""
+    device = q.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(dequantize_rows_mxfp4, q, stream, scales, k, dtype, out)
+    _check_mxfp4(q, device, "q")
+    shape = q.shape
+    k = 2 * shape[-1] if k is None else operator.index(k)
+    if k < 1 or _row_bytes(k) != shape[-1]:
+        _refuse("k: a row of %d bytes holds %d to %d values", shape[-1], 2 * shape[-1] - 31, 2 * shape[-1])
+    rows = _rows_of(q)
+    m = rows.shape[0]
+    _check_scales(scales, m, k, device, "scales")
+    dtype = dtype if out is None else out.dtype
+    kind, want = _FLOATS.get(dtype), shape[:-1] + (k,)
+    if kind is None:
+        _refuse("dtype: " + _FLOAT_NAMES, dtype)
+    if out is None:
+        out = torch.empty(want, dtype=dtype, device=q.device)
+    elif out.shape != want or out.get_device() != device or (out.stride(-1) != 1 and k > 1):
+        _refuse("out: %s on q's device, values of a row next to each other", list(want))
+    if m:
+        y = _rows_to(out)
+        status = _lib.load().tsb_dequantize_rows_mxfp4(rows.data_ptr(), rows.stride(0), scales.data_ptr(), y.data_ptr(), kind, y.stride(0), m, k, _current_raw_stream(device))
+        if status:
+            check(status)
+    return out
+
+
+def inner_prod_mxfp4(x, x_scales, w, w_scales, bias=None, residual=None, activation=ACT_NONE, leaky=0.0, out_dtype=None, out=None,
+                     residual_after_activation=False, kernel=KERNEL_AUTO, stream=None):
+    """x [..., k] times w [n, k] transposed, both in 4 bits with a power of two for every 32 values of a row, sums in fp32:
+    ``activation(sum + bias + residual)`` (or ``activation(...) + residual``), [..., n].
+
+    w and w_scales are what quantize_rows_mxfp4 makes of a float weight tensor; x and x_scales what it (or rms_norm) makes of activations, or x is
+    floating with ``x_scales=None``: then its rows are quantized in the call.  ``residual`` has the output's type and shape.  ``out_dtype`` is
+    x's type (of 4-bit rows: float32) unless given; ``out`` takes the result where it is given (it may be ``residual``, and no other operand)."""
+    if out is None and stream is None and kernel == KERNEL_AUTO:
+        done = (_native or _ordinary()).inner_prod_mxfp4(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, bool(residual_after_activation))
+        if done is not None:
+            return done
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(inner_prod_mxfp4, x, stream, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, out, residual_after_activation, kernel)
+    x_dtype, shape = x.dtype, x.shape
+    _check_mxfp4(w, device, "w")
+    if w.dim() != 2:
+        _refuse("w: a matrix")
+    n, k = w.shape[0], 2 * w.shape[1]
+    if x_scales is None:
+        if x_dtype not in _FLOATS:
+            _refuse("x.dtype: 4 bits with x_scales, without " + _FLOAT_NAMES, x_dtype)
+        if not shape or shape[-1] < 1 or _row_bytes(shape[-1]) != w.shape[1]:
+            _refuse("w_tensor.size(1) == 16 * ceil(x_tensor.size(-1) / 32)")
+        k = shape[-1]
+    else:
+        _check_mxfp4(x, device, "x")
+        if shape[-1] != w.shape[1]:
+            _refuse("w_tensor.size(1) == x_tensor.size(-1)")
+    rows, w = _rows_of(x), _rows_of(w)
+    m = rows.shape[0]
+    _check_scales(w_scales, n, k, device, "w_scales")
+    scales_at = bias_at = 0
+    if x_scales is not None:
+        _check_scales(x_scales, m, k, device, "x_scales")
+        scales_at = x_scales.data_ptr()
+    if bias is not None:
+        _check_vector(bias, n, device, "bias")
+        bias_at = bias.data_ptr()
+    dtype = out_dtype if out_dtype is not None else out.dtype if out is not None else x_dtype if x_scales is None else _float32
+    kind = _FLOATS.get(dtype)
+    if kind is None:
+        _refuse("out_dtype: " + _FLOAT_NAMES, dtype)
+    want = shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(want, dtype=dtype, device=x.device)
+    elif out.dtype is not dtype or out.shape != want or out.get_device() != device or (out.stride(-1) != 1 and n > 1):
+        _refuse("out: of out_dtype, [..., n] on x's device, values of a row next to each other")
+    residual_at = residual_step = 0
+    if residual is not None:
+        if residual.dtype is not dtype or residual.shape != want or residual.get_device() != device:
+            _refuse("residual: of the output's type and shape on x's device")
+    if not (m and n):
+        return out
+    y = _rows_to(out)
+    if residual is not None:
+        residual = _rows_of(residual)
+        residual_at, residual_step = residual.data_ptr(), residual.stride(0)
+    lib = _lib.load()
+    args = _lib.INNER_PROD_MXFP4_ARGS.pack(m, n, k, rows.data_ptr(), rows.stride(0), scales_at, w.data_ptr(), w.stride(0), w_scales.data_ptr(), bias_at, residual_at,
+                                           residual_step, y.data_ptr(), y.stride(0), _TYPE.get(x_dtype, _lib.TYPE_MXFP4), kind, activation, leaky,
+                                           1 if residual_after_activation else 0, kernel)
+    workspace = size = 0
+    if x_scales is None:
+        size = lib.tsb_inner_prod_mxfp4_workspace_bytes(args)
+        if size:
+            room = torch.empty((size,), dtype=_uint8, device=x.device)
+            workspace = room.data_ptr()
+    status = lib.tsb_inner_prod_mxfp4(args, workspace, size, _current_raw_stream(device))
+    if status:
+        check(status)
+    return out
+
+
+def rms_norm(x, gamma=None, residual=None, eps=1e-6, out_dtype=None, out=None, scales=None, sum_out=None, stream=None):
+    """Root-mean-square norm of the rows of x [..., k] (fp32, fp16 or bf16): ``h / sqrt(mean(h * h) + eps) * gamma`` with h = x + residual (x's
+    type) where a residual of x's type and shape is given, else x.
+
+    The result has x's type and shape; with ``out_dtype=torch.int8`` it is (q, scales) as quantize_rows gives them, what inner_prod_quantized reads,
+    with ``out_dtype=torch.float4_e2m1fn_x2`` (q, scales) as quantize_rows_mxfp4 gives them, what inner_prod_mxfp4 reads.  With a residual h comes
+    as one result more: y, h or q, scales, h.  ``out``, ``scales`` and ``sum_out`` (h; it may be ``residual`` or x) take the results where they are given."""
+    if out is None and scales is None and sum_out is None and stream is None:
+        done = (_native or _ordinary()).rms_norm(x, gamma, residual, eps, out_dtype)
+        if done is not None:
+            return done
+    device = x.get_device()
+    if device < 0 or stream is not None or device != _current_device():
+        return _elsewhere(rms_norm, x, stream, gamma, residual, eps, out_dtype, out, scales, sum_out)
+    kind, shape = _FLOATS.get(x.dtype), x.shape
+    if kind is None:
+        _refuse("x.dtype: " + _FLOAT_NAMES, x.dtype)
+    if not shape or shape[-1] < 1:
+        _refuse("x_tensor.size(-1) > 0")
+    dtype = out_dtype if out_dtype is not None else x.dtype if out is None else out.dtype
+    packed = dtype is _mxfp4 or (dtype is _uint8 and out is not None and out_dtype is None)
+    if dtype is not x.dtype and dtype is not _int8 and not packed:
+        _refuse("out_dtype: x's type, int8 or float4_e2m1fn_x2, not %s", dtype)
+    if residual is not None and (residual.dtype is not x.dtype or residual.shape != shape or residual.get_device() != device):
+        _refuse("residual: of x's type and shape on x's device")
+    rows = _rows_of(x)
+    m, k = rows.shape
+    gamma_at = residual_at = residual_step = sum_at = sum_step = scales_at = 0
+    if gamma is not None:
+        _check_vector(gamma, k, device, "gamma")
+        gamma_at = gamma.data_ptr()
+    want = shape[:-1] + (_row_bytes(k),) if packed else shape
+    if out is not None:
+        if (out.dtype is not dtype and not (packed and out.dtype is _uint8)) or out.shape != want or out.get_device() != device or (out.stride(-1) != 1 and want[-1] > 1):
+            _refuse("out: %s of out_dtype on x's device, values of a row next to each other", list(want))
+    elif dtype is _int8:
+        # rows start a multiple of 16 bytes apart, as quantize_rows has them
+        out = torch.empty(shape[:-1] + ((k + 15) // 16 * 16,), dtype=_int8, device=x.device)[..., :k]
+    else:
+        out = torch.empty(want, dtype=dtype, device=x.device)
+    if dtype is x.dtype:
+        if scales is not None:
+            _refuse("scales come with out_dtype int8 or float4_e2m1fn_x2")
+    elif scales is not None:
+        if packed:
+            _check_scales(scales, m, k, device, "scales")
+        else:
+            _check_vector(scales, m, device, "scales")
+    else:
+        scales = torch.empty(_scale_shape(m, k), dtype=_e8m0, device=x.device) if packed else torch.empty(shape[:-1], dtype=_float32, device=x.device)
+    if residual is None:
+        if sum_out is not None:
+            _refuse("sum_out comes with a residual")
+    elif sum_out is None:
+        sum_out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif sum_out.dtype is not x.dtype or sum_out.shape != shape or sum_out.get_device() != device or (sum_out.stride(-1) != 1 and k > 1):
+        _refuse("sum_out: of x's type and shape on x's device, values of a row next to each other")
+    if m:
+        y = _rows_to(out)
+        if residual is not None:
+            residual = _rows_of(residual)
+            residual_at, residual_step = residual.data_ptr(), residual.stride(0)
+            h = _rows_to(sum_out)
+            sum_at, sum_step = h.data_ptr(), h.stride(0)
+        if scales is not None:
+            scales_at = scales.data_ptr()
+        desc = _lib.RMS_NORM_DESC.pack(m, k, rows.data_ptr(), rows.stride(0), residual_at, residual_step, sum_at, sum_step, gamma_at, y.data_ptr(), y.stride(0), scales_at, eps,
+                                       kind, _lib.TYPE_MXFP4 if packed else _TYPE[dtype])
+        status = _lib.load().tsb_rms_norm(desc, _current_raw_stream(device))
+        if status:
+            check(status)
+    done = (out,) + ((scales,) if scales is not None else ()) + ((sum_out,) if residual is not None else ())
+    return done if len(done) > 1 else out
