@@ -504,9 +504,12 @@ typedef struct tsb_inner_prod_mxfp4_args {
     int kernel;                      /* TSB_KERNEL_AUTO; another one is tests' (TSB_ERR_UNSUPPORTED where it cannot) */
 } tsb_inner_prod_mxfp4_args;
 
-/* Scratch of a call with floating rows, as for tsb_inner_prod_i8. */
+/* Scratch of a call with floating rows and failure detection, as for tsb_inner_prod_i8; the status word is one of its own, with a
+ * code (1..5, which wait) in it. */
 TSB_API size_t tsb_inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *args);
 TSB_API int tsb_inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *args, void *workspace, size_t workspace_bytes, void *stream);
+TSB_API int tsb_inner_prod_mxfp4_status(void *stream);
+TSB_API int tsb_inner_prod_mxfp4_status_decode(int status_word);
 
 /*
  * Root-mean-square norm of rows, with the addition of a residual in front of it and rows quantized for a product behind it.

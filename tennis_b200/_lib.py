@@ -112,6 +112,8 @@ SYMBOLS = {
     "tsb_dequantize_rows_mxfp4": (_i, [_vp, _i64, _vp, _vp, _i, _i64, _i64, _i64, _vp]),
     "tsb_inner_prod_mxfp4_workspace_bytes": (_sz, [ctypes.c_char_p]),
     "tsb_inner_prod_mxfp4": (_i, [ctypes.c_char_p, _vp, _sz, _vp]),
+    "tsb_inner_prod_mxfp4_status": (_i, [_vp]),
+    "tsb_inner_prod_mxfp4_status_decode": (_i, [_i]),
     "tsb_rms_norm": (_i, [ctypes.c_char_p, _vp]),
     "tsb_kernel_launch_count": (_i64, []),
 }

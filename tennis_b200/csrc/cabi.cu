@@ -48,6 +48,10 @@ int64_t mxfp4_row_bytes(int64_t);
 int64_t mxfp4_scale_bytes(int64_t, int64_t);
 size_t inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *);
 int inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *, void *, size_t, cudaStream_t);
+namespace tc {
+int inner_prod_mxfp4_status(cudaStream_t);
+int inner_prod_mxfp4_status_decode(int);
+}
 int rms_norm(const tsb_rms_norm_desc *, cudaStream_t);
 
 namespace {
@@ -178,6 +182,8 @@ size_t tsb_inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *arg
 int tsb_inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *args, void *workspace, size_t workspace_bytes, void *stream) {
     return inner_prod_mxfp4(args, workspace, workspace_bytes, (cudaStream_t)stream);
 }
+int tsb_inner_prod_mxfp4_status(void *stream) { return tc::inner_prod_mxfp4_status((cudaStream_t)stream); }
+int tsb_inner_prod_mxfp4_status_decode(int status_word) { return tc::inner_prod_mxfp4_status_decode(status_word); }
 int tsb_rms_norm(const tsb_rms_norm_desc *desc, void *stream) { return rms_norm(desc, (cudaStream_t)stream); }
 
 int tsb_pool_out_dim(int x, int pad_lo, int pad_hi, int k, int stride) {

@@ -120,7 +120,10 @@ size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 int run(const InnerProdMxfp4Params &p, int y_type, int kernel, int early, cudaStream_t stream) {
     (void)early;
-    if (kernel == TSB_KERNEL_TCGEN05) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_mxfp4: no tensor-core kernel");
+    const char *why = "";
+    const bool tc_can = tc::inner_prod_can(p, &why);
+    if (kernel == TSB_KERNEL_TCGEN05 && !tc_can) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_mxfp4: no tensor-core kernel: %s", why);
+    if (kernel != TSB_KERNEL_DIRECT && tc_can) return tc::inner_prod(p, y_type, stream);
     switch (y_type) {
         case TSB_TYPE_F32: return launch_direct<float>(p, stream);
         case TSB_TYPE_F16: return launch_direct<__half>(p, stream);

@@ -41,4 +41,12 @@ __device__ __forceinline__ void finish_values(const InnerProdMxfp4Params &p, con
 }
 #endif
 
+// inner_prod_mxfp4_tc.cu: the tensor-core kernel
+namespace tc {
+bool inner_prod_can(const InnerProdMxfp4Params &p, const char **why);     // whether it takes these operands, and if not, why
+int inner_prod(const InnerProdMxfp4Params &p, int y_type, cudaStream_t stream);
+int inner_prod_mxfp4_status(cudaStream_t stream);
+int inner_prod_mxfp4_status_decode(int word);
+}  // namespace tc
+
 }  // namespace tsb

@@ -22,32 +22,17 @@
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and
 // all roles go to the common exit.
 #include "inner_prod_i8.h"
-#include "tc_ptx.cuh"
-
-#include <cudaTypedefs.h>
-
-#include <algorithm>
+#include "inner_prod_tiles.cuh"
 
 namespace tsb {
 namespace tc {
 namespace {
 
-constexpr int kKBytes = 128;                 // bytes of K a stage
-constexpr int kGroupM = 16;                  // token tiles that neighbouring CTAs share
-constexpr uint32_t kABytes = kBM * kKBytes;
-constexpr int kCh = 32;                      // channels of a step of the epilogue
-constexpr uint32_t kOutRows = 2048;          // bytes of a step of a warp's
-constexpr uint32_t kSmem = 227 * 1024;
-constexpr int kMaxStages = 8;
-
 // code of the wait that ran out: 1 stage free, 2 stage full, 3 sums free, 4 sums complete
 __device__ int g_status;
 
-struct TcParams {
+struct TcParams : Walk {
     InnerProdParams p;
-    int tiles_m, tiles_n, kblocks;
-    int group_m;                  // token tiles that neighbouring CTAs share: a power of two
-    uint32_t per_group, inverse;  // tiles of such a group, 2^32 / that
 };
 
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory
@@ -66,28 +51,6 @@ struct Layout {
     static constexpr int kStages = (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) < kMaxStages
                                        ? (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) : kMaxStages;
     static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kParts + kBars;
-};
-
-__device__ __forceinline__ void tile_of(const TcParams &t, int i, int &m_tile, int &n_tile) {
-    // (every warp of the epilogue does this for every tile: no division but in the last group)
-    int g = (int)__umulhi((uint32_t)i, t.inverse), r = i - g * (int)t.per_group;      // the quotient or one less
-    if (r >= (int)t.per_group) {
-        ++g;
-        r -= (int)t.per_group;
-    }
-    const int rows = t.tiles_m - g * t.group_m;
-    n_tile = rows >= t.group_m ? r >> (31 - __clz(t.group_m)) : r / rows;
-    m_tile = g * t.group_m + r - n_tile * min(rows, t.group_m);
-}
-
-// A warp's staged outputs, rows of kCh channels: in the order of a tensor map's 64- or 128-byte swizzle, so that the fragments' writes (eight
-// rows at a time, a 16-byte unit each or half a unit to a lane) and the rows' reads meet a bank once or twice.
-template <typename T>
-struct Staged {
-    static constexpr int kRowBytes = kCh * sizeof(T), kUnits = kRowBytes / 16;
-    static constexpr int kRows = 2048 / kRowBytes;            // tokens of a step: 32 of 2-byte values, 16 of 4-byte ones
-    static __device__ __forceinline__ uint32_t unit(int r, int u) { return (uint32_t)(r * kRowBytes + ((u ^ (kUnits == 4 ? (r >> 1) & 3 : r & 7)) << 4)); }
-    static __device__ __forceinline__ uint32_t value(int r, int c) { return unit(r, c * (int)sizeof(T) / 16) + c * (uint32_t)sizeof(T) % 16; }
 };
 
 // A lane's channels of a tile: 8 j + 2 (lane % 4) and the next one, for every j; zeros for channels that do not exist.
@@ -112,57 +75,6 @@ struct Channels {
         }
     }
 };
-
-// The residual of such a step into `rows`, once the copy that reads these rows last has done so.
-template <typename T>
-__device__ __forceinline__ void fetch_residual(const InnerProdParams &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
-    using S = Staged<T>;
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) bulk_wait_read();
-    __syncwarp();
-    if (res_vec && c0 + kCh <= p.n) {
-        constexpr int kN = Vec16<T>::kN, kStep = 32 / S::kUnits;
-        const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
-        const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
-        const int64_t step = kStep * p.residual_pitch;
-#pragma unroll
-        for (int r = 0; r < S::kRows; r += kStep, from += step)
-            if (r + r0 < live) *reinterpret_cast<uint4 *>(rows + S::unit(r + r0, u0)) = *reinterpret_cast<const uint4 *>(from);
-    } else {
-        // value by value, neighbouring lanes neighbouring channels
-        const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
-        T some[8];
-        for (int r = 0; r < live; r += 8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i, from += p.residual_pitch)
-                if (r + i < live && c0 + lane < p.n) some[i] = *from;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (r + i < live && c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, lane)) = some[i];
-        }
-    }
-    __syncwarp();
-}
-
-// The same without waiting for it: whole pieces alone (whole_residual), by asynchronous copies, a group of them in any case.
-__device__ __forceinline__ bool whole_residual(const InnerProdParams &p, int c0, bool res_vec) { return res_vec && c0 + kCh <= p.n; }
-template <typename T>
-__device__ __forceinline__ void start_residual(const InnerProdParams &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
-    using S = Staged<T>;
-    const int lane = threadIdx.x & 31;
-    if (lane == 0) bulk_wait_read();
-    __syncwarp();
-    if (live > 0 && whole_residual(p, c0, res_vec)) {
-        constexpr int kStep = 32 / S::kUnits;
-        const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
-        const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * Vec16<T>::kN;
-        const int64_t step = kStep * p.residual_pitch;
-#pragma unroll
-        for (int r = 0; r < S::kRows; r += kStep, from += step)
-            if (r + r0 < live) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(rows + S::unit(r + r0, u0))), "l"(from) : "memory");
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-}
 
 // kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; xs: the scales of tokens m0 + lane / 4 and every eighth behind it; to: where in a staged row of eight
@@ -504,44 +416,6 @@ done:
     }
 }
 
-// cuTensorMapEncodeTiled, looked up once
-PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
-    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        cudaDriverEntryPointQueryResult q;
-        void *f = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) f = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
-    }();
-    return fn;
-}
-
-// Tiles of `box_rows` rows x 128 bytes of an int8 matrix
-int encode(CUtensorMap *map, const int8_t *at, int64_t rows, int cols, int64_t pitch, int box_rows) {
-    const auto fn = encode_tiled();
-    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
-    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? pitch : (cols + 15) / 16 * 16)};
-    cuuint32_t box[2] = {(cuuint32_t)kKBytes, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(at), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: cuTensorMapEncodeTiled failed with %d", (int)r);
-    return TSB_OK;
-}
-
-// The boxes that a warp writes
-template <typename T>
-int encode_output(CUtensorMap *map, const InnerProdParams &p) {
-    const auto fn = encode_tiled();
-    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
-    cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m};
-    cuuint64_t strides[1] = {(cuuint64_t)(p.m > 1 ? p.y_pitch * (int64_t)sizeof(T) : ((int64_t)p.n * (int64_t)sizeof(T) + 15) / 16 * 16)};
-    cuuint32_t box[2] = {kCh, Staged<T>::kRows}, estr[2] = {1, 1};
-    const CUresult r = fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_i8: cuTensorMapEncodeTiled(y) failed with %d", (int)r);
-    return TSB_OK;
-}
-
 template <typename T, int BN, bool RES, bool PAIR = false, int SPLIT = 1>
 int launch(const InnerProdParams &p, cudaStream_t stream) {
     using L = Layout<T, BN, RES, PAIR, SPLIT>;
@@ -560,11 +434,7 @@ int launch(const InnerProdParams &p, cudaStream_t stream) {
         raised.done();
     }
     constexpr int kCluster = PAIR ? 2 : SPLIT;
-    TcParams t = {p, (int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes)};
-    // (of few output channels, tiles of the same tokens follow each other: then a CTA of an even grid stays with its channels)
-    t.group_m = t.tiles_n <= 4 ? 1 : kGroupM;
-    t.per_group = (uint32_t)(t.group_m * t.tiles_n);
-    t.inverse = (uint32_t)std::min<uint64_t>(UINT32_MAX, ((uint64_t)1 << 32) / t.per_group);
+    const TcParams t = {walk_of((int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(p.k, kKBytes)), p};
     const int grid = kCluster * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, SPLIT > 1 ? INT32_MAX : 148 / kCluster);      // (split: a tile a cluster)
     TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, my, t, (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_i8_tc_kernel");

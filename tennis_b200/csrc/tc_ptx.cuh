@@ -179,6 +179,19 @@ __device__ __forceinline__ void mma_i8_if(uint32_t d_tmem, uint64_t adesc, uint6
         "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on));
 }
+// 4-bit operands with a scale for every 32 values of K: the scales lie in tensor memory, a row's four of 128 values of K in a column's 32 bits, 32 rows down the
+// lanes and 128 in four columns; the instruction descriptor says which two of the four an MMA (64 values of K) takes.
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// 512 bytes of scales, 32 rows of 16 bytes, to four columns of tensor memory, for each of its four groups of lanes
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
 // ---- two CTAs of a cluster on one tile: the even one's issuing warp multiplies for both
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -208,6 +221,17 @@ __device__ __forceinline__ void pair_mma_i8(uint32_t d_tmem, uint64_t adesc, uin
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pair_mma_mxf4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// each CTA's from its own shared memory to its own tensor memory
+__device__ __forceinline__ void pair_copy_scales(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, int (&v)[32]) {
     asm volatile(
@@ -285,6 +309,13 @@ __device__ __forceinline__ uint64_t smem_desc_sliding(uint32_t saddr) {
 template <int BN>
 __device__ __forceinline__ constexpr uint32_t instr_desc() {
     return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+}
+
+// Instruction descriptor of 4-bit operands with scales of powers of two for 32 values (kind::mxf4): A and B e2m1, both K-major, M rows (of both CTAs of a pair
+// together), N = BN; pair: which two of a column's four scales are taken, 0 or 1.
+template <int BN>
+__device__ __forceinline__ constexpr uint32_t instr_desc_mxf4(int m, int pair) {
+    return (uint32_t)(2 * pair) << 4 | 1u << 7 | 1u << 10 | (uint32_t)(BN >> 3) << 17 | 1u << 23 | (uint32_t)(m >> 7) << 27 | (uint32_t)(2 * pair) << 29;
 }
 
 }  // namespace tc

@@ -989,6 +989,12 @@ def inner_prod_mxfp4(x, x_scales, w, w_scales, bias=None, residual=None, activat
     return out
 
 
+def inner_prod_mxfp4_status(device=None, stream=None):
+    """inner_prod_status for inner_prod_mxfp4."""
+    with torch.cuda.device(device):
+        check(_lib.load().tsb_inner_prod_mxfp4_status(_stream_ptr(stream)))
+
+
 def rms_norm(x, gamma=None, residual=None, eps=1e-6, out_dtype=None, out=None, scales=None, sum_out=None, stream=None):
     """Root-mean-square norm of the rows of x [..., k] (fp32, fp16 or bf16): ``h / sqrt(mean(h * h) + eps) * gamma`` with h = x + residual (x's
     type) where a residual of x's type and shape is given, else x.

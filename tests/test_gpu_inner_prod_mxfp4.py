@@ -97,6 +97,7 @@ def test_large_products(m, n, k):
         assert torch.equal(call(d, out_dtype=out), want.to(out))
     r = torch.randn((m, n), device="cuda", dtype=torch.bfloat16)
     assert torch.equal(ops.inner_prod_mxfp4(d["x"], d["xs"], d["w"], d["ws"], d["bias"], r, out_dtype=torch.bfloat16), (want + r.float()).bfloat16())
+    ops.inner_prod_mxfp4_status()
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 500, 4096), (20, 300, 8192), (50, 260, 1500), (200, 300, 4096), (900, 1100, 8192)])

@@ -162,3 +162,18 @@ def test_plain_norm_and_product():
     assert np.allclose(v, [[1.2, 3.2, 0.0, 0.0]]) and torch.equal(h, x)
     y, _ = plain.inner_prod(np.array([[1.0, 2.0]]), np.array([[3.0, -4.0], [1.0, 1.0]]), bias=np.array([0.0, 1.0]), act=1)
     assert y.tolist() == [[0.0, 4.0]]
+
+
+def test_every_wait_code_has_a_name_of_its_own(lib):
+    from tennis_b200 import _lib
+    kernel = open(ROOT + "/tennis_b200/csrc/inner_prod_mxfp4_tc.cu").read()
+    codes = sorted({int(c) for c in re.findall(r"give_up\((\d+)\)", kernel)})
+    assert codes == list(range(1, len(codes) + 1))
+    names = set()
+    for code in codes:
+        assert lib.tsb_inner_prod_mxfp4_status_decode(code) == _lib.ERR_DEVICE_TIMEOUT
+        names.add(re.search(r"the wait for (.*) ran out;", lib.tsb_last_error().decode()).group(1))
+    assert len(names) == len(codes) and "an unknown event" not in names
+    assert lib.tsb_inner_prod_mxfp4_status_decode(codes[-1] + 1) == _lib.ERR_DEVICE_TIMEOUT and "an unknown event" in lib.tsb_last_error().decode()
+    assert lib.tsb_inner_prod_mxfp4_status_decode(0) == 0
+    assert "code (1..%d, which wait) in it" % codes[-1] in open(ROOT + "/include/tennis_b200.h").read()
