@@ -505,7 +505,7 @@ typedef struct tsb_inner_prod_mxfp4_args {
 } tsb_inner_prod_mxfp4_args;
 
 /* Scratch of a call with floating rows and failure detection, as for tsb_inner_prod_i8; the status word is one of its own, with a
- * code (1..5, which wait) in it. */
+ * code (1..6, which wait) in it. */
 TSB_API size_t tsb_inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *args);
 TSB_API int tsb_inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *args, void *workspace, size_t workspace_bytes, void *stream);
 TSB_API int tsb_inner_prod_mxfp4_status(void *stream);

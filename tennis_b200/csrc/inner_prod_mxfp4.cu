@@ -119,10 +119,10 @@ int check_args(const tsb_inner_prod_mxfp4_args *a) {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 int run(const InnerProdMxfp4Params &p, int y_type, int kernel, int early, cudaStream_t stream) {
-    (void)early;
     const char *why = "";
     const bool tc_can = tc::inner_prod_can(p, &why);
     if (kernel == TSB_KERNEL_TCGEN05 && !tc_can) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_mxfp4: no tensor-core kernel: %s", why);
+    if (kernel == TSB_KERNEL_AUTO && tc_can && p.m <= few::kMaxMxfp4Tokens) return few::inner_prod(p, y_type, early, stream);
     if (kernel != TSB_KERNEL_DIRECT && tc_can) return tc::inner_prod(p, y_type, stream);
     switch (y_type) {
         case TSB_TYPE_F32: return launch_direct<float>(p, stream);
@@ -153,9 +153,14 @@ InnerProdMxfp4Params params_of(const tsb_inner_prod_mxfp4_args *a) {
     return p;
 }
 
+// Whether floating rows are quantized by the kernel that multiplies them.
+bool quantizes_inside(const tsb_inner_prod_mxfp4_args *a, const InnerProdMxfp4Params &p) {
+    return a->kernel == TSB_KERNEL_AUTO && tc::weights_fit(p) && few::can_quantize(p, a->x_type, a->y_type);
+}
+
 // Workspace of floating rows: the rows in 4 bits, then their scales.
-size_t workspace_of(const tsb_inner_prod_mxfp4_args *a) {
-    if (a->x_type == TSB_TYPE_MXFP4) return 0;
+size_t workspace_of(const tsb_inner_prod_mxfp4_args *a, const InnerProdMxfp4Params &p) {
+    if (a->x_type == TSB_TYPE_MXFP4 || quantizes_inside(a, p)) return 0;
     return align256((size_t)(a->m * mx::row_bytes(a->k))) + align256((size_t)mx::scale_bytes(a->m, a->k));
 }
 
@@ -164,7 +169,7 @@ size_t workspace_of(const tsb_inner_prod_mxfp4_args *a) {
 int quantize_rows_mxfp4(const void *, int, int64_t, void *, int64_t, void *, int64_t, int64_t, cudaStream_t);
 
 size_t inner_prod_mxfp4_workspace_bytes(const tsb_inner_prod_mxfp4_args *a) {
-    return check_args(a) != TSB_OK || a->m == 0 || a->n == 0 ? 0 : workspace_of(a);
+    return check_args(a) != TSB_OK || a->m == 0 || a->n == 0 ? 0 : workspace_of(a, params_of(a));
 }
 
 int inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *a, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
@@ -172,7 +177,8 @@ int inner_prod_mxfp4(const tsb_inner_prod_mxfp4_args *a, void *workspace, size_t
     if (st != TSB_OK || a->m == 0 || a->n == 0) return st;
     InnerProdMxfp4Params p = params_of(a);
     if (a->x_type == TSB_TYPE_MXFP4) return run(p, a->y_type, a->kernel, 0, stream);
-    const size_t need = workspace_of(a);
+    if (quantizes_inside(a, p)) return few::inner_prod_quantize(p, a->y_type, p.x_pitch, (int)a->k, stream);
+    const size_t need = workspace_of(a, p);
     if (!workspace || workspace_bytes < need)
         return fail(TSB_ERR_WORKSPACE_TOO_SMALL, "inner_prod_mxfp4: %zu bytes of workspace, %zu needed", workspace ? workspace_bytes : (size_t)0, need);
     if (reinterpret_cast<uintptr_t>(workspace) % 256) return fail(TSB_ERR_INVALID_ARGUMENT, "inner_prod_mxfp4: the workspace must be 256-byte aligned");

@@ -44,9 +44,19 @@ __device__ __forceinline__ void finish_values(const InnerProdMxfp4Params &p, con
 // inner_prod_mxfp4_tc.cu: the tensor-core kernel
 namespace tc {
 bool inner_prod_can(const InnerProdMxfp4Params &p, const char **why);     // whether it takes these operands, and if not, why
+bool weights_fit(const InnerProdMxfp4Params &p);                           // the part of that that concerns w
 int inner_prod(const InnerProdMxfp4Params &p, int y_type, cudaStream_t stream);
+int mxfp4_status_word(int **at);                                          // of the current device, for the kernels of few tokens too
 int inner_prod_mxfp4_status(cudaStream_t stream);
 int inner_prod_mxfp4_status_decode(int word);
 }  // namespace tc
+
+// inner_prod_mxfp4_few.cu: the kernel of few tokens
+namespace few {
+constexpr int kMaxMxfp4Tokens = 64;
+int inner_prod(const InnerProdMxfp4Params &p, int y_type, int early, cudaStream_t stream);       // early: weights may be read before the kernel in front is done
+bool can_quantize(const InnerProdMxfp4Params &p, int x_type, int y_type);                        // whether the next one takes these floating rows
+int inner_prod_quantize(const InnerProdMxfp4Params &p, int y_type, int64_t x_pitch, int cols, cudaStream_t stream);
+}  // namespace few
 
 }  // namespace tsb

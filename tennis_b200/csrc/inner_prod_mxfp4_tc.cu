@@ -22,14 +22,12 @@ namespace {
 
 using Params = InnerProdMxfp4Params;
 
-// code of the wait that ran out: 1 stage free, 2 stage full, 3 sums free, 4 sums complete, 5 shared columns free
+// code of the wait that ran out: 1 stage free, 2 stage full, 3 sums free, 4 sums complete, 5 shared columns free, 6 (few tokens) tokens quantized
 __device__ int g_mxfp4_status;
 
 struct Mxfp4Params : Walk {
     Params p;
 };
-
-constexpr uint32_t kScales = 1024;           // bytes of a stage's scales of 128 rows
 
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory, and all channels' scales
 template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
@@ -444,18 +442,6 @@ done:
     }
 }
 
-// The scales of a matrix as words of four: `tiles` runs of 128 a row of 128 rows' tiles; a box holds two runs of `box_rows` such rows
-int encode_scales(CUtensorMap *map, const uint8_t *at, int64_t rows, int64_t tiles, int box_rows) {
-    const auto fn = encode_tiled();
-    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
-    cuuint64_t dims[2] = {(cuuint64_t)tiles * 128, (cuuint64_t)ceil_div64(rows, mx::kTileRows)}, strides[1] = {(cuuint64_t)tiles * mx::kTileBytes};
-    cuuint32_t box[2] = {256, (cuuint32_t)box_rows}, estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<uint8_t *>(at), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_mxfp4: cuTensorMapEncodeTiled failed with %d", (int)r);
-    return TSB_OK;
-}
-
 template <typename T, int BN, bool RES, bool PAIR = false, int SPLIT = 1>
 int launch(const Params &p, cudaStream_t stream) {
     using L = Layout<T, BN, RES, PAIR, SPLIT>;
@@ -505,6 +491,21 @@ int pick(const Params &p, cudaStream_t stream) {
     return c64 <= c128 ? launch<T, 64, RES>(p, stream) : launch<T, 128, RES>(p, stream);
 }
 
+// The status word's address on the current device
+int status_word(int **at) {
+    static std::atomic<int *> known[64];
+    int device = 0;
+    TSB_CUDA(cudaGetDevice(&device));
+    std::atomic<int *> *slot = device >= 0 && device < 64 ? &known[device] : nullptr;
+    *at = slot ? slot->load(std::memory_order_acquire) : nullptr;
+    if (*at) return TSB_OK;
+    void *found = nullptr;
+    TSB_CUDA(cudaGetSymbolAddress(&found, g_mxfp4_status));
+    *at = static_cast<int *>(found);
+    if (slot) slot->store(*at, std::memory_order_release);
+    return TSB_OK;
+}
+
 bool operand_fits(const uint8_t *at, const uint8_t *scales, int64_t rows, int64_t pitch, int groups) {
     return (reinterpret_cast<uintptr_t>(at) | reinterpret_cast<uintptr_t>(scales)) % 16 == 0 &&
            (rows == 1 || (pitch % 16 == 0 && pitch >= (int64_t)groups * (mx::kGroup / 2) && pitch < (int64_t)1 << 40));
@@ -512,8 +513,10 @@ bool operand_fits(const uint8_t *at, const uint8_t *scales, int64_t rows, int64_
 
 }  // namespace
 
+bool weights_fit(const Params &p) { return operand_fits(p.w, p.w_scales, p.n, p.w_pitch, p.groups); }
+
 bool inner_prod_can(const Params &p, const char **why) {
-    if (!operand_fits(p.x, p.x_scales, p.m, p.x_pitch, p.groups) || !operand_fits(p.w, p.w_scales, p.n, p.w_pitch, p.groups)) {
+    if (!operand_fits(p.x, p.x_scales, p.m, p.x_pitch, p.groups) || !weights_fit(p)) {
         *why = "an operand's address or pitch is no multiple of 16 bytes, or its rows overlap";
         return false;
     }
@@ -529,19 +532,21 @@ int inner_prod(const Params &p, int y_type, cudaStream_t stream) {
     }
 }
 
+int mxfp4_status_word(int **at) { return status_word(at); }
+
 // What a status word stands for.
 int inner_prod_mxfp4_status_decode(int word) {
     if (word == 0) return TSB_OK;
-    static const char *const kWaits[] = {"a stage to be free", "a stage to be loaded", "sums to be read", "sums to be complete", "shared columns to be read"};
+    static const char *const kWaits[] = {"a stage to be free", "a stage to be loaded", "sums to be read", "sums to be complete", "shared columns to be read", "tokens to be quantized"};
     return fail(TSB_ERR_DEVICE_TIMEOUT, "inner_prod_mxfp4: the wait for %s ran out; results since the last check are not to be used",
-                word >= 1 && word <= 5 ? kWaits[word - 1] : "an unknown event");
+                word >= 1 && word <= 6 ? kWaits[word - 1] : "an unknown event");
 }
 
 // The device's status word: waits for the stream, reads and clears it.
 int inner_prod_mxfp4_status(cudaStream_t stream) {
-    int word = 0, zero = 0;
-    void *at = nullptr;
-    TSB_CUDA(cudaGetSymbolAddress(&at, g_mxfp4_status));
+    int word = 0, zero = 0, *at = nullptr;
+    const int st = mxfp4_status_word(&at);
+    if (st != TSB_OK) return st;
     TSB_CUDA(cudaMemcpyAsync(&word, at, sizeof(word), cudaMemcpyDeviceToHost, stream));
     TSB_CUDA(cudaStreamSynchronize(stream));
     if (word == 0) return TSB_OK;

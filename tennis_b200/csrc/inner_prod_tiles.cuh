@@ -20,6 +20,7 @@ constexpr int kCh = 32;                      // channels of a step of the epilog
 constexpr uint32_t kOutRows = 2048;          // bytes of a step of a warp's
 constexpr uint32_t kSmem = 227 * 1024;
 constexpr int kMaxStages = 8;
+constexpr uint32_t kScales = 1024;           // bytes of a stage's scales of 128 rows in 4 bits
 
 // Tiles in the order in which CTAs take them.
 struct Walk {
@@ -146,6 +147,18 @@ int encode_output(CUtensorMap *map, const P &p) {
     const CUresult r = fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner product: cuTensorMapEncodeTiled(y) failed with %d", (int)r);
+    return TSB_OK;
+}
+
+// The scales of a 4-bit matrix as words of four: `tiles` runs of 128 a row of 128 rows' tiles; a box holds two runs of `box_rows` such rows
+inline int encode_scales(CUtensorMap *map, const uint8_t *at, int64_t rows, int64_t tiles, int box_rows) {
+    const auto fn = encode_tiled();
+    if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
+    cuuint64_t dims[2] = {(cuuint64_t)tiles * 128, (cuuint64_t)ceil_div64(rows, 128)}, strides[1] = {(cuuint64_t)tiles * 512};
+    cuuint32_t box[2] = {256, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<uint8_t *>(at), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner product: cuTensorMapEncodeTiled failed with %d", (int)r);
     return TSB_OK;
 }
 

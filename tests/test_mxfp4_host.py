@@ -166,7 +166,7 @@ def test_plain_norm_and_product():
 
 def test_every_wait_code_has_a_name_of_its_own(lib):
     from tennis_b200 import _lib
-    kernel = open(ROOT + "/tennis_b200/csrc/inner_prod_mxfp4_tc.cu").read()
+    kernel = "".join(open(ROOT + "/tennis_b200/csrc/inner_prod_mxfp4_%s.cu" % name).read() for name in ("tc", "few"))
     codes = sorted({int(c) for c in re.findall(r"give_up\((\d+)\)", kernel)})
     assert codes == list(range(1, len(codes) + 1))
     names = set()
