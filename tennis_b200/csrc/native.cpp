@@ -1,4 +1,4 @@
-// The ordinary calls of ops.quantize_rows, inner_prod_quantized, group_norm_nhwc, quantize_rows_mxfp4, inner_prod_mxfp4 and rms_norm, from Python
+// The ordinary calls of ops.quantize_rows, inner_prod_quantized, group_norm_nhwc, (de)quantize_rows_mxfp4, inner_prod_mxfp4 and rms_norm, from Python
 // straight to the C ABI: tensors on the current device and stream, rows and images that lie one after the other, outputs that are allocated.  A kernel of these can be done in
 // 2 us, where the checks, the allocations and the call take some 8 us in Python and half of that here.
 //
@@ -268,6 +268,27 @@ PyObject *quantize_rows_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t coun
     END_HANDLE_TH_ERRORS
 }
 
+// dequantize_rows_mxfp4(q, scales, k, dtype) -> y
+PyObject *dequantize_rows_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    const Tensor *q = count == 4 ? tensor(args[0], -1) : nullptr;
+    int type;
+    int64_t rows, pitch;
+    const void *scales;
+    if (!q || !is_fp4(*q) || !rows_of(*q, &rows, &pitch) || !THPDtype_Check(args[3])) Py_RETURN_NONE;
+    const at::ScalarType out = reinterpret_cast<THPDtype *>(args[3])->scalar_type;
+    const int64_t k = args[2] == Py_None ? 2 * q->size(-1) : PyLong_AsLongLong(args[2]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (k < 1 || row_bytes(k) != q->size(-1) || !type_of(out, &type) || !scales_of(args[1], rows, k, q->get_device(), &scales)) Py_RETURN_NONE;
+    const Tensor y = dense(*q, k, out);
+    if (tsb_dequantize_rows_mxfp4(q->const_data_ptr(), pitch, scales, y.mutable_data_ptr(), type, k, rows, k, stream_of(q->get_device())) != TSB_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // inner_prod_mxfp4(x, x_scales, w, w_scales, bias, residual, activation, leaky, out_dtype, residual_after) -> y
 PyObject *inner_prod_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t count) {
     HANDLE_TH_ERRORS
@@ -388,6 +409,7 @@ PyMethodDef kMethods[] = {
     {"inner_prod", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(inner_prod)), METH_FASTCALL, nullptr},
     {"group_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(group_norm)), METH_FASTCALL, nullptr},
     {"quantize_rows_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(quantize_rows_mxfp4)), METH_FASTCALL, nullptr},
+    {"dequantize_rows_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(dequantize_rows_mxfp4)), METH_FASTCALL, nullptr},
     {"inner_prod_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(inner_prod_mxfp4)), METH_FASTCALL, nullptr},
     {"rms_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(rms_norm)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

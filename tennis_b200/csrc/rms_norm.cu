@@ -115,7 +115,13 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
     // (4 bits: whole tiles of scales, so that all lanes of a warp that has any of a row take part)
     const int vectors = (p.cols + kN - 1) / kN, turns = (vectors + step - 1) / step;
     const int64_t first = WARP ? (int64_t)blockIdx.x * warps + (threadIdx.x >> 5) : blockIdx.x, stride = WARP ? (int64_t)gridDim.x * warps : gridDim.x;
-    for (int64_t r = first; r < p.rows; r += stride) {
+    // (4 bits: the last 128 rows' scales have room for 128 rows, and what no row has is zero)
+    const int64_t room_rows = OUT == kMxfp4 ? (p.rows + mx::kTileRows - 1) / mx::kTileRows * mx::kTileRows : p.rows;
+    for (int64_t r = first; r < room_rows; r += stride) {
+        if (OUT == kMxfp4 && r >= p.rows) {
+            for (int t = at; t < p.tiles; t += step) mx::store_scales(static_cast<uint8_t *>(p.scales) + mx::word_at(r, t, p.tiles), 0, p.scales_aligned);
+            continue;
+        }
         const T *xr = static_cast<const T *>(p.x) + r * p.x_pitch;
         const T *rr = RES ? static_cast<const T *>(p.residual) + r * p.residual_pitch : nullptr;
         T *hr = RES && p.sum ? static_cast<T *>(p.sum) + r * p.sum_pitch : nullptr;
@@ -229,12 +235,7 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
                 uint32_t word;
                 const uint32_t codes = mx::quantize_lanes<kN>(v, &word);
                 if ((int64_t)u * kN < used) mx::store_codes<kN>(yr + u * (kN / 2), codes, p.y_aligned);
-                if (u % kLanes == 0 && u / kLanes < p.tiles) {
-                    mx::store_scales(scales + mx::word_at(r, u / kLanes, p.tiles), word, p.scales_aligned);
-                    // the places behind the last row
-                    if (r == p.rows - 1)
-                        for (int64_t e = r + 1; e % mx::kTileRows; ++e) mx::store_scales(scales + mx::word_at(e, u / kLanes, p.tiles), 0, p.scales_aligned);
-                }
+                if (u % kLanes == 0 && u / kLanes < p.tiles) mx::store_scales(scales + mx::word_at(r, u / kLanes, p.tiles), word, p.scales_aligned);
             });
         }
         if constexpr (!WARP) __syncthreads();      // (the next row's sums)
@@ -245,16 +246,17 @@ template <typename T, Out OUT, bool RES>
 int launch(const NormParams &p, cudaStream_t stream) {
     constexpr int kN = Vec16<T>::kN;
     const int vectors = ceil_div(p.cols, kN);
+    const int64_t rows = OUT == kMxfp4 ? ceil_div64(p.rows, mx::kTileRows) * mx::kTileRows : p.rows;
     auto go = [&](auto kernel, int64_t blocks, int threads) {
         TSB_CUDA(launch_pdl(kernel, dim3((int)std::min<int64_t>(blocks, 148 * 64)), dim3(threads), 0, stream, p));
         TSB_LAUNCHED("rms_norm_kernel");
         return TSB_OK;
     };
-    if (vectors <= 32) return go(rms_norm_kernel<T, OUT, RES, 1, true>, ceil_div64(p.rows, kWarpRowThreads / 32), kWarpRowThreads);
-    if (vectors <= 64) return go(rms_norm_kernel<T, OUT, RES, 2, true>, ceil_div64(p.rows, kWarpRowThreads / 32), kWarpRowThreads);
-    if (vectors <= kMost && p.rows <= 148 * 2) return go(rms_norm_kernel<T, OUT, RES, 1, false>, p.rows, round_up(vectors, 32));
-    if (vectors <= 4 * kMost) return go(rms_norm_kernel<T, OUT, RES, 4, false>, p.rows, round_up(ceil_div(vectors, 4), 32));
-    return go(rms_norm_kernel<T, OUT, RES, 0, false>, p.rows, kMost);
+    if (vectors <= 32) return go(rms_norm_kernel<T, OUT, RES, 1, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
+    if (vectors <= 64) return go(rms_norm_kernel<T, OUT, RES, 2, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
+    if (vectors <= kMost && p.rows <= 148 * 2) return go(rms_norm_kernel<T, OUT, RES, 1, false>, rows, round_up(vectors, 32));
+    if (vectors <= 4 * kMost) return go(rms_norm_kernel<T, OUT, RES, 4, false>, rows, round_up(ceil_div(vectors, 4), 32));
+    return go(rms_norm_kernel<T, OUT, RES, 0, false>, rows, kMost);
 }
 
 template <typename T, Out OUT>

@@ -887,6 +887,10 @@ def quantize_rows_mxfp4(x, out=None, scales=None, stream=None):
 def dequantize_rows_mxfp4(q, scales, k=None, dtype=torch.float32, out=None, stream=None):
     """The values [..., k] that 4-bit rows q [..., 16 * ceil(k / 32)] with these scales stand for, rounded once to ``dtype`` (``out`` takes
     them where it is given, and says their type).  k: twice q's last size unless given."""
+    if out is None and stream is None:
+        done = (_native or _ordinary()).dequantize_rows_mxfp4(q, scales, k, dtype)
+        if done is not None:
+            return done
     device = q.get_device()
     if device < 0 or stream is not None or device != _current_device():
         return _elsewhere(dequantize_rows_mxfp4, q, stream, scales, k, dtype, out)

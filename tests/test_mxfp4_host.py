@@ -125,6 +125,7 @@ def test_the_module_of_ordinary_calls():
     from tennis_b200 import ops
     native, x = ops._ordinary(), torch.zeros((2, 64))
     assert native.quantize_rows_mxfp4(x) is None and native.quantize_rows_mxfp4("x") is None and native.quantize_rows_mxfp4() is None
+    assert native.dequantize_rows_mxfp4(*[None] * 4) is None and native.dequantize_rows_mxfp4(x, x, None, torch.float32) is None and native.dequantize_rows_mxfp4(x) is None
     assert native.inner_prod_mxfp4(*[None] * 10) is None and native.inner_prod_mxfp4(x, None, x, x, None, None, 0, 0.0, None, False) is None
     assert native.rms_norm(*[None] * 5) is None and native.rms_norm(x, None, None, 1e-6, None) is None and native.rms_norm() is None
 
