@@ -75,10 +75,8 @@ __device__ __forceinline__ void quantize_tokens(const FewParams &t, int kb0, int
         for (int i = 0; i < kTurns; ++i) {
             if (first + i * kQuantizers * kAtOnce >= units) break;
             const uint32_t u = first + i * kQuantizers * kAtOnce + lane / kLanes, token = __umulhi(u, inverse), tile = u - token * tiles;
-            float v[kN];
-            Vec16<X>::get(held[i], v);
             uint32_t word;
-            const uint32_t codes = mx::quantize_lanes<kN>(v, &word);
+            const uint32_t codes = mx::quantize_vector<X>(held[i], &word);
             if (u < units) {
                 uint8_t *block = to + (tile >> 1) * S::kTokens;
                 const uint32_t b = (tile & 1) * 64 + in * (kN / 2);

@@ -58,26 +58,84 @@ __device__ __forceinline__ void values_of(uint32_t codes, float (&v)[N]) {
 }
 
 // A warp whose lanes hold neighbouring runs of kN values of a row (kN = 4 or 8, values that do not exist are zero) quantizes them: the lane's
-// codes, and the word of scales of its tile, the same in all lanes of the tile.  All lanes take part.
+// codes, and the word of scales of its tile, the same in all lanes of the tile.  most: the largest magnitude's bits of the lane's values.  All lanes take part.
 template <int kN>
-__device__ __forceinline__ uint32_t quantize_lanes(const float (&v)[kN], uint32_t *scales) {
+__device__ __forceinline__ uint32_t quantize_lanes(const float (&v)[kN], uint32_t most, uint32_t *scales) {
     constexpr int kLanes = kGroup / kN;          // of a group
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kN; ++i) most = max(most, magnitude(v[i]));
 #pragma unroll
     for (int d = 1; d < kLanes; d *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
     const uint32_t byte = scale_byte(most);
     const float by = inverse_scale(byte);
     float t[kN];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) t[i] = __fmul_rn(v[i], by);
+    for (int i = 0; i < kN; i += 2) {
+        const float2 r = mul2(make_float2(v[i], v[i + 1]), make_float2(by, by));
+        t[i] = r.x;
+        t[i + 1] = r.y;
+    }
     uint32_t word = byte << (8 * ((threadIdx.x & 31) / kLanes % kTileGroups));
     word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
     word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
     *scales = word;
     if constexpr (kN == 8) return codes8(t);
     else return codes4(t);
+}
+// The same of 16 bytes of a floating row, and of 32 neighbouring ones.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize_vector(const uint4 &q, uint32_t *scales) {
+    Largest<T> largest;
+    largest.add(q);
+    float v[Vec16<T>::kN];
+    Vec16<T>::get(q, v);
+    return quantize_lanes<Vec16<T>::kN>(v, largest.bits(), scales);
+}
+template <typename T>
+__device__ __forceinline__ void quantize_bytes(const uint4 (&q)[2], uint32_t (&codes)[4 / sizeof(T)], uint32_t *scales) {
+    constexpr int kHalf = Vec16<T>::kN, kLanes = kGroup / (2 * kHalf);
+    Largest<T> largest;
+    largest.add(q[0]);
+    largest.add(q[1]);
+    uint32_t most = largest.bits();
+#pragma unroll
+    for (int d = 1; d < kLanes; d *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+    const uint32_t byte = scale_byte(most);
+    const float by = inverse_scale(byte);
+    float t[2 * kHalf];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[kHalf];
+        Vec16<T>::get(q[h], v);
+#pragma unroll
+        for (int i = 0; i < kHalf; i += 2) {
+            const float2 r = mul2(make_float2(v[i], v[i + 1]), make_float2(by, by));
+            t[h * kHalf + i] = r.x;
+            t[h * kHalf + i + 1] = r.y;
+        }
+    }
+    uint32_t word = byte << (8 * ((threadIdx.x & 31) / kLanes % kTileGroups));
+    word |= __shfl_xor_sync(0xffffffffu, word, kLanes);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2 * kLanes);
+    *scales = word;
+#pragma unroll
+    for (int h = 0; h < kHalf / 4; ++h) {
+        const float some[8] = {t[8 * h], t[8 * h + 1], t[8 * h + 2], t[8 * h + 3], t[8 * h + 4], t[8 * h + 5], t[8 * h + 6], t[8 * h + 7]};
+        codes[h] = codes8(some);
+    }
+}
+// 16 bytes of values of type T of a group with a scale
+template <typename T>
+__device__ __forceinline__ uint4 values_vector(uint32_t codes, uint32_t byte) {
+    constexpr int kN = Vec16<T>::kN;
+    float v[kN];
+    values_of<kN>(codes, v);
+    const float by = scale_value(byte);
+#pragma unroll
+    for (int i = 0; i < kN; i += 2) {
+        const float2 r = mul2(make_float2(v[i], v[i + 1]), make_float2(by, by));
+        v[i] = r.x;
+        v[i + 1] = r.y;
+    }
+    return Vec16<T>::put(v);
 }
 // Such a lane's codes to `to`, kN / 2 bytes
 template <int kN>

@@ -27,26 +27,31 @@ struct NormParams {
     int aligned, sum_aligned, y_aligned, gamma_aligned, scales_aligned;      // aligned: of what is read
 };
 
-// Vector u of gamma; ones where there is none, and where a row has ended
-template <int N>
+// Vector u of gamma; ones where there is none, and where a row has ended.  WHOLE: vectors are whole and lie on 16 bytes.
+template <bool WHOLE, int N>
 __device__ __forceinline__ void load_gamma(const NormParams &p, int u, float (&g)[N]) {
-    if (p.gamma && p.gamma_aligned && u * N + N <= p.cols) {
+    if (p.gamma && (WHOLE || (p.gamma_aligned && u * N + N <= p.cols))) {
+        const float4 *from = reinterpret_cast<const float4 *>(p.gamma + u * N);
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const float4 v = *reinterpret_cast<const float4 *>(p.gamma + u * N + i);
+            const float4 v = from[i / 4];
             g[i] = v.x; g[i + 1] = v.y; g[i + 2] = v.z; g[i + 3] = v.w;
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) g[i] = p.gamma && u * N + i < p.cols ? p.gamma[u * N + i] : 1.0f;
+    for (int i = 0; i < N; ++i) g[i] = !WHOLE && p.gamma && u * N + i < p.cols ? p.gamma[u * N + i] : 1.0f;
 }
 
-template <typename T, typename Y>
-__device__ __forceinline__ void store_values(T *row, int u, int cols, const Y &values, bool aligned) {
-    constexpr int kN = 16 / sizeof(T);
-    if (aligned && u * kN + kN <= cols) {
-        *reinterpret_cast<uint4 *>(row + u * kN) = values;
+template <bool WHOLE, typename T>
+__device__ __forceinline__ uint4 load_vector(const T *row, int u, int cols, bool aligned) {
+    return WHOLE ? reinterpret_cast<const uint4 *>(row)[u] : mx::load_values(row, (int64_t)u * Vec16<T>::kN, cols, aligned);
+}
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void store_vector(T *row, int u, int cols, const uint4 &values, bool aligned) {
+    constexpr int kN = Vec16<T>::kN;
+    if (WHOLE || (aligned && u * kN + kN <= cols)) {
+        reinterpret_cast<uint4 *>(row)[u] = values;
     } else {
         const T *v = reinterpret_cast<const T *>(&values);
 #pragma unroll
@@ -66,6 +71,7 @@ __device__ __forceinline__ uint4 add_rounded(const uint4 &a, const uint4 &b) {
     return Vec16<T>::put(x);
 }
 
+// s + the squares of a vector, in 64 bits
 template <typename T>
 __device__ __forceinline__ double squares(const uint4 &h, double s) {
     constexpr int kN = Vec16<T>::kN;
@@ -103,8 +109,9 @@ __device__ __forceinline__ uint32_t row_max(uint32_t most, uint32_t *part) {
     return most;
 }
 
-// V: vectors a thread holds; 0: any number, read again for each use.  WARP: a row belongs to a warp, else to the block.
-template <typename T, Out OUT, bool RES, int V, bool WARP>
+// V: vectors a thread holds; 0: any number, read again for each use.  WARP: a row belongs to a warp, else to the block.  WHOLE: rows are whole 16-byte vectors that lie on
+// 16 bytes, their results likewise (an instance of its own: checks of every vector are half of the instructions of the general one).
+template <typename T, Out OUT, bool RES, int V, bool WARP, bool WHOLE>
 __global__ void __launch_bounds__(WARP ? kWarpRowThreads : kMost)
 rms_norm_kernel(const __grid_constant__ NormParams p) {
     constexpr int kN = Vec16<T>::kN;
@@ -127,11 +134,11 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
         T *hr = RES && p.sum ? static_cast<T *>(p.sum) + r * p.sum_pitch : nullptr;
         // h from x and the residual, and h again where it is not held: of the sum, which may have taken the place of one of them
         auto fresh = [&](int u) {
-            uint4 h = mx::load_values(xr, (int64_t)u * kN, p.cols, p.aligned);
-            if constexpr (RES) h = add_rounded<T>(h, mx::load_values(rr, (int64_t)u * kN, p.cols, p.aligned));
+            uint4 h = load_vector<WHOLE>(xr, u, p.cols, p.aligned);
+            if constexpr (RES) h = add_rounded<T>(h, load_vector<WHOLE>(rr, u, p.cols, p.aligned));
             return h;
         };
-        auto again = [&](int u) { return RES && hr ? mx::load_values(const_cast<const T *>(hr), (int64_t)u * kN, p.cols, p.sum_aligned) : fresh(u); };
+        auto again = [&](int u) { return RES && hr ? load_vector<WHOLE>(const_cast<const T *>(hr), u, p.cols, p.sum_aligned) : fresh(u); };
         uint4 held[V > 0 ? V : 1];
         double s = 0.0;
         if constexpr (V > 0) {
@@ -139,24 +146,24 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 held[i] = make_uint4(0, 0, 0, 0);
-                if (at + i * step < vectors) held[i] = mx::load_values(xr, (int64_t)(at + i * step) * kN, p.cols, p.aligned);
+                if (at + i * step < vectors) held[i] = load_vector<WHOLE>(xr, at + i * step, p.cols, p.aligned);
                 if constexpr (RES) {
                     res[i] = make_uint4(0, 0, 0, 0);
-                    if (at + i * step < vectors) res[i] = mx::load_values(rr, (int64_t)(at + i * step) * kN, p.cols, p.aligned);
+                    if (at + i * step < vectors) res[i] = load_vector<WHOLE>(rr, at + i * step, p.cols, p.aligned);
                 }
             }
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if constexpr (RES) {
                     held[i] = add_rounded<T>(held[i], res[i]);
-                    if (hr && at + i * step < vectors) store_values(hr, at + i * step, p.cols, held[i], p.sum_aligned);
+                    if (hr && at + i * step < vectors) store_vector<WHOLE>(hr, at + i * step, p.cols, held[i], p.sum_aligned);
                 }
                 s = squares<T>(held[i], s);
             }
         } else {
             for (int u = at; u < vectors; u += step) {
                 const uint4 h = fresh(u);
-                if (RES && hr) store_values(hr, u, p.cols, h, p.sum_aligned);
+                if (RES && hr) store_vector<WHOLE>(hr, u, p.cols, h, p.sum_aligned);
                 s = squares<T>(h, s);
             }
         }
@@ -164,10 +171,26 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
         const float by = (float)(1.0 / sqrt(s / (double)p.cols + p.eps));
         auto normed = [&](const uint4 &h, int u, float (&v)[kN]) {
             float g[kN];
-            load_gamma<kN>(p, u, g);
+            load_gamma<WHOLE>(p, u, g);
             Vec16<T>::get(h, v);
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[i] = __fmul_rn(__fmul_rn(v[i], by), g[i]);
+            for (int i = 0; i < kN; i += 2) {
+                const float2 r = mul2(mul2(make_float2(v[i], v[i + 1]), make_float2(by, by)), make_float2(g[i], g[i + 1]));
+                v[i] = r.x;
+                v[i + 1] = r.y;
+            }
+        };
+        // (a row that is not finite: what lies behind its end is NaN)
+        auto clear_behind = [&](int u, float (&v)[kN]) {
+            if (!WHOLE && (int64_t)u * kN + kN > p.cols)
+#pragma unroll
+                for (int i = 0; i < kN; ++i)
+                    if ((int64_t)u * kN + i >= p.cols) v[i] = 0.0f;
+        };
+        auto largest = [&](const float (&v)[kN], float most) {
+#pragma unroll
+            for (int i = 0; i < kN; i += 2) most = max_magnitude(most, v[i], v[i + 1]);
+            return most;
         };
         // body(turn, vector, its h): of all vectors; ALL: and of as many behind the row's end as the other lanes of a warp have
         auto each = [&](auto all, const auto &body) {
@@ -188,18 +211,17 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             each(Live(), [&](int u, const uint4 &h) {
                 float v[kN];
                 normed(h, u, v);
-                store_values(static_cast<T *>(p.y) + r * p.y_pitch, u, p.cols, Vec16<T>::put(v), p.y_aligned);
+                store_vector<WHOLE>(static_cast<T *>(p.y) + r * p.y_pitch, u, p.cols, Vec16<T>::put(v), p.y_aligned);
             });
         } else if constexpr (OUT == kInt8) {
-            uint32_t most = 0;
+            float most = 0.0f;
             each(Live(), [&](int u, const uint4 &h) {
                 float v[kN];
                 normed(h, u, v);
-#pragma unroll
-                for (int i = 0; i < kN; ++i)
-                    if (u * kN + i < p.cols) most = max(most, magnitude(v[i]));      // (a row that is not finite: what lies behind its end is NaN)
+                clear_behind(u, v);
+                most = largest(v, most);
             });
-            const RowScale scale(row_max<WARP>(most, maxima));
+            const RowScale scale(row_max<WARP>(__float_as_uint(most), maxima));
             if (at == 0) static_cast<float *>(p.scales)[r] = scale.scale;
             int8_t *yr = static_cast<int8_t *>(p.y) + r * p.y_pitch;
             each(Live(), [&](int u, const uint4 &h) {
@@ -213,7 +235,7 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
                     quantize16<float>(scale, some, &w[q / 4]);
                 }
                 int8_t *to = yr + u * kN;
-                if (p.y_aligned && u * kN + kN <= p.cols) {
+                if (WHOLE || (p.y_aligned && u * kN + kN <= p.cols)) {
                     if constexpr (kN == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
                     else *reinterpret_cast<uint32_t *>(to) = w[0];
                 } else {
@@ -224,18 +246,19 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             });
         } else {
             const int used = (p.cols + mx::kGroup - 1) / mx::kGroup * mx::kGroup;
-            uint8_t *yr = static_cast<uint8_t *>(p.y) + r * p.y_pitch, *scales = static_cast<uint8_t *>(p.scales);
+            uint8_t *yr = static_cast<uint8_t *>(p.y) + r * p.y_pitch, *scales = static_cast<uint8_t *>(p.scales) + mx::word_at(r, 0, p.tiles);
             constexpr int kLanes = 128 / kN;      // of a tile of scales
             each(All(), [&](int u, const uint4 &h) {
                 float v[kN];
                 normed(h, u, v);
+                if (u >= vectors)
 #pragma unroll
-                for (int i = 0; i < kN; ++i)
-                    if ((int64_t)u * kN + i >= p.cols) v[i] = 0.0f;
+                    for (int i = 0; i < kN; ++i) v[i] = 0.0f;
+                clear_behind(u, v);
                 uint32_t word;
-                const uint32_t codes = mx::quantize_lanes<kN>(v, &word);
-                if ((int64_t)u * kN < used) mx::store_codes<kN>(yr + u * (kN / 2), codes, p.y_aligned);
-                if (u % kLanes == 0 && u / kLanes < p.tiles) mx::store_scales(scales + mx::word_at(r, u / kLanes, p.tiles), word, p.scales_aligned);
+                const uint32_t codes = mx::quantize_lanes<kN>(v, __float_as_uint(largest(v, 0.0f)), &word);
+                if (u * kN < used) mx::store_codes<kN>(yr + u * (kN / 2), codes, WHOLE || p.y_aligned);
+                if (u % kLanes == 0 && u / kLanes < p.tiles) mx::store_scales(scales + u / kLanes * (int64_t)mx::kTileBytes, word, WHOLE || p.scales_aligned);
             });
         }
         if constexpr (!WARP) __syncthreads();      // (the next row's sums)
@@ -252,11 +275,16 @@ int launch(const NormParams &p, cudaStream_t stream) {
         TSB_LAUNCHED("rms_norm_kernel");
         return TSB_OK;
     };
-    if (vectors <= 32) return go(rms_norm_kernel<T, OUT, RES, 1, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
-    if (vectors <= 64) return go(rms_norm_kernel<T, OUT, RES, 2, true>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
-    if (vectors <= kMost && p.rows <= 148 * 2) return go(rms_norm_kernel<T, OUT, RES, 1, false>, rows, round_up(vectors, 32));
-    if (vectors <= 4 * kMost) return go(rms_norm_kernel<T, OUT, RES, 4, false>, rows, round_up(ceil_div(vectors, 4), 32));
-    return go(rms_norm_kernel<T, OUT, RES, 0, false>, rows, kMost);
+    const bool whole = p.cols % kN == 0 && p.aligned && p.y_aligned && (p.sum_aligned || !p.sum) && p.gamma_aligned && p.scales_aligned;
+    auto pick = [&](auto is_whole) {
+        constexpr bool kWhole = decltype(is_whole)::value;
+        if (vectors <= 32) return go(rms_norm_kernel<T, OUT, RES, 1, true, kWhole>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
+        if (vectors <= 64) return go(rms_norm_kernel<T, OUT, RES, 2, true, kWhole>, ceil_div64(rows, kWarpRowThreads / 32), kWarpRowThreads);
+        if (vectors <= kMost && p.rows <= 148 * 2) return go(rms_norm_kernel<T, OUT, RES, 1, false, kWhole>, rows, round_up(vectors, 32));
+        return go(rms_norm_kernel<T, OUT, RES, 4, false, kWhole>, rows, round_up(ceil_div(vectors, 4), 32));
+    };
+    if (vectors > 4 * kMost) return go(rms_norm_kernel<T, OUT, RES, 0, false, false>, rows, kMost);
+    return whole ? pick(std::true_type()) : pick(std::false_type());
 }
 
 template <typename T, Out OUT>
