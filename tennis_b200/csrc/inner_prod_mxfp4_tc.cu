@@ -32,64 +32,74 @@ struct Mxfp4Params : Walk {
 // PAIR: tiles of two CTAs, each with 128 of 256 tokens and half of the channels' rows of w in its shared memory, and all channels' scales
 template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
 struct Layout {
+    // A step of the epilogue is 2 KB of y in rows of 128 bytes: a copy costs the engine that moves it 4.5 clocks a row of up to 128 bytes (100352 x 256 x 64, which
+    // that engine bounds, 20.5 -> 15.6 us).  Pairs, whose columns of sums are handed on 32 at a time, and splits take rows of 32 channels.
+    static constexpr int kChannels = PAIR || SPLIT > 1 ? kCh : 128 / (int)sizeof(T);
+    using Step = Staged<T, kChannels>;
     static constexpr bool kAhead = RES && SPLIT == 1;                             // residuals of a step come while the one in front of it is worked on
     static constexpr uint32_t kOutWarp = kAhead ? 2 * kOutRows : kOutRows;        // a warp's staged outputs (and the next step's residuals)
-    static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) share the channels of a tile
+    static constexpr int kEpiWarps = BN >= 128 ? 16 : 8;                          // four (or two) for each quarter of the tokens
     static constexpr int kThreads = 32 * (2 + kEpiWarps);
+    // those four share the channels, and where there are fewer steps' channels than that, the rows of the quarter
+    static constexpr int kShares = kEpiWarps / 4 < BN / kChannels ? kEpiWarps / 4 : BN / kChannels, kRowShares = kEpiWarps / 4 / kShares;
     static constexpr int kBRows = PAIR ? BN / 2 : BN;
     static constexpr uint32_t kBBytes = kBRows * kKBytes;
     static constexpr int kScaleTiles = (BN + 127) / 128;                          // of 128 channels
     static constexpr uint32_t kScalesAt = kABytes + kBBytes;
+    static constexpr uint32_t kWeights = kBBytes + kScaleTiles * kScales;         // of a stage
     static constexpr uint32_t kStage = kScalesAt + (1 + kScaleTiles) * kScales;
     static constexpr uint32_t kOut = kEpiWarps * kOutWarp;
     static constexpr uint32_t kParts = (SPLIT - 1) * kBM * kCh * 4;               // the other CTAs' sums of this CTA's channels
-    static constexpr uint32_t kBars = 256;
-    static constexpr int kStages = (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) < kMaxStages
-                                       ? (int)((kSmem - 1024 - kOut - kParts - kBars) / kStage) : kMaxStages;
-    static constexpr uint32_t kBytes = 1024 + kStages * kStage + kOut + kParts + kBars;
-    // columns of tensor memory: the sums' buffers, x's scales (of a stage: twice four), w's (twice four for every 128 channels)
+    static constexpr uint32_t kFixed = 1024 + 1024 + kOut + kParts;               // barriers, and what the alignment of the ring takes
+    static constexpr int kStages = (int)((kSmem - kFixed) / kStage) < kMaxStages ? (int)((kSmem - kFixed) / kStage) : kMaxStages;      // at most
+    // columns of tensor memory: the sums' buffers, x's scales (of a stage: twice four), w's (twice four for every 128 channels).  Where every CTA has one tile, one buffer.
     static constexpr bool kShared = BN == 256;
-    static constexpr uint32_t kSecond = kShared ? 224 : BN, kScaleColumns = kShared ? 480 : 256;
-    static_assert(kSecond + BN <= kScaleColumns && kScaleColumns + 8 + 8 * kScaleTiles <= 512, "sums and scales fit tensor memory");
+    static constexpr uint32_t kSecond = kShared ? 224 : BN;
+    __host__ __device__ static constexpr uint32_t scale_columns(bool one) { return kShared ? 480 : one ? BN : 2 * BN; }
+    __host__ __device__ static constexpr uint32_t columns(bool one) { return BN == 64 ? (one ? 128 : 256) : BN == 128 && one ? 256 : 512; }
 };
 
 // A lane's channels' biases of a step: channels 8 j + 2 (lane % 4) and the next one, for every j; zeros for channels that do not exist.
-__device__ __forceinline__ void load_bias(const Params &p, int c0, float2 (&bias)[kCh / 8]) {
+template <int J>
+__device__ __forceinline__ void load_bias(const Params &p, int c0, float2 (&bias)[J]) {
 #pragma unroll
-    for (int j = 0; j < kCh / 8; ++j) {
+    for (int j = 0; j < J; ++j) {
         const int c = c0 + 8 * j + 2 * (threadIdx.x & 3);
         bias[j] = make_float2(p.bias && c < p.n ? p.bias[c] : 0.0f, p.bias && c + 1 < p.n ? p.bias[c + 1] : 0.0f);
     }
 }
 
-// kCh channels of Staged<T>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
+// CH channels of Staged<T, CH>::kRows tokens, of which `live` exist: sums in tensor memory at `taddr` -> y, by way of `rows` in shared memory.
 // m0, c0: the first token and channel; to: where in a staged row of eight the lane's pairs of channels 8 j lie; tile_store: y is written by a copy of
 // its own accord that is under way when this returns, else by the lanes.  fetched: the residual is in `rows` already.  loaded(): called once
 // the sums are in registers.  GIVEN: the sums are in `given` already.
-template <typename T, bool RES, bool GIVEN = false, typename Loaded>
-__device__ __forceinline__ void epilogue_rows(const Params &p, const CUtensorMap *map_y, uint32_t taddr, const float *given, int64_t m0, int live, int c0, const float2 (&bias)[kCh / 8],
-                                              uint8_t *rows, const uint32_t (&to)[kCh / 8], bool tile_store, bool res_vec, bool fetched, const Loaded &loaded) {
-    using S = Staged<T>;
-    constexpr int kN = Vec16<T>::kN, kHalves = S::kRows / 16, kValues = kHalves * kCh / 2;     // values of a unit; runs of 16 rows; values of a lane
+template <typename T, int CH, bool RES, bool GIVEN = false, typename Loaded>
+__device__ __forceinline__ void epilogue_rows(const Params &p, const CUtensorMap *map_y, uint32_t taddr, const float *given, int64_t m0, int live, int c0, const float2 (&bias)[CH / 8],
+                                              uint8_t *rows, const uint32_t (&to)[CH / 8], bool tile_store, bool res_vec, bool fetched, const Loaded &loaded) {
+    using S = Staged<T, CH>;
+    constexpr int kN = Vec16<T>::kN, kHalves = S::kRows / 16, kPieces = CH / 32, kValues = kHalves * CH / 2;     // values of a unit; runs of 16 rows, of 32 channels; values of a lane
     const int lane = threadIdx.x & 31;
-    // value i of a lane: channels 8 j + 2 (lane % 4) + i % 2 of j = i / 4 % 4, of the row lane / 4, plus 8 for i & 2, plus 16 a half
+    // value i of a lane: channels 8 j + 2 (lane % 4) + i % 2 of j = i / 4 % (CH / 8), of the row lane / 4, plus 8 for i & 2, plus 16 a half
     float v[kValues];
     if constexpr (GIVEN) {
 #pragma unroll
         for (int i = 0; i < kValues; ++i) v[i] = given[i];
-        if (RES && !fetched) fetch_residual<T>(p, m0, live, c0, rows, res_vec);
+        if (RES && !fetched) fetch_residual<T, CH>(p, m0, live, c0, rows, res_vec);
     } else {
         int acc[kValues];
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16), *reinterpret_cast<int (*)[kCh / 2]>(&acc[h * kCh / 2]));
-        if (RES && !fetched) fetch_residual<T>(p, m0, live, c0, rows, res_vec);
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c)
+                tmem_ld_rows16(taddr + ((uint32_t)(h * 16) << 16) + 32 * c, *reinterpret_cast<int (*)[16]>(&acc[(h * kPieces + c) * 16]));
+        if (RES && !fetched) fetch_residual<T, CH>(p, m0, live, c0, rows, res_vec);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < kValues; ++i) v[i] = __int_as_float(acc[i]);
         loaded();
     }
-    auto at = [&](int i) { return rows + to[i / 4 % (kCh / 8)] + ((i & 2) * 4 + i / (kCh / 2) * 16) * S::kRowBytes; };
-    finish_values<T, RES>(p, [&](int i) { return i & 1 ? bias[i / 4 % (kCh / 8)].y : bias[i / 4 % (kCh / 8)].x; },
+    auto at = [&](int i) { return rows + to[i / 4 % (CH / 8)] + ((i & 2) * 4 + i / (CH / 2) * 16) * S::kRowBytes; };
+    finish_values<T, RES>(p, [&](int i) { return i & 1 ? bias[i / 4 % (CH / 8)].y : bias[i / 4 % (CH / 8)].x; },
                           [&](int i) { return to_f32(reinterpret_cast<const T *>(at(i))[i & 1]); }, v);      // (a lane's outputs go where its residuals were)
     if (!RES && lane == 0) bulk_wait_read();
     __syncwarp();
@@ -102,7 +112,7 @@ __device__ __forceinline__ void epilogue_rows(const Params &p, const CUtensorMap
             *reinterpret_cast<uint32_t *>(at(i)) = *reinterpret_cast<const uint32_t *>(pair);
         }
     }
-    if (tile_store && (c0 + kCh <= p.n || p.n % kN == 0)) {      // (such a copy stops at 16 bytes, not at the value, where y ends)
+    if (tile_store && (c0 + CH <= p.n || p.n % kN == 0)) {      // (such a copy stops at 16 bytes, not at the value, where y ends)
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -114,7 +124,9 @@ __device__ __forceinline__ void epilogue_rows(const Params &p, const CUtensorMap
         T *y = static_cast<T *>(p.y) + m0 * p.y_pitch + c0 + lane;
 #pragma unroll 4
         for (int r = 0; r < live; ++r, y += p.y_pitch)
-            if (c0 + lane < p.n) *y = *reinterpret_cast<const T *>(rows + S::value(r, lane));
+#pragma unroll
+            for (int c = 0; c < CH; c += 32)
+                if (c0 + c + lane < p.n) y[c] = *reinterpret_cast<const T *>(rows + S::value(r, c + lane));
         __syncwarp();
     }
 }
@@ -122,15 +134,17 @@ __device__ __forceinline__ void epilogue_rows(const Params &p, const CUtensorMap
 template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
 __global__ void __launch_bounds__(Layout<T, BN, RES, PAIR, SPLIT>::kThreads, 1)
 inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_xs,
-                           const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ Mxfp4Params t, int tile_store, int res_vec) {
+                           const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ Mxfp4Params t, int stages, int one, int keep, int tile_store, int res_vec) {
     static_assert(SPLIT == 1 || (!PAIR && BN == kCh * SPLIT), "split: kCh channels of the tile for each CTA");
     static_assert(PAIR == (BN == 256), "the widest tiles are pairs'");
+    static_assert(Layout<T, BN, RES, PAIR, SPLIT>::scale_columns(true) + 8 + 8 * Layout<T, BN, RES, PAIR, SPLIT>::kScaleTiles <= Layout<T, BN, RES, PAIR, SPLIT>::columns(true) &&
+                      Layout<T, BN, RES, PAIR, SPLIT>::scale_columns(false) + 8 + 8 * Layout<T, BN, RES, PAIR, SPLIT>::kScaleTiles <= Layout<T, BN, RES, PAIR, SPLIT>::columns(false),
+                  "sums and scales fit tensor memory");
     using L = Layout<T, BN, RES, PAIR, SPLIT>;
     extern __shared__ uint8_t smem_raw[];
-    const uint32_t raw = smem_u32(smem_raw);
-    const uint32_t base = (raw + 1023u) & ~1023u;
-    uint8_t *out_rows = smem_raw + (base - raw) + L::kStages * L::kStage;
-    uint8_t *parts = out_rows + L::kOut, *bars_ptr = parts + L::kParts;
+    const uint32_t raw = smem_u32(smem_raw), lowest = (raw + 1023u) & ~1023u;
+    uint8_t *const bars_ptr = smem_raw + (lowest - raw), *const out_rows = bars_ptr + 1024, *const parts = out_rows + L::kOut;
+    const uint32_t base = smem_u32(parts + L::kParts);       // of the ring
     const uint32_t bar_full = smem_u32(bars_ptr), bar_empty = bar_full + 8 * kMaxStages, bar_tfull = bar_empty + 8 * kMaxStages, bar_tempty = bar_tfull + 16, bar_shared = bar_tempty + 16;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars_ptr + 8 * (2 * kMaxStages + 6));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(bars_ptr + 8 * (2 * kMaxStages + 6) + 4);
@@ -143,7 +157,7 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
     auto rows_of = [&](int m_tile) { return PAIR ? 2 * m_tile + rank : m_tile; };      // this CTA's 128 tokens of a tile
 
     if (warp == 0) {
-        if (lane < L::kStages) {
+        if (lane < stages) {
             mbar_init(bar_full + 8 * lane, 1);
             mbar_init(bar_empty + 8 * lane, 1);
         }
@@ -158,6 +172,7 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
             prefetch_tensormap(&map_w);
             prefetch_tensormap(&map_xs);
             prefetch_tensormap(&map_ws);
+            prefetch_tensormap(&map_y);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
@@ -165,10 +180,10 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
     if (warp == 1) {
         const uint32_t slot = smem_u32(const_cast<uint32_t *>(tmem_slot));
         if constexpr (PAIR) {
-            pair_tmem_alloc(slot, 512);
+            pair_tmem_alloc(slot, L::columns(one));
             pair_tmem_relinquish();
         } else {
-            tmem_alloc(slot, 512);
+            tmem_alloc(slot, L::columns(one));
             tmem_relinquish();
         }
     }
@@ -189,16 +204,18 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
     if (warp == 0) {
         // Both CTAs of a pair load their halves; the bytes of both count at the even one's barrier.  Neither can be a round ahead: its
         // own stage is free only when the MMAs that read both have completed.
-        uint32_t s = 0;
+        // `keep`: K's blocks divide the ring, and the CTA stays with its channels: the weights of its first tile serve the others too.
+        uint32_t stage = 0, round = 1, at = base;
+        int loads = 0;
         const uint32_t lead_full = PAIR ? map_to_rank(bar_full, 0) : bar_full;
         for (int i = first; i < tiles; i += step) {
             int mt, nt;
             tile_of(t, i, mt, nt);
-            for (int kb = kb0; kb < kb1; ++kb, ++s) {
-                const uint32_t stage = s % L::kStages, round = s / L::kStages, at = base + stage * L::kStage;
-                if (!mbar_wait_warp(bar_empty + 8 * stage, (round & 1) ^ 1, abort_flag)) { give_up(1); goto done; }
+            for (int kb = kb0; kb < kb1; ++kb, ++loads) {
+                if (!mbar_wait_warp(bar_empty + 8 * stage, round, abort_flag)) { give_up(1); goto done; }
+                const bool weights = !keep || loads < stages;
                 if (elect_one()) {
-                    if (!PAIR || rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, PAIR ? 2 * L::kStage : L::kStage);
+                    if (!PAIR || rank == 0) mbar_arrive_expect_tx(bar_full + 8 * stage, PAIR ? 2 * L::kStage : weights ? L::kStage : L::kStage - L::kWeights);
                     const uint32_t full = lead_full + 8 * stage;
                     // (scales: words of four, a tile's 128 after each other, two tiles a block of K)
                     if constexpr (PAIR) {
@@ -208,24 +225,34 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
                         pair_tma_load_2d(at + L::kScalesAt + kScales, &map_ws, full, kb * 256, nt * L::kScaleTiles);
                     } else {
                         tma_load_2d(at, &map_x, full, kb * kKBytes, rows_of(mt) * kBM);
-                        tma_load_2d(at + kABytes, &map_w, full, kb * kKBytes, nt * BN);
                         tma_load_2d(at + L::kScalesAt, &map_xs, full, kb * 256, rows_of(mt));
-                        tma_load_2d(at + L::kScalesAt + kScales, &map_ws, full, kb * 256, BN < 128 ? nt * BN / 128 : nt);
+                        if (weights) {
+                            tma_load_2d(at + kABytes, &map_w, full, kb * kKBytes, nt * BN);
+                            tma_load_2d(at + L::kScalesAt + kScales, &map_ws, full, kb * 256, BN < 128 ? nt * BN / 128 : nt);
+                        }
                     }
                 }
                 __syncwarp();
+                at += L::kStage;
+                if (++stage == (uint32_t)stages) {
+                    stage = 0;
+                    at = base;
+                    round ^= 1;
+                }
             }
         }
         if constexpr (PAIR) {
-            // no arrival from the other CTA is to come when this one leaves
-            for (uint32_t back = min(s, (uint32_t)L::kStages); back > 0; --back)
-                if (!mbar_wait_warp(bar_empty + 8 * ((s - back) % L::kStages), (s - back) / L::kStages & 1, abort_flag)) { give_up(1); goto done; }
+            // no arrival from the other CTA is to come when this one leaves: the last rounds' stages, from the one that is loaded longest ago
+            for (int back = min(loads, stages); back > 0; --back) {
+                const uint32_t behind = (uint32_t)(loads - back) % (uint32_t)stages;
+                if (!mbar_wait_warp(bar_empty + 8 * behind, (uint32_t)(loads - back) / (uint32_t)stages & 1, abort_flag)) { give_up(1); goto done; }
+            }
         }
     } else if (warp == 1) {
-        uint32_t s = 0, n = 0;
+        uint32_t stage = 0, round = 0, at = base, n = 0;
         constexpr uint64_t kDescHi = smem_desc_hi<kKBytes>(8 * kKBytes);
         constexpr uint32_t kInstr[2] = {instr_desc_mxf4<BN>(PAIR ? 2 * kBM : kBM, 0), instr_desc_mxf4<BN>(PAIR ? 2 * kBM : kBM, 1)};
-        const uint32_t sfa = tmem + L::kScaleColumns, sfb = sfa + 8;
+        const uint32_t sfa = tmem + L::scale_columns(one), sfb = sfa + 8;
         if (!PAIR || rank == 0)
             for (int i = first; i < tiles; i += step, ++n) {
                 const uint32_t acc = n & 1;
@@ -241,12 +268,10 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
                     tile_of(t, i, mt, nt);
                     odd = nt * BN % 128 / 32;
                 }
-                for (int kb = kb0; kb < kb1; ++kb, ++s) {
-                    const uint32_t stage = s % L::kStages, round = s / L::kStages;
-                    if (!mbar_wait_warp(bar_full + 8 * stage, round & 1, abort_flag)) { give_up(2); goto done; }
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!mbar_wait_warp(bar_full + 8 * stage, round, abort_flag)) { give_up(2); goto done; }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t at = base + stage * L::kStage;
                         const uint64_t a = kDescHi | (at >> 4), b = kDescHi | ((at + kABytes) >> 4);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {                // 128 values of K, the half of a stage
@@ -275,27 +300,36 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
                         }
                     }
                     __syncwarp();
+                    at += L::kStage;
+                    if (++stage == (uint32_t)stages) {
+                        stage = 0;
+                        at = base;
+                        round ^= 1;
+                    }
                 }
             }
     } else {
         const int e = warp - 2, quarter = warp & 3;      // tensor memory lanes of this warp: 32 * (warp % 4)
-        constexpr int kShare = BN / (L::kEpiWarps / 4), kSteps = kShare / kCh;
-        const int share = e / 4 * kShare;                // its channels of the tile
+        using S = typename L::Step;
+        constexpr int kChannels = L::kChannels, kShare = BN / L::kShares, kSteps = kShare / kChannels, kRows = S::kRows, kQuarter = 32 / L::kRowShares;
+        static_assert(kRows <= kQuarter, "a step's rows are a warp's");
+        const int share = e / 4 % L::kShares * kShare;   // its channels of the tile, and from which of the quarter's rows on it has kQuarter of them
+        const int row0 = quarter * 32 + e / 4 / L::kShares * kQuarter;
         // Its steps' channels from there.  (The columns that the buffers share are the last ones of the first buffer and the first ones of the second: the
         // warps of either take them in their first step.)
-        const int turned = L::kShared && e / 4 == L::kEpiWarps / 4 - 1 ? kSteps - 1 : 0;
-        auto channel_of = [&](int c) { return share + (c ^ turned) * kCh; };
+        const int turned = L::kShared && e / 4 == L::kShares - 1 ? kSteps - 1 : 0;
+        auto channel_of = [&](int c) { return share + (c ^ turned) * kChannels; };
         uint8_t *rows = out_rows + e * L::kOutWarp;
-        uint32_t n = 0, to[kCh / 8];
+        uint32_t n = 0, to[kChannels / 8];
 #pragma unroll
-        for (int j = 0; j < kCh / 8; ++j) to[j] = Staged<T>::value(lane >> 2, 8 * j + 2 * (lane & 3));
+        for (int j = 0; j < kChannels / 8; ++j) to[j] = S::value(lane >> 2, 8 * j + 2 * (lane & 3));
         int mt, nt, channels_of = -1;
-        float2 bias[kSteps][kCh / 8];
+        float2 bias[kSteps][kChannels / 8];
         tile_of(t, first, mt, nt);
         uint32_t turn = 0;                               // which half of its staging a step takes
         if constexpr (L::kAhead) {
-            const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32;
-            start_residual<T>(t.p, m0, (int)max((int64_t)0, min((int64_t)Staged<T>::kRows, t.p.m - m0)), nt * BN + channel_of(0), rows, res_vec != 0);
+            const int64_t m0 = (int64_t)rows_of(mt) * kBM + row0;
+            start_residual<T, kChannels>(t.p, m0, (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), nt * BN + channel_of(0), rows, res_vec != 0);
         }
         const uint32_t lead_tempty = PAIR ? map_to_rank(bar_tempty, 0) : bar_tempty, lead_shared = PAIR ? map_to_rank(bar_shared, 0) : bar_shared;
         for (int i = first; i < tiles; i += step, ++n) {
@@ -307,12 +341,11 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
             channels_of = nt;
             int next_mt = mt, next_nt = nt;
             if (i + step < tiles) tile_of(t, i + step, next_mt, next_nt);
-            constexpr int kRows = Staged<T>::kRows;
             if constexpr (RES) {                       // (the first step's, while the sums are not there yet)
-                const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32;
+                const int64_t m0 = (int64_t)rows_of(mt) * kBM + row0;
                 const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + channel_of(0);
-                if (live > 0 && c0 < t.p.n && (SPLIT == 1 || e / 4 == rank) && !(L::kAhead && whole_residual(t.p, c0, res_vec != 0)))
-                    fetch_residual<T>(t.p, m0, live, c0, rows + (L::kAhead ? kOutRows * (turn & 1) : 0), res_vec != 0);
+                if (live > 0 && c0 < t.p.n && (SPLIT == 1 || e / 4 == rank) && !(L::kAhead && whole_residual<kChannels>(t.p, c0, res_vec != 0)))
+                    fetch_residual<T, kChannels>(t.p, m0, live, c0, rows + (L::kAhead ? kOutRows * (turn & 1) : 0), res_vec != 0);
             }
             if (!mbar_wait_warp(bar_tfull + 8 * acc, (n >> 1) & 1, abort_flag)) { give_up(4); goto done; }
             tc_fence_after();
@@ -357,7 +390,7 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
                         const int64_t m0 = (int64_t)mt * kBM + quarter * 32 + r;
                         const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + share;
                         if (live > 0 && c0 < t.p.n)
-                            epilogue_rows<T, RES, true>(t.p, &map_y, 0, sum + r / 16 * (kLane / 2), m0, live, c0, bias[0], rows, to, tile_store != 0, res_vec != 0, RES && r == 0, [] {});
+                            epilogue_rows<T, kChannels, RES, true>(t.p, &map_y, 0, sum + r / 16 * (kLane / 2), m0, live, c0, bias[0], rows, to, tile_store != 0, res_vec != 0, RES && r == 0, [] {});
                     }
                 }
                 goto done;
@@ -365,24 +398,24 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
 #pragma unroll
             for (int c = 0; c < (SPLIT > 1 ? 0 : kSteps); ++c)
 #pragma unroll
-                for (int r = 0; r < 32; r += kRows) {
-                    const int64_t m0 = (int64_t)rows_of(mt) * kBM + quarter * 32 + r;
+                for (int r = 0; r < kQuarter; r += kRows) {
+                    const int64_t m0 = (int64_t)rows_of(mt) * kBM + row0 + r;
                     const int live = (int)max((int64_t)0, min((int64_t)kRows, t.p.m - m0)), c0 = nt * BN + channel_of(c);
                     bool fetched = RES && c == 0 && r == 0;
                     uint8_t *staged = rows;
                     if constexpr (L::kAhead) {
                         staged = rows + kOutRows * (turn++ & 1);
-                        const bool last = c == kSteps - 1 && r + kRows == 32;       // of the tile: the next step is the next tile's first
-                        const int next_r = last ? 0 : (r + kRows) % 32, next_c = last ? 0 : c + (r + kRows) / 32;
-                        const int64_t next_m0 = (int64_t)rows_of(last ? next_mt : mt) * kBM + quarter * 32 + next_r;
+                        const bool last = c == kSteps - 1 && r + kRows == kQuarter;      // of the tile: the next step is the next tile's first
+                        const int next_r = last ? 0 : (r + kRows) % kQuarter, next_c = last ? 0 : c + (r + kRows) / kQuarter;
+                        const int64_t next_m0 = (int64_t)rows_of(last ? next_mt : mt) * kBM + row0 + next_r;
                         const int next_live = last && i + step >= tiles ? 0 : (int)max((int64_t)0, min((int64_t)kRows, t.p.m - next_m0));
-                        start_residual<T>(t.p, next_m0, next_live, (last ? next_nt : nt) * BN + channel_of(next_c), rows + kOutRows * (turn & 1), res_vec != 0);
+                        start_residual<T, kChannels>(t.p, next_m0, next_live, (last ? next_nt : nt) * BN + channel_of(next_c), rows + kOutRows * (turn & 1), res_vec != 0);
                         asm volatile("cp.async.wait_group 1;" ::: "memory");              // this step's
                         __syncwarp();
-                        fetched = fetched || whole_residual(t.p, c0, res_vec != 0);
+                        fetched = fetched || whole_residual<kChannels>(t.p, c0, res_vec != 0);
                     }
                     // the shared columns: the last share's of the first buffer, the first share's of the second
-                    const bool tells = L::kShared && c == 0 && r + kRows == 32 && e / 4 == (acc ? 0 : L::kEpiWarps / 4 - 1);
+                    const bool tells = L::kShared && c == 0 && r + kRows == kQuarter && e / 4 == (acc ? 0 : L::kShares - 1);
                     auto tell = [&] {
                         if (tells) {
                             tc_fence_before();
@@ -391,7 +424,7 @@ inner_prod_mxfp4_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __gr
                         }
                     };
                     if (live > 0 && c0 < t.p.n)
-                        epilogue_rows<T, RES>(t.p, &map_y, tmem + acc * L::kSecond + ((uint32_t)(quarter * 32 + r) << 16) + channel_of(c), nullptr, m0, live, c0, bias[c], staged, to, tile_store != 0,
+                        epilogue_rows<T, kChannels, RES>(t.p, &map_y, tmem + acc * L::kSecond + ((uint32_t)(row0 + r) << 16) + channel_of(c), nullptr, m0, live, c0, bias[c], staged, to, tile_store != 0,
                                               res_vec != 0, fetched, tell);
                     else tell();
                 }
@@ -437,8 +470,8 @@ done:
     }
     if (warp == 1) {
         tc_fence_after();
-        if constexpr (PAIR) pair_tmem_dealloc(tmem, 512);
-        else tmem_dealloc(tmem, 512);
+        if constexpr (PAIR) pair_tmem_dealloc(tmem, L::columns(one));
+        else tmem_dealloc(tmem, L::columns(one));
     }
 }
 
@@ -455,17 +488,27 @@ int launch(const Params &p, cudaStream_t stream) {
     const int type = sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16;
     const bool tile_store = aligned16(p.y, p.y_pitch, type) && p.y_pitch < (int64_t)1 << 37, res_vec = p.residual && aligned16(p.residual, p.residual_pitch, type);
     if (!tile_store) my = mx;
-    else if ((st = encode_output<T>(&my, p)) != TSB_OK) return st;
+    else if ((st = encode_output<T, L::kChannels>(&my, p)) != TSB_OK) return st;
     auto kernel = inner_prod_mxfp4_tc_kernel<T, BN, RES, PAIR, SPLIT>;
     static DeviceOnce raised;
     if (raised.first()) {
-        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kBytes));
+        TSB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem));
         raised.done();
     }
     constexpr int kCluster = PAIR ? 2 : SPLIT;
     const Mxfp4Params t = {walk_of((int)ceil_div64(p.m, PAIR ? 2 * kBM : kBM), ceil_div(p.n, BN), ceil_div(bytes, kKBytes)), p};
-    const int grid = kCluster * (int)std::min<int64_t>((int64_t)t.tiles_m * t.tiles_n, SPLIT > 1 ? INT32_MAX : 148 / kCluster);      // (split: a tile a cluster)
-    TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(grid), dim3(L::kThreads), L::kBytes, stream, mx, mw, mxs, mws, my, t, (int)tile_store, (int)res_vec));
+    const int64_t tiles_all = (int64_t)t.tiles_m * t.tiles_n;
+    int clusters = (int)std::min<int64_t>(tiles_all, SPLIT > 1 ? INT32_MAX : 148 / kCluster);      // (split: a tile a cluster)
+    const int one = clusters == tiles_all;
+    // Of few output channels, tiles of the same tokens follow each other: on a grid that is a multiple of them a CTA stays with its channels.
+    if (!one && !PAIR && t.group_m == 1) clusters -= clusters % t.tiles_n;
+    // No more stages than a CTA has blocks of K: what fits beside another kernel's CTAs starts while those run.
+    const int64_t loads = ceil_div64(tiles_all, clusters) * (SPLIT > 1 ? ceil_div(t.kblocks, SPLIT) : t.kblocks);
+    int stages = (int)std::min<int64_t>(L::kStages, loads);
+    const int keep = !PAIR && SPLIT == 1 && !one && t.group_m == 1 && t.kblocks <= stages;
+    if (keep) stages -= stages % t.kblocks;
+    TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(kCluster * clusters), dim3(L::kThreads), L::kFixed + stages * L::kStage, stream, mx, mw, mxs, mws, my, t, stages, one, keep,
+                                (int)tile_store, (int)res_vec));
     TSB_LAUNCHED("inner_prod_mxfp4_tc_kernel");
     return TSB_OK;
 }
@@ -480,10 +523,10 @@ int pick(const Params &p, cudaStream_t stream) {
         return rounds * (kblocks * 2 * (int64_t)(128 + bn / ctas) + 9 * bn + (ctas - 1) * 3500);
     };
     const int64_t c64 = clocks(64, 1), c128 = clocks(128, 1), pair = clocks(256, 2);
-    // Few tiles: two or four CTAs a tile, each with a part of K, and 2000 clocks for handing sums over.
+    // Few tiles: two or four CTAs a tile, each with a part of K, and 1000 clocks a CTA for handing sums over.
     auto split_clocks = [&](int ctas) {
         const int64_t tiles = ceil_div64(p.m, kBM) * ceil_div(p.n, kCh * ctas);
-        return tiles * ctas > 148 || kblocks < ctas ? INT64_MAX : ceil_div64(kblocks, ctas) * 2 * (128 + kCh * ctas) + 9 * kCh * ctas + 2000;
+        return tiles * ctas > 148 || kblocks < ctas ? INT64_MAX : ceil_div64(kblocks, ctas) * 2 * (128 + kCh * ctas) + 9 * kCh * ctas + 1000 * ctas;
     };
     const int64_t split2 = split_clocks(2), split4 = split_clocks(4), whole = std::min({c64, c128, pair});
     if (std::min(split2, split4) < whole) return split4 <= split2 ? launch<T, 128, RES, false, 4>(p, stream) : launch<T, 64, RES, false, 2>(p, stream);

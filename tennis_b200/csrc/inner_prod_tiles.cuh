@@ -50,24 +50,24 @@ __device__ __forceinline__ void tile_of(const Walk &t, int i, int &m_tile, int &
     m_tile = g * t.group_m + r - n_tile * min(rows, t.group_m);
 }
 
-// A warp's staged outputs, rows of kCh channels: in the order of a tensor map's 64- or 128-byte swizzle, so that the fragments' writes (eight
+// A warp's staged outputs, rows of CH channels: in the order of a tensor map's 64- or 128-byte swizzle, so that the fragments' writes (eight
 // rows at a time, a 16-byte unit each or half a unit to a lane) and the rows' reads meet a bank once or twice.
-template <typename T>
+template <typename T, int CH = kCh>
 struct Staged {
-    static constexpr int kRowBytes = kCh * sizeof(T), kUnits = kRowBytes / 16;
-    static constexpr int kRows = 2048 / kRowBytes;            // tokens of a step: 32 of 2-byte values, 16 of 4-byte ones
+    static constexpr int kRowBytes = CH * sizeof(T), kUnits = kRowBytes / 16;
+    static constexpr int kRows = 2048 / kRowBytes;            // tokens of a step: 32 in rows of 64 bytes, 16 in rows of 128 bytes
     static __device__ __forceinline__ uint32_t unit(int r, int u) { return (uint32_t)(r * kRowBytes + ((u ^ (kUnits == 4 ? (r >> 1) & 3 : r & 7)) << 4)); }
     static __device__ __forceinline__ uint32_t value(int r, int c) { return unit(r, c * (int)sizeof(T) / 16) + c * (uint32_t)sizeof(T) % 16; }
 };
 
 // The residual of such a step into `rows`, once the copy that reads these rows last has done so.
-template <typename T, typename P>
+template <typename T, int CH = kCh, typename P>
 __device__ __forceinline__ void fetch_residual(const P &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
-    using S = Staged<T>;
+    using S = Staged<T, CH>;
     const int lane = threadIdx.x & 31;
     if (lane == 0) bulk_wait_read();
     __syncwarp();
-    if (res_vec && c0 + kCh <= p.n) {
+    if (res_vec && c0 + CH <= p.n) {
         constexpr int kN = Vec16<T>::kN, kStep = 32 / S::kUnits;
         const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
         const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * kN;
@@ -76,38 +76,44 @@ __device__ __forceinline__ void fetch_residual(const P &p, int64_t m0, int live,
         for (int r = 0; r < S::kRows; r += kStep, from += step)
             if (r + r0 < live) *reinterpret_cast<uint4 *>(rows + S::unit(r + r0, u0)) = *reinterpret_cast<const uint4 *>(from);
     } else {
-        // value by value, neighbouring lanes neighbouring channels
+        // value by value, neighbouring lanes neighbouring channels, as many loads under way as registers allow
+        constexpr int kPieces = CH / 32, kAtOnce = CH == kCh ? 8 : 16;
         const T *from = static_cast<const T *>(p.residual) + m0 * p.residual_pitch + c0 + lane;
-        T some[8];
-        for (int r = 0; r < live; r += 8) {
+        T some[kPieces][kAtOnce];
+        for (int r = 0; r < live; r += kAtOnce) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i, from += p.residual_pitch)
-                if (r + i < live && c0 + lane < p.n) some[i] = *from;
+            for (int i = 0; i < kAtOnce; ++i, from += p.residual_pitch)
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (r + i < live && c0 + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, lane)) = some[i];
+                for (int c = 0; c < kPieces; ++c)
+                    if (r + i < live && c0 + 32 * c + lane < p.n) some[c][i] = from[32 * c];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+                for (int c = 0; c < kPieces; ++c)
+                    if (r + i < live && c0 + 32 * c + lane < p.n) *reinterpret_cast<T *>(rows + S::value(r + i, 32 * c + lane)) = some[c][i];
         }
     }
     __syncwarp();
 }
 
-// The same without waiting for it: whole pieces alone (whole_residual), by asynchronous copies, a group of them in any case.
-template <typename P>
-__device__ __forceinline__ bool whole_residual(const P &p, int c0, bool res_vec) { return res_vec && c0 + kCh <= p.n; }
-template <typename T, typename P>
+// The same without waiting for it: whole pieces alone (whole_residual), by asynchronous copies, a group of them in any case.  (Of wider steps, whose 16-byte units are eight
+// values, pieces of whole units too.)
+template <int CH = kCh, typename P>
+__device__ __forceinline__ bool whole_residual(const P &p, int c0, bool res_vec) { return res_vec && (c0 + CH <= p.n || (CH != kCh && p.n % 8 == 0)); }
+template <typename T, int CH = kCh, typename P>
 __device__ __forceinline__ void start_residual(const P &p, int64_t m0, int live, int c0, uint8_t *rows, bool res_vec) {
-    using S = Staged<T>;
+    using S = Staged<T, CH>;
     const int lane = threadIdx.x & 31;
     if (lane == 0) bulk_wait_read();
     __syncwarp();
-    if (live > 0 && whole_residual(p, c0, res_vec)) {
+    if (live > 0 && whole_residual<CH>(p, c0, res_vec)) {
         constexpr int kStep = 32 / S::kUnits;
         const int r0 = lane / S::kUnits, u0 = lane % S::kUnits;
         const T *from = static_cast<const T *>(p.residual) + (m0 + r0) * p.residual_pitch + c0 + u0 * Vec16<T>::kN;
         const int64_t step = kStep * p.residual_pitch;
 #pragma unroll
         for (int r = 0; r < S::kRows; r += kStep, from += step)
-            if (r + r0 < live) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(rows + S::unit(r + r0, u0))), "l"(from) : "memory");
+            if (r + r0 < live && (CH == kCh || c0 + u0 * Vec16<T>::kN < p.n)) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(rows + S::unit(r + r0, u0))), "l"(from) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -137,15 +143,15 @@ inline int encode(CUtensorMap *map, const void *at, int64_t rows, int cols, int6
 }
 
 // The boxes that a warp writes
-template <typename T, typename P>
+template <typename T, int CH = kCh, typename P>
 int encode_output(CUtensorMap *map, const P &p) {
     const auto fn = encode_tiled();
     if (!fn) return fail(TSB_ERR_UNSUPPORTED, "driver lacks cuTensorMapEncodeTiled");
     cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m};
     cuuint64_t strides[1] = {(cuuint64_t)(p.m > 1 ? p.y_pitch * (int64_t)sizeof(T) : ((int64_t)p.n * (int64_t)sizeof(T) + 15) / 16 * 16)};
-    cuuint32_t box[2] = {kCh, Staged<T>::kRows}, estr[2] = {1, 1};
+    cuuint32_t box[2] = {CH, Staged<T, CH>::kRows}, estr[2] = {1, 1};
     const CUresult r = fn(map, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          sizeof(T) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          Staged<T, CH>::kRowBytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(TSB_ERR_UNSUPPORTED, "inner product: cuTensorMapEncodeTiled(y) failed with %d", (int)r);
     return TSB_OK;
 }
