@@ -3,6 +3,8 @@
 
 #include "typed.cuh"
 
+#include <type_traits>
+
 namespace tsb {
 namespace mx {
 
@@ -122,20 +124,67 @@ __device__ __forceinline__ void quantize_bytes(const uint4 (&q)[2], uint32_t (&c
         codes[h] = codes8(some);
     }
 }
-// 16 bytes of values of type T of a group with a scale
+// Eight codes as bf16 values (fp16: their upper bytes differ, their lower ones are zero), pairs of them: bytes out of tables by the codes themselves, a sign from a table whose
+// every byte has its highest bit set, which a selector with the code's sign bit repeats.
+template <typename T>
+__device__ __forceinline__ void short_values8(uint32_t codes, uint32_t (&pairs)[4]) {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t four = codes >> (16 * h), at = four & 0x7777u;
+        uint32_t sign;                                       // 0x80, and 0xff of a negative code
+        asm("prmt.b32 %0, %1, %1, %2;" : "=r"(sign) : "r"(0x80808080u), "r"(four));
+        const uint32_t upper = (sign << 7 & 0x80808080u) | (kBf16 ? __byte_perm(0x3f3f3f00u, 0x40404040u, at) : __byte_perm(0x3e3c3800u, 0x46444240u, at));
+        const uint32_t lower = kBf16 ? __byte_perm(0xc0800000u, 0xc0804000u, at) : 0u;
+        pairs[2 * h] = __byte_perm(lower, upper, 0x5140);
+        pairs[2 * h + 1] = __byte_perm(lower, upper, 0x7362);
+    }
+}
+// 16 bytes of values of type T of a group with a scale: one rounding, to T
 template <typename T>
 __device__ __forceinline__ uint4 values_vector(uint32_t codes, uint32_t byte) {
-    constexpr int kN = Vec16<T>::kN;
-    float v[kN];
-    values_of<kN>(codes, v);
-    const float by = scale_value(byte);
+    if constexpr (sizeof(T) == 4) {
+        uint32_t pairs[4];
+        short_values8<__nv_bfloat16>(codes, pairs);      // (four of the eight)
+        const float by = scale_value(byte);
+        float v[4];
 #pragma unroll
-    for (int i = 0; i < kN; i += 2) {
-        const float2 r = mul2(make_float2(v[i], v[i + 1]), make_float2(by, by));
-        v[i] = r.x;
-        v[i + 1] = r.y;
+        for (int i = 0; i < 2; ++i) {
+            const float2 r = mul2(make_float2(__uint_as_float(pairs[i] << 16), __uint_as_float(pairs[i] & 0xffff0000u)), make_float2(by, by));
+            v[2 * i] = r.x;
+            v[2 * i + 1] = r.y;
+        }
+        return Vec16<T>::put(v);
+    } else {
+        uint32_t pairs[4];
+        short_values8<T>(codes, pairs);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            // (every scale is a bf16 number)
+            const uint32_t one = byte == 255 ? 0x7fffu : byte == 0 ? 0x0040u : byte << 7, by = one | one << 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162 *>(&pairs[i]), *reinterpret_cast<const __nv_bfloat162 *>(&by));
+                pairs[i] = *reinterpret_cast<const uint32_t *>(&r);
+            }
+        } else if (byte >= 113 && byte <= 142) {
+            // (2^-14 to 2^15 are fp16's normal powers of two)
+            const uint32_t one = (byte - 112) << 10, by = one | one << 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&pairs[i]), *reinterpret_cast<const __half2 *>(&by));
+                pairs[i] = *reinterpret_cast<const uint32_t *>(&r);
+            }
+        } else {
+            const float by = scale_value(byte);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&pairs[i]));
+                const __half2 r = __floats2half2_rn(__fmul_rn(v.x, by), __fmul_rn(v.y, by));
+                pairs[i] = *reinterpret_cast<const uint32_t *>(&r);
+            }
+        }
+        return make_uint4(pairs[0], pairs[1], pairs[2], pairs[3]);
     }
-    return Vec16<T>::put(v);
 }
 // Such a lane's codes to `to`, kN / 2 bytes
 template <int kN>

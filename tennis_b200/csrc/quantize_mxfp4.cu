@@ -98,37 +98,66 @@ quantize_rows_mxfp4_kernel(const T *x, int64_t x_pitch, uint8_t *q, int64_t q_pi
     }
 }
 
-// Rows of few tiles: a 16-byte vector a lane and turn.
+// Rows of few tiles: a group a lane, which reads 64 (fp32: 128) bytes of it; four lanes a tile, one row behind the other.  (With a group among lanes, as above, and where it lies
+// worked out for every 16 bytes, 200000 x 64 bf16 took 24 us, so 7.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-quantize_rows_mxfp4_narrow_kernel(const T *x, int64_t x_pitch, uint8_t *q, int64_t q_pitch, uint8_t *scales, int64_t rows, int64_t room_rows, int64_t cols, int tiles, uint32_t inverse,
-                           int x_aligned, int q_aligned, int s_aligned) {
-    constexpr int kN = Vec16<T>::kN;
-    using W = Tiles<kN>;
+quantize_rows_mxfp4_narrow_kernel(const T *x, int64_t x_pitch, uint8_t *q, int64_t q_pitch, uint8_t *scales, int64_t rows, int64_t room_rows, int cols, int tiles, uint32_t inverse,
+                                  int x_aligned, int q_aligned, int s_aligned) {
+    constexpr int kN = Vec16<T>::kN, kVectors = mx::kGroup / kN;
     pdl_sync();
-    const int in = (threadIdx.x & 31) % W::kLanes;
-    const int64_t used = (cols + mx::kGroup - 1) / mx::kGroup * mx::kGroup;      // values of a row with those that fill up its last group
-    const W walk(tiles, inverse);
-    uint4 held[W::kTurns];
+    const uint32_t u = blockIdx.x * kThreads + threadIdx.x, groups = 4 * (uint32_t)tiles;
+    uint32_t row = __umulhi(u, inverse);                     // the quotient or one less (inverse: 2^32 / groups, rounded down)
+    if (u - row * groups >= groups) ++row;
+    const int64_t r = row;
+    const int c = (int)(u - row * groups) * mx::kGroup;
+    const bool live = r < rows && c < cols;
+    uint4 held[kVectors];
+    const T *from = x + r * x_pitch + c;
+    if (live && x_aligned && c + mx::kGroup <= cols) {
 #pragma unroll
-    for (int i = 0; i < W::kTurns; ++i) {
-        int64_t r;
-        int t;
-        walk.at(i, r, t);
-        held[i] = make_uint4(0, 0, 0, 0);
-        if (r < rows && t < tiles) held[i] = mx::load_values(x + r * x_pitch, (int64_t)t * 128 + in * kN, cols, x_aligned);
-    }
+        for (int i = 0; i < kVectors; ++i) held[i] = reinterpret_cast<const uint4 *>(from)[i];
+    } else {
 #pragma unroll
-    for (int i = 0; i < W::kTurns; ++i) {
-        int64_t r;
-        int t;
-        walk.at(i, r, t);
-        uint32_t word;
-        const uint32_t codes = mx::quantize_vector<T>(held[i], &word);
-        const int64_t c = (int64_t)t * 128 + in * kN;
-        if (r < rows && c < used) mx::store_codes<kN>(q + r * q_pitch + c / 2, codes, q_aligned);
-        if (r < room_rows && t < tiles && in == 0) mx::store_scales(scales + mx::word_at(r, t, tiles), word, s_aligned);
+        for (int i = 0; i < kVectors; ++i) {
+            held[i] = make_uint4(0, 0, 0, 0);
+            if (live) held[i] = mx::load_values(from, i * kN, cols - c, x_aligned);
+        }
     }
+    Largest<T> largest;
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) largest.add(held[i]);
+    const uint32_t byte = mx::scale_byte(largest.bits());
+    uint32_t word = byte << (8 * (threadIdx.x % 4));
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    if (live) {
+        const float by = mx::inverse_scale(byte);
+        float v[mx::kGroup];
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            float some[kN];
+            Vec16<T>::get(held[i], some);
+#pragma unroll
+            for (int j = 0; j < kN; j += 2) {
+                const float2 t = mul2(make_float2(some[j], some[j + 1]), make_float2(by, by));
+                v[i * kN + j] = t.x;
+                v[i * kN + j + 1] = t.y;
+            }
+        }
+        uint32_t codes[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float some[8] = {v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3], v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]};
+            codes[i] = mx::codes8(some);
+        }
+        uint8_t *to = q + r * q_pitch + c / 2;
+        if (q_aligned) *reinterpret_cast<uint4 *>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx::store_codes<8>(to + 4 * i, codes[i], false);
+    }
+    if (threadIdx.x % 4 == 0 && r < room_rows) mx::store_scales(scales + mx::word_at(r, c / 128, tiles), word, s_aligned);
 }
 
 // Runs of other rows' values to y: 16 bytes of y a lane and turn.  `whole`: rows of codes start on their lanes' bytes and rows of y on 16 bytes.
@@ -231,9 +260,10 @@ int launch_quantize(const void *x, int64_t x_pitch, uint8_t *q, int64_t q_pitch,
     const auto address = reinterpret_cast<uintptr_t>(x);
     const int x_aligned = aligned16(x, x_pitch, sizeof(T) == 4 ? TSB_TYPE_F32 : TSB_TYPE_F16);
     const int q_aligned = reinterpret_cast<uintptr_t>(q) % 4 == 0 && q_pitch % 4 == 0, s_aligned = reinterpret_cast<uintptr_t>(scales) % 4 == 0;
-    if (W::narrow(room_rows, tiles)) {
-        TSB_CUDA(launch_pdl(quantize_rows_mxfp4_narrow_kernel<T>, dim3((int)W::blocks(room_rows, tiles)), dim3(kThreads), 0, stream, static_cast<const T *>(x), x_pitch, q, q_pitch, scales, rows,
-                            room_rows, cols, (int)tiles, W::inverse_of(tiles), x_aligned, q_aligned, s_aligned));
+    if (W::narrow(4 * room_rows, tiles)) {
+        const int q_wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_pitch % 16 == 0;
+        TSB_CUDA(launch_pdl(quantize_rows_mxfp4_narrow_kernel<T>, dim3((int)ceil_div64(4 * room_rows * tiles, kThreads)), dim3(kThreads), 0, stream, static_cast<const T *>(x), x_pitch, q, q_pitch,
+                            scales, rows, room_rows, (int)cols, (int)tiles, W::inverse_of(4 * tiles), x_aligned, q_wide, s_aligned));
         TSB_LAUNCHED("quantize_rows_mxfp4_narrow_kernel");
         return TSB_OK;
     }

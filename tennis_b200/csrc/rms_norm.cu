@@ -82,20 +82,24 @@ __device__ __forceinline__ double squares(const uint4 &h, double s) {
     return s;
 }
 
-// The sum over the row's threads: of a warp, or of the block by way of `part`
+// The reciprocal deviation from the squares' sums of the row's threads: of a warp, or of the block by way of `part` and `result`, where one warp alone takes
+// the root and divides (in 64 bits these are some hundred instructions: done by all, a fifth of the kernel's).
 template <bool WARP>
-__device__ __forceinline__ double row_sum(double s, double *part) {
+__device__ __forceinline__ float reciprocal_deviation(double s, const NormParams &p, double *part, float *result) {
 #pragma unroll
     for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if constexpr (!WARP) {
-        const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-        if (lane == 0) part[threadIdx.x >> 5] = s;
-        __syncthreads();
+    if constexpr (WARP) return (float)(1.0 / sqrt(s / (double)p.cols + p.eps));
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
         s = lane < warps ? part[lane] : 0.0;
 #pragma unroll
         for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (lane == 0) *result = (float)(1.0 / sqrt(s / (double)p.cols + p.eps));
     }
-    return s;
+    __syncthreads();
+    return *result;
 }
 template <bool WARP>
 __device__ __forceinline__ uint32_t row_max(uint32_t most, uint32_t *part) {
@@ -117,6 +121,7 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
     constexpr int kN = Vec16<T>::kN;
     __shared__ double sums[kMost / 32];
     __shared__ uint32_t maxima[kMost / 32];
+    __shared__ float deviation;
     pdl_sync();
     const int warps = blockDim.x >> 5, at = WARP ? threadIdx.x & 31 : threadIdx.x, step = WARP ? 32 : blockDim.x;
     // (4 bits: whole tiles of scales, so that all lanes of a warp that has any of a row take part)
@@ -167,8 +172,7 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
                 s = squares<T>(h, s);
             }
         }
-        s = row_sum<WARP>(s, sums);
-        const float by = (float)(1.0 / sqrt(s / (double)p.cols + p.eps));
+        const float by = reciprocal_deviation<WARP>(s, p, sums, &deviation);
         auto normed = [&](const uint4 &h, int u, float (&v)[kN]) {
             float g[kN];
             load_gamma<WHOLE>(p, u, g);
@@ -197,26 +201,28 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             if constexpr (V > 0) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
-                    if (decltype(all)::value ? i < turns : at + i * step < vectors) body(at + i * step, held[i]);
+                    if (decltype(all)::value ? i < turns : at + i * step < vectors) body(i, at + i * step, held[i]);
             } else {
                 for (int i = 0; i < turns; ++i) {
                     const int u = at + i * step;
-                    if (decltype(all)::value || u < vectors) body(u, u < vectors ? again(u) : make_uint4(0, 0, 0, 0));
+                    if (decltype(all)::value || u < vectors) body(0, u, u < vectors ? again(u) : make_uint4(0, 0, 0, 0));
                 }
             }
         };
         using Live = std::false_type;
         using All = std::true_type;
         if constexpr (OUT == kSame) {
-            each(Live(), [&](int u, const uint4 &h) {
+            each(Live(), [&](int, int u, const uint4 &h) {
                 float v[kN];
                 normed(h, u, v);
                 store_vector<WHOLE>(static_cast<T *>(p.y) + r * p.y_pitch, u, p.cols, Vec16<T>::put(v), p.y_aligned);
             });
         } else if constexpr (OUT == kInt8) {
-            float most = 0.0f;
-            each(Live(), [&](int u, const uint4 &h) {
-                float v[kN];
+            // (up to sixteen values are kept between the maximum and the rounding, so that gamma is read once; 32 of a thread's 64 registers would be too many)
+            constexpr bool kKeep = V > 0 && V * kN <= 16;
+            float most = 0.0f, kept[kKeep ? V : 1][kN];
+            each(Live(), [&](int i, int u, const uint4 &h) {
+                float (&v)[kN] = kept[kKeep ? i : 0];
                 normed(h, u, v);
                 clear_behind(u, v);
                 most = largest(v, most);
@@ -224,16 +230,11 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             const RowScale scale(row_max<WARP>(__float_as_uint(most), maxima));
             if (at == 0) static_cast<float *>(p.scales)[r] = scale.scale;
             int8_t *yr = static_cast<int8_t *>(p.y) + r * p.y_pitch;
-            each(Live(), [&](int u, const uint4 &h) {
-                float v[kN];
-                normed(h, u, v);
+            each(Live(), [&](int i, int u, const uint4 &h) {
+                float (&v)[kN] = kept[kKeep ? i : 0];
+                if (!kKeep) normed(h, u, v);
                 uint32_t w[kN / 4];
-#pragma unroll
-                for (int q = 0; q < kN; q += 4) {
-                    uint4 some;
-                    some.x = __float_as_uint(v[q]); some.y = __float_as_uint(v[q + 1]); some.z = __float_as_uint(v[q + 2]); some.w = __float_as_uint(v[q + 3]);
-                    quantize16<float>(scale, some, &w[q / 4]);
-                }
+                quantize_values(scale, v, w);
                 int8_t *to = yr + u * kN;
                 if (WHOLE || (p.y_aligned && u * kN + kN <= p.cols)) {
                     if constexpr (kN == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
@@ -248,7 +249,7 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             const int used = (p.cols + mx::kGroup - 1) / mx::kGroup * mx::kGroup;
             uint8_t *yr = static_cast<uint8_t *>(p.y) + r * p.y_pitch, *scales = static_cast<uint8_t *>(p.scales) + mx::word_at(r, 0, p.tiles);
             constexpr int kLanes = 128 / kN;      // of a tile of scales
-            each(All(), [&](int u, const uint4 &h) {
+            each(All(), [&](int, int u, const uint4 &h) {
                 float v[kN];
                 normed(h, u, v);
                 if (u >= vectors)
