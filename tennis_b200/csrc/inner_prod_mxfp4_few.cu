@@ -341,7 +341,9 @@ int launch(const Params &p, int64_t x_pitch, int cols, int early, cudaStream_t s
     }
     const int ctas = ceil_div(p.n, kBM) * CL, blocks = ceil_div(t.kblocks, CL);
     const int room = (int)(ctas <= 148 ? kSmem : kSmem / 2 - 1024) - (int)S::fixed(blocks);
+    // (two stages or more: a cluster's CTA so takes 46 KB or more, four a multiprocessor fit its tensor memory, and none waits for columns that one of another cluster holds)
     t.stages = std::max(2, std::min({blocks, S::kMost + 0, room / (int)S::kStage}));
+    static_assert(CL == 1 || 1024 + S::kBars + S::kParts + (S::kQuantize ? S::kTokens : 0) + 2 * S::kStage > 46 * 1024, "four CTAs a multiprocessor at most");
     TSB_CUDA(launch_pdl_cluster(CL, kernel, dim3(ctas), dim3(S::kThreads), S::fixed(blocks) + t.stages * S::kStage, stream, mw, mws, mx, mxs, t));
     TSB_LAUNCHED("inner_prod_mxfp4_few_kernel");
     return TSB_OK;

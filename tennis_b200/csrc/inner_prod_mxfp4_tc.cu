@@ -502,9 +502,14 @@ int launch(const Params &p, cudaStream_t stream) {
     const int one = clusters == tiles_all;
     // Of few output channels, tiles of the same tokens follow each other: on a grid that is a multiple of them a CTA stays with its channels.
     if (!one && !PAIR && t.group_m == 1) clusters -= clusters % t.tiles_n;
-    // No more stages than a CTA has blocks of K: what fits beside another kernel's CTAs starts while those run.
+    // No more stages than a CTA has blocks of K: what fits beside another kernel's CTAs starts while those run.  CTAs of a cluster hold tensor memory while they wait for each
+    // other, so what fits a multiprocessor by its shared memory has to fit by its tensor memory too: a pair, which needs all of that, takes the shared memory as well, and
+    // splits (119 KB for 256 columns, 61 KB for 128) and clusters of few tokens (47 KB or more for 128) never come to more than 512 columns.
     const int64_t loads = ceil_div64(tiles_all, clusters) * (SPLIT > 1 ? ceil_div(t.kblocks, SPLIT) : t.kblocks);
-    int stages = (int)std::min<int64_t>(L::kStages, loads);
+    int stages = PAIR ? L::kStages : (int)std::min<int64_t>(L::kStages, loads);
+    static_assert(!PAIR || L::kFixed + L::kStages * L::kStage > 180 * 1024, "nothing that waits for a cluster fits beside a pair's CTA");
+    static_assert(SPLIT != 4 || L::kFixed + L::kStage > 76 * 1024, "two splits of 256 columns a multiprocessor at most");
+    static_assert(SPLIT != 2 || L::kFixed + L::kStage > 46 * 1024, "four splits of 128 columns a multiprocessor at most");
     const int keep = !PAIR && SPLIT == 1 && !one && t.group_m == 1 && t.kblocks <= stages;
     if (keep) stages -= stages % t.kblocks;
     TSB_CUDA(launch_pdl_cluster(kCluster, kernel, dim3(kCluster * clusters), dim3(L::kThreads), L::kFixed + stages * L::kStage, stream, mx, mw, mxs, mws, my, t, stages, one, keep,

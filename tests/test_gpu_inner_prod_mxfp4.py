@@ -292,3 +292,64 @@ def test_refusals():
     for kw, text in ((dict(activation=5), "activation 5"), (dict(activation=-1), "activation -1"), (dict(kernel=9), "kernel 9")):
         with pytest.raises(_lib.TsbError, match=text):
             ops.inner_prod_mxfp4(x, xs, w, ws, **kw)
+
+
+FIRST = """
+import sys, torch
+sys.path.insert(0, %r)
+from tennis_b200 import ops
+dev = torch.device("cuda")
+w, ws = torch.zeros((512, 64), dtype=torch.uint8, device=dev), torch.zeros((4, 1, 32, 4, 4), dtype=torch.uint8, device=dev)
+w.fill_(0x22), ws.fill_(127)
+x, gamma = torch.full((%d, 128), 2.0, device=dev, dtype=torch.bfloat16), torch.ones(128, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s, h = ops.rms_norm(x, gamma, x, 0.0, torch.float4_e2m1fn_x2)
+    y = ops.inner_prod_mxfp4(q, s, w, ws)
+    z = ops.inner_prod_mxfp4(x, None, w, ws)
+    v = ops.dequantize_rows_mxfp4(*ops.quantize_rows_mxfp4(x))
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 128.0).all() and (z == 256.0).all() and (v == 2.0).all() and (h == 4.0).all()
+ops.inner_prod_mxfp4_status()
+"""
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_first_calls_of_a_process_may_be_captured(m):
+    import subprocess
+    import sys
+    from conftest import ROOT
+    done = subprocess.run([sys.executable, "-c", FIRST % (ROOT, m)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout[-2000:]
+
+
+def test_kernels_beside_each_other():
+    """Calls of every kernel on four streams at once: they share multiprocessors, and their tensor memory."""
+    from tennis_b200 import ops
+    sizes = [(2048, 2048, 512), (16, 4096, 1024), (128, 4096, 1024), (100, 512, 2048), (1, 1000, 4096), (600, 600, 600), (40, 300, 300), (4096, 512, 256)]
+    cases = [case(m, n, k, torch.bfloat16, i) for i, (m, n, k) in enumerate(sizes)]
+    want = [call(d, out_dtype=torch.bfloat16) for d in cases]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for round in range(10):
+        got = []
+        for side in streams:
+            side.wait_stream(torch.cuda.current_stream())
+        for i, d in enumerate(cases * 2):
+            got.append(call(cases[(i * 3 + round) % len(cases)], out_dtype=torch.bfloat16, stream=streams[i % 4]))
+        for side in streams:
+            torch.cuda.current_stream().wait_stream(side)
+        for i, y in enumerate(got):
+            assert torch.equal(y, want[(i * 3 + round) % len(cases)])
+    ops.inner_prod_mxfp4_status()
+
+
+def test_a_timed_out_wait_is_reported_once_and_named():
+    """No kernel is made to time out: the code that a timed-out wait would leave is looked up on the host (the library decodes it), and a healthy device has none."""
+    from tennis_b200 import _lib, ops
+    call(case(300, 300, 300, torch.float32))
+    ops.inner_prod_mxfp4_status()
+    ops.inner_prod_mxfp4_status(torch.device("cuda"), torch.cuda.current_stream())
+    with pytest.raises(_lib.TsbError, match="a stage to be loaded"):
+        _lib.check(_lib.load().tsb_inner_prod_mxfp4_status_decode(2))
