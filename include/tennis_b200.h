@@ -352,7 +352,7 @@ TSB_API int tsb_concat_i8_nhwc(const int8_t *a, int channels_a, const int8_t *b,
                                void *stream);
 
 /*
- * quantize with a scale for each row, taken from the row (this and the next two operators have no counterpart in the
+ * quantize with a scale for each row, taken from the row (this and the operators below have no counterpart in the
  * reference, whose quantize scales are attributes; they are what int8 networks of matrix products and group norms need
  * next to its convolutions).
  *   a = max_c |x[r][c]|;  y[r][c] = half_even(x[r][c] * fp32(127 / a));  scales[r] = fp32(a / 127)
@@ -478,7 +478,7 @@ TSB_API int tsb_dequantize_rows_mxfp4(const void *q, int64_t q_pitch, const void
  *     values, the call or the rows of other tiles: the same call gives the same bits.  Steps behind the sum as in tsb_inner_prod_i8.
  *   - x: 4-bit rows with x_scales, or floating rows without: those are quantized as tsb_quantize_rows_mxfp4 does it.
  *   - w, w_scales: n rows of k values, as tsb_quantize_rows_mxfp4 lays out a weight tensor.  Rows are read to the end of their last
- *     group, where zeros lie behind the k values.
+ *     group, where zeros lie behind the k values; scales to the end of their tiles, where places without a group hold zero.
  *   - Any pitch and alignment is right; 4-bit operands at multiples of 16 bytes run on the tensor cores.
  *   - y does not overlap the other tensors, but may be the residual itself (same address and pitch).
  *   - m = 0 or n = 0: nothing is done.
