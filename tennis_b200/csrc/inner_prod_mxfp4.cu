@@ -122,7 +122,7 @@ int run(const InnerProdMxfp4Params &p, int y_type, int kernel, int early, cudaSt
     const char *why = "";
     const bool tc_can = tc::inner_prod_can(p, &why);
     if (kernel == TSB_KERNEL_TCGEN05 && !tc_can) return fail(TSB_ERR_UNSUPPORTED, "inner_prod_mxfp4: no tensor-core kernel: %s", why);
-    if (kernel == TSB_KERNEL_AUTO && tc_can && p.m <= few::kMaxMxfp4Tokens) return few::inner_prod(p, y_type, early, stream);
+    if (kernel == TSB_KERNEL_AUTO && tc_can && few::takes(p)) return few::inner_prod(p, y_type, early, stream);
     if (kernel != TSB_KERNEL_DIRECT && tc_can) return tc::inner_prod(p, y_type, stream);
     switch (y_type) {
         case TSB_TYPE_F32: return launch_direct<float>(p, stream);

@@ -21,6 +21,46 @@ struct InnerProdMxfp4Params {
 };
 
 #ifdef __CUDACC__
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// gelu of values that become results of 16 bits: v / 2 + |v| / 2 - |v| / 2 erfc(|v| / sqrt(2)), with erfc by Abramowitz and Stegun's formula 7.1.26, P(t) exp(-x^2) of t = 1 / (1 + 0.3275911 x) and a
+// polynomial of degree five, which is off by 1.5e-7 at most: |v| 2^-23.7 of a value whose half step is 2^-12 of itself or more.  (erff and the rest are some 60 instructions a value,
+// these 12: 333 x 777 x 1021 with a residual 6.1 -> 5.5 us.)
+__device__ __forceinline__ float2 gelu_short(float2 v) {
+    const float2 a = make_float2(fminf(fabsf(v.x), 16.0f), fminf(fabsf(v.y), 16.0f));      // (erfc is 0 there; an infinity's would be infinity times 0)
+    const float2 d = fma2(a, both(0.23164190f), both(1.0f));                                // 0.3275911 / sqrt(2)
+    const float2 t = make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
+    const float2 q = mul2(mul2(a, both(-0.72134752f)), a);                                  // -log2(e) / 2
+    const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+    float2 p = fma2(both(1.061405429f), t, both(-1.453152027f));
+    p = fma2(p, t, both(1.421413741f));
+    p = fma2(p, t, both(-0.284496736f));
+    p = fma2(p, t, both(0.254829592f));
+    const float2 tail = mul2(mul2(mul2(p, t), e), mul2(a, both(-0.5f)));
+    // (a NaN is one here, whatever the minimum above made of it, and minus infinity becomes one)
+    const float2 rising = fma2(make_float2(fabsf(v.x), fabsf(v.y)), both(0.5f), mul2(v, both(0.5f)));
+    return add2(rising, tail);
+}
+// The activation as activate() takes it, gelu of 16-bit results as above.
+template <int ACT, typename T, int N>
+__device__ __forceinline__ void activate_sums(float (&v)[N], float leaky) {
+    if constexpr (ACT == TSB_ACT_GELU && sizeof(T) == 2 && N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 y = gelu_short(make_float2(v[i], v[i + 1]));
+            v[i] = y.x;
+            v[i + 1] = y.y;
+        }
+    } else {
+        activate<ACT, T>(v, leaky);
+    }
+}
+
 // N sums: + bias (a missing one is 0), + residual, activation (+ residual); every step is rounded by itself.
 // bias(i), res(i): value i's.  RES: false where there is certainly no residual.
 template <typename T, bool RES = true, int N, typename Bias, typename Res>
@@ -33,7 +73,7 @@ __device__ __forceinline__ void finish_values(const InnerProdMxfp4Params &p, con
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
     }
-    by_activation(p.activation, [&](auto act) { activate<decltype(act)::value, T>(v, p.leaky); });
+    by_activation(p.activation, [&](auto act) { activate_sums<decltype(act)::value, T>(v, p.leaky); });
     if (RES && p.residual && p.residual_after) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __fadd_rn(v[i], res(i));
@@ -53,7 +93,9 @@ int inner_prod_mxfp4_status_decode(int word);
 
 // inner_prod_mxfp4_few.cu: the kernel of few tokens
 namespace few {
-constexpr int kMaxMxfp4Tokens = 64;
+// Whether it is the sooner one: up to 32 tokens, and up to 64 of more than 1024 values each (64 tokens, by it and by tiles: 300 x 300 3.7 and 3.2 us, 8000 x 300 4.3 and 3.8,
+// 2000 x 4000 4.7 and 5.1, 300 x 8192 5.1 and 7.9; 32 tokens 2.7 and 3.1, 3.2 and 3.8, 3.8 and 5.3, 4.3 and 7.8).
+inline bool takes(const InnerProdMxfp4Params &p) { return p.m <= 32 || (p.m <= 64 && p.groups > 32); }
 int inner_prod(const InnerProdMxfp4Params &p, int y_type, int early, cudaStream_t stream);       // early: weights may be read before the kernel in front is done
 bool can_quantize(const InnerProdMxfp4Params &p, int x_type, int y_type);                        // whether the next one takes these floating rows
 int inner_prod_quantize(const InnerProdMxfp4Params &p, int y_type, int64_t x_pitch, int cols, cudaStream_t stream);

@@ -7,8 +7,8 @@
 //   loads      weights and their scales through a ring of TMA boxes, 256 values of K of 128 rows each
 //   tokens     4-bit rows, by TMA through the same ring; or floating rows, which the CTA quantizes into shared memory, its part of K alone, while
 //              its weights are on their way
-//   roles      warp 0 loads, warp 1 multiplies, warps 2 to 5 finish (a lane has a channel of all tokens, so rows of y are written 32 channels at a
-//              time); warps 2 to 9 quantize
+//   roles      warp 0 loads, warp 1 multiplies, warps 2 to 5 (of more than 16 tokens 2 to 9) finish: a lane has a channel of all tokens, so rows of y are
+//              written 32 channels at a time; warps 2 to 9 quantize
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and all roles go to the common exit.
 #include "inner_prod_mxfp4.h"
@@ -35,7 +35,8 @@ struct Shape {
     static constexpr uint32_t kScalesAt = kABytes, kTokensAt = kABytes + kScales;     // within a stage
     static constexpr uint32_t kStage = kTokensAt + (kQuantize ? 0 : kTokens);
     static constexpr int kMost = 10;                                                  // stages
-    static constexpr int kThreads = 32 * (2 + (kQuantize ? kQuantizers : 4));
+    static constexpr int kFinishers = NT > 16 ? 8 : 4;                                // warps; eight: two a quarter of the channels, which take turns
+    static constexpr int kThreads = 32 * (2 + (kQuantize && kQuantizers > kFinishers ? kQuantizers : kFinishers));
     static constexpr int kMine = NT / CL;                                             // tokens that a CTA finishes
     static constexpr uint32_t kParts = CL > 1 ? NT * kBM * 4 : 0;                     // all CTAs' sums of those
     static constexpr uint32_t kBars = 256;
@@ -141,7 +142,8 @@ inner_prod_mxfp4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int c = tile * kBM + (warp & 3) * 32 + lane;       // a finishing lane's channel
-    const bool finishes = warp >= 2 && warp < 6;
+    const bool finishes = warp >= 2 && warp < 2 + S::kFinishers;
+    const int turn = (warp - 2) / 4 % 2, turns = S::kFinishers / 4;
     auto give_up = [&](int code) {
         if (!*abort_flag) { *abort_flag = 1; atomicExch(t.status, code); }
     };
@@ -243,6 +245,7 @@ done:
 #pragma unroll
                 for (int m0 = 0; m0 < NT; m0 += 16) {
                     if (m0 >= m) break;
+                    if (turns == 2 && m0 / 16 % 2 != turn) continue;
                     int part[16];
                     tmem_ld16(lanes + m0, part);
                     tmem_ld_wait();
@@ -264,6 +267,7 @@ done:
 #pragma unroll
                 for (int m0 = 0; m0 < NT; m0 += 16) {
                     if (m0 >= m) break;
+                    if (turns == 2 && m0 / 16 % 2 != turn) continue;
                     int part[16];
                     tmem_ld16(lanes + m0, part);
                     tmem_ld_wait();
@@ -280,6 +284,7 @@ done:
                 for (int i = 0; i < S::kMine; i += 4) {
                     const int m0 = rank * S::kMine + i;
                     if (m0 >= m) break;
+                    if (turns == 2 && i / 4 % 2 != turn) continue;
                     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int r = 0; r < CL; ++r) {

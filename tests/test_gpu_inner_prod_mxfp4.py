@@ -71,6 +71,40 @@ def test_activations(m, n, k, act, leaky):
             check(call(d, activation=act, leaky=leaky, out_dtype=out, residual_after_activation=after), d, act, leaky, after)
 
 
+@pytest.mark.parametrize("m", [1, 12, 40, 150, 400])
+@pytest.mark.parametrize("act", [1, 3, 4])
+def test_activations_of_the_largest_values(m, act):
+    """Values to the ends of fp32, infinities and NaN, side by side: what is far below zero becomes zero (an infinity NaN, 0 times it, as
+    the formulas say), and none changes its neighbour.  Sums of zero leave the bias itself."""
+    from tennis_b200 import ops
+    ends = [-1e4, 3.0, -1e30, -3.3e38, -44.0, -43.0, float("nan"), -1.0, -float("inf"), -2.0, float("inf"), -90.0, 3.3e38, -200.0, 1e-30, -3.3e38]
+    for n in (16, 200):
+        bias = torch.tensor((ends * 13)[:n], device="cuda")
+        v = bias.double().cpu()
+        want = v.clamp(min=0.0).nan_to_num(nan=0.0, posinf=float("inf")) if act == 1 else v / (1.0 + torch.exp(-v)) if act == 3 else 0.5 * v * (1.0 + torch.erf(v * 0.5 ** 0.5))
+        for out in FLOATS:
+            d = case(m, n, 48, out, 3)
+            got = ops.inner_prod_mxfp4(torch.zeros_like(d["x"].view(torch.uint8)), d["xs"], d["w"], d["ws"], bias, activation=act, out_dtype=out).cpu()
+            # fp32: silu by 8 half steps of its value, gelu by 24 of 1; one rounding to 16 bits; 10^-17 as plain.activation's quotient
+            torch.testing.assert_close(got.double(), want.to(out).double().expand(m, n), rtol=2 * torch.finfo(out).eps + 8 * plain.EPS32,
+                                       atol=24 * plain.EPS32 if act == 4 else 1e-17, equal_nan=True)
+
+
+@pytest.mark.parametrize("out", FLOATS, ids=str)
+def test_gelu_between(out):
+    """gelu from -7 to 7: within |v| 2^-22 (the formula of 16-bit results is off by 1.5e-7 |v| / 2, its fp32 steps by some 2^-23 |v|; erff's form by as much) and one rounding."""
+    from tennis_b200 import ops
+    n = 4096
+    bias = torch.linspace(-7.0, 7.0, n, device="cuda")
+    v = bias.double().cpu()
+    want = 0.5 * v * torch.erfc(-v * 0.5 ** 0.5)
+    for m in (1, 40, 300):
+        d = case(m, n, 48, out, 3)
+        got = ops.inner_prod_mxfp4(torch.zeros_like(d["x"].view(torch.uint8)), d["xs"], d["w"], d["ws"], bias, activation=4, out_dtype=out).cpu().double()
+        room = v.abs() * 2.0 ** -22 + (0.0 if out == torch.float32 else want.abs() * torch.finfo(out).eps / 2 + (2.0 ** -25 if out == torch.float16 else 0.0))
+        assert ((got - want).abs() <= room).all()
+
+
 @pytest.mark.parametrize("m", [1, 6, 30, 60, 140, 700])
 def test_kernels_agree(m):
     """Exact sums: the kernels have the same bits, whatever rows are computed with a row."""
