@@ -8,7 +8,8 @@ namespace tsb {
 namespace {
 
 // ---- CUDA-core kernel: any alignment, any pitch -----------------------------------------------------------------------
-// A block computes 64 tokens x 64 output channels, 16 values a thread (4 x 4), two groups of K at a time as fp32 values in shared memory.
+// A block computes 64 tokens x 64 output channels, 16 values a thread (4 x 4), two groups of K at a time as fp32 values in shared memory.  Bound by fused multiply-adds and
+// the shared-memory reads that feed them (8192^3 42.8 ms): for operands that the copies of the other kernels cannot read.
 constexpr int kTile = 64, kTileK = 64, kThreads = 256;
 constexpr int kRow = kTileK + 1;         // words of a staged row; odd, so that neighbouring rows lie in different banks
 

@@ -12,6 +12,10 @@
 //              distributed shared memory and writes its own 32; the parts are added in a fixed order
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of token tiles, whose operands the L2 then serves
 //
+// Measured, bf16 out: 8192^3 182 us (6.0 PFLOP/s; for seconds, at the power limit, 225), 4096^3 28.8 us (with a residual 38.5), 2048 x 4096 x 4096 16.4 us, 128 x 4096 x 4096
+// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 15.6 us, where stores bound it (silu: 20.3, where the special-function unit does).  Of 8192^3 loads and shared memory alone take
+// 132 us, the scales' copies nothing.
+//
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and all roles go to the common exit.
 #include "inner_prod_mxfp4.h"
 #include "inner_prod_tiles.cuh"

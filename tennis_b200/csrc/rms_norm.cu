@@ -2,7 +2,10 @@
 //
 // Bound by memory: a row is read once (two tensors of it with a residual), held in registers as the sums' own type while the squares are added up, and written
 // with its sum.  Squares are added in 64 bits, so that the mean does not depend on how a row is shared out (but in the 50th bit), and with it neither do
-// the 8- or 4-bit values behind it.  A row belongs to a warp, which needs no barrier, or to a block of as many warps as it needs.
+// the 8- or 4-bit values behind it.  A row belongs to a warp, which needs no barrier, or to a block of as many warps as it needs: of many rows, threads with four
+// vectors each (loads in flight), of few, more threads with one (a short way from load to store).
+// Measured, bf16 rows of 16384 x 8192: 92 us (5.8 TB/s), with a residual 158 (6.8), to int8 147 (6.4), to 4 bits 136 (6.5), without a residual to int8 113 (3.6: instructions, two
+// passes over gamma); 2048 x 4096 with a residual to 4 bits 12.6 us; 1 x 4096 2.5 us.
 #include "mxfp4.cuh"
 
 #include <algorithm>
