@@ -42,10 +42,10 @@ struct Shape {
     static constexpr int kThreads = 32 * (2 + (kQuantize && kQuantizers > kFinishers ? kQuantizers : kFinishers));
     static constexpr int kMine = NT / CL;                                             // tokens that a CTA finishes
     static constexpr uint32_t kParts = CL > 1 ? NT * kBM * 4 : 0;                     // all CTAs' sums of those
-    static constexpr uint32_t kBars = 256;
+    static constexpr uint32_t kBars = 1024;                                           // (what follows lies on 1024 bytes)
     // columns of tensor memory: sums, weights' scales, tokens' scales
     static constexpr uint32_t kScaleColumns = 64, kColumns = 128;
-    static uint32_t fixed(int blocks) { return 1024 + kBars + kParts + (kQuantize ? blocks * kTokens : 0); }      // bytes beside the ring
+    static uint32_t fixed(int blocks) { return 1024 + kBars + kParts + (kQuantize ? blocks * kTokens : 0); }      // bytes beside the ring, and what its alignment takes
 };
 
 struct FewParams {
@@ -111,7 +111,7 @@ inner_prod_mxfp4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     using S = Shape<X, NT, CL>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t *const bars = smem_raw + (base - smem_u32(smem_raw)), *const parts = bars + 1024, *const ring = parts + S::kParts;
+    uint8_t *const bars = smem_raw + (base - smem_u32(smem_raw)), *const parts = bars + S::kBars, *const ring = parts + S::kParts;
     uint8_t *const tokens = ring + t.stages * S::kStage;
     const uint32_t bar_full = smem_u32(bars), bar_empty = bar_full + 8 * S::kMost, bar_sums = bar_empty + 8 * S::kMost, bar_tokens = bar_sums + 8;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + 8 * (2 * S::kMost + 2));
@@ -131,6 +131,10 @@ inner_prod_mxfp4_few_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             *abort_flag = 0;
             prefetch_tensormap(&map_w);
             prefetch_tensormap(&map_ws);
+            if (!S::kQuantize) {
+                prefetch_tensormap(&map_x);
+                prefetch_tensormap(&map_xs);
+            }
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
@@ -357,7 +361,8 @@ int launch(const Params &p, int64_t x_pitch, int cols, int early, cudaStream_t s
     return TSB_OK;
 }
 
-// CTAs that share a tile: as many as one on every multiprocessor leave, and no more than there are blocks of K.
+// CTAs that share a tile: as many as two on every multiprocessor leave, and no more than there are blocks of K.  (32 tokens through 8192 x 8192, by one, two and four CTAs a
+// tile 11.4, 9.3 and 9.2 us; one token through 4096 x 4096 6.8, 5.2 and 4.4, through 16384 x 8192 16.5, 14.6 and 16.2.)
 int cluster_of(const Params &p) {
     const int tiles = ceil_div(p.n, kBM), kblocks = ceil_div(p.groups * (mx::kGroup / 2), kKBytes);
     int cluster = 1;
@@ -393,7 +398,7 @@ int inner_prod(const Params &p, int y_type, int early, cudaStream_t stream) {
 }
 
 // Rows that the kernel quantizes itself: what a CTA's part takes it is less than a launch of quantize_rows_mxfp4 in front (2.2 us) up to some 16 Ki values (4096 x 4096, by the
-// kernel and by a launch: 1 token 4.4 and 6.5 us, 8 tokens 5.2 and 6.7, 16 tokens 7.0 and 6.9).
+// kernel and by a launch: 1 token 4.1 and 6.5 us, 8 tokens 4.9 and 6.7, 16 tokens 6.2 and 6.9).
 bool can_quantize(const Params &p, int x_type, int y_type) {
     const int64_t blocks = ceil_div(ceil_div(p.groups * (mx::kGroup / 2), kKBytes), cluster_of(p));
     return x_type == y_type && p.m <= 16 && p.m * blocks <= 64 && blocks * (16 * kKBytes + kScales) <= kMaxResident;

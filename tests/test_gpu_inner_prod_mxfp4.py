@@ -387,3 +387,38 @@ def test_a_timed_out_wait_is_reported_once_and_named():
     ops.inner_prod_mxfp4_status(torch.device("cuda"), torch.cuda.current_stream())
     with pytest.raises(_lib.TsbError, match="a stage to be loaded"):
         _lib.check(_lib.load().tsb_inner_prod_mxfp4_status_decode(2))
+
+
+@pytest.mark.parametrize("m,n", [(5, 256), (40, 264), (300, 256), (700, 136)])
+def test_what_lies_around_the_result_stays(m, n):
+    """Rows above and below y, and columns beside it, at widths that copies write whole and at others."""
+    for out in FLOATS:
+        for odd in (0, 1):
+            d = case(m, n - odd, 640, out, m)
+            tall = torch.full((m + 9, n + 16), 7.0, dtype=out, device="cuda")
+            to = tall[3:m + 3, 8:8 + n - odd]
+            assert torch.equal(call(d, out=to), call(d, out_dtype=out))
+            tall[3:m + 3, 8:8 + n - odd] = 7.0
+            assert (tall == 7.0).all()
+
+
+def test_offsets_beyond_32_bits():
+    """A result of more than 2^31 values and operands of more than 2^31 bytes: the rows at the end are those of a call for them alone."""
+    from tennis_b200 import ops
+    d = case(300, 8192, 64, torch.bfloat16, 1, residual=False)
+    m = 270000                                                  # 128 rows' tiles of scales again and again, so a row's lie where they should
+    x = d["x"].view(torch.uint8)[:128].repeat(m // 128 + 1, 1)[:m]
+    xs = d["xs"].view(torch.uint8)[:1].repeat(m // 128 + 1, 1, 1, 1, 1)
+    y = ops.inner_prod_mxfp4(x, xs, d["w"], d["ws"], d["bias"], out_dtype=torch.bfloat16)
+    assert y.numel() > 2 ** 31
+    want = ops.inner_prod_mxfp4(d["x"][:128], d["xs"][:1], d["w"], d["ws"], d["bias"], out_dtype=torch.bfloat16)
+    assert torch.equal(y[:128], want) and torch.equal(y[m - m % 128:], want[:m % 128]) and torch.equal(y[128 * 2000:128 * 2001], want)
+    del y
+    d = case(300, 24, 8192, torch.float32, 2, residual=False)
+    m = 128 * 4200
+    x = d["x"].view(torch.uint8)[:128].repeat(m // 128, 1)
+    xs = d["xs"].view(torch.uint8)[:1].repeat(m // 128, 1, 1, 1, 1)
+    assert x.numel() > 2 ** 31
+    y = ops.inner_prod_mxfp4(x, xs, d["w"], d["ws"], d["bias"])
+    want = ops.inner_prod_mxfp4(d["x"][:128], d["xs"][:1], d["w"], d["ws"], d["bias"])
+    assert torch.equal(y.view(-1, 128, 24), want.expand(m // 128, 128, 24))
