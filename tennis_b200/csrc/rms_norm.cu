@@ -4,8 +4,8 @@
 // with its sum.  Squares are added in 64 bits, so that the mean does not depend on how a row is shared out (but in the 50th bit), and with it neither do
 // the 8- or 4-bit values behind it.  A row belongs to a warp, which needs no barrier, or to a block of as many warps as it needs: of many rows, threads with four
 // vectors each (loads in flight), of few, more threads with one (a short way from load to store).
-// Measured, bf16 rows of 16384 x 8192: 92 us (5.8 TB/s), with a residual 158 (6.8), to int8 147 (6.4), to 4 bits 136 (6.5), without a residual to int8 113 (3.6: instructions, two
-// passes over gamma); 2048 x 4096 with a residual to 4 bits 12.6 us; 1 x 4096 2.5 us.
+// Measured, bf16 rows of 16384 x 8192: 92 us (5.8 TB/s), with a residual 158 (6.8), to int8 143 (6.6; for seconds, at the power limit, 155 to 163), to 4 bits 135 (6.5), without a
+// residual to int8 112 (3.6: instructions, two passes over gamma); 2048 x 4096 with a residual to 4 bits 12.6 us; 1 x 4096 2.5 us.
 #include "mxfp4.cuh"
 
 #include <algorithm>
@@ -34,7 +34,7 @@ struct NormParams {
 template <bool WHOLE, int N>
 __device__ __forceinline__ void load_gamma(const NormParams &p, int u, float (&g)[N]) {
     if (p.gamma && (WHOLE || (p.gamma_aligned && u * N + N <= p.cols))) {
-        const float4 *from = reinterpret_cast<const float4 *>(p.gamma + u * N);
+        const float4 *from = reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(p.gamma) + (uint32_t)u * (N * 4u));
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
             const float4 v = from[i / 4];
@@ -48,13 +48,14 @@ __device__ __forceinline__ void load_gamma(const NormParams &p, int u, float (&g
 
 template <bool WHOLE, typename T>
 __device__ __forceinline__ uint4 load_vector(const T *row, int u, int cols, bool aligned) {
-    return WHOLE ? reinterpret_cast<const uint4 *>(row)[u] : mx::load_values(row, (int64_t)u * Vec16<T>::kN, cols, aligned);
+    // (a row's address and an unsigned offset of 32 bits: one instruction's operands)
+    return WHOLE ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(row) + (uint32_t)u * 16u) : mx::load_values(row, (int64_t)u * Vec16<T>::kN, cols, aligned);
 }
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void store_vector(T *row, int u, int cols, const uint4 &values, bool aligned) {
     constexpr int kN = Vec16<T>::kN;
     if (WHOLE || (aligned && u * kN + kN <= cols)) {
-        reinterpret_cast<uint4 *>(row)[u] = values;
+        *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(row) + (uint32_t)u * 16u) = values;
     } else {
         const T *v = reinterpret_cast<const T *>(&values);
 #pragma unroll
@@ -70,7 +71,11 @@ __device__ __forceinline__ uint4 add_rounded(const uint4 &a, const uint4 &b) {
     Vec16<T>::get(a, x);
     Vec16<T>::get(b, r);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) x[i] = __fadd_rn(x[i], r[i]);
+    for (int i = 0; i < kN; i += 2) {
+        const float2 s = add2(make_float2(x[i], x[i + 1]), make_float2(r[i], r[i + 1]));
+        x[i] = s.x;
+        x[i + 1] = s.y;
+    }
     return Vec16<T>::put(x);
 }
 
@@ -233,12 +238,12 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             const RowScale scale(row_max<WARP>(__float_as_uint(most), maxima));
             if (at == 0) static_cast<float *>(p.scales)[r] = scale.scale;
             int8_t *yr = static_cast<int8_t *>(p.y) + r * p.y_pitch;
-            each(Live(), [&](int i, int u, const uint4 &h) {
+            auto write = [&](auto finite, int i, int u, const uint4 &h) {
                 float (&v)[kN] = kept[kKeep ? i : 0];
                 if (!kKeep) normed(h, u, v);
                 uint32_t w[kN / 4];
-                quantize_values(scale, v, w);
-                int8_t *to = yr + u * kN;
+                quantize_values<decltype(finite)::value>(scale, v, w);
+                int8_t *to = yr + (uint32_t)(u * kN);
                 if (WHOLE || (p.y_aligned && u * kN + kN <= p.cols)) {
                     if constexpr (kN == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[1]);
                     else *reinterpret_cast<uint32_t *>(to) = w[0];
@@ -247,7 +252,10 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
                     for (int i = 0; i < kN; ++i)
                         if (u * kN + i < p.cols) to[i] = (int8_t)(w[i / 4] >> (8 * (i % 4)));
                 }
-            });
+            };
+            // (chosen once for a row)
+            if (scale.finite) each(Live(), [&](int i, int u, const uint4 &h) { write(std::true_type(), i, u, h); });
+            else each(Live(), [&](int i, int u, const uint4 &h) { write(std::false_type(), i, u, h); });
         } else {
             const int used = (p.cols + mx::kGroup - 1) / mx::kGroup * mx::kGroup;
             uint8_t *yr = static_cast<uint8_t *>(p.y) + r * p.y_pitch, *scales = static_cast<uint8_t *>(p.scales) + mx::word_at(r, 0, p.tiles);

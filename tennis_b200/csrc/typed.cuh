@@ -158,20 +158,20 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
-// quantize16 of fp32 values in registers, products by twos.
-template <int N>
+// quantize16 of fp32 values in registers, products by twos.  FINITE: of a row of numbers.
+template <bool FINITE, int N>
 __device__ __forceinline__ void quantize_values(const RowScale &q, const float (&v)[N], uint32_t (&to)[N / 4]) {
     uint32_t r[N];
-    if (q.finite) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
+    for (int i = 0; i < N; i += 2) {
+        if constexpr (FINITE) {
             const float2 t = mul2(make_float2(v[i], v[i + 1]), make_float2(q.by, q.by));
             r[i] = __float_as_uint(__fadd_rn(t.x, 12582912.0f));
             r[i + 1] = __float_as_uint(__fadd_rn(t.y, 12582912.0f));
+        } else {
+            r[i] = (uint32_t)q(v[i]);
+            r[i + 1] = (uint32_t)q(v[i + 1]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r[i] = (uint32_t)q(v[i]);
     }
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) to[i] = __byte_perm(__byte_perm(r[4 * i], r[4 * i + 1], 0x0040), __byte_perm(r[4 * i + 2], r[4 * i + 3], 0x0040), 0x5410);
