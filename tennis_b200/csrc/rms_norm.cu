@@ -261,12 +261,12 @@ rms_norm_kernel(const __grid_constant__ NormParams p) {
             uint8_t *yr = static_cast<uint8_t *>(p.y) + r * p.y_pitch, *scales = static_cast<uint8_t *>(p.scales) + mx::word_at(r, 0, p.tiles);
             constexpr int kLanes = 128 / kN;      // of a tile of scales
             each(All(), [&](int, int u, const uint4 &h) {
-                float v[kN];
-                normed(h, u, v);
-                if (u >= vectors)
-#pragma unroll
-                    for (int i = 0; i < kN; ++i) v[i] = 0.0f;
-                clear_behind(u, v);
+                // (behind the row's end there is nothing of gamma to read)
+                float v[kN] = {};
+                if (u < vectors) {
+                    normed(h, u, v);
+                    clear_behind(u, v);
+                }
                 uint32_t word;
                 const uint32_t codes = mx::quantize_lanes<kN>(v, __float_as_uint(largest(v, 0.0f)), &word);
                 if (u * kN < used) mx::store_codes<kN>(yr + u * (kN / 2), codes, WHOLE || p.y_aligned);

@@ -164,6 +164,23 @@ def test_streams_and_graphs():
     check(got, x, g, r, torch.int8)
 
 
+def last_in_memory(t):
+    """t as the last bytes of an allocation."""
+    room = torch.empty(32 << 20, dtype=torch.uint8, device="cuda")[-t.numel() * t.element_size():].view(t.dtype).view(t.shape)
+    return room.copy_(t)
+
+
+@pytest.mark.parametrize("k", [8, 64, 264, 320, 520, 1000, 1032, 4104, 8200])
+def test_nothing_is_read_behind_the_ends(k):
+    """Rows of whole vectors whose scales' tiles, and whose threads, reach beyond them."""
+    from tennis_b200 import ops
+    for dtype in FLOATS:
+        x, r, gamma = (last_in_memory(t) for t in (features(3, k, dtype, k), features(3, k, dtype, k + 1), weights(k)))
+        for out in (dtype, torch.int8, FP4):
+            check(ops.rms_norm(x, gamma, out_dtype=out), x, gamma, None, out)
+            check(ops.rms_norm(x, gamma, r, out_dtype=out), x, gamma, r, out)
+
+
 def test_many_rows():
     """Offsets beyond 2^31 bytes."""
     from tennis_b200 import ops
