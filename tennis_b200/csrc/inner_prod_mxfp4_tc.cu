@@ -13,7 +13,7 @@
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of token tiles, whose operands the L2 then serves
 //
 // Measured, bf16 out: 8192^3 182 us (6.0 PFLOP/s; for seconds, at the power limit, 225), 4096^3 28.8 us (with a residual 38.5), 2048 x 4096 x 4096 16.4 us, 128 x 4096 x 4096
-// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 15.6 us, where stores bound it (silu: 20.3, where the special-function unit does).  Of 8192^3 loads and shared memory alone take
+// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 14.1 us, half of them stores (silu: 19.2, where the special-function unit bounds it).  Of 8192^3 loads and shared memory alone take
 // 132 us, the scales' copies nothing.
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and all roles go to the common exit.
@@ -37,7 +37,7 @@ struct Mxfp4Params : Walk {
 template <typename T, int BN, bool RES, bool PAIR, int SPLIT>
 struct Layout {
     // A step of the epilogue is 2 KB of y in rows of 128 bytes: a copy costs the engine that moves it 4.5 clocks a row of up to 128 bytes (100352 x 256 x 64, which
-    // that engine bounds, 20.5 -> 15.6 us).  Pairs, whose columns of sums are handed on 32 at a time, and splits take rows of 32 channels.
+    // that engine bound, 20.5 -> 15.6 us).  Pairs, whose columns of sums are handed on 32 at a time, and splits take rows of 32 channels.
     static constexpr int kChannels = PAIR || SPLIT > 1 ? kCh : 128 / (int)sizeof(T);
     using Step = Staged<T, kChannels>;
     static constexpr bool kAhead = RES && SPLIT == 1;                             // residuals of a step come while the one in front of it is worked on

@@ -158,7 +158,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
-// quantize16 of fp32 values in registers, products by twos.  FINITE: of a row of numbers.
+// quantize16 of fp32 values in registers, products by twos (and sums not: a packed sum of a packed product is one fused operation as compiled here, one rounding in place
+// of two).  FINITE: of a row of numbers.
 template <bool FINITE, int N>
 __device__ __forceinline__ void quantize_values(const RowScale &q, const float (&v)[N], uint32_t (&to)[N / 4]) {
     uint32_t r[N];
