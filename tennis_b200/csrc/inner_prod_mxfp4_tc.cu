@@ -13,7 +13,7 @@
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of token tiles, whose operands the L2 then serves
 //
 // Measured, bf16 out: 8192^3 182 us (6.0 PFLOP/s; for seconds, at the power limit, 225), 4096^3 28.8 us (with a residual 38.5), 2048 x 4096 x 4096 16.4 us, 128 x 4096 x 4096
-// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 14.1 us, half of them stores (silu: 19.2, where the special-function unit bounds it).  Of 8192^3 loads and shared memory alone take
+// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 14.1 us, half of them stores (silu: 19.2, where its instructions and the special-function unit bound it).  Of 8192^3 loads and shared memory alone take
 // 132 us, the scales' copies nothing.
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and all roles go to the common exit.
