@@ -30,11 +30,18 @@ struct NormParams {
     int aligned, sum_aligned, y_aligned, gamma_aligned, scales_aligned;      // aligned: of what is read
 };
 
+// Where vector u of a row lies, N elements each.  WHOLE: such rows have 4 * kMost vectors at most, and an address and an unsigned offset of 32 bits are one instruction's
+// operands; other rows may be longer than 2^32 bytes.
+template <bool WHOLE, int N, typename E>
+__device__ __forceinline__ E *vector_at(E *row, int u) {
+    return WHOLE ? reinterpret_cast<E *>(reinterpret_cast<uintptr_t>(row) + (uint32_t)u * (uint32_t)(N * sizeof(E))) : row + (int64_t)u * N;
+}
+
 // Vector u of gamma; ones where there is none, and where a row has ended.  WHOLE: vectors are whole and lie on 16 bytes.
 template <bool WHOLE, int N>
 __device__ __forceinline__ void load_gamma(const NormParams &p, int u, float (&g)[N]) {
     if (p.gamma && (WHOLE || (p.gamma_aligned && u * N + N <= p.cols))) {
-        const float4 *from = reinterpret_cast<const float4 *>(reinterpret_cast<const char *>(p.gamma) + (uint32_t)u * (N * 4u));
+        const float4 *from = reinterpret_cast<const float4 *>(vector_at<WHOLE, N>(p.gamma, u));
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
             const float4 v = from[i / 4];
@@ -48,14 +55,13 @@ __device__ __forceinline__ void load_gamma(const NormParams &p, int u, float (&g
 
 template <bool WHOLE, typename T>
 __device__ __forceinline__ uint4 load_vector(const T *row, int u, int cols, bool aligned) {
-    // (a row's address and an unsigned offset of 32 bits: one instruction's operands)
-    return WHOLE ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(row) + (uint32_t)u * 16u) : mx::load_values(row, (int64_t)u * Vec16<T>::kN, cols, aligned);
+    return WHOLE ? *reinterpret_cast<const uint4 *>(vector_at<WHOLE, Vec16<T>::kN>(row, u)) : mx::load_values(row, (int64_t)u * Vec16<T>::kN, cols, aligned);
 }
 template <bool WHOLE, typename T>
 __device__ __forceinline__ void store_vector(T *row, int u, int cols, const uint4 &values, bool aligned) {
     constexpr int kN = Vec16<T>::kN;
     if (WHOLE || (aligned && u * kN + kN <= cols)) {
-        *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(row) + (uint32_t)u * 16u) = values;
+        *reinterpret_cast<uint4 *>(vector_at<WHOLE, kN>(row, u)) = values;
     } else {
         const T *v = reinterpret_cast<const T *>(&values);
 #pragma unroll

@@ -208,3 +208,49 @@ def test_refusals():
     for eps in (-1.0, float("nan"), float("inf")):
         with pytest.raises(Exception, match="eps"):
             ops.rms_norm(x, g, eps=eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_rows_longer_than_2_to_the_30(dtype):
+    """One row whose gamma, and of fp32 whose values, lie beyond 2^32 bytes: every result, the end's and the beginning's.  Values are small whole numbers, so the squares'
+    sum is exact in 64 bits in any order and the reciprocal deviation is one fp32 number; v is its two fp32 products."""
+    from tennis_b200 import ops
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("40 GB of memory")
+    k, piece, dev = (1 << 30) + 1_000_003, 1 << 26, torch.device("cuda")
+    g = torch.Generator(device=dev).manual_seed(k)
+    x, r = (torch.empty((1, k), dtype=torch.int8, device=dev).random_(-3, 4, generator=g).to(dtype) for _ in range(2))
+    gamma = torch.rand(k, device=dev, generator=g).add_(0.5)
+
+    def pieces(total):
+        return [slice(at, min(at + piece, total)) for at in range(0, total, piece)]
+
+    for residual in (None, r):
+        def h_of(at):
+            return x[0, at].float() if residual is None else x[0, at].float() + r[0, at].float()
+
+        squares = sum(float((h_of(at).double() ** 2).sum()) for at in pieces(k))
+        by = np.float32(1.0 / np.sqrt(squares / k + 1e-6))
+
+        def v_of(at):
+            return h_of(at) * float(by) * gamma[at]
+
+        largest = max(float(v_of(at).abs().max()) for at in pieces(k))
+        for out in (dtype, torch.int8, FP4):
+            got = ops.rms_norm(x, gamma, residual, 1e-6, out)
+            got = got if isinstance(got, tuple) else (got,)
+            if residual is not None:
+                assert all(torch.equal(got[-1][0, at], h_of(at).to(dtype)) for at in pieces(k))
+            if out == dtype:
+                assert all(torch.equal(got[0][0, at], v_of(at).to(dtype)) for at in pieces(k))
+            elif out == torch.int8:
+                assert got[1].item() == np.float32(largest) / np.float32(127)
+                factor = float(np.float32(127) / np.float32(largest))
+                assert all(torch.equal(got[0][0, at], (v_of(at) * factor).round().to(torch.int8)) for at in pieces(k))
+            else:
+                q, s = bits(got[0]), bits(got[1]).view(-1, 128, 4)
+                for at in pieces(k):
+                    want_q, want_s = (bits(t) for t in ops.quantize_rows_mxfp4(v_of(at).view(1, -1)))
+                    first = at.start // 128
+                    assert torch.equal(q[0, at.start // 2:][:want_q.shape[1]], want_q[0]) and torch.equal(s[first:first + want_s.shape[1]], want_s.view(-1, 128, 4))
+            del got
