@@ -9,36 +9,68 @@ namespace {
 
 // ---- CUDA-core kernel: any alignment, any pitch -----------------------------------------------------------------------
 // A block computes 64 tokens x 64 output channels, 16 values a thread (4 x 4), two groups of K at a time as fp32 values in shared memory.  Bound by fused multiply-adds and
-// the shared-memory reads that feed them (8192^3 42.8 ms): for operands that the copies of the other kernels cannot read.
+// the shared-memory reads that feed them (8192^3 43.7 ms): for operands that the copies of the other kernels cannot read.
+// Under the two largest scales, 2^126 and 2^127, a value may lie beyond fp32 and its product with the other operand's not: where one of a block's groups has such a
+// scale, values are staged without their scales, and a group's sum of products, which is exact then (at most 32 * 36, multiples of a quarter), joins the others times both scales.
 constexpr int kTile = 64, kTileK = 64, kThreads = 256;
 constexpr int kRow = kTileK + 1;         // words of a staged row; odd, so that neighbouring rows lie in different banks
+constexpr int kTileGroups = kTileK / mx::kGroup;
+constexpr int kLarge = 253;              // the lowest byte of such a scale (255 is NaN, not one)
 
-// Sixteen values of row r from value k on (half of a group) into a staged row; zeros where the row or the group does not exist
-__device__ __forceinline__ void stage16(const uint8_t *q, int64_t pitch, const uint8_t *scales, int64_t r, bool exists, int k, int groups, float *to) {
-    const int g = k / mx::kGroup;
-    float v[8];
-    if (!exists || g >= groups) {
+// Sixteen codes of a row, half of a group, and the byte of its scale; zeros where the row or the group does not exist.
+struct Half {
+    uint32_t codes[2] = {0, 0};
+    int byte = 0;
+    __device__ __forceinline__ Half(const uint8_t *q, int64_t pitch, const uint8_t *scales, int64_t r, bool exists, int k, int groups) {
+        const int g = k / mx::kGroup;
+        if (!exists || g >= groups) return;
+        const uint8_t *from = q + r * pitch + k / 2;
+        byte = scales[mx::word_at(r, g / mx::kTileGroups, (groups + mx::kTileGroups - 1) / mx::kTileGroups) + g % mx::kTileGroups];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) to[i] = 0.0f;
-        return;
+        for (int b = 0; b < 8; ++b) codes[b / 4] |= (uint32_t)from[b] << (8 * (b % 4));
     }
-    const uint8_t *from = q + r * pitch + k / 2;
-    const float by = mx::scale_value(scales[mx::word_at(r, g / mx::kTileGroups, (groups + mx::kTileGroups - 1) / mx::kTileGroups) + g % mx::kTileGroups]);
+    __device__ __forceinline__ bool large() const { return byte >= kLarge && byte < 255; }
+    // its values, without their scale where they are kept `apart` from it, into a staged row
+    __device__ __forceinline__ void stage(bool apart, float *to) const {
+        const float by = mx::scale_value(apart && byte < 255 ? 127 : byte);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t codes = 0;
+        for (int h = 0; h < 2; ++h) {
+            float v[8];
+            mx::values_of<8>(codes[h], v);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) codes |= (uint32_t)from[4 * h + b] << (8 * b);
-        mx::values_of<8>(codes, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) to[8 * h + i] = __fmul_rn(v[i], by);
+            for (int i = 0; i < 8; ++i) to[8 * h + i] = __fmul_rn(v[i], by);
+        }
     }
+};
+
+// acc[i][j] + the products of values q0 to q1 - 1 of staged tokens tm + 16 i and channels tn + 16 j
+__device__ __forceinline__ void multiply(const float (&sx)[kTile][kRow], const float (&sw)[kTile][kRow], int tm, int tn, int q0, int q1, float (&acc)[4][4]) {
+#pragma unroll 4
+    for (int q = q0; q < q1; ++q) {
+        float a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = sx[tm + 16 * i][q];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = sw[tn + 16 * j][q];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+    }
+}
+
+// sum + part * 2^e, one rounding.  part: 0, or from 2^-2 to 2^11 in magnitude (or NaN); beyond +-200 e is of no account: such a product is infinite, or nothing beside any sum.
+__device__ __forceinline__ float add_scaled(float part, int e, float sum) {
+    e = min(max(e, -200), 200);
+    const int half = e >> 1;
+    return fmaf(__fmul_rn(part, __int_as_float((half + 127) << 23)), __int_as_float((e - half + 127) << 23), sum);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 inner_prod_mxfp4_direct_kernel(const __grid_constant__ InnerProdMxfp4Params p) {
     __shared__ float sx[kTile][kRow], sw[kTile][kRow];
+    __shared__ int ex[kTileGroups][kTile], ew[kTileGroups][kTile];   // exponents of the groups' scales, where values are staged without
     pdl_sync();
     const int n_tiles = (p.n + kTile - 1) / kTile;
     const int64_t tiles = (p.m + kTile - 1) / kTile * n_tiles;
@@ -49,21 +81,27 @@ inner_prod_mxfp4_direct_kernel(const __grid_constant__ InnerProdMxfp4Params p) {
         const int n0 = (int)(t % n_tiles) * kTile;
         float acc[4][4] = {};
         for (int k0 = 0; k0 < p.groups * mx::kGroup; k0 += kTileK) {
+            const Half x(p.x, p.x_pitch, p.x_scales, m0 + lr, m0 + lr < p.m, k0 + lk, p.groups), w(p.w, p.w_pitch, p.w_scales, n0 + lr, n0 + lr < p.n, k0 + lk, p.groups);
+            const bool apart = __syncthreads_or(x.large() || w.large());      // (and nobody reads the staged values of the turn before any more)
+            x.stage(apart, &sx[lr][lk]);
+            w.stage(apart, &sw[lr][lk]);
+            if (apart && lk % mx::kGroup == 0) {
+                ex[lk / mx::kGroup][lr] = x.byte - 127;
+                ew[lk / mx::kGroup][lr] = w.byte - 127;
+            }
             __syncthreads();
-            stage16(p.x, p.x_pitch, p.x_scales, m0 + lr, m0 + lr < p.m, k0 + lk, p.groups, &sx[lr][lk]);
-            stage16(p.w, p.w_pitch, p.w_scales, n0 + lr, n0 + lr < p.n, k0 + lk, p.groups, &sw[lr][lk]);
-            __syncthreads();
-#pragma unroll 4
-            for (int q = 0; q < kTileK; ++q) {
-                float a[4], b[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = sx[tm + 16 * i][q];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b[j] = sw[tn + 16 * j][q];
+            if (!apart) {
+                multiply(sx, sw, tm, tn, 0, kTileK, acc);
+                continue;
+            }
+#pragma unroll 1
+            for (int g = 0; g < kTileGroups; ++g) {
+                float part[4][4] = {};
+                multiply(sx, sw, tm, tn, g * mx::kGroup, (g + 1) * mx::kGroup, part);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+                    for (int j = 0; j < 4; ++j) acc[i][j] = add_scaled(part[i][j], ex[g][tm + 16 * i] + ew[g][tn + 16 * j], acc[i][j]);
             }
         }
 #pragma unroll

@@ -422,3 +422,29 @@ def test_offsets_beyond_32_bits():
     y = ops.inner_prod_mxfp4(x, xs, d["w"], d["ws"], d["bias"])
     want = ops.inner_prod_mxfp4(d["x"][:128], d["xs"][:1], d["w"], d["ws"], d["bias"])
     assert torch.equal(y.view(-1, 128, 24), want.expand(m // 128, 128, 24))
+
+
+@pytest.mark.parametrize("m", [1, 20, 50, 200])
+def test_scales_at_the_ends_of_operands_off_16_bytes(m):
+    """A value under its own scale may lie beyond fp32 where the product does not: every kernel has the sums' very bits.  Sums are multiples of a quarter of the smallest two
+    scales' product and, of scales that spread over six powers of two together, below 36 * 256 * 2^6 = 2^19.2 times that: exact in fp32 in any order."""
+    from tennis_b200 import _lib, ops
+    n, k = 130, 256
+    for low, high in ((250, 0), (0, 250), (251, 3), (5, 248)):
+        g = torch.Generator(device="cuda").manual_seed(m + low)
+        for layout in (dict(), dict(x_at=8), dict(w_at=1), dict(x_pitch=k // 2 + 1, w_pitch=k // 2 + 3)):
+            x, _ = rows(m, k, g, pitch=layout.get("x_pitch"), at=layout.get("x_at", 0))
+            w, _ = rows(n, k, g, pitch=layout.get("w_pitch"), at=layout.get("w_at", 0))
+            xs, ws = (torch.randint(at, at + 4, (count, k // 32), dtype=torch.uint8, device="cuda", generator=g) for at, count in ((low, m), (high, n)))
+            xs[m // 2, 3], ws[7, 5] = 255, 255                # (not finite: NaN in their row and column alone)
+            xt, wt = ops.mxfp4_scale_tiles(xs), ops.mxfp4_scale_tiles(ws)
+            want = torch.from_numpy(plain.decode(x, xt) @ plain.decode(w, wt).T)
+            assert want.isnan().sum() == m + n - 1
+            for kernel in (_lib.KERNEL_AUTO, _lib.KERNEL_DIRECT):
+                got = ops.inner_prod_mxfp4(x, xt, w, wt, kernel=kernel).cpu()
+                assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.double().nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    x, w = (torch.full((count, k // 2), 0x22, dtype=torch.uint8, device="cuda") for count in (m, n))      # ones
+    w[::2] = 0
+    xt, wt = (ops.mxfp4_scale_tiles(torch.full((count, k // 32), byte, dtype=torch.uint8, device="cuda")) for count, byte in ((m, 254), (n, 250)))
+    got = ops.inner_prod_mxfp4(x, xt, w, wt, kernel=_lib.KERNEL_DIRECT)      # 2^127 times 2^123, and times nothing
+    assert (got[:, ::2] == 0).all() and (got[:, 1::2] == float("inf")).all()
