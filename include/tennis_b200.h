@@ -475,7 +475,8 @@ TSB_API int tsb_dequantize_rows_mxfp4(const void *q, int64_t q_pitch, const void
  * inner product on 4-bit rows: y[m][n] = activation(sum_k x[m][k] * w[n][k] (+ bias[n]) (+ residual[m][n])) of the values that codes
  * and scales stand for.
  *   - Products are exact, sums are held in fp32; their order, and with it the last bits, depend on the kernel that the sizes choose, but not on the
- *     values, the call or the rows of other tiles: the same call gives the same bits.  Steps behind the sum as in tsb_inner_prod_i8.
+ *     values, the call or the rows of other tiles: the same call gives the same bits.  Steps behind the sum as in tsb_inner_prod_i8, but for gelu of 16-bit results: off by 2^-15 of
+ *     itself at most before it is rounded, down to v = -13; from there on, where it is less than 10^-37, it becomes 0.
  *   - x: 4-bit rows with x_scales, or floating rows without: those are quantized as tsb_quantize_rows_mxfp4 does it.
  *   - w, w_scales: n rows of k values, as tsb_quantize_rows_mxfp4 lays out a weight tensor.  Rows are read to the end of their last
  *     group, where zeros lie behind the k values; scales to the end of their tiles, where places without a group hold zero.

@@ -28,23 +28,26 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     return d;
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
-// gelu of values that become results of 16 bits: v / 2 + |v| / 2 - |v| / 2 erfc(|v| / sqrt(2)), with erfc by Abramowitz and Stegun's formula 7.1.26, P(t) exp(-x^2) of t = 1 / (1 + 0.3275911 x) and a
-// polynomial of degree five, which is off by 1.5e-7 at most: |v| 2^-23.7 of a value whose half step is 2^-12 of itself or more.  (erff and the rest are some 60 instructions a value,
-// these 12: 333 x 777 x 1021 with a residual 6.1 -> 5.5 us.)
+// gelu of values that become results of 16 bits: v / 2 + |v| / 2 - |v| / 2 erfc(|v| / sqrt(2)).  With b = |v| sqrt(log2(e) / 2) and t = 1 / (b + 2.451) that is exp2(-b^2) b t P(t), a polynomial of
+// degree six that was fitted by linear programming, so that erfc is off by 5.3e-8 at most and by 6.7e-6 of itself: below zero, where the result is the last term alone, the second counts.  With
+// the roundings of fp32 the result is off by 2^-16 of itself at most (2^-19 from v = -1 on), a sixteenth of half a step of fp16 at most, down to v = -13, and is zero below -13.3.  (erff and the rest are some
+// 60 instructions a value, these 12: 333 x 777 x 1021 with a residual 6.1 -> 5.4 us.)
 __device__ __forceinline__ float2 gelu_short(float2 v) {
-    const float2 a = make_float2(fminf(fabsf(v.x), 16.0f), fminf(fabsf(v.y), 16.0f));      // (erfc is 0 there; an infinity's would be infinity times 0)
-    const float2 d = fma2(a, both(0.23164190f), both(1.0f));                                // 0.3275911 / sqrt(2)
+    const float2 w = mul2(make_float2(fabsf(v.x), fabsf(v.y)), both(0.849321783f));
+    const float2 b = make_float2(fminf(w.x, 13.6f), fminf(w.y, 13.6f));      // (erfc is 0 there; an infinity's would be infinity times 0)
+    const float2 d = add2(b, both(2.4512701f));
     const float2 t = make_float2(reciprocal_approx(d.x), reciprocal_approx(d.y));
-    const float2 q = mul2(mul2(a, both(-0.72134752f)), a);                                  // -log2(e) / 2
-    const float2 e = make_float2(exp2_approx(q.x), exp2_approx(q.y));
-    float2 p = fma2(both(1.061405429f), t, both(-1.453152027f));
-    p = fma2(p, t, both(1.421413741f));
-    p = fma2(p, t, both(-0.284496736f));
-    p = fma2(p, t, both(0.254829592f));
-    const float2 tail = mul2(mul2(mul2(p, t), e), mul2(a, both(-0.5f)));
+    const float2 q = mul2(b, b);
+    const float2 e = make_float2(exp2_approx(-q.x), exp2_approx(-q.y));
+    float2 p = fma2(both(-27.3318176f), t, both(47.4502983f));
+    p = fma2(p, t, both(-23.1390343f));
+    p = fma2(p, t, both(-0.0789856464f));
+    p = fma2(p, t, both(-2.50978255f));
+    p = fma2(p, t, both(-0.955673873f));
+    p = fma2(p, t, both(-0.399428397f));
     // (a NaN is one here, whatever the minimum above made of it, and minus infinity becomes one)
     const float2 rising = fma2(make_float2(fabsf(v.x), fabsf(v.y)), both(0.5f), mul2(v, both(0.5f)));
-    return add2(rising, tail);
+    return fma2(mul2(mul2(p, t), e), b, rising);
 }
 // The activation as activate() takes it, gelu of 16-bit results as above.
 template <int ACT, typename T, int N>

@@ -448,3 +448,21 @@ def test_scales_at_the_ends_of_operands_off_16_bytes(m):
     xt, wt = (ops.mxfp4_scale_tiles(torch.full((count, k // 32), byte, dtype=torch.uint8, device="cuda")) for count, byte in ((m, 254), (n, 250)))
     got = ops.inner_prod_mxfp4(x, xt, w, wt, kernel=_lib.KERNEL_DIRECT)      # 2^127 times 2^123, and times nothing
     assert (got[:, ::2] == 0).all() and (got[:, 1::2] == float("inf")).all()
+
+
+@pytest.mark.parametrize("out", [torch.float16, torch.bfloat16], ids=str)
+def test_gelu_of_short_results_far_below_zero(out):
+    """gelu of 16-bit results is off by 2^-15 of itself before it is rounded, below zero too, where it is far smaller than its argument: so by (1 + 2^-8) times that and half a step behind
+    it, of fp16's smallest numbers 2^-25.  From v = -13 on; what is below -13.3 is less than 2^-126 and becomes zero."""
+    from tennis_b200 import ops
+    v = torch.cat([torch.linspace(-13.0, 0.0, 6000), torch.linspace(0.0, 8.0, 2000), -torch.logspace(-6, -1, 180), torch.tensor([-13.4, -16.0, -17.0, -40.0, -1e3, -1e30, 16.0, 1e3, 6e4, 0.0])]).cuda()
+    n = v.numel()
+    assert n % 8 == 6
+    x = v.double().cpu()
+    want = 0.5 * x * torch.erfc(-x * 0.5 ** 0.5)
+    want[x < -13.3] = 0.0
+    room = want.abs() * (torch.finfo(out).eps / 2 + 2.0 ** -15 * (1 + 2.0 ** -8)) + (2.0 ** -25 if out == torch.float16 else 2.0 ** -134)
+    for m in (1, 40, 300):
+        d = case(m, n, 48, out, 3)
+        got = ops.inner_prod_mxfp4(torch.zeros_like(d["x"].view(torch.uint8)), d["xs"], d["w"], d["ws"], v, activation=4, out_dtype=out).cpu().double()
+        assert ((got - want).abs() <= room).all(), float(((got - want).abs() / room).max())
