@@ -229,7 +229,17 @@ PyObject *group_norm(PyObject *, PyObject *const *args, Py_ssize_t count) {
 }
 
 // ---- 4 bits
-constexpr at::ScalarType kFp4 = at::ScalarType::Float4_e2m1fn_x2, kE8m0 = at::ScalarType::Float8_e8m0fnu;
+// (a PyTorch without these types: bytes, as in ops.py)
+#if TSB_TORCH_FP4
+constexpr at::ScalarType kFp4 = at::ScalarType::Float4_e2m1fn_x2;
+#else
+constexpr at::ScalarType kFp4 = at::kByte;
+#endif
+#if TSB_TORCH_E8M0
+constexpr at::ScalarType kE8m0 = at::ScalarType::Float8_e8m0fnu;
+#else
+constexpr at::ScalarType kE8m0 = at::kByte;
+#endif
 int64_t row_bytes(int64_t k) { return (k + 31) / 32 * 16; }
 
 // Values and their scales, which are of use together alone, in one allocation (a second one takes 0.7 us of a call of 5): a tensor of `type` of `sizes`, `step` elements between rows of

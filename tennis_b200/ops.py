@@ -528,7 +528,9 @@ _TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloa
 _FLOATS = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 _FLOAT_NAMES = "float32, float16 or bfloat16, not %s"
 _int8, _float32 = torch.int8, torch.float32
-_mxfp4, _e8m0, _uint8 = torch.float4_e2m1fn_x2, torch.float8_e8m0fnu, torch.uint8
+_uint8 = torch.uint8
+# (a PyTorch without the types of 4-bit values or their scales: their bytes, which are taken everywhere, in their place)
+_mxfp4, _e8m0 = getattr(torch, "float4_e2m1fn_x2", _uint8), getattr(torch, "float8_e8m0fnu", _uint8)
 
 
 _native = None
@@ -811,7 +813,8 @@ def _pixel_step(x):
 # ---- layers in 4 bits: quantize_rows_mxfp4, dequantize_rows_mxfp4, inner_prod_mxfp4; rms_norm, in front of products in 8 or 4 bits ----------
 # Devices, streams, and which calls go through native.cpp: as above.  A 4-bit matrix [m, k] is a tensor of torch.float4_e2m1fn_x2 (two
 # values an element), [m, 16 * ceil(k / 32)], and its scales are one of torch.float8_e8m0fnu, [ceil(m / 128), ceil(k / 128), 32, 4, 4] in the order that the
-# tensor cores read (mxfp4_scale_tiles makes it of scales row by row); uint8 tensors of the same bytes are taken too.
+# tensor cores read (mxfp4_scale_tiles makes it of scales row by row); uint8 tensors of the same bytes are taken too, and are what comes out where PyTorch has
+# no such types.
 def _row_bytes(k):
     return (k + 31) // 32 * 16
 

@@ -178,3 +178,30 @@ def test_every_wait_code_has_a_name_of_its_own(lib):
     assert lib.tsb_inner_prod_mxfp4_status_decode(codes[-1] + 1) == _lib.ERR_DEVICE_TIMEOUT and "an unknown event" in lib.tsb_last_error().decode()
     assert lib.tsb_inner_prod_mxfp4_status_decode(0) == 0
     assert "code (1..%d, which wait) in it" % codes[-1] in open(ROOT + "/include/tennis_b200.h").read()
+
+
+OLDER = """
+import sys, torch
+del torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+sys.path.insert(0, %r)
+import tennis_b200
+from tennis_b200 import ops, nets
+s = torch.arange(2 * 5, dtype=torch.uint8).view(2, 5)
+t = ops.mxfp4_scale_tiles(s)
+assert t.dtype == torch.uint8 and t.shape == (1, 2, 32, 4, 4) and t[0, 1, 1, 0, 0] == 9
+for call in (lambda: ops.quantize_rows_mxfp4(torch.zeros(2, 64)), lambda: ops.rms_norm(torch.zeros(2, 64), out_dtype=torch.uint8)):
+    try:
+        call()
+    except ops.EjectionException as e:
+        assert "is_cuda" in str(e)
+    else:
+        raise AssertionError("a host tensor was taken")
+"""
+
+
+def test_the_package_needs_no_4_bit_types():
+    """A PyTorch without the types of 4-bit values and their scales: the package imports, and works on their bytes."""
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", OLDER % ROOT], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout[-2000:]
