@@ -38,7 +38,7 @@ extern "C" {
 #define TSB_ACT_NONE 0
 #define TSB_ACT_RELU 1       /* src/kernels/cpu/relu.cpp:30-52 */
 #define TSB_ACT_LEAKY_RELU 2 /* src/kernels/cpu/leaky_relu.cpp:39-67, attribute "scale" */
-/* ... and, beyond the convolutions' three, after tsb_inner_prod_i8 and tsb_group_norm_nhwc */
+/* ... and, beyond the convolutions' three, after tsb_inner_prod_i8, tsb_inner_prod_mxfp4 and tsb_group_norm_nhwc */
 #define TSB_ACT_SILU 3       /* v / (1 + exp(-v)); 0 below v = -87, where that is less than 10^-35 */
 #define TSB_ACT_GELU 4       /* v / 2 * (1 + erf(v / sqrt(2))), in fp32 steps: far below zero the sum's rounding shows, up to |v| 2^-24 */
 
@@ -514,7 +514,8 @@ TSB_API int tsb_inner_prod_mxfp4_status_decode(int status_word);
 
 /*
  * Root-mean-square norm of rows, with the addition of a residual in front of it and rows quantized for a product behind it.
- *   h = x (+ residual, one fp32 addition rounded to x's type);  s = fp32(1 / sqrt(sum h^2 / cols + eps)), sum and root in 64 bits
+ *   h = x (+ residual, one fp32 addition rounded to x's type);  s = fp32(1 / sqrt(sum h^2 / cols + eps)), sum and root in 64 bits; the order of
+ *   that sum goes by sizes and alignment, which shows in s of fewer than one row in a million
  *   v = (h * s) * gamma[c], two separately rounded fp32 products
  *   y_type x_type             y = v, rounded to that type
  *   y_type TSB_TYPE_I8        y and scales as tsb_quantize_rows_i8 makes them of v (scales: float [rows])

@@ -14,7 +14,7 @@ namespace {
 // scale, values are staged without their scales, and a group's sum of products, which is exact then (at most 32 * 36, multiples of a quarter), joins the others times both scales.
 constexpr int kTile = 64, kTileK = 64, kThreads = 256;
 constexpr int kRow = kTileK + 1;         // words of a staged row; odd, so that neighbouring rows lie in different banks
-constexpr int kTileGroups = kTileK / mx::kGroup;
+constexpr int kTurnGroups = kTileK / mx::kGroup;      // of a turn of the loop over K
 constexpr int kLarge = 253;              // the lowest byte of such a scale (255 is NaN, not one)
 
 // Sixteen codes of a row, half of a group, and the byte of its scale; zeros where the row or the group does not exist.
@@ -70,7 +70,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads)
 inner_prod_mxfp4_direct_kernel(const __grid_constant__ InnerProdMxfp4Params p) {
     __shared__ float sx[kTile][kRow], sw[kTile][kRow];
-    __shared__ int ex[kTileGroups][kTile], ew[kTileGroups][kTile];   // exponents of the groups' scales, where values are staged without
+    __shared__ int ex[kTurnGroups][kTile], ew[kTurnGroups][kTile];   // exponents of the groups' scales, where values are staged without
     pdl_sync();
     const int n_tiles = (p.n + kTile - 1) / kTile;
     const int64_t tiles = (p.m + kTile - 1) / kTile * n_tiles;
@@ -95,7 +95,7 @@ inner_prod_mxfp4_direct_kernel(const __grid_constant__ InnerProdMxfp4Params p) {
                 continue;
             }
 #pragma unroll 1
-            for (int g = 0; g < kTileGroups; ++g) {
+            for (int g = 0; g < kTurnGroups; ++g) {
                 float part[4][4] = {};
                 multiply(sx, sw, tm, tn, g * mx::kGroup, (g + 1) * mx::kGroup, part);
 #pragma unroll

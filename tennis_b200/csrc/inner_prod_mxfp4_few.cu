@@ -3,7 +3,7 @@
 //   tile       128 output channels on the rows of an MMA, up to 64 tokens on its columns: what the tensor cores multiply for tokens that do not exist costs
 //              less than the weights' way from memory
 //   split      the CTAs of a cluster share a tile's K, so that a layer of few channels reads from all multiprocessors; their sums meet in the
-//              shared memory of the CTA that finishes a token (token t: CTA t modulo the cluster's size), added in the order of ranks
+//              shared memory of the CTA that finishes a token (each has neighbouring ones, all that fit an MMA in equal parts), added in the order of ranks
 //   loads      weights and their scales through a ring of TMA boxes, 256 values of K of 128 rows each
 //   tokens     4-bit rows, by TMA through the same ring; or floating rows, which the CTA quantizes into shared memory, its part of K alone, while
 //              its weights are on their way

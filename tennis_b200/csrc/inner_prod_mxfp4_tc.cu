@@ -12,9 +12,9 @@
 //              distributed shared memory and writes its own 32; the parts are added in a fixed order
 //   grid       persistent, one CTA per multiprocessor; neighbouring CTAs work on a block of token tiles, whose operands the L2 then serves
 //
-// Measured, bf16 out: 8192^3 182 us (6.0 PFLOP/s; for seconds, at the power limit, 225), 4096^3 28.8 us (with a residual 38.5), 2048 x 4096 x 4096 16.4 us, 128 x 4096 x 4096
-// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 14.1 us, half of them stores (silu: 19.2, where its instructions and the special-function unit bound it).  Of 8192^3 loads and shared memory alone take
-// 132 us, the scales' copies nothing.
+// Measured, bf16 out: 8192^3 184 us (6.0 PFLOP/s; for seconds, at the power limit, 223), 4096^3 29.7 us (with a residual 39.3), 2048 x 4096 x 4096 16.7 us, 128 x 4096 x 4096
+// 5.3 us, 1000^3 3.6 us; 100352 x 256 x 64 14.1 us, half of them stores (silu 19.2, gelu 22.0, where their instructions and the special-function unit bound it).  Of 8192^3 loads and shared memory
+// alone take 132 us, the scales' copies nothing.
 //
 // Every wait on a barrier is bounded; one that runs out records a code in the status word, raises the CTA's abort flag, and all roles go to the common exit.
 #include "inner_prod_mxfp4.h"
@@ -508,7 +508,8 @@ int launch(const Params &p, cudaStream_t stream) {
     if (!one && !PAIR && t.group_m == 1) clusters -= clusters % t.tiles_n;
     // No more stages than a CTA has blocks of K: what fits beside another kernel's CTAs starts while those run.  CTAs of a cluster hold tensor memory while they wait for each
     // other, so what fits a multiprocessor by its shared memory has to fit by its tensor memory too: a pair, which needs all of that, takes the shared memory as well, and
-    // splits (119 KB for 256 columns, 61 KB for 128) and clusters of few tokens (47 KB or more for 128) never come to more than 512 columns.
+    // splits (119 KB for 256 columns, 61 KB for 128) and clusters of few tokens (47 KB or more for 128) never come to more than 512 columns.  (The clusters of the int8 product and
+    // of the convolution take all of them, and 208 KB or more of shared memory, beside which none of these fits.)
     const int64_t loads = ceil_div64(tiles_all, clusters) * (SPLIT > 1 ? ceil_div(t.kblocks, SPLIT) : t.kblocks);
     int stages = PAIR ? L::kStages : (int)std::min<int64_t>(L::kStages, loads);
     static_assert(!PAIR || L::kFixed + L::kStages * L::kStage > 180 * 1024, "nothing that waits for a cluster fits beside a pair's CTA");

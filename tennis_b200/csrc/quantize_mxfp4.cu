@@ -3,7 +3,8 @@
 // Bound by memory.  A warp takes neighbouring values of a row: the largest magnitude of a group is found among the lanes that hold it, so nothing goes
 // through shared memory.  Instructions are what it takes to get there (at 19 a value, with 64-bit indexes and checks for every 16 bytes, 8192 x 16384
 // bf16 took 91 us): rows of more than a run go by runs whose ends are checked once.
-// Measured: 8192 x 16384 bf16 49 us (7.0 TB/s), back 52 us (6.5 TB/s); 16384 x 8192 fp32 85 and 93 us; 200000 x 64 bf16 7.1 and 15 us; 16 x 4096 bf16 2.2 and 2.0 us.
+// Measured: 8192 x 16384 bf16 49 us (7.0 TB/s), back 52 us (6.5 TB/s); 16384 x 8192 fp32 85 and 93 us; 200000 x 64 bf16 7.1 and 15 us; 16 x 4096 bf16 1.5 and 1.6 us; rows off 16 bytes,
+// value by value, 32768 x 1111 bf16 48 and 80 us.
 #include "mxfp4.cuh"
 
 #include <algorithm>

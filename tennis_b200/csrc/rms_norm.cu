@@ -1,11 +1,11 @@
 // Root-mean-square norm of rows: the residual's addition in front of it, int8 or 4-bit rows for a product behind it, in one pass.
 //
 // Bound by memory: a row is read once (two tensors of it with a residual), held in registers as the sums' own type while the squares are added up, and written
-// with its sum.  Squares are added in 64 bits, so that the mean does not depend on how a row is shared out (but in the 50th bit), and with it neither do
-// the 8- or 4-bit values behind it.  A row belongs to a warp, which needs no barrier, or to a block of as many warps as it needs: of many rows, threads with four
+// with its sum.  Squares are added in 64 bits: how a row is shared out, which goes by the number of rows and by alignment too, shows in the mean's 50th bit, and in the fp32
+// reciprocal deviation, and so in the results, of fewer than one row in a million.  A row belongs to a warp, which needs no barrier, or to a block of as many warps as it needs: of many rows, threads with four
 // vectors each (loads in flight), of few, more threads with one (a short way from load to store).
-// Measured, bf16 rows of 16384 x 8192: 92 us (5.8 TB/s), with a residual 158 (6.8), to int8 143 (6.6; for seconds, at the power limit, 155 to 163), to 4 bits 135 (6.5), without a
-// residual to int8 112 (3.6: instructions, two passes over gamma); 2048 x 4096 with a residual to 4 bits 12.6 us; 1 x 4096 2.5 us.
+// Measured, bf16 rows of 16384 x 8192: 92 us (5.8 TB/s), with a residual 158 (6.8), to int8 143 (6.6; for seconds, at the power limit, 155 to 163), to 4 bits 136 (6.5), without a
+// residual to int8 108 (3.7: instructions, two passes over gamma); 2048 x 4096 with a residual to 4 bits 12.7 us; 1 x 4096 2.5 us.
 #include "mxfp4.cuh"
 
 #include <algorithm>

@@ -855,7 +855,8 @@ def quantize_rows_mxfp4(x, out=None, scales=None, stream=None):
     """4-bit values of x [..., k] (fp32, fp16 or bf16) with a power of two for every 32 of a row: (q, scales), as tsb_quantize_rows_mxfp4 says.
 
     q is [..., 16 * ceil(k / 32)] float4_e2m1fn_x2, scales [ceil(m / 128), ceil(k / 128), 32, 4, 4] float8_e8m0fnu over the m rows of x.  The
-    rows are tokens of an activation, or output channels of a weight tensor.  ``out`` and ``scales`` take the results where they are given."""
+    rows are tokens of an activation, or output channels of a weight tensor.  ``out`` and ``scales`` take the results where they are given; else both may
+    lie in one storage (clone() one that is kept, or written to a file, without the other)."""
     if out is None and scales is None and stream is None:
         done = (_native or _ordinary()).quantize_rows_mxfp4(x)
         if done is not None:
@@ -1008,7 +1009,8 @@ def rms_norm(x, gamma=None, residual=None, eps=1e-6, out_dtype=None, out=None, s
 
     The result has x's type and shape; with ``out_dtype=torch.int8`` it is (q, scales) as quantize_rows gives them, what inner_prod_quantized reads,
     with ``out_dtype=torch.float4_e2m1fn_x2`` (q, scales) as quantize_rows_mxfp4 gives them, what inner_prod_mxfp4 reads.  With a residual h comes
-    as one result more: y, h or q, scales, h.  ``out``, ``scales`` and ``sum_out`` (h; it may be ``residual`` or x) take the results where they are given."""
+    as one result more: y, h or q, scales, h.  ``out``, ``scales`` and ``sum_out`` (h; it may be ``residual`` or x) take the results where they are given; q and
+    scales that are not may lie in one storage, as quantize_rows_mxfp4's."""
     if out is None and scales is None and sum_out is None and stream is None:
         done = (_native or _ordinary()).rms_norm(x, gamma, residual, eps, out_dtype)
         if done is not None:
